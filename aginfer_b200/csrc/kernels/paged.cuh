@@ -1,0 +1,220 @@
+// Paged K/V cache: what its kernels share, and the kernel that appends a step's keys and values to it.
+//
+// A cache is two pools [pages][kv_heads][head_dim / 64][page][64] of bf16, one of keys and one of values; the 16-byte chunk c of
+// a token's 64-column block lies at position c ^ (token & 7).  A run of consecutive tokens of one page, head and block is
+// therefore one contiguous run of memory and the byte image of a 128B-swizzled shared-memory tile: one bulk copy brings it in,
+// and both ldmatrix and tcgen05.mma read it without bank conflicts.
+//
+// A batch is `sequences` of them: rows starts[b] .. starts[b + 1) are the new tokens of sequence b, lengths[b] the tokens that it
+// holds once they are in, table[b * width + i] the page of its tokens [i * page, (i + 1) * page).  Row r of sequence b stands at
+// index lengths[b] - (starts[b + 1] - r) of its sequence; a row at a negative index is not appended and sees no key.
+//
+// starts, lengths and table are read on the device, so that one launch serves every step of a replayed graph.  What they must not
+// say is checked here: a page outside the pool or an index outside the table leaves a code in the status word and nothing is
+// read or written there.
+#pragma once
+
+#include "common.cuh"
+
+namespace paged {
+
+enum Status : unsigned {
+  kBadPage = 0x400,      // a table names a page outside the pool
+  kBadLength = 0x500,    // a sequence is longer than its row of the table
+  kMisaligned = 0x600,   // a tensor that is moved in 16-byte pieces does not start at a multiple of 16 bytes
+};
+
+__device__ __forceinline__ void report(unsigned* status, unsigned code) { atomicCAS(status, 0u, code); }
+
+// The sequence that holds a row: the number of sequences that end at or before it (`sequences` where none holds it).
+// Called by whole warps.
+__device__ __forceinline__ unsigned sequence_of(const int* starts, unsigned sequences, unsigned row) {
+  unsigned before = 0;
+  for (unsigned i = threadIdx.x & 31; i < sequences; i += 32) before += __ldg(starts + i + 1) <= int(row) ? 1u : 0u;
+  return __reduce_add_sync(0xffffffffu, before);
+}
+
+// The index of a row of sequence `seq` in it; whatever the tensors hold, the difference wraps and does not trap.
+__device__ __forceinline__ int index_of(const int* starts, const int* lengths, unsigned seq, unsigned row) {
+  return int(unsigned(__ldg(lengths + seq)) - (unsigned(__ldg(starts + seq + 1)) - row));
+}
+
+__device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<size_t>(p) & 15) == 0; }
+
+// Offset, in 64-column rows, of token t of a page's block.
+__device__ __forceinline__ size_t block_offset(unsigned page_id, unsigned kv_heads, unsigned head, unsigned blocks, unsigned block,
+                                               unsigned page) {
+  return ((size_t(page_id) * kv_heads + head) * blocks + block) * page;
+}
+
+}  // namespace paged
+
+// Queries and keys of a step's new tokens turned by their positions (half-split pairs, see rope.cuh), queries written to `q_out`,
+// keys and values to their pages.  Bound by memory: every row is read and written once.  Angles are formed in 64 bits: at
+// position 100000 a product in 32 bits would already be off by more than a bf16 rounding of the result; the sixty-four frequencies
+// are computed once a block and kept for its rows.
+// A block takes rows blockIdx.x, + gridDim.x, ...; a thread turns eight pairs of a head at a time (two 16-byte vectors), and
+// requests them before it computes the angles.
+// s0 says where a position comes from (below).  log2_theta + log2_theta_rest: log2 of theta in two pieces.
+// block = 128.  head_dim 64 or 128, strides multiples of 8.
+constexpr unsigned kPositionsFromCache = 0xffffffffu;   // s0: the index in the sequence, plus *offset where has_offset
+constexpr unsigned kPositionsOneAxis = 0xfffffffeu;     // s0: pos[row]; otherwise pos[3][rows] with sections s0, s1, rest
+extern "C" __global__ void __launch_bounds__(128)
+agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_column, unsigned v_column, bf16* q_out, bf16* k_pool,
+                   bf16* v_pool, const int* starts, const int* lengths, const int* table, const int* pos, const int* offset,
+                   unsigned* status, unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width,
+                   unsigned q_heads, unsigned kv_heads, unsigned head_dim, unsigned q_stride, unsigned kv_stride,
+                   unsigned out_stride, float log2_theta, float log2_theta_rest, unsigned s0, unsigned s1, unsigned ladder,
+                   unsigned has_offset) {
+  __shared__ __align__(16) float cosine[64], sine[64];
+  grid_dependency_wait();
+  const unsigned half = head_dim / 2, vecs = half / 8, turned = (q_heads + kv_heads) * vecs;
+  const unsigned blocks = head_dim / 64, copied = kv_heads * head_dim / 8;
+  k += k_column;
+  v += v_column;
+  if (!(paged::aligned16(q) && paged::aligned16(k) && paged::aligned16(v) && paged::aligned16(q_out) && paged::aligned16(k_pool) &&
+        paged::aligned16(v_pool))) {
+    if (threadIdx.x == 0) paged::report(status, paged::kMisaligned);
+    return;
+  }
+  const unsigned pair = threadIdx.x;
+  // turns per position of this thread's pair
+  double frequency = 0.;
+  if (pair < half)
+    frequency = exp2(-(double(log2_theta) + double(log2_theta_rest)) * (double(pair % ladder) / double(ladder))) * 0.15915494309189534;
+  for (unsigned row = blockIdx.x; row < rows; row += gridDim.x) {
+    const unsigned seq = paged::sequence_of(starts, sequences, row);
+    if (seq >= sequences) continue;      // the same for the whole block
+    const int index = paged::index_of(starts, lengths, seq, row);
+    unsigned page_id = 0;
+    bool stored = index >= 0;
+    if (stored) {
+      if (unsigned(index) / page >= width) {
+        stored = false;
+        if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
+      } else {
+        page_id = unsigned(__ldg(table + size_t(seq) * width + unsigned(index) / page));
+        if (page_id >= pages) {
+          stored = false;
+          if (threadIdx.x == 0) paged::report(status, paged::kBadPage);
+        }
+      }
+    }
+    const unsigned token = unsigned(index) % page;
+    const bf16* const q_row = q + size_t(row) * q_stride;
+    const bf16* const k_row = k + size_t(row) * kv_stride;
+    __syncthreads();      // the angles of the row before are no longer needed
+    if (pair < half) {
+      int at;
+      if (s0 == kPositionsFromCache) at = int(unsigned(index) + (has_offset ? unsigned(__ldg(offset)) : 0u));
+      else if (s0 == kPositionsOneAxis) at = __ldg(pos + row);
+      else at = __ldg(pos + size_t(pair < s0 ? 0u : pair < s0 + s1 ? 1u : 2u) * rows + row);
+      const double turns = double(at) * frequency;
+      sincospif(2.f * float(turns - rint(turns)), &sine[pair], &cosine[pair]);
+    }
+    __syncthreads();
+    for (unsigned item = threadIdx.x; item < turned; item += 128) {
+      const unsigned head = item / vecs, c = item - head * vecs;
+      const bf16* from = (head < q_heads ? q_row + head * head_dim : k_row + (head - q_heads) * head_dim) + c * 8;
+      float a[8], b[8], x[8], y[8];
+      unpack8(*reinterpret_cast<const Bf16x8*>(from), a);
+      unpack8(*reinterpret_cast<const Bf16x8*>(from + half), b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float co = cosine[c * 8 + j], si = sine[c * 8 + j];
+        x[j] = a[j] * co - b[j] * si;
+        y[j] = b[j] * co + a[j] * si;
+      }
+      if (head < q_heads) {
+        bf16* to = q_out + size_t(row) * out_stride + head * head_dim + c * 8;
+        *reinterpret_cast<Bf16x8*>(to) = pack8(x);
+        *reinterpret_cast<Bf16x8*>(to + half) = pack8(y);
+      } else if (stored) {
+        // chunk c of the head's first half, chunk c + vecs of the whole row: columns of one block (64 wide) or of two
+        const unsigned lo = c, hi = c + vecs;
+        bf16* first = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, lo / 8, page) + token) * 64;
+        bf16* second = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, hi / 8, page) + token) * 64;
+        *reinterpret_cast<Bf16x8*>(first + (((lo & 7) ^ (token & 7)) * 8)) = pack8(x);
+        *reinterpret_cast<Bf16x8*>(second + (((hi & 7) ^ (token & 7)) * 8)) = pack8(y);
+      }
+    }
+    if (stored)
+      for (unsigned item = threadIdx.x; item < copied; item += 128) {
+        const unsigned head = item / (blocks * 8), c = item % (blocks * 8);
+        bf16* to = v_pool + (paged::block_offset(page_id, kv_heads, head, blocks, c / 8, page) + token) * 64;
+        *reinterpret_cast<uint4*>(to + (((c & 7) ^ (token & 7)) * 8)) =
+            *reinterpret_cast<const uint4*>(v + size_t(row) * kv_stride + head * head_dim + c * 8);
+      }
+  }
+}
+
+// Attention of a batch's new tokens over its pages, a warp per row and head walking the keys one by one.
+// prefix_pages > 0: every row sees all *prefix_length tokens of the pages in prefix_table before its own sequence's.
+// grid = (rows, ceil(q_heads / 4)), block = 128.
+extern "C" __global__ void __launch_bounds__(128)
+agi_paged_attention_rows_bf16(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const int* starts, const int* lengths,
+                              const int* table, const int* prefix_table, const int* prefix_length, unsigned* status,
+                              unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width,
+                              unsigned prefix_pages, unsigned q_heads, unsigned kv_heads, unsigned head_dim, unsigned q_stride,
+                              unsigned o_stride, unsigned window, unsigned sinks, float scale) {
+  grid_dependency_wait();
+  const unsigned row = blockIdx.x, head = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (head >= q_heads) return;
+  if (!(paged::aligned16(q) && paged::aligned16(o) && paged::aligned16(k_pool) && paged::aligned16(v_pool))) {
+    paged::report(status, paged::kMisaligned);
+    return;
+  }
+  const unsigned seq = paged::sequence_of(starts, sequences, row);
+  if (seq >= sequences) return;
+  const int index = paged::index_of(starts, lengths, seq, row);
+  const unsigned blocks = head_dim / 64, kv_head = head / (q_heads / kv_heads), pairs = head_dim / 64;
+  const bf16* q_row = q + size_t(row) * q_stride + head * head_dim;
+  float mine[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
+  for (unsigned b = 0; b < pairs; ++b) {
+    mine[2 * b] = __bfloat162float(q_row[b * 64 + lane * 2]) * scale;
+    mine[2 * b + 1] = __bfloat162float(q_row[b * 64 + lane * 2 + 1]) * scale;
+  }
+  auto see = [&](const int* pages_of, unsigned j) {
+    const unsigned page_id = unsigned(pages_of[j / page]), token = j % page;
+    if (page_id >= pages) {
+      paged::report(status, paged::kBadPage);
+      return;
+    }
+    float s = 0.f, value[4];
+    for (unsigned b = 0; b < pairs; ++b) {
+      const size_t at = (paged::block_offset(page_id, kv_heads, kv_head, blocks, b, page) + token) * 64 +
+                        (((lane / 4) ^ (token & 7)) * 8) + (lane & 3) * 2;
+      s += mine[2 * b] * __bfloat162float(k_pool[at]) + mine[2 * b + 1] * __bfloat162float(k_pool[at + 1]);
+      value[2 * b] = __bfloat162float(v_pool[at]);
+      value[2 * b + 1] = __bfloat162float(v_pool[at + 1]);
+    }
+    s = warp_sum(s);
+    const float peak = fmaxf(top, s);
+    if (peak == -INFINITY) return;
+    const float old = __expf(top - peak), p = __expf(s - peak);
+    sum = sum * old + p;
+    for (unsigned i = 0; i < 2 * pairs; ++i) acc[i] = acc[i] * old + p * value[i];
+    top = peak;
+  };
+  if (prefix_pages > 0) {
+    unsigned count = unsigned(max(0, *prefix_length));
+    if (count > prefix_pages * page) {
+      paged::report(status, paged::kBadLength);
+      count = prefix_pages * page;
+    }
+    for (unsigned j = 0; j < count; ++j) see(prefix_table, j);
+  }
+  if (index >= 0) {
+    unsigned end = unsigned(index) + 1;
+    if (end > width * page) {
+      paged::report(status, paged::kBadLength);
+      end = width * page;
+    }
+    for (unsigned j = 0; j < end; ++j)
+      if (window == 0 || unsigned(index) - j < window || j < sinks) see(table + size_t(seq) * width, j);
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  for (unsigned b = 0; b < pairs; ++b)
+    *reinterpret_cast<bf162*>(o + size_t(row) * o_stride + head * head_dim + b * 64 + lane * 2) =
+        __floats2bfloat162_rn(acc[2 * b] * inv, acc[2 * b + 1] * inv);
+}

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import functools
 import math
+import struct
 from dataclasses import dataclass, field
 from typing import Any, Mapping, Sequence
 
@@ -450,6 +451,56 @@ def dit_block_geometry(T: int, D: int, heads: int, head_dim: int, mlp: int, ctx:
     return {"slots": slots, "region": region, "shared_bytes": DIT_HEADER_BYTES + region + slots * DIT_SLOT_BYTES}
 
 
+# ---- paged K/V cache (csrc/kernels/paged.cuh) ---------------------------------------------------------------
+PAGE_TOKENS = (16, 32, 64, 128)          # tokens of a page
+PAGED_HEAD_DIMS = (64, 128)
+POSITIONS_FROM_CACHE, POSITIONS_ONE_AXIS = 0xffffffff, 0xfffffffe
+
+
+@dataclass(frozen=True)
+class PagedCache:
+    """A paged K/V cache and the batch of sequences that a launch works on.
+
+    ``k`` and ``v`` are pools [pages, kv_heads, head_dim / 64, page, 64] of bf16 in the layout of ``layout.pack_kv_pages``
+    (tensors of the caller, declared as outputs of the profile where ``kv_append`` writes them; a buffer bound as an output
+    keeps what it holds).  ``table`` [sequences, pages_per_sequence], ``lengths`` [sequences] and ``starts`` [sequences + 1] are
+    I32: rows starts[b] .. starts[b + 1) of the launch are the new tokens of sequence b, lengths[b] counts the tokens that it
+    holds once they are in, table[b, i] is the page of its tokens i * page and on.  All three are read on the device when the
+    launch runs, so one packaged recipe serves every step; sequences without new tokens and of length zero are fine.  A page
+    outside the pool or a sequence longer than its table leaves 0x400 or 0x500 in the status word and is not followed; a
+    tensor that does not start on a 16-byte boundary leaves 0x600."""
+    k: Pointer
+    v: Pointer
+    table: Pointer
+    lengths: Pointer
+    starts: Pointer
+    sequences: int
+    pages: int
+    page: int
+    pages_per_sequence: int
+    kv_heads: int
+    head_dim: int
+
+    def __post_init__(self) -> None:
+        if self.page not in PAGE_TOKENS:
+            raise ValueError(f"a page holds {PAGE_TOKENS} tokens, not {self.page}")
+        if self.head_dim not in PAGED_HEAD_DIMS:
+            raise ValueError(f"a paged cache holds heads {PAGED_HEAD_DIMS} wide, not {self.head_dim}")
+        if min(self.sequences, self.pages, self.pages_per_sequence, self.kv_heads) < 1:
+            raise ValueError("a paged cache has at least one sequence, page and head")
+        if self.sequences > PAGED_MAX_SEQUENCES:
+            raise ValueError(f"a launch works on at most {PAGED_MAX_SEQUENCES} sequences, not {self.sequences}")
+        if self.pages_per_sequence * self.page >= 1 << 30 or self.pages >= 1 << 31:
+            raise ValueError("a sequence holds fewer than 2^30 tokens and a pool fewer than 2^31 pages")
+
+    @property
+    def pool_shape(self) -> list[int]:
+        return [self.pages, self.kv_heads, self.head_dim // 64, self.page, 64]
+
+
+PAGED_MAX_SEQUENCES = 4096
+
+
 def grid_for(work_items: int, threads: int = 256, cap: int = SM_COUNT * 8) -> int:
     return max(1, min(cap, ceil_div(work_items, threads)))
 
@@ -731,6 +782,126 @@ class RecipeBuilder:
             return
         self.launch("agi_attention_bf16", (ceil_div(q_rows, 8), q_heads, 1), (256, 1, 1), args,
                     op=f"attention_{mask}", algorithm="warp_per_row")
+
+    # ---- paged K/V cache --------------------------------------------------------------------
+    def _declared(self, what: str, pointer: Pointer, dtype: str, elements: int, shape: Sequence[int] | None = None) -> None:
+        """A caller's tensor has to be declared with this dtype and at least so many elements (or exactly this shape)."""
+        if not isinstance(pointer, Tensor):
+            return
+        assert self._profile is not None, "begin_profile first"
+        found = next((t for t in self._profile.inputs + self._profile.outputs if t["name"] == pointer.name), None)
+        if found is None:
+            raise ValueError(f"{what}: the profile has no tensor {pointer.name!r}")
+        if found["dtype"] != dtype or math.prod(found["shape"]) < elements or (shape is not None and list(found["shape"]) != list(shape)):
+            want = f"{list(shape)}" if shape is not None else f"at least {elements} elements"
+            raise ValueError(f"{what}: tensor {pointer.name!r} is {found['dtype']} {list(found['shape'])}, not {dtype} with {want}")
+
+    def _paged_batch(self, cache: PagedCache, rows: int, q_heads: int) -> None:
+        if rows < 1 or rows >= 1 << 24:
+            raise ValueError(f"a launch works on 1 to 2^24 - 1 rows, not {rows}")
+        if q_heads < 1 or q_heads % cache.kv_heads:
+            raise ValueError(f"{q_heads} query heads do not share {cache.kv_heads} key heads evenly")
+        for what, p in (("keys", cache.k), ("values", cache.v)):
+            self._declared(what, p, "BF16", 0, cache.pool_shape)
+        self._declared("table", cache.table, "I32", cache.sequences * cache.pages_per_sequence)
+        self._declared("lengths", cache.lengths, "I32", cache.sequences)
+        self._declared("starts", cache.starts, "I32", cache.sequences + 1)
+
+    def _paged_rows(self, what: str, pointer: Pointer, rows: int, columns: int, stride: int | None) -> int:
+        """The row pitch of a [rows, columns] operand; 16-byte vectors need rows that start on one."""
+        stride = stride or columns
+        if stride < columns or stride % 8:
+            raise ValueError(f"{what}: a row pitch of {stride} elements is no multiple of 8 that holds {columns}")
+        if isinstance(pointer, Arena) and pointer.offset % 16:
+            raise ValueError(f"{what}: does not start on a 16-byte boundary")
+        self._declared(what, pointer, "BF16", (rows - 1) * stride + columns)
+        return stride
+
+    def kv_append(self, q: Pointer, q_out: Pointer, cache: PagedCache, *, rows: int, q_heads: int, theta: float,
+                  row_stride: int | None = None, out_stride: int | None = None, k: Pointer | None = None, v: Pointer | None = None,
+                  kv_stride: int | None = None, positions: Pointer | None = None, sections: Sequence[int] | None = None,
+                  ladder: int | None = None, offset: Pointer | None = None) -> None:
+        """The new tokens' queries turned by their positions into ``q_out`` (which may be ``q``), keys turned and values as they
+        are into the pages of ``cache``.  ``q``: rows of queries | keys | values side by side (pitch ``row_stride``), or the
+        queries alone with ``k`` and ``v`` (pitch ``kv_stride``) beside them.  A position is the token's index in its sequence
+        plus the I32 at ``offset`` (a shared prefix in front of the sequences), or it comes from ``positions``: I32 [rows], or with
+        ``sections`` (pairs of the time, height and width axes) [3, rows].  ``ladder`` as in ``mrope``."""
+        self._paged_batch(cache, rows, q_heads)
+        d, kv_dim = cache.head_dim, cache.kv_heads * cache.head_dim
+        if (k is None) != (v is None) or (k is None and kv_stride is not None):
+            raise ValueError("keys and values both stand beside the queries or both come with a pitch of their own")
+        if offset is not None and positions is not None:
+            raise ValueError("an offset goes with positions that follow from the cache")
+        if sections is not None and (positions is None or len(sections) != 3 or sum(sections) != d // 2 or min(sections) < 0):
+            raise ValueError(f"sections are three counts of {d // 2} rotary pairs in all and need positions")
+        if not theta > 0 or (ladder is not None and not 1 <= ladder <= d // 2):
+            raise ValueError("theta is positive and a ladder has one to head_dim / 2 pairs")
+        q_dim = q_heads * d
+        row_stride = self._paged_rows("queries", q, rows, q_dim + (2 * kv_dim if k is None else 0), row_stride)
+        out_stride = self._paged_rows("turned queries", q_out, rows, q_dim, out_stride)
+        if k is None:
+            k, v, k_column, v_column, kv_stride = q, q, q_dim, q_dim + kv_dim, row_stride
+        else:
+            kv_stride, k_column, v_column = self._paged_rows("keys", k, rows, kv_dim, kv_stride), 0, 0
+            self._paged_rows("values", v, rows, kv_dim, kv_stride)
+        for name in (p.name for p in (q_out, cache.k, cache.v) if isinstance(p, Tensor)):
+            if all(t["name"] != name for t in self._profile.outputs):
+                raise ValueError(f"{name!r} is written: it has to be an output of the profile")
+        if positions is not None:
+            self._declared("positions", positions, "I32", rows * (1 if sections is None else 3))
+        if offset is not None:
+            self._declared("offset", offset, "I32", 1)
+        s0, s1 = (sections[0], sections[1]) if sections is not None else (POSITIONS_FROM_CACHE if positions is None else POSITIONS_ONE_AXIS, 0)
+        log2_theta = struct.unpack("f", struct.pack("f", math.log2(theta)))[0]
+        dummy = Arena(0)
+        self.launch("agi_kv_append_bf16", (min(rows, SM_COUNT * 8), 1, 1), (128, 1, 1),
+                    [q, k, v, U32(k_column), U32(v_column), q_out, cache.k, cache.v, cache.starts, cache.lengths, cache.table,
+                     positions or dummy, offset or dummy, Arena(STATUS_WORD), U32(rows), U32(cache.sequences), U32(cache.pages),
+                     U32(cache.page), U32(cache.pages_per_sequence), U32(q_heads), U32(cache.kv_heads), U32(d), U32(row_stride),
+                     U32(kv_stride), U32(out_stride), F32(log2_theta), F32(math.log2(theta) - log2_theta), U32(s0), U32(s1),
+                     U32(ladder or d // 2), U32(0 if offset is None else 1)], op="kv_append", algorithm="row_per_block")
+
+    def paged_attention(self, q: Pointer, o: Pointer, cache: PagedCache, *, rows: int, q_heads: int, longest: int | None = None,
+                        window: int = 0, sinks: int = 0, q_stride: int | None = None, o_stride: int | None = None,
+                        scale: float | None = None) -> None:
+        """Causal attention of the new tokens over their sequences' pages (their own keys among them: ``kv_append`` comes first).
+        ``window``: a token sees itself and the ``window`` - 1 before it (0: everything), and the first ``sinks`` tokens.
+        ``longest``: the most new tokens that one sequence has (``rows`` where it is left out); it says which kernel is
+        launched, the result does not depend on it.  A row that sees nothing is zero; rows of no sequence are left alone."""
+        self._paged_attention(q, o, cache, None, rows=rows, q_heads=q_heads, longest=longest, window=window, sinks=sinks,
+                              q_stride=q_stride, o_stride=o_stride, scale=scale, op="paged_attention")
+
+    def prefix_attention(self, q: Pointer, o: Pointer, cache: PagedCache, prefix_table: Pointer, prefix_length: Pointer, *,
+                         prefix_pages: int, rows: int, q_heads: int, longest: int | None = None, q_stride: int | None = None,
+                         o_stride: int | None = None, scale: float | None = None) -> None:
+        """``paged_attention`` for sequences that all go on from one prefix: a row sees all of the prefix, then its own sequence
+        up to itself (``cache`` holds what comes after the prefix).  ``prefix_table`` I32 [prefix_pages] names the prefix's pages in
+        the same pools, ``prefix_length`` I32 [1] counts its tokens.  The prefix is read once for the whole batch."""
+        if prefix_pages < 1 or prefix_pages * cache.page >= 1 << 30:
+            raise ValueError("a prefix has at least one page and fewer than 2^30 tokens")
+        self._declared("prefix_table", prefix_table, "I32", prefix_pages)
+        self._declared("prefix_length", prefix_length, "I32", 1)
+        self._paged_attention(q, o, cache, (prefix_table, prefix_length, prefix_pages), rows=rows, q_heads=q_heads, longest=longest,
+                              window=0, sinks=0, q_stride=q_stride, o_stride=o_stride, scale=scale, op="prefix_attention")
+
+    def _paged_attention(self, q: Pointer, o: Pointer, cache: PagedCache, prefix: tuple[Pointer, Pointer, int] | None, *, rows: int,
+                         q_heads: int, longest: int | None, window: int, sinks: int, q_stride: int | None, o_stride: int | None,
+                         scale: float | None, op: str) -> None:
+        self._paged_batch(cache, rows, q_heads)
+        longest = rows if longest is None else longest
+        if not 1 <= longest <= rows:
+            raise ValueError(f"the longest sequence brings 1 to {rows} rows, not {longest}")
+        if not (0 <= window < 1 << 30 and 0 <= sinks < 1 << 30) or (sinks and not window):
+            raise ValueError("window and sinks are counts of tokens, and sinks go with a window")
+        q_stride = self._paged_rows("queries", q, rows, q_heads * cache.head_dim, q_stride)
+        o_stride = self._paged_rows("outputs", o, rows, q_heads * cache.head_dim, o_stride)
+        dummy = Arena(0)
+        prefix_table, prefix_length, prefix_pages = prefix or (dummy, dummy, 0)
+        self.launch("agi_paged_attention_rows_bf16", (rows, ceil_div(q_heads, 4), 1), (128, 1, 1),
+                    [q, o, cache.k, cache.v, cache.starts, cache.lengths, cache.table, prefix_table, prefix_length, Arena(STATUS_WORD),
+                     U32(rows), U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence), U32(prefix_pages),
+                     U32(q_heads), U32(cache.kv_heads), U32(cache.head_dim), U32(q_stride), U32(o_stride), U32(window), U32(sinks),
+                     F32(scale if scale is not None else cache.head_dim ** -0.5)], op=op, algorithm="warp_per_row")
 
     def swiglu(self, gate: Pointer, up: Pointer, out: Pointer, rows: int, cols: int, in_stride: int,
                out_stride: int | None = None, amax: Pointer | None = None) -> None:

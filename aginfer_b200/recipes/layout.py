@@ -51,3 +51,27 @@ def unpack_kblock_swizzled(p, rows: int):
     blocks = torch.gather(raw, 2, index)
     flat = blocks.permute(1, 0, 2, 3).reshape(rp, kb * 128)[:rows].contiguous()
     return flat.view(p.dtype)
+
+
+def pack_kv_pages(t):
+    """Keys or values [pages, page, kv_heads, head_dim] (2-byte dtype, head_dim a multiple of 64) -> the pool of a paged cache,
+    [pages, kv_heads, head_dim / 64, page, 64]: 16-byte chunk c of a token's 64 columns sits at position ``c ^ (token & 7)``, so
+    that consecutive tokens of a page, head and block are the image of a 128-byte-swizzled shared-memory tile."""
+    pages, page, heads, d = t.shape
+    blocks = t.reshape(pages, page, heads, d // 64, 8, 8).permute(0, 2, 3, 1, 4, 5)       # [..., token, chunk, 8]
+    return _swap_chunks(blocks).reshape(pages, heads, d // 64, page, 64)
+
+
+def unpack_kv_pages(p):
+    """Inverse of ``pack_kv_pages``."""
+    pages, heads, blocks, page, _ = p.shape
+    t = _swap_chunks(p.reshape(pages, heads, blocks, page, 8, 8))
+    return t.permute(0, 3, 1, 2, 4, 5).reshape(pages, page, heads, blocks * 64)
+
+
+def _swap_chunks(t):
+    """[..., token, chunk, 8] with chunk c of token r exchanged with chunk c ^ (r & 7) (its own inverse)."""
+    import torch
+    tokens = torch.arange(t.shape[-3], device=t.device)
+    source = torch.arange(8, device=t.device)[None, :] ^ (tokens % 8)[:, None]
+    return torch.gather(t, -2, source[:, :, None].expand(t.shape)).contiguous()

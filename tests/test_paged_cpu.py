@@ -1,0 +1,102 @@
+"""Paged K/V cache without a GPU: the pool's layout, what the entry points refuse, and that a recipe of them packages."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from aginfer_b200.recipes import Arena, PagedCache, RecipeBuilder, Tensor, io
+from aginfer_b200.recipes.layout import pack_kv_pages, unpack_kv_pages
+
+CACHE = dict(k=Tensor("k"), v=Tensor("v"), table=Tensor("table"), lengths=Tensor("lengths"), starts=Tensor("starts"), sequences=3, pages=9, page=16,
+             pages_per_sequence=4, kv_heads=2, head_dim=128)
+ROWS, HEADS = 5, 8
+
+
+def builder() -> RecipeBuilder:
+    r = RecipeBuilder({"w": ("BF16", (8,))})
+    pool = [9, 2, 2, 16, 64]
+    r.begin_profile("default", [io("q", "BF16", [ROWS, HEADS * 128]), io("qkv", "BF16", [ROWS, (HEADS + 4) * 128]), io("table", "I32", [3, 4]),
+                                io("lengths", "I32", [3]), io("starts", "I32", [4]), io("positions", "I32", [3, ROWS]), io("at", "I32", [1]),
+                                io("pages", "I32", [6]), io("k_in", "BF16", pool)],
+                    [io("o", "BF16", [ROWS, HEADS * 128]), io("k", "BF16", pool), io("v", "BF16", pool)])
+    return r
+
+
+def append(r, **kw):
+    cache = PagedCache(**CACHE | kw.pop("cache", {}))
+    r.kv_append(kw.pop("x", Tensor("qkv")), kw.pop("out", Tensor("o")), cache, **dict(rows=ROWS, q_heads=HEADS, theta=1e6) | kw)
+
+
+def attend(r, **kw):
+    cache = PagedCache(**CACHE | kw.pop("cache", {}))
+    r.paged_attention(kw.pop("q", Tensor("q")), kw.pop("o", Tensor("o")), cache, **dict(rows=ROWS, q_heads=HEADS) | kw)
+
+
+def share(r, **kw):
+    cache = PagedCache(**CACHE | kw.pop("cache", {}))
+    r.prefix_attention(Tensor("q"), Tensor("o"), cache, kw.pop("table", Tensor("pages")), kw.pop("length", Tensor("at")),
+                       **dict(rows=ROWS, q_heads=HEADS, prefix_pages=6) | kw)
+
+
+def test_pages_pack_and_unpack():
+    for page, heads, d in ((16, 2, 64), (128, 1, 128)):
+        t = torch.arange(3 * page * heads * d).reshape(3, page, heads, d).to(torch.int16)
+        p = pack_kv_pages(t)
+        assert p.shape == (3, heads, d // 64, page, 64) and torch.equal(unpack_kv_pages(p), t)
+        token, column = 13, d - 3       # one element by hand
+        chunk = (column % 64 // 8) ^ (token & 7)
+        assert p[2, heads - 1, column // 64, token, chunk * 8 + column % 8] == t[2, token, heads - 1, column]
+
+
+def test_the_operators_package_together():
+    r = builder()
+    append(r)
+    append(r, positions=Tensor("positions"), sections=(16, 24, 24))
+    append(r, offset=Tensor("at"))
+    attend(r)
+    attend(r, window=100, sinks=4, longest=2, scale=0.1)
+    share(r)
+    share(r, longest=1)
+    plan = r.plan()
+    assert [t["op"] for t in r.tactic_database()["tactics"] if t["op"] != "prologue"] and plan["shape_dispatch"][0]["launches"]
+
+
+@pytest.mark.parametrize("change", [dict(page=8), dict(page=48), dict(head_dim=80), dict(head_dim=256), dict(sequences=0), dict(pages=0),
+                                    dict(pages_per_sequence=0), dict(kv_heads=0), dict(sequences=5000), dict(pages_per_sequence=1 << 27)], ids=str)
+def test_caches_that_are_refused(change):
+    with pytest.raises(ValueError):
+        PagedCache(**CACHE | change)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(rows=0), dict(rows=1 << 24), dict(q_heads=7), dict(q_heads=0), dict(rows=6), dict(cache=dict(pages=8)), dict(cache=dict(page=32)),
+    dict(cache=dict(kv_heads=1)), dict(cache=dict(sequences=4)), dict(cache=dict(pages_per_sequence=5)), dict(cache=dict(k=Tensor("lengths"))),
+    dict(cache=dict(k=Tensor("nothing"))), dict(cache=dict(lengths=Tensor("q")))], ids=str)
+@pytest.mark.parametrize("call", [append, attend, share])
+def test_batches_that_are_refused(call, kw):
+    with pytest.raises(ValueError):
+        call(builder(), **kw)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(row_stride=1000), dict(row_stride=(HEADS + 4) * 128 + 4), dict(out_stride=1000), dict(k=Tensor("q")), dict(kv_stride=256),
+    dict(sections=(16, 24, 24)), dict(positions=Tensor("positions"), sections=(16, 24, 25)), dict(positions=Tensor("positions"), sections=(64,)),
+    dict(positions=Tensor("positions"), sections=(-1, 1, 64)), dict(positions=Tensor("lengths")), dict(offset=Tensor("q")),
+    dict(positions=Tensor("positions"), offset=Tensor("at")), dict(theta=0.0), dict(ladder=65), dict(cache=dict(k=Tensor("k_in"))),
+    dict(x=Tensor("q")), dict(x=Arena(8)), dict(out=Tensor("qkv"))], ids=str)
+def test_appends_that_are_refused(kw):
+    with pytest.raises(ValueError):
+        append(builder(), **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(longest=0), dict(longest=6), dict(window=-1), dict(sinks=3), dict(window=4, sinks=-1), dict(q_stride=1025),
+                                dict(o_stride=512), dict(q=Arena(24)), dict(o=Tensor("lengths")), dict(window=1 << 30)], ids=str)
+def test_attention_that_is_refused(kw):
+    with pytest.raises(ValueError):
+        attend(builder(), **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(prefix_pages=0), dict(prefix_pages=7), dict(prefix_pages=1 << 28), dict(table=Tensor("q")), dict(length=Tensor("q"))], ids=str)
+def test_prefixes_that_are_refused(kw):
+    with pytest.raises(ValueError):
+        share(builder(), **kw)
