@@ -39,12 +39,71 @@ __device__ __forceinline__ int index_of(const int* starts, const int* lengths, u
   return int(unsigned(__ldg(lengths + seq)) - (unsigned(__ldg(starts + seq + 1)) - row));
 }
 
+// 2^x, zero for minus infinity; relative error 2^-22.
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<size_t>(p) & 15) == 0; }
 
 // Offset, in 64-column rows, of token t of a page's block.
 __device__ __forceinline__ size_t block_offset(unsigned page_id, unsigned kv_heads, unsigned head, unsigned blocks, unsigned block,
                                                unsigned page) {
   return ((size_t(page_id) * kv_heads + head) * blocks + block) * page;
+}
+
+// The batch as the attention kernels take it.
+struct Batch {
+  const int *starts, *lengths, *table;
+  unsigned* status;
+  unsigned rows, sequences, pages, page, width;
+};
+
+// A sequence of it: its first row, its new tokens, the index of the first of them (negative: in front of the sequence) and the
+// tokens that it holds.  Rows out of order leave it without new tokens, a length beyond the table is cut to it.
+struct Span {
+  unsigned row, fresh;
+  int first;
+  unsigned length;
+};
+__device__ __forceinline__ Span span_of(const Batch& b, unsigned seq) {
+  const int from = __ldg(b.starts + seq), to = __ldg(b.starts + seq + 1), length = __ldg(b.lengths + seq);
+  const unsigned room = b.width * b.page;
+  const bool ordered = from >= 0 && to >= from && unsigned(to) <= b.rows;
+  if (!ordered || length > int(room)) report(b.status, kBadLength);
+  Span s;
+  s.row = ordered ? unsigned(from) : 0u;
+  s.fresh = ordered ? unsigned(to - from) : 0u;
+  s.length = min(unsigned(max(length, 0)), room);
+  s.first = int(s.length) - int(s.fresh);
+  return s;
+}
+
+// The key tiles that rows at indices [low, high] see: those of the first `sinks` tokens that lie before the window of the first
+// row, then those from that window to the last row.  At least one, which may hold no visible key: it makes a row that sees
+// nothing zero.
+struct Visible {
+  unsigned end, start, sink_end;            // keys [0, sink_end) and [start, end)
+  unsigned sink_tiles, window_tile, count;
+  __device__ __forceinline__ unsigned tile(unsigned i) const { return i < sink_tiles ? i : window_tile + (i - sink_tiles); }
+};
+template <unsigned kTile>
+__device__ __forceinline__ Visible visible_of(int low, int high, unsigned length, unsigned window, unsigned sinks) {
+  Visible v;
+  v.end = min(unsigned(max(high + 1, 0)), length);
+  v.start = window == 0 ? 0u : unsigned(max(low - int(window) + 1, 0));
+  v.sink_end = min(sinks, v.start);
+  v.sink_tiles = (v.sink_end + kTile - 1) / kTile;
+  v.window_tile = max(v.start / kTile, v.sink_tiles);
+  const unsigned tiles = (v.end + kTile - 1) / kTile;
+  v.count = max(v.sink_tiles + (tiles > v.window_tile ? tiles - v.window_tile : 0u), 1u);
+  return v;
+}
+__device__ __forceinline__ bool sees(int index, unsigned key, unsigned window, unsigned sinks) {
+  const int back = index - int(key);
+  return back >= 0 && (window == 0 || unsigned(back) < window || key < sinks);
 }
 
 }  // namespace paged

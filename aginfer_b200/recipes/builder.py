@@ -499,6 +499,23 @@ class PagedCache:
 
 
 PAGED_MAX_SEQUENCES = 4096
+PAGED_FEW_ROWS = 32                      # rows (new tokens x query heads of a key head) of a sequence that mma.sync tiles take
+PAGED_FEW_KEYS = 64                      # keys of a tile
+PAGED_FEW_LEAST = 2
+
+
+def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> dict[str, int]:
+    """Launch geometry of ``agi_paged_few_bf16_*``: 16-row MMA tiles of an item ``m``, CTAs, ring depth.  The CTAs share out all
+    key tiles of the batch evenly, so there are as many as the SMs hold, or as the tables have room for tiles."""
+    m = 1 if longest * group <= 16 else 2
+    per_sm = 3 - m
+    stage = 4 * PAGED_FEW_KEYS * cache.head_dim
+    exchange = 4 * 16 * 32 * 4
+    stages = min(8, ((227 - per_sm) * 1024 // per_sm - 2048 - exchange) // stage)
+    blocks = min(cache.sequences, rows) * ceil_div(longest * group, 16 * m) * cache.kv_heads
+    tiles = blocks * ceil_div(cache.pages_per_sequence * cache.page, PAGED_FEW_KEYS)
+    return {"m": m, "grid": min(SM_COUNT * per_sm, ceil_div(tiles, PAGED_FEW_LEAST)), "stages": stages, "least": PAGED_FEW_LEAST,
+            "shared_bytes": stages * stage + exchange + 1024}
 
 
 def grid_for(work_items: int, threads: int = 256, cap: int = SM_COUNT * 8) -> int:
@@ -896,12 +913,24 @@ class RecipeBuilder:
         q_stride = self._paged_rows("queries", q, rows, q_heads * cache.head_dim, q_stride)
         o_stride = self._paged_rows("outputs", o, rows, q_heads * cache.head_dim, o_stride)
         dummy = Arena(0)
+        scale = scale if scale is not None else cache.head_dim ** -0.5
+        batch = [cache.starts, cache.lengths, cache.table]
+        group = q_heads // cache.kv_heads
+        if prefix is None and longest * group <= PAGED_FEW_ROWS:
+            t = paged_few_tiling(cache, rows, longest, group)
+            scratch, counters = self._tc_scratch
+            self.launch(f"agi_paged_few_bf16_d{cache.head_dim}_m{t['m']}", (t["grid"], 1, 1), (160, 1, 1),
+                        [q, o, cache.k, cache.v, *batch, scratch, counters, Arena(STATUS_WORD), U32(rows), U32(cache.sequences), U32(cache.pages),
+                         U32(cache.page), U32(cache.pages_per_sequence), U32(q_heads), U32(cache.kv_heads), U32(q_stride), U32(o_stride),
+                         U32(window), U32(sinks), F32(scale * math.log2(math.e)), U32(t["stages"]), U32(t["least"])],
+                        shared_bytes=t["shared_bytes"], op=op, algorithm=f"mma_key_tiles_m{t['m']}")
+            return
         prefix_table, prefix_length, prefix_pages = prefix or (dummy, dummy, 0)
         self.launch("agi_paged_attention_rows_bf16", (rows, ceil_div(q_heads, 4), 1), (128, 1, 1),
                     [q, o, cache.k, cache.v, cache.starts, cache.lengths, cache.table, prefix_table, prefix_length, Arena(STATUS_WORD),
                      U32(rows), U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence), U32(prefix_pages),
                      U32(q_heads), U32(cache.kv_heads), U32(cache.head_dim), U32(q_stride), U32(o_stride), U32(window), U32(sinks),
-                     F32(scale if scale is not None else cache.head_dim ** -0.5)], op=op, algorithm="warp_per_row")
+                     F32(scale)], op=op, algorithm="warp_per_row")
 
     def swiglu(self, gate: Pointer, up: Pointer, out: Pointer, rows: int, cols: int, in_stride: int,
                out_stride: int | None = None, amax: Pointer | None = None) -> None:
