@@ -30,13 +30,13 @@ __device__ __forceinline__ void report(unsigned* status, unsigned code) { atomic
 // Called by whole warps.
 __device__ __forceinline__ unsigned sequence_of(const int* starts, unsigned sequences, unsigned row) {
   unsigned before = 0;
-  for (unsigned i = threadIdx.x & 31; i < sequences; i += 32) before += __ldg(starts + i + 1) <= int(row) ? 1u : 0u;
+  for (unsigned i = threadIdx.x & 31; i < sequences; i += 32) before += *(starts + i + 1) <= int(row) ? 1u : 0u;
   return __reduce_add_sync(0xffffffffu, before);
 }
 
 // The index of a row of sequence `seq` in it; whatever the tensors hold, the difference wraps and does not trap.
 __device__ __forceinline__ int index_of(const int* starts, const int* lengths, unsigned seq, unsigned row) {
-  return int(unsigned(__ldg(lengths + seq)) - (unsigned(__ldg(starts + seq + 1)) - row));
+  return int(unsigned(*(lengths + seq)) - (unsigned(*(starts + seq + 1)) - row));
 }
 
 // 2^x, zero for minus infinity; relative error 2^-22.
@@ -69,7 +69,7 @@ struct Span {
   unsigned length;
 };
 __device__ __forceinline__ Span span_of(const Batch& b, unsigned seq) {
-  const int from = __ldg(b.starts + seq), to = __ldg(b.starts + seq + 1), length = __ldg(b.lengths + seq);
+  const int from = *(b.starts + seq), to = *(b.starts + seq + 1), length = *(b.lengths + seq);
   const unsigned room = b.width * b.page;
   const bool ordered = from >= 0 && to >= from && unsigned(to) <= b.rows;
   if (!ordered || length > int(room)) report(b.status, kBadLength);
@@ -152,7 +152,7 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
         stored = false;
         if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
       } else {
-        page_id = unsigned(__ldg(table + size_t(seq) * width + unsigned(index) / page));
+        page_id = unsigned(*(table + size_t(seq) * width + unsigned(index) / page));
         if (page_id >= pages) {
           stored = false;
           if (threadIdx.x == 0) paged::report(status, paged::kBadPage);
@@ -165,9 +165,9 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
     __syncthreads();      // the angles of the row before are no longer needed
     if (pair < half) {
       int at;
-      if (s0 == kPositionsFromCache) at = int(unsigned(index) + (has_offset ? unsigned(__ldg(offset)) : 0u));
-      else if (s0 == kPositionsOneAxis) at = __ldg(pos + row);
-      else at = __ldg(pos + size_t(pair < s0 ? 0u : pair < s0 + s1 ? 1u : 2u) * rows + row);
+      if (s0 == kPositionsFromCache) at = int(unsigned(index) + (has_offset ? unsigned(*offset) : 0u));
+      else if (s0 == kPositionsOneAxis) at = *(pos + row);
+      else at = *(pos + size_t(pair < s0 ? 0u : pair < s0 + s1 ? 1u : 2u) * rows + row);
       const double turns = double(at) * frequency;
       sincospif(2.f * float(turns - rint(turns)), &sine[pair], &cosine[pair]);
     }
@@ -205,75 +205,4 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
             *reinterpret_cast<const uint4*>(v + size_t(row) * kv_stride + head * head_dim + c * 8);
       }
   }
-}
-
-// Attention of a batch's new tokens over its pages, a warp per row and head walking the keys one by one.
-// prefix_pages > 0: every row sees all *prefix_length tokens of the pages in prefix_table before its own sequence's.
-// grid = (rows, ceil(q_heads / 4)), block = 128.
-extern "C" __global__ void __launch_bounds__(128)
-agi_paged_attention_rows_bf16(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const int* starts, const int* lengths,
-                              const int* table, const int* prefix_table, const int* prefix_length, unsigned* status,
-                              unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width,
-                              unsigned prefix_pages, unsigned q_heads, unsigned kv_heads, unsigned head_dim, unsigned q_stride,
-                              unsigned o_stride, unsigned window, unsigned sinks, float scale) {
-  grid_dependency_wait();
-  const unsigned row = blockIdx.x, head = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x & 31;
-  if (head >= q_heads) return;
-  if (!(paged::aligned16(q) && paged::aligned16(o) && paged::aligned16(k_pool) && paged::aligned16(v_pool))) {
-    paged::report(status, paged::kMisaligned);
-    return;
-  }
-  const unsigned seq = paged::sequence_of(starts, sequences, row);
-  if (seq >= sequences) return;
-  const int index = paged::index_of(starts, lengths, seq, row);
-  const unsigned blocks = head_dim / 64, kv_head = head / (q_heads / kv_heads), pairs = head_dim / 64;
-  const bf16* q_row = q + size_t(row) * q_stride + head * head_dim;
-  float mine[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
-  for (unsigned b = 0; b < pairs; ++b) {
-    mine[2 * b] = __bfloat162float(q_row[b * 64 + lane * 2]) * scale;
-    mine[2 * b + 1] = __bfloat162float(q_row[b * 64 + lane * 2 + 1]) * scale;
-  }
-  auto see = [&](const int* pages_of, unsigned j) {
-    const unsigned page_id = unsigned(pages_of[j / page]), token = j % page;
-    if (page_id >= pages) {
-      paged::report(status, paged::kBadPage);
-      return;
-    }
-    float s = 0.f, value[4];
-    for (unsigned b = 0; b < pairs; ++b) {
-      const size_t at = (paged::block_offset(page_id, kv_heads, kv_head, blocks, b, page) + token) * 64 +
-                        (((lane / 4) ^ (token & 7)) * 8) + (lane & 3) * 2;
-      s += mine[2 * b] * __bfloat162float(k_pool[at]) + mine[2 * b + 1] * __bfloat162float(k_pool[at + 1]);
-      value[2 * b] = __bfloat162float(v_pool[at]);
-      value[2 * b + 1] = __bfloat162float(v_pool[at + 1]);
-    }
-    s = warp_sum(s);
-    const float peak = fmaxf(top, s);
-    if (peak == -INFINITY) return;
-    const float old = __expf(top - peak), p = __expf(s - peak);
-    sum = sum * old + p;
-    for (unsigned i = 0; i < 2 * pairs; ++i) acc[i] = acc[i] * old + p * value[i];
-    top = peak;
-  };
-  if (prefix_pages > 0) {
-    unsigned count = unsigned(max(0, *prefix_length));
-    if (count > prefix_pages * page) {
-      paged::report(status, paged::kBadLength);
-      count = prefix_pages * page;
-    }
-    for (unsigned j = 0; j < count; ++j) see(prefix_table, j);
-  }
-  if (index >= 0) {
-    unsigned end = unsigned(index) + 1;
-    if (end > width * page) {
-      paged::report(status, paged::kBadLength);
-      end = width * page;
-    }
-    for (unsigned j = 0; j < end; ++j)
-      if (window == 0 || unsigned(index) - j < window || j < sinks) see(table + size_t(seq) * width, j);
-  }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  for (unsigned b = 0; b < pairs; ++b)
-    *reinterpret_cast<bf162*>(o + size_t(row) * o_stride + head * head_dim + b * 64 + lane * 2) =
-        __floats2bfloat162_rn(acc[2 * b] * inv, acc[2 * b + 1] * inv);
 }

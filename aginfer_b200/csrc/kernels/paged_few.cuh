@@ -54,9 +54,10 @@ struct Scratch {
 };
 
 template <int HD16, int kM>
-__device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const Batch& batch, float* scratch,
-                                               unsigned* counters, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride,
-                                               unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned least) {
+__device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const Batch& batch, float* own_sums,
+                                               float* own_ends, float* scratch, unsigned* counters, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride,
+                                               unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned least,
+                                               unsigned own_only) {
   constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kRows = 16 * kM;
   constexpr unsigned kTileBytes = kKeys * kDim * 2, kStageBytes = 2 * kTileBytes, kBlockBytes = kKeys * 128;
   constexpr unsigned kMaxStages = 8;
@@ -160,7 +161,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         const bool wanted = live && token < it.seen.end && (token < it.seen.sink_end || token + run > it.seen.start);
         return wanted ? min(run, it.seen.end - token) : 0u;
       };
-      auto page_of = [&](unsigned t) { return unsigned(__ldg(pages_of + (it.seen.tile(t) * kKeys + piece * run) / batch.page)); };
+      auto page_of = [&](unsigned t) { return unsigned(pages_of[(it.seen.tile(t) * kKeys + piece * run) / batch.page]); };
       unsigned count = tokens_of(begin), page_id = count ? page_of(begin) : 0u;
       for (unsigned t = begin; t < end; ++t) {
         if (page_id >= batch.pages) {
@@ -210,8 +211,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         const bf16* from_row = q + size_t(span.row + token) * q_stride + (head * group + (row0 + r) % group) * kDim + 2 * t4;
 #pragma unroll
         for (int ks = 0; ks < HD16; ++ks) {
-          qa[m][ks][h] = live ? __ldg(reinterpret_cast<const unsigned*>(from_row + ks * 16)) : 0u;
-          qa[m][ks][h + 2] = live ? __ldg(reinterpret_cast<const unsigned*>(from_row + ks * 16 + 8)) : 0u;
+          qa[m][ks][h] = live ? __ldcg(reinterpret_cast<const unsigned*>(from_row + ks * 16)) : 0u;
+          qa[m][ks][h + 2] = live ? __ldcg(reinterpret_cast<const unsigned*>(from_row + ks * 16 + 8)) : 0u;
         }
       }
     float top[kM][2], sum[kM][2], out[kM][2 * HD16][4];
@@ -315,7 +316,19 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     // ---- the four warps' shares meet: maxima and weights first, then the outputs, 32 columns at a time ----
     const bool whole_item = begin == 0 && end == it.seen.count;
     const unsigned slot = begin > 0 ? 0u : 1u;
-    auto row_of = [&](unsigned r) { return o + size_t(span.row + (row0 + r) / group) * o_stride + (head * group + (row0 + r) % group) * kDim; };
+    // four columns of a row, divided, or as they are with the row's maximum and weight
+    auto leave = [&](unsigned r, unsigned c, float4 v, float peak, float weight) {
+      const unsigned row = span.row + (row0 + r) / group, q_head = head * group + (row0 + r) % group;
+      if (own_only) {
+        const size_t flat = size_t(row) * q_heads + q_head;
+        *reinterpret_cast<float4*>(own_sums + flat * kDim + c) = v;
+        if (c == 0) *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(peak, weight);
+        return;
+      }
+      const float inv = weight > 0.f ? 1.f / weight : 0.f;
+      const bf162 pair[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv), __floats2bfloat162_rn(v.z * inv, v.w * inv)};
+      *reinterpret_cast<uint2*>(o + size_t(row) * o_stride + q_head * kDim + c) = *reinterpret_cast<const uint2*>(pair);
+    };
 #pragma unroll
     for (int m = 0; m < kM; ++m)
 #pragma unroll
@@ -361,9 +374,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
           }
           if (r < rows) {
             if (whole_item) {
-              const float inv = weight > 0.f ? 1.f / weight : 0.f;
-              bf162 pair[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv), __floats2bfloat162_rn(v.z * inv, v.w * inv)};
-              *reinterpret_cast<uint2*>(row_of(r) + c0 + c) = *reinterpret_cast<const uint2*>(pair);
+              leave(r, c0 + c, v, peak, weight);
             } else {
               *reinterpret_cast<float4*>(parts.sum(blockIdx.x, slot, r) + c0 + c) = v;
               if (c0 == 0 && c == 0) *reinterpret_cast<float2*>(parts.end(blockIdx.x, slot, r)) = make_float2(peak, weight);
@@ -396,9 +407,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         v.x += part.x * f; v.y += part.y * f; v.z += part.z * f; v.w += part.w * f;
         weight += end_of.y * f;
       }
-      const float inv = weight > 0.f ? 1.f / weight : 0.f;
-      bf162 pair[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv), __floats2bfloat162_rn(v.z * inv, v.w * inv)};
-      *reinterpret_cast<uint2*>(row_of(r) + c) = *reinterpret_cast<const uint2*>(pair);
+      leave(r, c, v, peak, weight);
     }
     if (tid == 0) counters[first_cta] = 0;               // as the next launch expects it
   });
@@ -407,16 +416,17 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 }  // namespace few
 
 // grid: any number of CTAs that `scratch` has room for, block = 160, dynamic shared memory = stages * 256 * head_dim + 8192 + 1024.
-// least: units that a CTA takes at the least; counters: one word per CTA, zero between launches.
+// least: units that a CTA takes at the least; counters: one word per CTA, zero between launches.  own_only: sums, maxima and
+// weights to own_sums [rows][q_heads][head_dim] and own_ends [rows][q_heads][2] instead of o (prefix attention adds the prefix to them).
 #define AGI_PAGED_FEW(NAME, HD16, M, PER_SM)                                                                                          \
   extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM)                                                                 \
   NAME(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const int* starts, const int* lengths, const int* table,       \
-       float* scratch, unsigned* counters, unsigned* status, unsigned rows, unsigned sequences, unsigned pages, unsigned page,        \
-       unsigned width, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride, unsigned window, unsigned sinks,    \
-       float scale_log2, unsigned stages, unsigned least) {                                                                           \
+       float* own_sums, float* own_ends, float* scratch, unsigned* counters, unsigned* status, unsigned rows, unsigned sequences,     \
+       unsigned pages, unsigned page, unsigned width, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride,      \
+       unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned least, unsigned own_only) {                       \
     const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                    \
-    few::attention_body<HD16, M>(q, o, k_pool, v_pool, batch, scratch, counters, q_heads, kv_heads, q_stride, o_stride, window,       \
-                                 sinks, scale_log2, stages, least);                                                                   \
+    few::attention_body<HD16, M>(q, o, k_pool, v_pool, batch, own_sums, own_ends, scratch, counters, q_heads, kv_heads, q_stride,     \
+                                 o_stride, window, sinks, scale_log2, stages, least, own_only);                                       \
   }
 AGI_PAGED_FEW(agi_paged_few_bf16_d64_m1, 4, 1, 2)
 AGI_PAGED_FEW(agi_paged_few_bf16_d64_m2, 4, 2, 1)

@@ -1,0 +1,702 @@
+// Attention over a paged cache for many rows a sequence and key head (prompts, chunks of prompts, a batch over a shared prefix), on
+// the fifth-generation tensor core: S = Q K^T and O += P V with tcgen05.mma, accumulators and P in tensor memory.
+//
+// An item is up to 256 rows of one sequence and key head, its query heads side by side as rows (row r of the sequence: token
+// r / group, query head r % group), so that a key head's keys are read once for all of them.  Key tiles hold 128 keys.  All key
+// tiles of all items form one line, of which every CTA (one an SM) takes an equal run, whatever the lengths and masks; an item that
+// a cut divides leaves unnormalised parts in scratch, which agi_paged_join_bf16 adds in order.
+//
+// Two streams share the tensor core: while one stream's scores are exponentiated by its four warps, the other's products run.
+// An item of more than 128 rows gives each stream 128 rows and every key tile; a smaller one gives both streams the same rows
+// and every other tile, and their outputs meet in shared memory.  A warp thread owns a row: it reads the row's 128 scores from
+// tensor memory, needs no shuffles for maximum and sum, and writes P back over them as bf16.  Outputs are rescaled only when a
+// row's maximum has grown by more than 2^8 since they were last scaled (all of it cancels in the quotient).
+//
+// Keys and values come in by one bulk copy per page (or its part in a tile) and 64-column block: the pool holds the image that
+// the tensor core reads, rows of keys K-major for S, the same image MN-major for P V.  Tokens behind a sequence's end are not
+// copied; their values are set to zero in shared memory, since weight zero does not make a NaN zero.
+//
+// Tensor memory (512 columns): scores and P of the streams at 0 and 128, outputs at 256 and 384.
+#pragma once
+
+#include "gemm_tc.cuh"
+#include "paged.cuh"
+
+namespace many {
+
+using namespace paged;
+
+constexpr unsigned kKeys = 128, kStreamRows = 128, kRows = 256, kThreads = 384;
+// Registers after the warp groups have traded: a row's 128 scores stay in registers (168 a thread, the launch's share, would spill 480
+// bytes), the group of the loading and the issuing warp gives its own for that (2 x 208 + 88 = 3 x 168).
+constexpr unsigned kSoftmaxRegs = 208, kHelperRegs = 88;
+constexpr unsigned kOutColumn = 256;
+constexpr float kSlack = 8.f;               // log2 of how far scores may exceed the maximum that weights are relative to
+
+// 32 columns of this thread's lane; the values may be used after tmem_loaded().
+__device__ __forceinline__ void tmem_load32(unsigned addr, float* v) {
+  unsigned* r = reinterpret_cast<unsigned*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(addr));
+}
+// Waits for loads; the empty statements tie the values to the wait, so that nothing that uses them moves in front of it.
+template <unsigned kCount>
+__device__ __forceinline__ void tmem_loaded(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (unsigned i = 0; i < kCount; ++i) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void tmem_store32(unsigned addr, const unsigned* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[128 x N] (+)= A . B with A (bf16 pairs) in tensor memory.
+__device__ __forceinline__ void mma_from_tmem(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b),
+               "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+// fp32 accumulators, bf16 operands, M = 128, N columns; B K-major or MN-major.
+__device__ __forceinline__ constexpr unsigned instruction(unsigned n, bool b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// 128-byte-swizzled MN-major operand: 64 columns (one 128-byte row of each key) to the next 64 `leading` bytes on, 8 keys to the
+// next 8 keys 1024 bytes on.
+__device__ __forceinline__ unsigned long long mn_descriptor(unsigned addr, unsigned leading) {
+  return (unsigned long long)((addr & 0x3FFFFu) >> 4) | ((unsigned long long)(leading >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Rows of an item and what they see.  kPrefix: all rows of the launch over the one shared prefix.
+struct Item {
+  unsigned row, fresh;       // first row of the sequence (or launch), new tokens
+  int first;                 // index of the first of them
+  unsigned row0, rows;       // rows of the item among the sequence's fresh * group
+  unsigned head;
+  Visible seen;
+};
+
+// Parts of items that runs cut, as in the kernel for few rows: slot 0 of a CTA where the item began before its run, slot 1 where it
+// goes on behind it.  A slot is [head_dim / 4][256 rows][4] sums and [256][2] (maximum in units of log2, weight).
+// note[cta]: the item that begins in slot 1 of a CTA (pieces = 0: none).
+struct Note {
+  unsigned pieces, row, row0, rows, head, unused[3];
+};
+template <unsigned kDim>
+struct Parts {
+  float* base;
+  Note* notes;
+  static constexpr size_t kSlot = size_t(kRows) * kDim + 2 * kRows;
+  __device__ __forceinline__ float4* sum(unsigned cta, unsigned slot, unsigned row, unsigned c4) const {
+    return reinterpret_cast<float4*>(base + (size_t(cta) * 2 + slot) * kSlot) + c4 * kRows + row;
+  }
+  __device__ __forceinline__ float2* end(unsigned cta, unsigned slot, unsigned row) const {
+    return reinterpret_cast<float2*>(base + (size_t(cta) * 2 + slot) * kSlot + size_t(kRows) * kDim) + row;
+  }
+};
+
+// own_sums, own_ends: the rows' own sequences' part of prefix attention, [rows][q_heads][head_dim] and [rows][q_heads][2], written by the
+// launch before (own_only).
+template <int HD16, bool kPrefix>
+__device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const Batch& batch,
+                                               const int* prefix_table, const int* prefix_length, unsigned prefix_pages, float* own_sums,
+                                               float* own_ends, float* scratch, Note* notes, unsigned q_heads, unsigned kv_heads, unsigned q_stride,
+                                               unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,
+                                               unsigned least, unsigned own_only) {
+  constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kBlockBytes = kKeys * 128, kSlotBytes = kBlocks * kBlockBytes;
+  constexpr unsigned kQBytes = kStreamRows * kDim * 2, kMaxStages = 12;
+  extern __shared__ unsigned char dynamic_smem[];
+  __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages], q_full[2], s_full[2], p_full[2], o_full[2];
+  __shared__ unsigned long long warp_base[12], run_total, run_first;
+  __shared__ float2 shared_end[kStreamRows];
+  __shared__ unsigned tile_base[12], tile_total, run_seq, run_block, gave_up, tmem_slot;
+  const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const unsigned base = (tc::smem_u32(dynamic_smem) + 1023u) & ~1023u;
+  unsigned char* const base_ptr = dynamic_smem + (base - tc::smem_u32(dynamic_smem));
+  const unsigned ring = base + 2 * kQBytes;
+  const unsigned group = q_heads / kv_heads;
+  const Parts<kDim> parts{scratch, notes};
+
+  if (tid == 0) {
+    for (unsigned s = 0; s < stages; ++s) {
+      tc::mbar_init(&full_bar[s], 1);
+      tc::mbar_init(&empty_bar[s], 1);
+    }
+    for (unsigned s = 0; s < 2; ++s) {
+      tc::mbar_init(&q_full[s], kStreamRows);
+      tc::mbar_init(&s_full[s], 1);
+      tc::mbar_init(&p_full[s], kStreamRows);
+      tc::mbar_init(&o_full[s], 1);
+    }
+    gave_up = 0;
+    run_seq = run_block = 0;
+    run_first = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tc::tmem_alloc(&tmem_slot, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const unsigned tmem = tmem_slot;
+  grid_dependency_wait();
+
+  const bool aligned = aligned16(q) && aligned16(o) && aligned16(k_pool) && aligned16(v_pool);
+  if (!aligned && tid == 0) report(batch.status, kMisaligned);
+
+  // ---- the run of this CTA: key tiles [from, to) of all ----
+  const unsigned sequences = kPrefix ? 1u : batch.sequences;
+  auto span_at = [&](unsigned seq) {
+    if (!kPrefix) return span_of(batch, seq);
+    Span s;
+    s.row = 0;
+    s.fresh = batch.rows;
+    s.first = 0;
+    const int length = *prefix_length;
+    const unsigned room = prefix_pages * batch.page;
+    if (length > int(room)) report(batch.status, kBadLength);
+    s.length = min(unsigned(max(length, 0)), room);
+    return s;
+  };
+  auto seen_at = [&](const Span& s, unsigned block) {
+    if (kPrefix) return visible_of<kKeys>(0, int(s.length) - 1, s.length, 0, 0);
+    const unsigned last = min((block + 1) * kRows, s.fresh * group) - 1;
+    return visible_of<kKeys>(s.first + int(block * kRows / group), s.first + int(last / group), s.length, window, sinks);
+  };
+  auto blocks_of = [&](const Span& s) { return (s.fresh * group + kRows - 1) / kRows; };
+  auto scan = [&](auto mine, auto* of_warp, auto* total) {      // exclusive over the block's threads
+    auto below = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const auto other = __shfl_up_sync(0xffffffffu, below, d);
+      if (lane >= unsigned(d)) below += other;
+    }
+    if (lane == 31) of_warp[warp] = below;
+    __syncthreads();
+    if (tid == 0) {
+      auto sum = mine - mine;
+      for (unsigned w = 0; w < kThreads / 32; ++w) {
+        const auto next = sum + of_warp[w];
+        of_warp[w] = sum;
+        sum = next;
+      }
+      *total = sum;
+    }
+    __syncthreads();
+    return below - mine + of_warp[warp];
+  };
+  // blocks of rows first: where the blocks of every sequence begin (in Q's memory, before Q is there) ...
+  unsigned* const block_begin = reinterpret_cast<unsigned*>(base_ptr);
+  const unsigned seq_share = (sequences + kThreads - 1) / kThreads, seq0 = min(tid * seq_share, sequences), seq1 = min(seq0 + seq_share, sequences);
+  unsigned blocks_mine = 0;
+  for (unsigned i = seq0; i < seq1; ++i) blocks_mine += blocks_of(span_at(i));
+  unsigned blocks_below = scan(blocks_mine, tile_base, &tile_total);
+  for (unsigned i = seq0; i < seq1; ++i) {
+    block_begin[i] = blocks_below;
+    blocks_below += blocks_of(span_at(i));
+  }
+  __syncthreads();
+  // ... then their key tiles: a run of blocks a thread
+  const unsigned all_blocks = tile_total, share = (all_blocks + kThreads - 1) / kThreads;
+  const unsigned b0 = min(tid * share, all_blocks), b1 = min(b0 + share, all_blocks);
+  auto holder = [&](unsigned b) {      // the sequence with block b: the last one that begins at or before it (none that has no block)
+    unsigned lo = 0, hi = sequences;
+    while (hi - lo > 1) {
+      const unsigned mid = (lo + hi) / 2;
+      if (block_begin[mid] <= b) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+  unsigned long long mine = 0;
+  for (unsigned b = b0; b < b1; ++b) {
+    const unsigned seq = holder(b);
+    mine += (unsigned long long)seen_at(span_at(seq), b - block_begin[seq]).count * kv_heads;
+  }
+  unsigned long long below = scan(mine, warp_base, &run_total);
+  const unsigned long long total = run_total, per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)least);
+  const unsigned long long from = min(per * blockIdx.x, total), to = aligned ? min(from + per, total) : from;
+  if (from < to && from >= below && from < below + mine) {
+    for (unsigned b = b0; b < b1; ++b) {
+      const unsigned seq = holder(b);
+      const unsigned long long units = (unsigned long long)seen_at(span_at(seq), b - block_begin[seq]).count * kv_heads;
+      if (from < below + units) {
+        run_seq = seq;
+        run_block = b - block_begin[seq];
+        run_first = below;
+        break;
+      }
+      below += units;
+    }
+  }
+  if (tid == 0) parts.notes[blockIdx.x].pieces = 0;
+  __syncthreads();
+
+  auto give_up = [&] { *(volatile unsigned*)&gave_up = 1; };
+  auto await = [&](unsigned long long* bar, unsigned parity, unsigned code) {
+    if (!*(volatile unsigned*)&gave_up && !tc::mbar_wait(bar, parity, batch.status, code)) give_up();
+  };
+  // f(item, first key tile, last key tile + 1, number of the item's first unit, sequence)
+  auto walk = [&](auto&& f) {
+    unsigned seq = run_seq, block = run_block;
+    unsigned long long first = run_first, unit = from;
+    while (unit < to && seq < sequences) {
+      const Span span = span_at(seq);
+      for (const unsigned blocks = blocks_of(span); unit < to && block < blocks; ++block) {
+        Item it;
+        it.row = span.row;
+        it.fresh = span.fresh;
+        it.first = span.first;
+        it.row0 = block * kRows;
+        it.rows = min(kRows, span.fresh * group - it.row0);
+        it.seen = seen_at(span, block);
+        const unsigned count = it.seen.count;
+        while (unit < to && unit < first + (unsigned long long)count * kv_heads) {
+          it.head = unsigned((unit - first) / count);
+          const unsigned begin = unsigned((unit - first) - (unsigned long long)it.head * count);
+          const unsigned end = unsigned(min((unsigned long long)count, begin + (to - unit)));
+          f(it, begin, end, first + (unsigned long long)it.head * count, seq);
+          unit += end - begin;
+        }
+        first += (unsigned long long)count * kv_heads;
+      }
+      block = 0;
+      ++seq;
+    }
+  };
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+  if (warp == 9) {
+    // ---- loading warp: a lane per piece (64-column block, page or part of one) of a tile; keys run ahead of values ----
+    const unsigned run = min(batch.page, kKeys), pieces = kKeys / run;
+    const unsigned block = (lane / pieces) % kBlocks, piece = lane % pieces;
+    const bool live = lane < kBlocks * pieces;
+    unsigned s = 0, phase = 1;
+    walk([&](const Item& it, unsigned begin, unsigned end, unsigned long long, unsigned seq) {
+      const int* const pages_of = kPrefix ? prefix_table : batch.table + size_t(seq) * batch.width;
+      auto bring = [&](unsigned t, bool values) {
+        const unsigned token = it.seen.tile(t) * kKeys + piece * run;
+        unsigned count = 0;
+        const bf16* from_page = nullptr;
+        if (live && token < it.seen.end && (token < it.seen.sink_end || token + run > it.seen.start)) {
+          const unsigned page_id = unsigned(*(pages_of + token / batch.page));
+          if (page_id < batch.pages) {
+            count = min(run, it.seen.end - token);
+            from_page = (values ? v_pool : k_pool) + (block_offset(page_id, kv_heads, it.head, kBlocks, block, batch.page) + token % batch.page) * 64;
+          } else {
+            report(batch.status, kBadPage);
+          }
+        }
+        const unsigned slot = ring + s * kSlotBytes, all = __reduce_add_sync(0xffffffffu, count * 128);
+        if (lane == 0) await(&empty_bar[s], phase, tc::kTimeoutEmpty | s);
+        __syncwarp();
+        if (values && all < kSlotBytes) {      // zero what is not copied
+          for (unsigned p = 0; p < pieces; ++p) {
+            const unsigned held = __shfl_sync(0xffffffffu, count, p);       // the same for every block of the piece
+            for (unsigned i = lane; i < (run - held) * 8 * kBlocks; i += 32) {
+              const unsigned b = i / ((run - held) * 8), rest = i % ((run - held) * 8);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(slot + b * kBlockBytes + (p * run + held) * 128 + rest * 16), "r"(0u)
+                           : "memory");
+            }
+          }
+          tc::fence_async_shared();
+          __syncwarp();
+        }
+        if (lane == 0) tc::expect_bytes(&full_bar[s], all);
+        __syncwarp();
+        if (count) tc::bulk_copy(slot + block * kBlockBytes + piece * run * 128, from_page, count * 128, &full_bar[s]);
+        if (++s == stages) { s = 0; phase ^= 1; }
+      };
+      const unsigned n = end - begin, lead = min(n, it.rows <= kStreamRows ? 2u : 1u);
+      for (unsigned j = 0; j < lead; ++j) bring(begin + j, false);
+      for (unsigned j = 0; j < n; ++j) {
+        bring(begin + j, true);
+        if (j + lead < n) bring(begin + j + lead, false);
+      }
+    });
+  } else if (warp == 8) {
+    // ---- one thread issues the products ----
+    if (elect_one()) {
+      constexpr unsigned kScores = instruction(kKeys, false), kOutputs = instruction(kDim, true);
+      unsigned s = 0, phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      auto scores = [&](unsigned stream, unsigned q_stream, unsigned slot) {
+        const unsigned long long a = tc::smem_descriptor(base + q_stream * kQBytes), b = tc::smem_descriptor(ring + slot * kSlotBytes);
+#pragma unroll
+        for (unsigned k = 0; k < HD16; ++k)
+          tc::mma<false>(tmem + stream * kKeys, a + (k / 4) * (kStreamRows * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2,
+                         kScores, k != 0);
+        tc::tc_commit(&s_full[stream]);
+      };
+      auto outputs = [&](unsigned stream, unsigned slot, bool accumulate) {
+        const unsigned long long b = mn_descriptor(ring + slot * kSlotBytes, kBlockBytes);
+#pragma unroll
+        for (unsigned k = 0; k < kKeys / 16; ++k)
+          mma_from_tmem(tmem + kOutColumn + stream * 128, tmem + stream * kKeys + k * 8, b + k * (16 * 128 >> 4), kOutputs, accumulate || k != 0);
+      };
+      auto arrived = [&] {      // the next slot of the ring has landed: its number
+        await(&full_bar[s], phase, tc::kTimeoutFull | s);
+        tc::tc_fence_after();
+        const unsigned slot = s;
+        if (++s == stages) { s = 0; phase ^= 1; }
+        return slot;
+      };
+      auto weighted = [&](unsigned stream) {
+        await(&p_full[stream], p_phase[stream], tc::kTimeoutAccum | 0x20 | stream);
+        p_phase[stream] ^= 1;
+        tc::tc_fence_after();
+      };
+      walk([&](const Item& it, unsigned begin, unsigned end, unsigned long long, unsigned) {
+        const unsigned n = end - begin;
+        const bool shared_rows = it.rows <= kStreamRows;
+        for (unsigned stream = 0; stream < (shared_rows ? 1u : 2u); ++stream) {
+          await(&q_full[stream], q_phase[stream], tc::kTimeoutAccum | 0x10 | stream);
+          q_phase[stream] ^= 1;
+        }
+        tc::tc_fence_after();
+        if (shared_rows) {
+          for (unsigned j = 0; j < min(n, 2u); ++j) {
+            const unsigned slot = arrived();
+            scores(j, 0, slot);
+            tc::tc_commit(&empty_bar[slot]);
+          }
+          for (unsigned j = 0; j < n; ++j) {
+            const unsigned stream = j & 1, slot = arrived();
+            weighted(stream);
+            outputs(stream, slot, j >= 2);
+            tc::tc_commit(&empty_bar[slot]);
+            if (j + 2 < n) {
+              const unsigned next = arrived();
+              scores(stream, 0, next);
+              tc::tc_commit(&empty_bar[next]);
+            } else {
+              tc::tc_commit(&o_full[stream]);
+            }
+          }
+        } else {
+          unsigned slot = arrived();
+          scores(0, 0, slot);
+          scores(1, 1, slot);
+          tc::tc_commit(&empty_bar[slot]);
+          for (unsigned j = 0; j < n; ++j) {
+            slot = arrived();
+            unsigned next = 0;
+            for (unsigned stream = 0; stream < 2; ++stream) {
+              weighted(stream);
+              outputs(stream, slot, j != 0);
+              if (stream == 1) tc::tc_commit(&empty_bar[slot]);
+              if (j + 1 < n) {
+                if (stream == 0) next = arrived();
+                scores(stream, stream, next);
+                if (stream == 1) tc::tc_commit(&empty_bar[next]);
+              } else {
+                tc::tc_commit(&o_full[stream]);
+              }
+            }
+          }
+        }
+      });
+    }
+    __syncwarp();
+  }
+  } else {
+    // ---- softmax and outputs: four warps a stream, a thread a row ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const unsigned stream = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;       // row of the stream
+    const unsigned lanes = (quarter * 32u) << 16;
+    const unsigned score_at = tmem + stream * kKeys + lanes, out_at = tmem + kOutColumn + stream * 128 + lanes;
+    unsigned char* const q_area = base_ptr + stream * kQBytes;
+    auto stream_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + stream) : "memory"); };
+    auto both_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
+    unsigned s_phase = 0, o_phase = 0;
+    walk([&](const Item& it, unsigned begin, unsigned end, unsigned long long item_first, unsigned) {
+      const unsigned n = end - begin;
+      const bool shared_rows = it.rows <= kStreamRows;
+      const unsigned rows_before = shared_rows ? 0u : stream * kStreamRows;                 // of the item's, in front of this stream's
+      const unsigned live = min(it.rows - rows_before, kStreamRows);
+      auto row_at = [&](unsigned i, unsigned stride) {                                      // offset of the stream's row i of q or o
+        const unsigned at = it.row0 + rows_before + i;
+        return size_t(it.row + at / group) * stride + (it.head * group + at % group) * kDim;
+      };
+      // Q into shared memory, swizzled (zero past the item's rows)
+      if (!shared_rows || stream == 0) {
+#pragma unroll 4
+        for (unsigned i = tid & 127; i < kStreamRows * (kDim / 8); i += 128) {
+          const unsigned row = i / (kDim / 8), c = i % (kDim / 8);
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (row < live) v = __ldcg(reinterpret_cast<const uint4*>(q + row_at(row, q_stride) + c * 8));
+          *reinterpret_cast<uint4*>(q_area + (c / 8) * (kStreamRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+        }
+        tc::fence_async_shared();
+        tc::mbar_arrive(&q_full[stream]);
+      }
+      const unsigned at = it.row0 + rows_before + r;
+      const bool is_live = r < live;
+      const int index = kPrefix ? 0x3fffffff : is_live ? it.first + int(at / group) : -1;
+      // the rows of this warp: does a tile need a mask?
+      const int low = it.first + int((it.row0 + rows_before + quarter * 32) / group);
+      const int high = it.first + int((it.row0 + rows_before + quarter * 32 + 31) / group);
+      float top = -INFINITY, sum = 0.f;       // what weights are relative to (in units of log2), their sum
+      unsigned done = 0;
+      for (unsigned j = shared_rows ? stream : 0u; j < n; j += shared_rows ? 2u : 1u, ++done) {
+        await(&s_full[stream], s_phase, tc::kTimeoutAccum | stream);
+        s_phase ^= 1;
+        __syncwarp();
+        tc::tc_fence_after();
+        float x[kKeys];
+#pragma unroll
+        for (unsigned c = 0; c < kKeys; c += 32) tmem_load32(score_at + c, x + c);
+        tmem_loaded<kKeys>(x);
+        const unsigned key0 = it.seen.tile(begin + j) * kKeys;
+        const bool whole = key0 + kKeys <= it.seen.end && (kPrefix || (int(key0 + kKeys) - 1 <= low && (window == 0 || int(key0) > high - int(window))));
+        if (!whole) {      // the row sees keys up to `last`, and of those the ones from `begins` on and the first `sinks`
+          const int last = min(index, int(it.seen.end) - 1) - int(key0), begins = kPrefix || window == 0 ? -1 : index - int(window) + 1 - int(key0);
+          const int sunk = int(sinks) - int(key0);
+#pragma unroll
+          for (int c = 0; c < int(kKeys); ++c)
+            if (c > last || (c < begins && c >= sunk)) x[c] = -INFINITY;
+        }
+        float peak[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (unsigned c = 4; c < kKeys; ++c) peak[c & 3] = fmaxf(peak[c & 3], x[c]);
+        const float now = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3])) * scale_log2;
+        if (__any_sync(0xffffffffu, now > top + kSlack)) {
+          const float next = fmaxf(top, now), factor = next == -INFINITY ? 1.f : exp2_of(top - next);
+          top = next;
+          sum *= factor;
+          if (done) {
+#pragma unroll
+            for (unsigned c = 0; c < kDim; c += 32) {
+              float v[32];
+              tmem_load32(out_at + c, v);
+              tmem_loaded<32>(v);
+#pragma unroll
+              for (unsigned i = 0; i < 32; ++i) v[i] *= factor;
+              tmem_store32(out_at + c, reinterpret_cast<const unsigned*>(v));
+            }
+            tmem_stored();
+          }
+        }
+        const float from_top = top == -INFINITY ? 0.f : top;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (unsigned half = 0; half < 2; ++half) {
+          unsigned packed[32];
+#pragma unroll
+          for (unsigned i = 0; i < 32; ++i) {
+            const unsigned c = half * 64 + 2 * i;
+            const float a = exp2_of(fmaf(x[c], scale_log2, -from_top)), b = exp2_of(fmaf(x[c + 1], scale_log2, -from_top));
+            part[(2 * i) & 3] += a;
+            part[(2 * i + 1) & 3] += b;
+            const bf162 pair = __floats2bfloat162_rn(a, b);
+            packed[i] = *reinterpret_cast<const unsigned*>(&pair);
+          }
+          tmem_store32(score_at + half * 32, packed);
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tmem_stored();
+        tc::tc_fence_before();
+        tc::mbar_arrive(&p_full[stream]);
+      }
+      float out[kDim];
+      if (done) {
+        await(&o_full[stream], o_phase, tc::kTimeoutAccum | 0x40 | stream);
+        o_phase ^= 1;
+        __syncwarp();
+        tc::tc_fence_after();
+#pragma unroll
+        for (unsigned c = 0; c < kDim; c += 32) tmem_load32(out_at + c, out + c);
+        tmem_loaded<kDim>(out);
+      } else {
+#pragma unroll
+        for (unsigned c = 0; c < kDim; ++c) out[c] = 0.f;
+      }
+      if (shared_rows) {      // the second stream's share to the first, through the memory of Q
+        float* const shared_out = reinterpret_cast<float*>(base_ptr);
+        both_sync();          // Q has been read by both streams' products
+        if (stream == 1) {
+#pragma unroll
+          for (unsigned c = 0; c < kDim; ++c) shared_out[c * kStreamRows + r] = out[c];
+          shared_end[r] = make_float2(top, sum);
+        }
+        both_sync();
+        if (stream == 0) {
+          const float2 other = shared_end[r];
+          const float next = fmaxf(top, other.x);
+          const float mine_by = top == -INFINITY ? 0.f : exp2_of(top - next), other_by = other.x == -INFINITY ? 0.f : exp2_of(other.x - next);
+#pragma unroll
+          for (unsigned c = 0; c < kDim; ++c) out[c] = out[c] * mine_by + shared_out[c * kStreamRows + r] * other_by;
+          sum = sum * mine_by + other.y * other_by;
+          top = next;
+        }
+        both_sync();          // Q's memory is free
+        if (stream == 1) return;
+      }
+      if (begin == 0 && end == it.seen.count) {
+        if (kPrefix || own_only) {
+          // rows of the launch are [row][q_head]; the own sequences' part is read (prefix) or written (own sequences, in front of it)
+          const size_t flat = size_t(it.row + at / group) * q_heads + it.head * group + at % group;
+          const bool covered = is_live && (!kPrefix || (int(it.row + at / group) >= batch.starts[0] && int(it.row + at / group) < batch.starts[batch.sequences]));
+          if (own_only) {
+            if (covered) {
+#pragma unroll
+              for (unsigned c = 0; c < kDim; c += 4)
+                *reinterpret_cast<float4*>(own_sums + flat * kDim + c) = make_float4(out[c], out[c + 1], out[c + 2], out[c + 3]);
+              *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(top, sum);
+            }
+            return;
+          }
+          if (covered) {
+            const float2 other = __ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2));
+            const float next = fmaxf(top, other.x);
+            const float mine_by = top == -INFINITY ? 0.f : exp2_of(top - next), other_by = other.x == -INFINITY ? 0.f : exp2_of(other.x - next);
+            sum = sum * mine_by + other.y * other_by;
+#pragma unroll
+            for (unsigned c = 0; c < kDim; c += 4) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c));
+              out[c] = out[c] * mine_by + v.x * other_by;
+              out[c + 1] = out[c + 1] * mine_by + v.y * other_by;
+              out[c + 2] = out[c + 2] * mine_by + v.z * other_by;
+              out[c + 3] = out[c + 3] * mine_by + v.w * other_by;
+            }
+            const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+            for (unsigned c = 0; c < kDim; c += 8) {
+              float v[8];
+#pragma unroll
+              for (unsigned i = 0; i < 8; ++i) v[i] = out[c + i] * inv;
+              *reinterpret_cast<Bf16x8*>(o + row_at(r, o_stride) + c) = pack8(v);
+            }
+          }
+          return;
+        }
+        // rows staged in Q's memory, so that they leave in whole lines
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+        for (unsigned c = 0; c < kDim; c += 8) {
+          float v[8];
+#pragma unroll
+          for (unsigned i = 0; i < 8; ++i) v[i] = out[c + i] * inv;
+          *reinterpret_cast<Bf16x8*>(q_area + (c / 64) * (kStreamRows * 128) + r * 128 + ((((c / 8) & 7) ^ (r & 7)) << 4)) = pack8(v);
+        }
+        stream_sync();
+#pragma unroll 4
+        for (unsigned i = tid & 127; i < live * (kDim / 8); i += 128) {
+          const unsigned row = i / (kDim / 8), c = i % (kDim / 8);
+          *reinterpret_cast<uint4*>(o + row_at(row, o_stride) + c * 8) =
+              *reinterpret_cast<const uint4*>(q_area + (c / 8) * (kStreamRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+        }
+        stream_sync();
+        return;
+      }
+      const unsigned slot = begin > 0 ? 0u : 1u;
+      if (is_live) {
+#pragma unroll
+        for (unsigned c = 0; c < kDim; c += 4) *parts.sum(blockIdx.x, slot, rows_before + r, c / 4) = make_float4(out[c], out[c + 1], out[c + 2], out[c + 3]);
+        *parts.end(blockIdx.x, slot, rows_before + r) = make_float2(top, sum);
+      }
+      if (begin == 0 && tid == 0) {
+        Note& note = parts.notes[blockIdx.x];
+        note.row = it.row;
+        note.row0 = it.row0;
+        note.rows = it.rows;
+        note.head = it.head;
+        note.pieces = unsigned((item_first + it.seen.count - 1) / per) - blockIdx.x + 1;
+      }
+    });
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc::tc_fence_after();
+    tc::tmem_free(tmem, 512);
+  }
+}
+
+// The parts of items that runs cut, added in order: CTA (i, cta) takes rows i * kJoinRows and on of the item that begins in slot 1 of `cta`.
+// A thread takes four columns of a row: eight rows of a column group are one line of a slot.
+constexpr unsigned kJoinRows = 8;
+template <int HD16, bool kPrefix>
+__device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned sequences, float* own_sums, float* own_ends, float* scratch, Note* notes,
+                                          unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {
+  constexpr unsigned kDim = HD16 * 16;
+  grid_dependency_wait();
+  const Parts<kDim> parts{scratch, notes};
+  const unsigned first = blockIdx.y, group = q_heads / kv_heads;
+  const uint4 a = __ldcg(reinterpret_cast<const uint4*>(notes + first));
+  const unsigned pieces = a.x, row_first = a.y, row0 = a.z, rows = a.w;
+  const unsigned r = blockIdx.x * kJoinRows + threadIdx.x % kJoinRows, c4 = threadIdx.x / kJoinRows;
+  if (pieces == 0 || r >= rows) return;
+  const unsigned head = __ldcg(&notes[first].head);
+  const unsigned row = row_first + (row0 + r) / group, q_head = head * group + (row0 + r) % group;
+  if (kPrefix && !(int(row) >= starts[0] && int(row) < starts[sequences])) return;
+  const size_t flat = size_t(row) * q_heads + q_head;
+  float top = -INFINITY, sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float2 end, const float4 part) {
+    if (end.x == -INFINITY) return;
+    const float next = fmaxf(top, end.x), mine_by = exp2_of(top - next), other_by = exp2_of(end.x - next);
+    v.x = v.x * mine_by + part.x * other_by;
+    v.y = v.y * mine_by + part.y * other_by;
+    v.z = v.z * mine_by + part.z * other_by;
+    v.w = v.w * mine_by + part.w * other_by;
+    sum = sum * mine_by + end.y * other_by;
+    top = next;
+  };
+#pragma unroll 4
+  for (unsigned p = 0; p < pieces; ++p) add(__ldcg(parts.end(first + p, p == 0, r)), __ldcg(parts.sum(first + p, p == 0, r, c4)));
+  if (own_only) {
+    *reinterpret_cast<float4*>(own_sums + flat * kDim + c4 * 4) = v;
+    if (c4 == 0) *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(top, sum);
+    return;
+  }
+  if (kPrefix) add(__ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c4 * 4)));
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const bf162 pair[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv), __floats2bfloat162_rn(v.z * inv, v.w * inv)};
+  *reinterpret_cast<uint2*>(o + size_t(row) * o_stride + q_head * kDim + c4 * 4) = *reinterpret_cast<const uint2*>(pair);
+}
+
+}  // namespace many
+
+// grid: one CTA an SM (or fewer), block = 384, dynamic shared memory = 512 * head_dim (Q) + stages * 256 * head_dim + 1024.
+// own_only: the rows' own sequences' part of prefix attention, left in own_sums and own_ends instead of o.
+#define AGI_PAGED_MANY(NAME, HD16, PREFIX)                                                                                              \
+  extern "C" __global__ void __launch_bounds__(many::kThreads, 1)                                                                       \
+  NAME(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const int* starts, const int* lengths, const int* table,         \
+       const int* prefix_table, const int* prefix_length, float* own_sums, float* own_ends, float* scratch, many::Note* notes,          \
+       unsigned* status, unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width, unsigned prefix_pages,       \
+       unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride, unsigned window, unsigned sinks, float scale_log2,    \
+       unsigned stages, unsigned least, unsigned own_only) {                                                                            \
+    const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                      \
+    many::attention_body<HD16, PREFIX>(q, o, k_pool, v_pool, batch, prefix_table, prefix_length, prefix_pages, own_sums, own_ends,      \
+                                       scratch, notes, q_heads, kv_heads, q_stride, o_stride, window, sinks, scale_log2, stages, least, \
+                                       own_only);                                                                                       \
+  }
+AGI_PAGED_MANY(agi_paged_many_bf16_d64, 4, false)
+AGI_PAGED_MANY(agi_paged_many_bf16_d128, 8, false)
+AGI_PAGED_MANY(agi_paged_prefix_bf16_d64, 4, true)
+AGI_PAGED_MANY(agi_paged_prefix_bf16_d128, 8, true)
+#undef AGI_PAGED_MANY
+
+// grid = (256 / 8, CTAs of the launch before), block = 2 * head_dim.
+#define AGI_PAGED_JOIN(NAME, HD16, PREFIX)                                                                                             \
+  extern "C" __global__ void __launch_bounds__(many::kJoinRows * HD16 * 4)                                                             \
+  NAME(bf16* o, const int* starts, unsigned sequences, float* own_sums, float* own_ends, float* scratch, many::Note* notes,            \
+       unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {                                                    \
+    many::join_body<HD16, PREFIX>(o, starts, sequences, own_sums, own_ends, scratch, notes, q_heads, kv_heads, o_stride, own_only);    \
+  }
+AGI_PAGED_JOIN(agi_paged_join_bf16_d64, 4, false)
+AGI_PAGED_JOIN(agi_paged_join_bf16_d128, 8, false)
+AGI_PAGED_JOIN(agi_paged_join_prefix_bf16_d64, 4, true)
+AGI_PAGED_JOIN(agi_paged_join_prefix_bf16_d128, 8, true)
+#undef AGI_PAGED_JOIN

@@ -518,6 +518,21 @@ def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> 
             "shared_bytes": stages * stage + exchange + 1024}
 
 
+PAGED_MANY_ROWS, PAGED_MANY_KEYS = 256, 128
+PAGED_MANY_LEAST = 2
+
+
+def paged_many_tiling(cache: PagedCache, blocks: int, tokens: int) -> dict[str, int]:
+    """Launch geometry of ``agi_paged_many_bf16_*`` and ``agi_paged_prefix_bf16_*`` for at most ``blocks`` blocks of 256 rows a key head over
+    at most ``tokens`` keys: CTAs (one an SM), ring depth, room for the parts of items that the CTAs' runs cut."""
+    d = cache.head_dim
+    units = blocks * cache.kv_heads * ceil_div(tokens, PAGED_MANY_KEYS)
+    grid = min(SM_COUNT, ceil_div(units, PAGED_MANY_LEAST))
+    stages = min(12, (MAX_DYNAMIC_SHARED - 1024 - 2048 - 512 * d) // (256 * d))
+    return {"grid": grid, "stages": stages, "least": PAGED_MANY_LEAST, "shared_bytes": 512 * d + stages * 256 * d + 1024,
+            "scratch_bytes": grid * 2 * (PAGED_MANY_ROWS * d + 2 * PAGED_MANY_ROWS) * 4}
+
+
 def grid_for(work_items: int, threads: int = 256, cap: int = SM_COUNT * 8) -> int:
     return max(1, min(cap, ceil_div(work_items, threads)))
 
@@ -910,27 +925,42 @@ class RecipeBuilder:
             raise ValueError(f"the longest sequence brings 1 to {rows} rows, not {longest}")
         if not (0 <= window < 1 << 30 and 0 <= sinks < 1 << 30) or (sinks and not window):
             raise ValueError("window and sinks are counts of tokens, and sinks go with a window")
+        scale = scale if scale is not None else cache.head_dim ** -0.5
+        if not 0 < scale < math.inf:
+            raise ValueError("the scale of the scores is positive")
         q_stride = self._paged_rows("queries", q, rows, q_heads * cache.head_dim, q_stride)
         o_stride = self._paged_rows("outputs", o, rows, q_heads * cache.head_dim, o_stride)
-        dummy = Arena(0)
-        scale = scale if scale is not None else cache.head_dim ** -0.5
+        dummy, group, d, mark = Arena(0), q_heads // cache.kv_heads, cache.head_dim, self.mark()
+        # prefix attention: the sequences' own part, unnormalised, goes in front of the prefix's launch
+        own = (self.alloc(rows * q_heads * d * 4), self.alloc(rows * q_heads * 8)) if prefix else (dummy, dummy)
+        shape = [U32(rows), U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence)]
+        heads = [U32(q_heads), U32(cache.kv_heads), U32(q_stride), U32(o_stride), U32(window), U32(sinks), F32(scale * math.log2(math.e))]
         batch = [cache.starts, cache.lengths, cache.table]
-        group = q_heads // cache.kv_heads
-        if prefix is None and longest * group <= PAGED_FEW_ROWS:
+
+        def many(kernel: str, join: str, blocks: int, tokens: int, shared: tuple[Pointer, Pointer, int], own_only: int) -> None:
+            t = paged_many_tiling(cache, blocks, tokens)
+            scratch, notes = self.alloc(t["scratch_bytes"]), self.alloc(t["grid"] * 32)
+            self.launch(f"{kernel}_d{d}", (t["grid"], 1, 1), (384, 1, 1),
+                        [q, o, cache.k, cache.v, *batch, shared[0], shared[1], *own, scratch, notes, Arena(STATUS_WORD), *shape, U32(shared[2]),
+                         *heads, U32(t["stages"]), U32(t["least"]), U32(own_only)],
+                        shared_bytes=t["shared_bytes"], op=op, algorithm="tcgen05_row_blocks")
+            self.launch(f"{join}_d{d}", (ceil_div(min(PAGED_MANY_ROWS, rows * group), 8), t["grid"], 1), (2 * d, 1, 1),
+                        [o, cache.starts, U32(cache.sequences), *own, scratch, notes, U32(q_heads), U32(cache.kv_heads), U32(o_stride),
+                         U32(own_only)], op=op, algorithm="join_parts")
+
+        if longest * group <= PAGED_FEW_ROWS:
             t = paged_few_tiling(cache, rows, longest, group)
             scratch, counters = self._tc_scratch
-            self.launch(f"agi_paged_few_bf16_d{cache.head_dim}_m{t['m']}", (t["grid"], 1, 1), (160, 1, 1),
-                        [q, o, cache.k, cache.v, *batch, scratch, counters, Arena(STATUS_WORD), U32(rows), U32(cache.sequences), U32(cache.pages),
-                         U32(cache.page), U32(cache.pages_per_sequence), U32(q_heads), U32(cache.kv_heads), U32(q_stride), U32(o_stride),
-                         U32(window), U32(sinks), F32(scale * math.log2(math.e)), U32(t["stages"]), U32(t["least"])],
+            self.launch(f"agi_paged_few_bf16_d{d}_m{t['m']}", (t["grid"], 1, 1), (160, 1, 1),
+                        [q, o, cache.k, cache.v, *batch, *own, scratch, counters, Arena(STATUS_WORD), *shape, *heads, U32(t["stages"]),
+                         U32(t["least"]), U32(1 if prefix else 0)],
                         shared_bytes=t["shared_bytes"], op=op, algorithm=f"mma_key_tiles_m{t['m']}")
-            return
-        prefix_table, prefix_length, prefix_pages = prefix or (dummy, dummy, 0)
-        self.launch("agi_paged_attention_rows_bf16", (rows, ceil_div(q_heads, 4), 1), (128, 1, 1),
-                    [q, o, cache.k, cache.v, cache.starts, cache.lengths, cache.table, prefix_table, prefix_length, Arena(STATUS_WORD),
-                     U32(rows), U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence), U32(prefix_pages),
-                     U32(q_heads), U32(cache.kv_heads), U32(cache.head_dim), U32(q_stride), U32(o_stride), U32(window), U32(sinks),
-                     F32(scale)], op=op, algorithm="warp_per_row")
+        else:
+            blocks = min(rows * group // PAGED_MANY_ROWS + min(cache.sequences, rows), cache.sequences * ceil_div(longest * group, PAGED_MANY_ROWS))
+            many("agi_paged_many_bf16", "agi_paged_join_bf16", blocks, cache.pages_per_sequence * cache.page, (dummy, dummy, 0), 1 if prefix else 0)
+        if prefix:
+            many("agi_paged_prefix_bf16", "agi_paged_join_prefix_bf16", ceil_div(rows * group, PAGED_MANY_ROWS), prefix[2] * cache.page, prefix, 0)
+        self.release(mark)
 
     def swiglu(self, gate: Pointer, up: Pointer, out: Pointer, rows: int, cols: int, in_stride: int,
                out_stride: int | None = None, amax: Pointer | None = None) -> None:

@@ -90,7 +90,8 @@ def test_appends_that_are_refused(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(longest=0), dict(longest=6), dict(window=-1), dict(sinks=3), dict(window=4, sinks=-1), dict(q_stride=1025),
-                                dict(o_stride=512), dict(q=Arena(24)), dict(o=Tensor("lengths")), dict(window=1 << 30)], ids=str)
+                                dict(o_stride=512), dict(q=Arena(24)), dict(o=Tensor("lengths")), dict(window=1 << 30), dict(scale=0.0),
+                                dict(scale=-1.0)], ids=str)
 def test_attention_that_is_refused(kw):
     with pytest.raises(ValueError):
         attend(builder(), **kw)
