@@ -62,24 +62,65 @@ struct Batch {
 };
 
 // A sequence of it: its first row, its new tokens, the index of the first of them (negative: in front of the sequence) and the
-// tokens that it holds.  Rows out of order leave it without new tokens, a length beyond the table is cut to it.
+// tokens that it holds; a length beyond the table is cut to it.
 struct Span {
   unsigned row, fresh;
   int first;
   unsigned length;
 };
 __device__ __forceinline__ Span span_of(const Batch& b, unsigned seq) {
-  const int from = *(b.starts + seq), to = *(b.starts + seq + 1), length = *(b.lengths + seq);
-  const unsigned room = b.width * b.page;
-  const bool ordered = from >= 0 && to >= from && unsigned(to) <= b.rows;
-  if (!ordered || length > int(room)) report(b.status, kBadLength);
+  const int from = b.starts[seq], to = b.starts[seq + 1], length = b.lengths[seq];
   Span s;
-  s.row = ordered ? unsigned(from) : 0u;
-  s.fresh = ordered ? unsigned(to - from) : 0u;
-  s.length = min(unsigned(max(length, 0)), room);
+  s.row = unsigned(from);
+  s.fresh = unsigned(to - from);
+  s.length = min(unsigned(max(length, 0)), b.width * b.page);
   s.first = int(s.length) - int(s.fresh);
   return s;
 }
+// What a launch checks of every sequence before it uses any: rows in order and a length that the table has room for.  Rows out of
+// order leave the whole launch without work, so that rows add up to no more than there are.
+__device__ __forceinline__ bool in_order(const Batch& b, unsigned seq) {
+  const int from = b.starts[seq], to = b.starts[seq + 1];
+  const bool ordered = from >= 0 && to >= from && unsigned(to) <= b.rows;
+  if (!ordered || b.lengths[seq] > int(b.width * b.page)) report(b.status, kBadLength);
+  return ordered;
+}
+
+// Sum over the threads in front of this one, and over all.  `of_warp`: a word per warp, used once a kernel.
+template <unsigned kThreads>
+__device__ __forceinline__ unsigned sum_before(unsigned mine, unsigned* of_warp, unsigned* all) {
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned below = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned other = __shfl_up_sync(0xffffffffu, below, d);
+    if (lane >= unsigned(d)) below += other;
+  }
+  if (lane == 31) of_warp[warp] = below;
+  __syncthreads();
+  below -= mine;
+  unsigned total = 0;
+#pragma unroll
+  for (unsigned w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) below += of_warp[w];
+    total += of_warp[w];
+  }
+  *all = total;
+  return below;
+}
+
+// Rows of a block are (token, query head of the key head) pairs, heads fastest: row i of one that begins at row `first` of its sequence.
+// The quotient by a reciprocal is exact: i + group stays far below 2^20.
+struct Rows {
+  unsigned token, head, group;
+  float reciprocal;
+  __device__ __forceinline__ Rows(unsigned first, unsigned group_) : token(first / group_), head(first % group_), group(group_), reciprocal(1.f / float(group_)) {}
+  __device__ __forceinline__ void at(unsigned i, unsigned& token_of, unsigned& head_of) const {
+    const unsigned t = __float2uint_rz((float(head + i) + 0.5f) * reciprocal);
+    token_of = token + t;
+    head_of = head + i - t * group;
+  }
+};
 
 // The key tiles that rows at indices [low, high] see: those of the first `sinks` tokens that lie before the window of the first
 // row, then those from that window to the last row.  At least one, which may hold no visible key: it makes a row that sees

@@ -30,8 +30,7 @@ constexpr unsigned kMergeColumns = 32;      // columns of the outputs that the f
 struct Items {
   Span span;
   Visible seen;
-  unsigned blocks;                    // row blocks of a key head
-  unsigned long long units;
+  unsigned blocks, units;             // row blocks of a key head; units of the sequence
 };
 template <unsigned kRows>
 __device__ __forceinline__ Items items_of(const Batch& batch, unsigned seq, unsigned group, unsigned kv_heads, unsigned window, unsigned sinks) {
@@ -39,7 +38,7 @@ __device__ __forceinline__ Items items_of(const Batch& batch, unsigned seq, unsi
   it.span = span_of(batch, seq);
   it.seen = visible_of<kKeys>(it.span.first, int(it.span.length) - 1, it.span.length, window, sinks);
   it.blocks = (it.span.fresh * group + kRows - 1) / kRows;
-  it.units = (unsigned long long)it.blocks * kv_heads * it.seen.count;
+  it.units = it.blocks * kv_heads * it.seen.count;
   return it;
 }
 
@@ -63,9 +62,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   constexpr unsigned kMaxStages = 8;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages];
-  __shared__ unsigned long long run_total, run_base[5];
-  __shared__ unsigned run_seq, gave_up, last_flag;
-  __shared__ unsigned long long run_first;
+  __shared__ unsigned run_base[kThreads / 32], run_seq, run_first, gave_up, last_flag;
   __shared__ float warp_max_of[4][kRows], warp_sum_of[4][kRows];
   const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const unsigned ring = (tc::smem_u32(dynamic_smem) + 1023u) & ~1023u;
@@ -78,7 +75,6 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       tc::mbar_init(&empty_bar[s], 4);
     }
     gave_up = 0;
-    run_seq = batch.sequences;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   grid_dependency_wait();
@@ -88,55 +84,42 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   }
 
   // ---- this CTA's run: units [from, to) of all, and the sequence that holds the first of them ----
-  unsigned long long mine = 0;
-  const unsigned share = (batch.sequences + kThreads - 1) / kThreads, seq0 = tid * share;
-  for (unsigned i = seq0; i < min(seq0 + share, batch.sequences); ++i) mine += items_of<kRows>(batch, i, group, kv_heads, window, sinks).units;
-  unsigned long long below = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const unsigned long long other = __shfl_up_sync(0xffffffffu, below, d);
-    if (lane >= unsigned(d)) below += other;
+  unsigned mine = 0, total;
+  bool ordered = true;
+  const unsigned share = (batch.sequences + kThreads - 1) / kThreads, seq0 = min(tid * share, batch.sequences), seq1 = min(seq0 + share, batch.sequences);
+#pragma unroll 1
+  for (unsigned i = seq0; i < seq1; ++i) {
+    ordered = in_order(batch, i) && ordered;
+    mine += items_of<kRows>(batch, i, group, kv_heads, window, sinks).units;
   }
-  if (lane == 31) run_base[warp] = below;
-  __syncthreads();
-  if (tid == 0) {
-    unsigned long long sum = 0;
-    for (unsigned w = 0; w < 5; ++w) {
-      const unsigned long long next = sum + run_base[w];
-      run_base[w] = sum;
-      sum = next;
-    }
-    run_total = sum;
-  }
-  __syncthreads();
-  const unsigned long long total = run_total;
-  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)least);
-  const unsigned long long from = min(per * blockIdx.x, total), to = min(from + per, total);
-  below += run_base[warp] - mine;                      // units in front of this thread's sequences
+  unsigned below = sum_before<kThreads>(mine, run_base, &total);
+  const unsigned per = max((total + gridDim.x - 1) / gridDim.x, least), from = min(per * blockIdx.x, total), to = min(from + per, total);
   if (from < to && from >= below && from < below + mine) {
-    unsigned i = seq0;
-    for (;; ++i) {
-      const unsigned long long units = items_of<kRows>(batch, i, group, kv_heads, window, sinks).units;
-      if (from < below + units) break;
+#pragma unroll 1
+    for (unsigned i = seq0; i < seq1; ++i) {
+      const unsigned units = items_of<kRows>(batch, i, group, kv_heads, window, sinks).units;
+      if (from < below + units) {
+        run_seq = i;
+        run_first = below;
+        break;
+      }
       below += units;
     }
-    run_seq = i;
-    run_first = below;
   }
-  __syncthreads();
-  if (from >= to) return;
+  if (__syncthreads_or(!ordered) || from >= to) return;
 
   // Walks the run item by item: f(sequence, key head, row block, its items, first tile, last tile + 1, first unit of the item).
   auto walk = [&](auto&& f) {
-    unsigned seq = run_seq;
-    unsigned long long first = run_first, unit = from;
+    unsigned seq = run_seq, first = run_first, unit = from;
+#pragma unroll 1
     while (unit < to && seq < batch.sequences) {
       const Items it = items_of<kRows>(batch, seq, group, kv_heads, window, sinks);
+#pragma unroll 1
       while (unit < to && unit < first + it.units) {
-        const unsigned long long at = (unit - first) / it.seen.count;      // which item of the sequence
-        const unsigned begin = unsigned(unit - first - at * it.seen.count);
-        const unsigned end = unsigned(min((unsigned long long)it.seen.count, begin + (to - unit)));
-        f(seq, unsigned(at / it.blocks), unsigned(at % it.blocks), it, begin, end, first + at * it.seen.count);
+        const unsigned at = (unit - first) / it.seen.count;                // which item of the sequence
+        const unsigned item_first = first + at * it.seen.count, begin = unit - item_first, end = min(it.seen.count, begin + (to - unit));
+        const unsigned head = at / it.blocks;
+        f(seq, head, at - head * it.blocks, it, begin, end, item_first);
         unit += end - begin;
       }
       first += it.units;
@@ -153,7 +136,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     const unsigned to_slot = (values ? kTileBytes : 0u) + block * kBlockBytes + piece * run * 128;
     const bf16* const pool = values ? v_pool : k_pool;
     unsigned s = 0, phase = 1;
-    walk([&](unsigned seq, unsigned head, unsigned, const Items& it, unsigned begin, unsigned end, unsigned long long) {
+    walk([&](unsigned seq, unsigned head, unsigned, const Items& it, unsigned begin, unsigned end, unsigned) {
       const int* const pages_of = batch.table + size_t(seq) * batch.width;
       // tokens of a tile that this lane brings in, and the page that holds them
       auto tokens_of = [&](unsigned t) {
@@ -195,9 +178,10 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   const unsigned g = lane >> 2, t4 = lane & 3;
   auto consumers_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
   unsigned s = 0, phase = 0;
-  walk([&](unsigned seq, unsigned head, unsigned block, const Items& it, unsigned begin, unsigned end, unsigned long long item_first) {
+  walk([&](unsigned seq, unsigned head, unsigned block, const Items& it, unsigned begin, unsigned end, unsigned item_first) {
     const Span& span = it.span;
     const unsigned row0 = block * kRows, rows = min(kRows, span.fresh * group - row0);
+    const Rows pairs(row0, group);
     // Q fragments: row r of the item is token r / group, query head head * group + r % group
     unsigned qa[kM][HD16][4];
     int index[kM][2];
@@ -205,10 +189,12 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     for (int m = 0; m < kM; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const unsigned r = m * 16 + g + h * 8, token = (row0 + r) / group;
+        const unsigned r = m * 16 + g + h * 8;
+        unsigned token, sub;
+        pairs.at(r, token, sub);
         const bool live = r < rows;
         index[m][h] = live ? span.first + int(token) : -1;
-        const bf16* from_row = q + size_t(span.row + token) * q_stride + (head * group + (row0 + r) % group) * kDim + 2 * t4;
+        const bf16* from_row = q + size_t(span.row + token) * q_stride + (head * group + sub) * kDim + 2 * t4;
 #pragma unroll
         for (int ks = 0; ks < HD16; ++ks) {
           qa[m][ks][h] = live ? __ldcg(reinterpret_cast<const unsigned*>(from_row + ks * 16)) : 0u;
@@ -223,7 +209,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 #pragma unroll
       for (int c = 0; c < 2 * HD16; ++c) out[m][c][0] = out[m][c][1] = out[m][c][2] = out[m][c][3] = 0.f;
     }
-    const int low = span.first + int(row0 / group);                 // the item's first row
+    const int low = span.first + int(pairs.token);                 // the item's first row
     for (unsigned t = begin; t < end; ++t) {
       if (!*(volatile unsigned*)&gave_up && !tc::mbar_wait(&full_bar[s], phase, batch.status, tc::kTimeoutFull | s)) *(volatile unsigned*)&gave_up = 1;
       __syncwarp();
@@ -318,7 +304,9 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     const unsigned slot = begin > 0 ? 0u : 1u;
     // four columns of a row, divided, or as they are with the row's maximum and weight
     auto leave = [&](unsigned r, unsigned c, float4 v, float peak, float weight) {
-      const unsigned row = span.row + (row0 + r) / group, q_head = head * group + (row0 + r) % group;
+      unsigned token, sub;
+      pairs.at(r, token, sub);
+      const unsigned row = span.row + token, q_head = head * group + sub;
       if (own_only) {
         const size_t flat = size_t(row) * q_heads + q_head;
         *reinterpret_cast<float4*>(own_sums + flat * kDim + c) = v;
@@ -341,44 +329,38 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         }
       }
     consumers_sync();
+    const unsigned r16 = tid / 8, c4 = (tid % 8) * 4;      // a thread per row and four of 32 columns
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-      float factor[2];
+      const unsigned r = m * 16 + r16;
+      const float peak = fmaxf(fmaxf(warp_max_of[0][r], warp_max_of[1][r]), fmaxf(warp_max_of[2][r], warp_max_of[3][r]));
+      float by[4], weight = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned r = m * 16 + g + h * 8;
-        float peak = fmaxf(fmaxf(warp_max_of[0][r], warp_max_of[1][r]), fmaxf(warp_max_of[2][r], warp_max_of[3][r]));
-        factor[h] = top[m][h] == -INFINITY ? 0.f : exp2_of(top[m][h] - peak);
+      for (int w = 0; w < 4; ++w) {
+        by[w] = peak == -INFINITY ? 0.f : exp2_of(warp_max_of[w][r] - peak);
+        weight += warp_sum_of[w][r] * by[w];
       }
 #pragma unroll
       for (unsigned c0 = 0; c0 < kDim; c0 += kMergeColumns) {
 #pragma unroll
         for (unsigned n = 0; n < kMergeColumns / 8; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float* cell = exchange + ((warp * 16 + g + h * 8) * kMergeColumns + n * 8 + 2 * t4);
-            *reinterpret_cast<float2*>(cell) = make_float2(out[m][c0 / 8 + n][2 * h] * factor[h], out[m][c0 / 8 + n][2 * h + 1] * factor[h]);
-          }
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float2*>(exchange + (warp * 16 + g + h * 8) * kMergeColumns + n * 8 + 2 * t4) =
+                make_float2(out[m][c0 / 8 + n][2 * h], out[m][c0 / 8 + n][2 * h + 1]);
         consumers_sync();
-        {   // a thread per row and four columns
-          const unsigned r16 = tid / 8, c = (tid % 8) * 4, r = m * 16 + r16;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          float peak = -INFINITY, weight = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) peak = fmaxf(peak, warp_max_of[w][r]);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float4 part = *reinterpret_cast<const float4*>(exchange + (w * 16 + r16) * kMergeColumns + c);
-            v.x += part.x; v.y += part.y; v.z += part.z; v.w += part.w;
-            weight += warp_max_of[w][r] == -INFINITY ? 0.f : warp_sum_of[w][r] * exp2_of(warp_max_of[w][r] - peak);
-          }
-          if (r < rows) {
-            if (whole_item) {
-              leave(r, c0 + c, v, peak, weight);
-            } else {
-              *reinterpret_cast<float4*>(parts.sum(blockIdx.x, slot, r) + c0 + c) = v;
-              if (c0 == 0 && c == 0) *reinterpret_cast<float2*>(parts.end(blockIdx.x, slot, r)) = make_float2(peak, weight);
-            }
+        for (int w = 0; w < 4; ++w) {
+          const float4 part = *reinterpret_cast<const float4*>(exchange + (w * 16 + r16) * kMergeColumns + c4);
+          v.x += part.x * by[w]; v.y += part.y * by[w]; v.z += part.z * by[w]; v.w += part.w * by[w];
+        }
+        if (r < rows) {
+          if (whole_item) {
+            leave(r, c0 + c4, v, peak, weight);
+          } else {
+            *reinterpret_cast<float4*>(parts.sum(blockIdx.x, slot, r) + c0 + c4) = v;
+            if (c0 == 0 && c4 == 0) *reinterpret_cast<float2*>(parts.end(blockIdx.x, slot, r)) = make_float2(peak, weight);
           }
         }
         consumers_sync();
@@ -387,7 +369,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     if (whole_item) return;
 
     // ---- an item of several CTAs: the last of them to arrive adds the parts, in order ----
-    const unsigned first_cta = unsigned(item_first / per), last_cta = unsigned((item_first + it.seen.count - 1) / per);
+    const unsigned first_cta = item_first / per, last_cta = (item_first + it.seen.count - 1) / per;
     __threadfence();
     consumers_sync();
     if (tid == 0) last_flag = atomicAdd(&counters[first_cta], 1u) == last_cta - first_cta;

@@ -81,7 +81,7 @@ __device__ __forceinline__ unsigned long long mn_descriptor(unsigned addr, unsig
 
 // Rows of an item and what they see.  kPrefix: all rows of the launch over the one shared prefix.
 struct Item {
-  unsigned row, fresh;       // first row of the sequence (or launch), new tokens
+  unsigned row;              // first row of the sequence (or launch)
   int first;                 // index of the first of them
   unsigned row0, rows;       // rows of the item among the sequence's fresh * group
   unsigned head;
@@ -109,6 +109,49 @@ struct Parts {
 
 // own_sums, own_ends: the rows' own sequences' part of prefix attention, [rows][q_heads][head_dim] and [rows][q_heads][2], written by the
 // launch before (own_only).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two values at a time.
+__device__ __forceinline__ unsigned long long pair_bits(float2 v) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 pair_of(unsigned long long bits) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(bits));
+  return v;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(d);
+}
+
+// Which of the 32 keys from `key` on a row at `index` of a sequence of `end` tokens sees, a bit each.
+__device__ __forceinline__ unsigned visible_bits(unsigned key, int index, unsigned end, unsigned window, unsigned sinks) {
+  auto first = [](int count) { return count <= 0 ? 0u : count >= 32 ? 0xffffffffu : (1u << count) - 1; };      // the bits of so many keys
+  const unsigned up_to = first(min(index + 1, int(end)) - int(key));
+  return window == 0 ? up_to : up_to & (~first(index + 1 - int(window) - int(key)) | first(int(sinks) - int(key)));
+}
+
+// Another part of a row's sums (its maximum and weight in `other`) is added to this one's: what both are multiplied by.
+__device__ __forceinline__ void join(float& top, float& sum, float2 other, float& mine_by, float& other_by) {
+  const float next = fmaxf(top, other.x);
+  mine_by = next == -INFINITY ? 0.f : exp2_of(top - next);
+  other_by = next == -INFINITY ? 0.f : exp2_of(other.x - next);
+  sum = sum * mine_by + other.y * other_by;
+  top = next;
+}
+
 template <int HD16, bool kPrefix>
 __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const Batch& batch,
                                                const int* prefix_table, const int* prefix_length, unsigned prefix_pages, float* own_sums,
@@ -119,9 +162,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   constexpr unsigned kQBytes = kStreamRows * kDim * 2, kMaxStages = 12;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages], q_full[2], s_full[2], p_full[2], o_full[2];
-  __shared__ unsigned long long warp_base[12], run_total, run_first;
   __shared__ float2 shared_end[kStreamRows];
-  __shared__ unsigned tile_base[12], tile_total, run_seq, run_block, gave_up, tmem_slot;
+  __shared__ unsigned block_base[kThreads / 32], tile_base[kThreads / 32], run_seq, run_block, run_first, gave_up, tmem_slot;
   const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const unsigned base = (tc::smem_u32(dynamic_smem) + 1023u) & ~1023u;
   unsigned char* const base_ptr = dynamic_smem + (base - tc::smem_u32(dynamic_smem));
@@ -159,15 +201,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   const unsigned sequences = kPrefix ? 1u : batch.sequences;
   auto span_at = [&](unsigned seq) {
     if (!kPrefix) return span_of(batch, seq);
-    Span s;
-    s.row = 0;
-    s.fresh = batch.rows;
-    s.first = 0;
-    const int length = *prefix_length;
-    const unsigned room = prefix_pages * batch.page;
-    if (length > int(room)) report(batch.status, kBadLength);
-    s.length = min(unsigned(max(length, 0)), room);
-    return s;
+    return Span{0u, batch.rows, 0, min(unsigned(max(*prefix_length, 0)), prefix_pages * batch.page)};
   };
   auto seen_at = [&](const Span& s, unsigned block) {
     if (kPrefix) return visible_of<kKeys>(0, int(s.length) - 1, s.length, 0, 0);
@@ -175,68 +209,57 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     return visible_of<kKeys>(s.first + int(block * kRows / group), s.first + int(last / group), s.length, window, sinks);
   };
   auto blocks_of = [&](const Span& s) { return (s.fresh * group + kRows - 1) / kRows; };
-  auto scan = [&](auto mine, auto* of_warp, auto* total) {      // exclusive over the block's threads
-    auto below = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const auto other = __shfl_up_sync(0xffffffffu, below, d);
-      if (lane >= unsigned(d)) below += other;
-    }
-    if (lane == 31) of_warp[warp] = below;
-    __syncthreads();
-    if (tid == 0) {
-      auto sum = mine - mine;
-      for (unsigned w = 0; w < kThreads / 32; ++w) {
-        const auto next = sum + of_warp[w];
-        of_warp[w] = sum;
-        sum = next;
-      }
-      *total = sum;
-    }
-    __syncthreads();
-    return below - mine + of_warp[warp];
-  };
   // blocks of rows first: where the blocks of every sequence begin (in Q's memory, before Q is there) ...
   unsigned* const block_begin = reinterpret_cast<unsigned*>(base_ptr);
   const unsigned seq_share = (sequences + kThreads - 1) / kThreads, seq0 = min(tid * seq_share, sequences), seq1 = min(seq0 + seq_share, sequences);
-  unsigned blocks_mine = 0;
-  for (unsigned i = seq0; i < seq1; ++i) blocks_mine += blocks_of(span_at(i));
-  unsigned blocks_below = scan(blocks_mine, tile_base, &tile_total);
+  unsigned blocks_mine = 0, all_blocks;
+  bool usable = aligned;
+#pragma unroll 1
+  for (unsigned i = seq0; i < seq1; ++i) {
+    usable = (kPrefix || in_order(batch, i)) && usable;
+    blocks_mine += blocks_of(span_at(i));
+  }
+  if (kPrefix && tid == 0 && *prefix_length > int(prefix_pages * batch.page)) report(batch.status, kBadLength);
+  unsigned blocks_below = sum_before<kThreads>(blocks_mine, block_base, &all_blocks);
+#pragma unroll 1
   for (unsigned i = seq0; i < seq1; ++i) {
     block_begin[i] = blocks_below;
     blocks_below += blocks_of(span_at(i));
   }
-  __syncthreads();
+  const bool stop = __syncthreads_or(!usable);
+  if (stop) all_blocks = 0;
   // ... then their key tiles: a run of blocks a thread
-  const unsigned all_blocks = tile_total, share = (all_blocks + kThreads - 1) / kThreads;
-  const unsigned b0 = min(tid * share, all_blocks), b1 = min(b0 + share, all_blocks);
-  auto holder = [&](unsigned b) {      // the sequence with block b: the last one that begins at or before it (none that has no block)
-    unsigned lo = 0, hi = sequences;
-    while (hi - lo > 1) {
-      const unsigned mid = (lo + hi) / 2;
-      if (block_begin[mid] <= b) lo = mid; else hi = mid;
-    }
-    return lo;
-  };
-  unsigned long long mine = 0;
-  for (unsigned b = b0; b < b1; ++b) {
-    const unsigned seq = holder(b);
-    mine += (unsigned long long)seen_at(span_at(seq), b - block_begin[seq]).count * kv_heads;
+  const unsigned share = (all_blocks + kThreads - 1) / kThreads, b0 = min(tid * share, all_blocks), b1 = min(b0 + share, all_blocks);
+  unsigned holder = 0;      // the sequence with block b0: the last one that begins at or before it
+  for (unsigned above = sequences; above - holder > 1;) {
+    const unsigned middle = (holder + above) / 2;
+    if (block_begin[middle] <= b0) holder = middle; else above = middle;
   }
-  unsigned long long below = scan(mine, warp_base, &run_total);
-  const unsigned long long total = run_total, per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)least);
-  const unsigned long long from = min(per * blockIdx.x, total), to = aligned ? min(from + per, total) : from;
-  if (from < to && from >= below && from < below + mine) {
+  unsigned mine = 0, total, below = 0, from = 0, to = 0, per = 1;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {      // counts the thread's tiles; then, in the thread that has it, finds the block of tile `from`
+    if (pass == 1) {
+      below = sum_before<kThreads>(mine, tile_base, &total);
+      per = max((total + gridDim.x - 1) / gridDim.x, least);
+      from = min(per * blockIdx.x, total);
+      to = min(from + per, total);
+      if (from >= to || from < below || from >= below + mine) break;
+    }
+    unsigned seq = holder;
+#pragma unroll 1
     for (unsigned b = b0; b < b1; ++b) {
-      const unsigned seq = holder(b);
-      const unsigned long long units = (unsigned long long)seen_at(span_at(seq), b - block_begin[seq]).count * kv_heads;
-      if (from < below + units) {
+      while (seq + 1 < sequences && block_begin[seq + 1] <= b) ++seq;
+      const unsigned tiles = seen_at(span_at(seq), b - block_begin[seq]).count * kv_heads;
+      if (pass == 0) {
+        mine += tiles;
+      } else if (from < below + tiles) {
         run_seq = seq;
         run_block = b - block_begin[seq];
         run_first = below;
         break;
+      } else {
+        below += tiles;
       }
-      below += units;
     }
   }
   if (tid == 0) parts.notes[blockIdx.x].pieces = 0;
@@ -248,30 +271,31 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   };
   // f(item, first key tile, last key tile + 1, number of the item's first unit, sequence)
   auto walk = [&](auto&& f) {
-    unsigned seq = run_seq, block = run_block;
-    unsigned long long first = run_first, unit = from;
+    unsigned seq = run_seq, block = run_block, first = run_first, unit = from;
+#pragma unroll 1
     while (unit < to && seq < sequences) {
       const Span span = span_at(seq);
-      for (const unsigned blocks = blocks_of(span); unit < to && block < blocks; ++block) {
-        Item it;
-        it.row = span.row;
-        it.fresh = span.fresh;
-        it.first = span.first;
-        it.row0 = block * kRows;
-        it.rows = min(kRows, span.fresh * group - it.row0);
-        it.seen = seen_at(span, block);
-        const unsigned count = it.seen.count;
-        while (unit < to && unit < first + (unsigned long long)count * kv_heads) {
-          it.head = unsigned((unit - first) / count);
-          const unsigned begin = unsigned((unit - first) - (unsigned long long)it.head * count);
-          const unsigned end = unsigned(min((unsigned long long)count, begin + (to - unit)));
-          f(it, begin, end, first + (unsigned long long)it.head * count, seq);
-          unit += end - begin;
-        }
-        first += (unsigned long long)count * kv_heads;
+      if (block >= blocks_of(span)) {
+        block = 0;
+        ++seq;
+        continue;
       }
-      block = 0;
-      ++seq;
+      Item it;
+      it.row = span.row;
+      it.first = span.first;
+      it.row0 = block * kRows;
+      it.rows = min(kRows, span.fresh * group - it.row0);
+      it.seen = seen_at(span, block);
+      const unsigned count = it.seen.count;
+#pragma unroll 1
+      while (unit < to && unit < first + count * kv_heads) {
+        it.head = (unit - first) / count;
+        const unsigned item_first = first + it.head * count, begin = unit - item_first, end = min(count, begin + (to - unit));
+        f(it, begin, end, item_first, seq);
+        unit += end - begin;
+      }
+      first += count * kv_heads;
+      ++block;
     }
   };
 
@@ -283,7 +307,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     const unsigned block = (lane / pieces) % kBlocks, piece = lane % pieces;
     const bool live = lane < kBlocks * pieces;
     unsigned s = 0, phase = 1;
-    walk([&](const Item& it, unsigned begin, unsigned end, unsigned long long, unsigned seq) {
+    walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned seq) {
       const int* const pages_of = kPrefix ? prefix_table : batch.table + size_t(seq) * batch.width;
       auto bring = [&](unsigned t, bool values) {
         const unsigned token = it.seen.tile(t) * kKeys + piece * run;
@@ -329,7 +353,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     // ---- one thread issues the products ----
     if (elect_one()) {
       constexpr unsigned kScores = instruction(kKeys, false), kOutputs = instruction(kDim, true);
-      unsigned s = 0, phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      unsigned s = 0, phase = 0, q_phases = 0, p_phases = 0;       // a bit per stream
       auto scores = [&](unsigned stream, unsigned q_stream, unsigned slot) {
         const unsigned long long a = tc::smem_descriptor(base + q_stream * kQBytes), b = tc::smem_descriptor(ring + slot * kSlotBytes);
 #pragma unroll
@@ -352,16 +376,16 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         return slot;
       };
       auto weighted = [&](unsigned stream) {
-        await(&p_full[stream], p_phase[stream], tc::kTimeoutAccum | 0x20 | stream);
-        p_phase[stream] ^= 1;
+        await(&p_full[stream], (p_phases >> stream) & 1, tc::kTimeoutAccum | 0x20 | stream);
+        p_phases ^= 1u << stream;
         tc::tc_fence_after();
       };
-      walk([&](const Item& it, unsigned begin, unsigned end, unsigned long long, unsigned) {
+      walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned) {
         const unsigned n = end - begin;
         const bool shared_rows = it.rows <= kStreamRows;
         for (unsigned stream = 0; stream < (shared_rows ? 1u : 2u); ++stream) {
-          await(&q_full[stream], q_phase[stream], tc::kTimeoutAccum | 0x10 | stream);
-          q_phase[stream] ^= 1;
+          await(&q_full[stream], (q_phases >> stream) & 1, tc::kTimeoutAccum | 0x10 | stream);
+          q_phases ^= 1u << stream;
         }
         tc::tc_fence_after();
         if (shared_rows) {
@@ -411,71 +435,93 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   }
   } else {
     // ---- softmax and outputs: four warps a stream, a thread a row ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const unsigned stream = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;       // row of the stream
     const unsigned lanes = (quarter * 32u) << 16;
     const unsigned score_at = tmem + stream * kKeys + lanes, out_at = tmem + kOutColumn + stream * 128 + lanes;
     unsigned char* const q_area = base_ptr + stream * kQBytes;
-    auto stream_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + stream) : "memory"); };
     auto both_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
+    auto stream_sync = [&] {
+      if (stream == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+      else asm volatile("bar.sync 2, 128;" ::: "memory");
+    };
     unsigned s_phase = 0, o_phase = 0;
-    walk([&](const Item& it, unsigned begin, unsigned end, unsigned long long item_first, unsigned) {
+    walk([&](const Item& it, unsigned begin, unsigned end, unsigned item_first, unsigned) {
       const unsigned n = end - begin;
       const bool shared_rows = it.rows <= kStreamRows;
       const unsigned rows_before = shared_rows ? 0u : stream * kStreamRows;                 // of the item's, in front of this stream's
       const unsigned live = min(it.rows - rows_before, kStreamRows);
+      const Rows pairs(it.row0 + rows_before, group);
       auto row_at = [&](unsigned i, unsigned stride) {                                      // offset of the stream's row i of q or o
-        const unsigned at = it.row0 + rows_before + i;
-        return size_t(it.row + at / group) * stride + (it.head * group + at % group) * kDim;
+        unsigned token, sub;
+        pairs.at(i, token, sub);
+        return size_t(it.row + token) * stride + (it.head * group + sub) * kDim;
       };
-      // Q into shared memory, swizzled (zero past the item's rows)
+      auto cell = [&](unsigned row, unsigned c) {                                           // 16-byte chunk c of a row of Q's memory
+        return reinterpret_cast<uint4*>(q_area + (c / 8) * (kStreamRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+      };
+      // Q into shared memory (zero past the item's rows)
       if (!shared_rows || stream == 0) {
-#pragma unroll 4
-        for (unsigned i = tid & 127; i < kStreamRows * (kDim / 8); i += 128) {
-          const unsigned row = i / (kDim / 8), c = i % (kDim / 8);
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (row < live) v = __ldcg(reinterpret_cast<const uint4*>(q + row_at(row, q_stride) + c * 8));
-          *reinterpret_cast<uint4*>(q_area + (c / 8) * (kStreamRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+        constexpr unsigned kBatch = 8;
+#pragma unroll 1
+        for (unsigned i0 = tid & 127; i0 < kStreamRows * (kDim / 8); i0 += 128 * kBatch) {
+          uint4 v[kBatch];
+#pragma unroll
+          for (unsigned b = 0; b < kBatch; ++b) {
+            const unsigned row = (i0 + b * 128) / (kDim / 8), c = (i0 + b * 128) % (kDim / 8);
+            v[b] = row < live ? __ldcg(reinterpret_cast<const uint4*>(q + row_at(row, q_stride) + c * 8)) : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (unsigned b = 0; b < kBatch; ++b) *cell((i0 + b * 128) / (kDim / 8), (i0 + b * 128) % (kDim / 8)) = v[b];
         }
         tc::fence_async_shared();
         tc::mbar_arrive(&q_full[stream]);
       }
-      const unsigned at = it.row0 + rows_before + r;
+      unsigned token, sub;
+      pairs.at(r, token, sub);
       const bool is_live = r < live;
-      const int index = kPrefix ? 0x3fffffff : is_live ? it.first + int(at / group) : -1;
+      const int index = kPrefix ? 0x3fffffff : is_live ? it.first + int(token) : -1;
       // the rows of this warp: does a tile need a mask?
-      const int low = it.first + int((it.row0 + rows_before + quarter * 32) / group);
-      const int high = it.first + int((it.row0 + rows_before + quarter * 32 + 31) / group);
+      const int low = it.first + int(__shfl_sync(0xffffffffu, token, 0)), high = it.first + int(__shfl_sync(0xffffffffu, token, 31));
       float top = -INFINITY, sum = 0.f;       // what weights are relative to (in units of log2), their sum
-      unsigned done = 0;
-      for (unsigned j = shared_rows ? stream : 0u; j < n; j += shared_rows ? 2u : 1u, ++done) {
+      bool done = false;
+#pragma unroll 1
+      for (unsigned j = shared_rows ? stream : 0u; j < n; j += shared_rows ? 2u : 1u) {
         await(&s_full[stream], s_phase, tc::kTimeoutAccum | stream);
         s_phase ^= 1;
         __syncwarp();
         tc::tc_fence_after();
-        float x[kKeys];
-#pragma unroll
-        for (unsigned c = 0; c < kKeys; c += 32) tmem_load32(score_at + c, x + c);
-        tmem_loaded<kKeys>(x);
         const unsigned key0 = it.seen.tile(begin + j) * kKeys;
         const bool whole = key0 + kKeys <= it.seen.end && (kPrefix || (int(key0 + kKeys) - 1 <= low && (window == 0 || int(key0) > high - int(window))));
-        if (!whole) {      // the row sees keys up to `last`, and of those the ones from `begins` on and the first `sinks`
-          const int last = min(index, int(it.seen.end) - 1) - int(key0), begins = kPrefix || window == 0 ? -1 : index - int(window) + 1 - int(key0);
-          const int sunk = int(sinks) - int(key0);
+        // the maximum of the row's scores; where the tile needs a mask, hidden ones become minus infinity in tensor memory
+        float now = -INFINITY;
+#pragma unroll 1
+        for (unsigned c0 = 0; c0 < kKeys; c0 += 64) {
+          float x[64];
+          tmem_load32(score_at + c0, x);
+          tmem_load32(score_at + c0 + 32, x + 32);
+          tmem_loaded<64>(x);
+          if (!whole) {
 #pragma unroll
-          for (int c = 0; c < int(kKeys); ++c)
-            if (c > last || (c < begins && c >= sunk)) x[c] = -INFINITY;
+            for (unsigned half = 0; half < 64; half += 32) {
+              const unsigned bits = visible_bits(key0 + c0 + half, index, it.seen.end, kPrefix ? 0u : window, sinks);
+#pragma unroll
+              for (unsigned i = 0; i < 32; ++i) x[half + i] = (bits >> i) & 1 ? x[half + i] : -INFINITY;
+              tmem_store32(score_at + c0 + half, reinterpret_cast<const unsigned*>(x + half));
+            }
+            tmem_stored();
+          }
+          float peak[4] = {now, x[0], x[1], x[2]};
+#pragma unroll
+          for (unsigned i = 3; i + 1 < 64; i += 2) peak[(i / 2) & 3] = max3(peak[(i / 2) & 3], x[i], x[i + 1]);
+          now = max3(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]), x[63]);
         }
-        float peak[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (unsigned c = 4; c < kKeys; ++c) peak[c & 3] = fmaxf(peak[c & 3], x[c]);
-        const float now = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3])) * scale_log2;
+        now *= scale_log2;
         if (__any_sync(0xffffffffu, now > top + kSlack)) {
           const float next = fmaxf(top, now), factor = next == -INFINITY ? 1.f : exp2_of(top - next);
           top = next;
           sum *= factor;
           if (done) {
-#pragma unroll
+#pragma unroll 1
             for (unsigned c = 0; c < kDim; c += 32) {
               float v[32];
               tmem_load32(out_at + c, v);
@@ -487,131 +533,139 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
             tmem_stored();
           }
         }
-        const float from_top = top == -INFINITY ? 0.f : top;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (unsigned half = 0; half < 2; ++half) {
+        const float2 by = make_float2(scale_log2, scale_log2), back = top == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-top, -top);
+        float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+        for (unsigned c0 = 0; c0 < kKeys; c0 += 64) {      // P takes half the columns: it never reaches scores that are still to be read
+          float x[64];
           unsigned packed[32];
+          tmem_load32(score_at + c0, x);
+          tmem_load32(score_at + c0 + 32, x + 32);
+          tmem_loaded<64>(x);
 #pragma unroll
           for (unsigned i = 0; i < 32; ++i) {
-            const unsigned c = half * 64 + 2 * i;
-            const float a = exp2_of(fmaf(x[c], scale_log2, -from_top)), b = exp2_of(fmaf(x[c + 1], scale_log2, -from_top));
-            part[(2 * i) & 3] += a;
-            part[(2 * i + 1) & 3] += b;
-            const bf162 pair = __floats2bfloat162_rn(a, b);
+            float2 p = fma2(make_float2(x[2 * i], x[2 * i + 1]), by, back);
+            p.x = exp2_of(p.x);
+            p.y = exp2_of(p.y);
+            part[i & 1] = add2(part[i & 1], p);
+            const bf162 pair = __floats2bfloat162_rn(p.x, p.y);
             packed[i] = *reinterpret_cast<const unsigned*>(&pair);
           }
-          tmem_store32(score_at + half * 32, packed);
+          tmem_store32(score_at + c0 / 2, packed);
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
         tmem_stored();
         tc::tc_fence_before();
         tc::mbar_arrive(&p_full[stream]);
+        done = true;
       }
-      float out[kDim];
       if (done) {
         await(&o_full[stream], o_phase, tc::kTimeoutAccum | 0x40 | stream);
         o_phase ^= 1;
         __syncwarp();
         tc::tc_fence_after();
-#pragma unroll
-        for (unsigned c = 0; c < kDim; c += 32) tmem_load32(out_at + c, out + c);
-        tmem_loaded<kDim>(out);
-      } else {
-#pragma unroll
-        for (unsigned c = 0; c < kDim; ++c) out[c] = 0.f;
       }
-      if (shared_rows) {      // the second stream's share to the first, through the memory of Q
-        float* const shared_out = reinterpret_cast<float*>(base_ptr);
+      // the stream's outputs, 32 columns at a time
+      auto columns = [&](unsigned c, float* v) {
+        if (done) {
+          tmem_load32(out_at + c, v);
+          tmem_loaded<32>(v);
+        } else {
+#pragma unroll
+          for (unsigned i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+      };
+      float* const shared_out = reinterpret_cast<float*>(base_ptr);      // [head_dim][128], in Q's memory
+      float mine_by = 1.f, other_by = 0.f;
+      if (shared_rows) {      // the second stream's share goes to the first
         both_sync();          // Q has been read by both streams' products
         if (stream == 1) {
+#pragma unroll 1
+          for (unsigned c0 = 0; c0 < kDim; c0 += 32) {
+            float v[32];
+            columns(c0, v);
 #pragma unroll
-          for (unsigned c = 0; c < kDim; ++c) shared_out[c * kStreamRows + r] = out[c];
+            for (unsigned i = 0; i < 32; ++i) shared_out[(c0 + i) * kStreamRows + r] = v[i];
+          }
           shared_end[r] = make_float2(top, sum);
         }
         both_sync();
-        if (stream == 0) {
-          const float2 other = shared_end[r];
-          const float next = fmaxf(top, other.x);
-          const float mine_by = top == -INFINITY ? 0.f : exp2_of(top - next), other_by = other.x == -INFINITY ? 0.f : exp2_of(other.x - next);
-#pragma unroll
-          for (unsigned c = 0; c < kDim; ++c) out[c] = out[c] * mine_by + shared_out[c * kStreamRows + r] * other_by;
-          sum = sum * mine_by + other.y * other_by;
-          top = next;
-        }
-        both_sync();          // Q's memory is free
-        if (stream == 1) return;
-      }
-      if (begin == 0 && end == it.seen.count) {
-        if (kPrefix || own_only) {
-          // rows of the launch are [row][q_head]; the own sequences' part is read (prefix) or written (own sequences, in front of it)
-          const size_t flat = size_t(it.row + at / group) * q_heads + it.head * group + at % group;
-          const bool covered = is_live && (!kPrefix || (int(it.row + at / group) >= batch.starts[0] && int(it.row + at / group) < batch.starts[batch.sequences]));
-          if (own_only) {
-            if (covered) {
-#pragma unroll
-              for (unsigned c = 0; c < kDim; c += 4)
-                *reinterpret_cast<float4*>(own_sums + flat * kDim + c) = make_float4(out[c], out[c + 1], out[c + 2], out[c + 3]);
-              *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(top, sum);
-            }
-            return;
-          }
-          if (covered) {
-            const float2 other = __ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2));
-            const float next = fmaxf(top, other.x);
-            const float mine_by = top == -INFINITY ? 0.f : exp2_of(top - next), other_by = other.x == -INFINITY ? 0.f : exp2_of(other.x - next);
-            sum = sum * mine_by + other.y * other_by;
-#pragma unroll
-            for (unsigned c = 0; c < kDim; c += 4) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c));
-              out[c] = out[c] * mine_by + v.x * other_by;
-              out[c + 1] = out[c + 1] * mine_by + v.y * other_by;
-              out[c + 2] = out[c + 2] * mine_by + v.z * other_by;
-              out[c + 3] = out[c + 3] * mine_by + v.w * other_by;
-            }
-            const float inv = sum > 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-            for (unsigned c = 0; c < kDim; c += 8) {
-              float v[8];
-#pragma unroll
-              for (unsigned i = 0; i < 8; ++i) v[i] = out[c + i] * inv;
-              *reinterpret_cast<Bf16x8*>(o + row_at(r, o_stride) + c) = pack8(v);
-            }
-          }
+        if (stream == 1) {
+          both_sync();        // Q's memory is free
           return;
         }
-        // rows staged in Q's memory, so that they leave in whole lines
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        join(top, sum, shared_end[r], mine_by, other_by);
+      }
+      const bool cut = begin != 0 || end != it.seen.count;
+      const unsigned slot = begin > 0 ? 0u : 1u;
+      // rows of no sequence are left alone
+      auto covered = [&](unsigned token_of) {
+        return !kPrefix || (int(it.row + token_of) >= batch.starts[0] && int(it.row + token_of) < batch.starts[batch.sequences]);
+      };
+      const size_t flat = size_t(it.row + token) * q_heads + it.head * group + sub;
+      const bool merges = kPrefix && !cut && is_live && covered(token);
+      float own_by = 0.f, all_by = 1.f;
+      if (merges) join(top, sum, __ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), all_by, own_by);
+      const bool divides = !cut && !own_only;
+      const float inv = !divides ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll 1
+      for (unsigned c0 = 0; c0 < kDim; c0 += 32) {
+        float v[32];
+        columns(c0, v);
+        if (shared_rows) {
 #pragma unroll
-        for (unsigned c = 0; c < kDim; c += 8) {
-          float v[8];
-#pragma unroll
-          for (unsigned i = 0; i < 8; ++i) v[i] = out[c + i] * inv;
-          *reinterpret_cast<Bf16x8*>(q_area + (c / 64) * (kStreamRows * 128) + r * 128 + ((((c / 8) & 7) ^ (r & 7)) << 4)) = pack8(v);
+          for (unsigned i = 0; i < 32; ++i) v[i] = v[i] * mine_by + shared_out[(c0 + i) * kStreamRows + r] * other_by;
         }
+        if (merges) {
+#pragma unroll
+          for (unsigned i = 0; i < 32; i += 4) {
+            const float4 w = __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c0 + i));
+            v[i] = v[i] * all_by + w.x * own_by;
+            v[i + 1] = v[i + 1] * all_by + w.y * own_by;
+            v[i + 2] = v[i + 2] * all_by + w.z * own_by;
+            v[i + 3] = v[i + 3] * all_by + w.w * own_by;
+          }
+        }
+        if (divides) {
+#pragma unroll
+          for (unsigned i = 0; i < 32; i += 8) {
+            float w[8];
+#pragma unroll
+            for (unsigned k = 0; k < 8; ++k) w[k] = v[i + k] * inv;
+            const Bf16x8 packed = pack8(w);
+            // rows are staged in Q's memory, so that they leave in whole lines; where it holds the other stream's share they leave as they are
+            if (!shared_rows) *cell(r, (c0 + i) / 8) = *reinterpret_cast<const uint4*>(&packed);
+            else if (is_live && covered(token)) *reinterpret_cast<Bf16x8*>(o + row_at(r, o_stride) + c0 + i) = packed;
+          }
+        } else if (is_live) {
+#pragma unroll
+          for (unsigned i = 0; i < 32; i += 4) {
+            float4* const to_row = cut ? parts.sum(blockIdx.x, slot, rows_before + r, (c0 + i) / 4) : reinterpret_cast<float4*>(own_sums + flat * kDim + c0 + i);
+            *to_row = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        }
+      }
+      if (!divides && is_live) *(cut ? parts.end(blockIdx.x, slot, rows_before + r) : reinterpret_cast<float2*>(own_ends + flat * 2)) = make_float2(top, sum);
+      if (shared_rows) {
+        both_sync();          // Q's memory is free
+      } else if (divides) {
         stream_sync();
 #pragma unroll 4
         for (unsigned i = tid & 127; i < live * (kDim / 8); i += 128) {
           const unsigned row = i / (kDim / 8), c = i % (kDim / 8);
-          *reinterpret_cast<uint4*>(o + row_at(row, o_stride) + c * 8) =
-              *reinterpret_cast<const uint4*>(q_area + (c / 8) * (kStreamRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+          unsigned token_of, sub_of;
+          pairs.at(row, token_of, sub_of);
+          if (covered(token_of)) *reinterpret_cast<uint4*>(o + row_at(row, o_stride) + c * 8) = *cell(row, c);
         }
         stream_sync();
-        return;
       }
-      const unsigned slot = begin > 0 ? 0u : 1u;
-      if (is_live) {
-#pragma unroll
-        for (unsigned c = 0; c < kDim; c += 4) *parts.sum(blockIdx.x, slot, rows_before + r, c / 4) = make_float4(out[c], out[c + 1], out[c + 2], out[c + 3]);
-        *parts.end(blockIdx.x, slot, rows_before + r) = make_float2(top, sum);
-      }
-      if (begin == 0 && tid == 0) {
+      if (cut && begin == 0 && tid == 0) {
         Note& note = parts.notes[blockIdx.x];
         note.row = it.row;
         note.row0 = it.row0;
         note.rows = it.rows;
         note.head = it.head;
-        note.pieces = unsigned((item_first + it.seen.count - 1) / per) - blockIdx.x + 1;
+        note.pieces = (item_first + it.seen.count - 1) / per - blockIdx.x + 1;
       }
     });
   }
@@ -644,16 +698,14 @@ __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned s
   float top = -INFINITY, sum = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](const float2 end, const float4 part) {
-    if (end.x == -INFINITY) return;
-    const float next = fmaxf(top, end.x), mine_by = exp2_of(top - next), other_by = exp2_of(end.x - next);
+    float mine_by, other_by;
+    join(top, sum, end, mine_by, other_by);
     v.x = v.x * mine_by + part.x * other_by;
     v.y = v.y * mine_by + part.y * other_by;
     v.z = v.z * mine_by + part.z * other_by;
     v.w = v.w * mine_by + part.w * other_by;
-    sum = sum * mine_by + end.y * other_by;
-    top = next;
   };
-#pragma unroll 4
+#pragma unroll 2
   for (unsigned p = 0; p < pieces; ++p) add(__ldcg(parts.end(first + p, p == 0, r)), __ldcg(parts.sum(first + p, p == 0, r, c4)));
   if (own_only) {
     *reinterpret_cast<float4*>(own_sums + flat * kDim + c4 * 4) = v;
