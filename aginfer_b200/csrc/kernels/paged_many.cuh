@@ -30,6 +30,8 @@ constexpr unsigned kKeys = 128, kStreamRows = 128, kRows = 256, kThreads = 384;
 // Registers after the warp groups have traded: a row's 128 scores stay in registers (168 a thread, the launch's share, would spill 480
 // bytes), the group of the loading and the issuing warp gives its own for that (2 x 208 + 88 = 3 x 168).
 constexpr unsigned kSoftmaxRegs = 208, kHelperRegs = 88;
+constexpr unsigned kStagePitch = 80;        // bytes of a row's 32 columns in a warp's staging memory, and 16 against bank conflicts
+constexpr unsigned kItemCost = 1;           // what an item costs besides its tiles (queries in, outputs out), in tiles
 constexpr unsigned kOutColumn = 256;
 constexpr float kSlack = 8.f;               // log2 of how far scores may exceed the maximum that weights are relative to
 
@@ -60,6 +62,12 @@ __device__ __forceinline__ void tmem_store32(unsigned addr, const unsigned* r) {
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_store16(unsigned addr, const unsigned* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+               "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -161,7 +169,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kBlockBytes = kKeys * 128, kSlotBytes = kBlocks * kBlockBytes;
   constexpr unsigned kQBytes = kStreamRows * kDim * 2, kMaxStages = 12;
   extern __shared__ unsigned char dynamic_smem[];
-  __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages], q_full[2], s_full[2], p_full[2], o_full[2];
+  __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages];
+  __shared__ __align__(8) unsigned long long q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
   __shared__ float2 shared_end[kStreamRows];
   __shared__ unsigned block_base[kThreads / 32], tile_base[kThreads / 32], run_seq, run_block, run_first, gave_up, tmem_slot;
   const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -177,10 +186,13 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       tc::mbar_init(&empty_bar[s], 1);
     }
     for (unsigned s = 0; s < 2; ++s) {
-      tc::mbar_init(&q_full[s], kStreamRows);
+      tc::mbar_init(&q_full[s], 32);
+      tc::mbar_init(&q_empty[s], 1);
       tc::mbar_init(&s_full[s], 1);
+      tc::mbar_init(&p_half[s], kStreamRows);
       tc::mbar_init(&p_full[s], kStreamRows);
       tc::mbar_init(&o_full[s], 1);
+      tc::mbar_init(&o_empty[s], kStreamRows);
     }
     gave_up = 0;
     run_seq = run_block = 0;
@@ -249,7 +261,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 #pragma unroll 1
     for (unsigned b = b0; b < b1; ++b) {
       while (seq + 1 < sequences && block_begin[seq + 1] <= b) ++seq;
-      const unsigned tiles = seen_at(span_at(seq), b - block_begin[seq]).count * kv_heads;
+      const unsigned tiles = (seen_at(span_at(seq), b - block_begin[seq]).count + kItemCost) * kv_heads;
       if (pass == 0) {
         mine += tiles;
       } else if (from < below + tiles) {
@@ -286,15 +298,17 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       it.row0 = block * kRows;
       it.rows = min(kRows, span.fresh * group - it.row0);
       it.seen = seen_at(span, block);
-      const unsigned count = it.seen.count;
+      const unsigned length = it.seen.count + kItemCost;
 #pragma unroll 1
-      while (unit < to && unit < first + count * kv_heads) {
-        it.head = (unit - first) / count;
-        const unsigned item_first = first + it.head * count, begin = unit - item_first, end = min(count, begin + (to - unit));
-        f(it, begin, end, item_first, seq);
-        unit += end - begin;
+      while (unit < to && unit < first + length * kv_heads) {
+        it.head = (unit - first) / length;
+        // the item's tiles stand behind the units that it costs besides; a run that ends among those leaves the item to the next one
+        const unsigned tiles_at = first + it.head * length + kItemCost, next = tiles_at + it.seen.count;
+        const unsigned begin = max(unit, tiles_at) - tiles_at, end = max(min(next, to), tiles_at) - tiles_at;
+        if (begin < end) f(it, begin, end, tiles_at, seq);
+        unit = next;
       }
-      first += count * kv_heads;
+      first += length * kv_heads;
       ++block;
     }
   };
@@ -353,7 +367,12 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     // ---- one thread issues the products ----
     if (elect_one()) {
       constexpr unsigned kScores = instruction(kKeys, false), kOutputs = instruction(kDim, true);
-      unsigned s = 0, phase = 0, q_phases = 0, p_phases = 0;       // a bit per stream
+      unsigned s = 0, phase = 0, q_phases = 0, p_phases = 0, o_phases = 3;       // a bit per stream
+      auto flips = [&](unsigned long long* bars, unsigned& phases, unsigned stream, unsigned code) {
+        await(&bars[stream], (phases >> stream) & 1, tc::kTimeoutAccum | code | stream);
+        phases ^= 1u << stream;
+        tc::tc_fence_after();
+      };
       auto scores = [&](unsigned stream, unsigned q_stream, unsigned slot) {
         const unsigned long long a = tc::smem_descriptor(base + q_stream * kQBytes), b = tc::smem_descriptor(ring + slot * kSlotBytes);
 #pragma unroll
@@ -362,12 +381,6 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
                          kScores, k != 0);
         tc::tc_commit(&s_full[stream]);
       };
-      auto outputs = [&](unsigned stream, unsigned slot, bool accumulate) {
-        const unsigned long long b = mn_descriptor(ring + slot * kSlotBytes, kBlockBytes);
-#pragma unroll
-        for (unsigned k = 0; k < kKeys / 16; ++k)
-          mma_from_tmem(tmem + kOutColumn + stream * 128, tmem + stream * kKeys + k * 8, b + k * (16 * 128 >> 4), kOutputs, accumulate || k != 0);
-      };
       auto arrived = [&] {      // the next slot of the ring has landed: its number
         await(&full_bar[s], phase, tc::kTimeoutFull | s);
         tc::tc_fence_after();
@@ -375,110 +388,103 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         if (++s == stages) { s = 0; phase ^= 1; }
         return slot;
       };
-      auto weighted = [&](unsigned stream) {
-        await(&p_full[stream], (p_phases >> stream) & 1, tc::kTimeoutAccum | 0x20 | stream);
-        p_phases ^= 1u << stream;
+      // P V of a stream's tile: the first half of the keys while the weights of the second half are still being formed
+      auto outputs = [&](unsigned stream, unsigned slot, bool first) {
+        const unsigned long long b = mn_descriptor(ring + slot * kSlotBytes, kBlockBytes);
+        const unsigned d = tmem + kOutColumn + stream * 128, a = tmem + stream * kKeys;
+        if (first) flips(o_empty, o_phases, stream, 0x80);
+        await(&p_half[stream], (p_phases >> stream) & 1, tc::kTimeoutAccum | 0x30 | stream);
         tc::tc_fence_after();
+#pragma unroll
+        for (unsigned k = 0; k < kKeys / 32; ++k) mma_from_tmem(d, a + k * 8, b + k * (16 * 128 >> 4), kOutputs, !first || k != 0);
+        flips(p_full, p_phases, stream, 0x20);
+#pragma unroll
+        for (unsigned k = kKeys / 32; k < kKeys / 16; ++k) mma_from_tmem(d, a + k * 8, b + k * (16 * 128 >> 4), kOutputs, 1);
       };
       walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned) {
         const unsigned n = end - begin;
         const bool shared_rows = it.rows <= kStreamRows;
-        for (unsigned stream = 0; stream < (shared_rows ? 1u : 2u); ++stream) {
-          await(&q_full[stream], (q_phases >> stream) & 1, tc::kTimeoutAccum | 0x10 | stream);
-          q_phases ^= 1u << stream;
-        }
-        tc::tc_fence_after();
-        if (shared_rows) {
-          for (unsigned j = 0; j < min(n, 2u); ++j) {
-            const unsigned slot = arrived();
-            scores(j, 0, slot);
-            tc::tc_commit(&empty_bar[slot]);
-          }
-          for (unsigned j = 0; j < n; ++j) {
-            const unsigned stream = j & 1, slot = arrived();
-            weighted(stream);
-            outputs(stream, slot, j >= 2);
-            tc::tc_commit(&empty_bar[slot]);
-            if (j + 2 < n) {
-              const unsigned next = arrived();
-              scores(stream, 0, next);
-              tc::tc_commit(&empty_bar[next]);
-            } else {
-              tc::tc_commit(&o_full[stream]);
+        // step i: scores of tile i (i < n), behind the outputs of the tile that used the same columns before
+        const unsigned lead = shared_rows ? min(n, 2u) : 1u;
+        unsigned values = 0, keys = 0;
+#pragma unroll 1
+        for (unsigned i = 0; i < n + lead; ++i) {
+#pragma unroll 1
+          for (unsigned half = 0; half < (shared_rows ? 1u : 2u); ++half) {
+            const unsigned stream = shared_rows ? (i >= lead ? (i - lead) & 1 : i) : half, area = shared_rows ? 0u : stream;
+            const bool last_use = shared_rows || half == 1;
+            if (i >= lead) {
+              const unsigned j = i - lead;
+              if (half == 0) values = arrived();
+              outputs(stream, values, j < lead);
+              if (last_use) tc::tc_commit(&empty_bar[values]);
+              if (j + lead >= n) tc::tc_commit(&o_full[stream]);
             }
-          }
-        } else {
-          unsigned slot = arrived();
-          scores(0, 0, slot);
-          scores(1, 1, slot);
-          tc::tc_commit(&empty_bar[slot]);
-          for (unsigned j = 0; j < n; ++j) {
-            slot = arrived();
-            unsigned next = 0;
-            for (unsigned stream = 0; stream < 2; ++stream) {
-              weighted(stream);
-              outputs(stream, slot, j != 0);
-              if (stream == 1) tc::tc_commit(&empty_bar[slot]);
-              if (j + 1 < n) {
-                if (stream == 0) next = arrived();
-                scores(stream, stream, next);
-                if (stream == 1) tc::tc_commit(&empty_bar[next]);
-              } else {
-                tc::tc_commit(&o_full[stream]);
-              }
+            if (i < n) {
+              if (half == 0) keys = arrived();
+              if (i == 0) flips(q_full, q_phases, area, 0x10);
+              scores(stream, area, keys);
+              if (last_use) tc::tc_commit(&empty_bar[keys]);
+              if (i == n - 1) tc::tc_commit(&q_empty[area]);
             }
           }
         }
       });
     }
     __syncwarp();
+  } else {
+    // ---- a warp per stream brings the queries in (zero past the item's rows), as soon as the item before has formed its last scores ----
+    const unsigned stream = warp - 10;
+    constexpr unsigned kChunks = kDim / 8, kStep = 32 / kChunks;      // 16-byte chunks of a row, rows that the warp copies at a time
+    const unsigned c = lane % kChunks, q_area = base + stream * kQBytes + (c / 8) * (kStreamRows * 128);
+    unsigned phase = 1;
+    walk([&](const Item& it, unsigned, unsigned, unsigned, unsigned) {
+      const bool shared_rows = it.rows <= kStreamRows;
+      if (shared_rows && stream == 1) return;
+      const unsigned rows_before = stream * kStreamRows, live = min(it.rows - rows_before, kStreamRows);
+      await(&q_empty[stream], phase, tc::kTimeoutAccum | 0x50 | stream);
+      phase ^= 1;
+      __syncwarp();
+      const unsigned first = it.row0 + rows_before + lane / kChunks, token_step = kStep / group, sub_step = kStep % group;
+      unsigned token = first / group, sub = first % group;
+#pragma unroll 4
+      for (unsigned row = lane / kChunks; row < kStreamRows; row += kStep) {
+        const bool held = row < live;
+        const bf16* from_row = q + (held ? size_t(it.row + token) * q_stride + (it.head * group + sub) * kDim : 0) + c * 8;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_area + row * 128 + (((c & 7) ^ (row & 7)) << 4)), "l"(from_row),
+                     "r"(held ? 16u : 0u) : "memory");
+        token += token_step;
+        sub += sub_step;
+        if (sub >= group) {
+          sub -= group;
+          ++token;
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      tc::fence_async_shared();
+      tc::mbar_arrive(&q_full[stream]);
+    });
   }
   } else {
     // ---- softmax and outputs: four warps a stream, a thread a row ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const unsigned stream = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;       // row of the stream
     const unsigned lanes = (quarter * 32u) << 16;
     const unsigned score_at = tmem + stream * kKeys + lanes, out_at = tmem + kOutColumn + stream * 128 + lanes;
-    unsigned char* const q_area = base_ptr + stream * kQBytes;
-    auto both_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
-    auto stream_sync = [&] {
-      if (stream == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-      else asm volatile("bar.sync 2, 128;" ::: "memory");
+    unsigned char* const staged = base_ptr + 2 * kQBytes + stages * kSlotBytes + warp * (32 * kStagePitch);
+    unsigned s_phase = 0, o_phases = 0, shared_items = 0;
+    auto outputs_done = [&](unsigned of_stream) {
+      await(&o_full[of_stream], (o_phases >> of_stream) & 1, tc::kTimeoutAccum | 0x40 | of_stream);
+      __syncwarp();
+      tc::tc_fence_after();
     };
-    unsigned s_phase = 0, o_phase = 0;
-    walk([&](const Item& it, unsigned begin, unsigned end, unsigned item_first, unsigned) {
+    walk([&](const Item& it, unsigned begin, unsigned end, unsigned tiles_at, unsigned) {
       const unsigned n = end - begin;
       const bool shared_rows = it.rows <= kStreamRows;
       const unsigned rows_before = shared_rows ? 0u : stream * kStreamRows;                 // of the item's, in front of this stream's
-      const unsigned live = min(it.rows - rows_before, kStreamRows);
-      const Rows pairs(it.row0 + rows_before, group);
-      auto row_at = [&](unsigned i, unsigned stride) {                                      // offset of the stream's row i of q or o
-        unsigned token, sub;
-        pairs.at(i, token, sub);
-        return size_t(it.row + token) * stride + (it.head * group + sub) * kDim;
-      };
-      auto cell = [&](unsigned row, unsigned c) {                                           // 16-byte chunk c of a row of Q's memory
-        return reinterpret_cast<uint4*>(q_area + (c / 8) * (kStreamRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
-      };
-      // Q into shared memory (zero past the item's rows)
-      if (!shared_rows || stream == 0) {
-        constexpr unsigned kBatch = 8;
-#pragma unroll 1
-        for (unsigned i0 = tid & 127; i0 < kStreamRows * (kDim / 8); i0 += 128 * kBatch) {
-          uint4 v[kBatch];
-#pragma unroll
-          for (unsigned b = 0; b < kBatch; ++b) {
-            const unsigned row = (i0 + b * 128) / (kDim / 8), c = (i0 + b * 128) % (kDim / 8);
-            v[b] = row < live ? __ldcg(reinterpret_cast<const uint4*>(q + row_at(row, q_stride) + c * 8)) : make_uint4(0u, 0u, 0u, 0u);
-          }
-#pragma unroll
-          for (unsigned b = 0; b < kBatch; ++b) *cell((i0 + b * 128) / (kDim / 8), (i0 + b * 128) % (kDim / 8)) = v[b];
-        }
-        tc::fence_async_shared();
-        tc::mbar_arrive(&q_full[stream]);
-      }
+      const bool is_live = rows_before + r < it.rows;
       unsigned token, sub;
-      pairs.at(r, token, sub);
-      const bool is_live = r < live;
+      Rows(it.row0 + rows_before, group).at(r, token, sub);
       const int index = kPrefix ? 0x3fffffff : is_live ? it.first + int(token) : -1;
       // the rows of this warp: does a tile need a mask?
       const int low = it.first + int(__shfl_sync(0xffffffffu, token, 0)), high = it.first + int(__shfl_sync(0xffffffffu, token, 31));
@@ -490,182 +496,156 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         s_phase ^= 1;
         __syncwarp();
         tc::tc_fence_after();
+        float x[kKeys];
+#pragma unroll
+        for (unsigned c = 0; c < kKeys; c += 32) tmem_load32(score_at + c, x + c);
         const unsigned key0 = it.seen.tile(begin + j) * kKeys;
         const bool whole = key0 + kKeys <= it.seen.end && (kPrefix || (int(key0 + kKeys) - 1 <= low && (window == 0 || int(key0) > high - int(window))));
-        // the maximum of the row's scores; where the tile needs a mask, hidden ones become minus infinity in tensor memory
-        float now = -INFINITY;
-#pragma unroll 1
-        for (unsigned c0 = 0; c0 < kKeys; c0 += 64) {
-          float x[64];
-          tmem_load32(score_at + c0, x);
-          tmem_load32(score_at + c0 + 32, x + 32);
-          tmem_loaded<64>(x);
-          if (!whole) {
+        tmem_loaded<kKeys>(x);
+        if (!whole) {
 #pragma unroll
-            for (unsigned half = 0; half < 64; half += 32) {
-              const unsigned bits = visible_bits(key0 + c0 + half, index, it.seen.end, kPrefix ? 0u : window, sinks);
+          for (unsigned c = 0; c < kKeys; c += 32) {
+            const unsigned bits = visible_bits(key0 + c, index, it.seen.end, kPrefix ? 0u : window, sinks);
 #pragma unroll
-              for (unsigned i = 0; i < 32; ++i) x[half + i] = (bits >> i) & 1 ? x[half + i] : -INFINITY;
-              tmem_store32(score_at + c0 + half, reinterpret_cast<const unsigned*>(x + half));
-            }
-            tmem_stored();
+            for (unsigned i = 0; i < 32; ++i) x[c + i] = (bits >> i) & 1 ? x[c + i] : -INFINITY;
           }
-          float peak[4] = {now, x[0], x[1], x[2]};
-#pragma unroll
-          for (unsigned i = 3; i + 1 < 64; i += 2) peak[(i / 2) & 3] = max3(peak[(i / 2) & 3], x[i], x[i + 1]);
-          now = max3(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]), x[63]);
         }
-        now *= scale_log2;
+        float peak[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (unsigned i = 4; i < kKeys; i += 2) peak[(i / 2) & 3] = max3(peak[(i / 2) & 3], x[i], x[i + 1]);
+        const float now = max3(fmaxf(peak[0], peak[1]), peak[2], peak[3]) * scale_log2;
         if (__any_sync(0xffffffffu, now > top + kSlack)) {
           const float next = fmaxf(top, now), factor = next == -INFINITY ? 1.f : exp2_of(top - next);
           top = next;
           sum *= factor;
           if (done) {
 #pragma unroll 1
-            for (unsigned c = 0; c < kDim; c += 32) {
-              float v[32];
-              tmem_load32(out_at + c, v);
-              tmem_loaded<32>(v);
+            for (unsigned c = 0; c < kDim; c += 16) {
+              float v[16];
+              tc::tmem_load16(out_at + c, v);
+              tmem_loaded<16>(v);
 #pragma unroll
-              for (unsigned i = 0; i < 32; ++i) v[i] *= factor;
-              tmem_store32(out_at + c, reinterpret_cast<const unsigned*>(v));
+              for (unsigned i = 0; i < 16; ++i) v[i] *= factor;
+              tmem_store16(out_at + c, reinterpret_cast<const unsigned*>(v));
             }
             tmem_stored();
           }
         }
         const float2 by = make_float2(scale_log2, scale_log2), back = top == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-top, -top);
         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-        for (unsigned c0 = 0; c0 < kKeys; c0 += 64) {      // P takes half the columns: it never reaches scores that are still to be read
-          float x[64];
+#pragma unroll
+        for (unsigned half = 0; half < 2; ++half) {
           unsigned packed[32];
-          tmem_load32(score_at + c0, x);
-          tmem_load32(score_at + c0 + 32, x + 32);
-          tmem_loaded<64>(x);
 #pragma unroll
           for (unsigned i = 0; i < 32; ++i) {
-            float2 p = fma2(make_float2(x[2 * i], x[2 * i + 1]), by, back);
+            float2 p = fma2(make_float2(x[half * 64 + 2 * i], x[half * 64 + 2 * i + 1]), by, back);
             p.x = exp2_of(p.x);
             p.y = exp2_of(p.y);
             part[i & 1] = add2(part[i & 1], p);
             const bf162 pair = __floats2bfloat162_rn(p.x, p.y);
             packed[i] = *reinterpret_cast<const unsigned*>(&pair);
           }
-          tmem_store32(score_at + c0 / 2, packed);
+          tmem_store32(score_at + half * 32, packed);
+          tmem_stored();
+          tc::tc_fence_before();
+          tc::mbar_arrive(half == 0 ? &p_half[stream] : &p_full[stream]);
         }
         sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-        tmem_stored();
-        tc::tc_fence_before();
-        tc::mbar_arrive(&p_full[stream]);
         done = true;
       }
-      if (done) {
-        await(&o_full[stream], o_phase, tc::kTimeoutAccum | 0x40 | stream);
-        o_phase ^= 1;
-        __syncwarp();
-        tc::tc_fence_after();
-      }
-      // the stream's outputs, 32 columns at a time
-      auto columns = [&](unsigned c, float* v) {
-        if (done) {
-          tmem_load32(out_at + c, v);
-          tmem_loaded<32>(v);
-        } else {
-#pragma unroll
-          for (unsigned i = 0; i < 32; ++i) v[i] = 0.f;
-        }
-      };
-      float* const shared_out = reinterpret_cast<float*>(base_ptr);      // [head_dim][128], in Q's memory
-      float mine_by = 1.f, other_by = 0.f;
-      if (shared_rows) {      // the second stream's share goes to the first
-        both_sync();          // Q has been read by both streams' products
+      const bool cut = begin != 0 || end != it.seen.count, both = shared_rows && n >= 2;
+      const unsigned slot = begin > 0 ? 0u : 1u;
+      float2 other = make_float2(-INFINITY, 0.f);
+      if (shared_rows) {      // the first stream adds the second one's share, which it reads where that left it
         if (stream == 1) {
-#pragma unroll 1
-          for (unsigned c0 = 0; c0 < kDim; c0 += 32) {
-            float v[32];
-            columns(c0, v);
-#pragma unroll
-            for (unsigned i = 0; i < 32; ++i) shared_out[(c0 + i) * kStreamRows + r] = v[i];
-          }
+          if (shared_items++) asm volatile("bar.sync 2, 256;" ::: "memory");      // that of the item before has been read
           shared_end[r] = make_float2(top, sum);
-        }
-        both_sync();
-        if (stream == 1) {
-          both_sync();        // Q's memory is free
+          asm volatile("bar.arrive 1, 256;" ::: "memory");
+          o_phases ^= both ? 3u : 1u;
           return;
         }
-        join(top, sum, shared_end[r], mine_by, other_by);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        other = shared_end[r];
+        asm volatile("bar.arrive 2, 256;" ::: "memory");
       }
-      const bool cut = begin != 0 || end != it.seen.count;
-      const unsigned slot = begin > 0 ? 0u : 1u;
+      outputs_done(stream);
+      if (both) outputs_done(1);
+      o_phases ^= shared_rows && !both ? 1u : 3u;
+      float mine_by = 1.f, other_by = 0.f;
+      if (both) join(top, sum, other, mine_by, other_by);
       // rows of no sequence are left alone
-      auto covered = [&](unsigned token_of) {
-        return !kPrefix || (int(it.row + token_of) >= batch.starts[0] && int(it.row + token_of) < batch.starts[batch.sequences]);
-      };
-      const size_t flat = size_t(it.row + token) * q_heads + it.head * group + sub;
-      const bool merges = kPrefix && !cut && is_live && covered(token);
-      float own_by = 0.f, all_by = 1.f;
-      if (merges) join(top, sum, __ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), all_by, own_by);
-      const bool divides = !cut && !own_only;
-      const float inv = !divides ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
+      const unsigned row = it.row + token;
+      const bool stays = is_live && (!kPrefix || (int(row) >= batch.starts[0] && int(row) < batch.starts[batch.sequences]));
+      const size_t flat = size_t(row) * q_heads + it.head * group + sub;
+      const bool merges = kPrefix && !cut && stays, divides = !cut && !own_only;
+      float own_by = 0.f;
+      if (merges) {
+        float all_by;
+        join(top, sum, __ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), all_by, own_by);
+        mine_by *= all_by;
+        other_by *= all_by;
+      }
+      if (divides) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        mine_by *= inv;
+        other_by *= inv;
+        own_by *= inv;
+      }
+      bf16* const to_row = o + size_t(row) * o_stride + (it.head * group + sub) * kDim;
 #pragma unroll 1
       for (unsigned c0 = 0; c0 < kDim; c0 += 32) {
         float v[32];
-        columns(c0, v);
-        if (shared_rows) {
+        tmem_load32(out_at + c0, v);
+        tmem_loaded<32>(v);
 #pragma unroll
-          for (unsigned i = 0; i < 32; ++i) v[i] = v[i] * mine_by + shared_out[(c0 + i) * kStreamRows + r] * other_by;
+        for (unsigned i = 0; i < 32; ++i) v[i] *= mine_by;
+        if (both) {
+          float w[32];
+          tmem_load32(out_at + 128 + c0, w);
+          tmem_loaded<32>(w);
+#pragma unroll
+          for (unsigned i = 0; i < 32; ++i) v[i] = fmaf(w[i], other_by, v[i]);
         }
         if (merges) {
 #pragma unroll
           for (unsigned i = 0; i < 32; i += 4) {
             const float4 w = __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c0 + i));
-            v[i] = v[i] * all_by + w.x * own_by;
-            v[i + 1] = v[i + 1] * all_by + w.y * own_by;
-            v[i + 2] = v[i + 2] * all_by + w.z * own_by;
-            v[i + 3] = v[i + 3] * all_by + w.w * own_by;
+            v[i] = fmaf(w.x, own_by, v[i]);
+            v[i + 1] = fmaf(w.y, own_by, v[i + 1]);
+            v[i + 2] = fmaf(w.z, own_by, v[i + 2]);
+            v[i + 3] = fmaf(w.w, own_by, v[i + 3]);
           }
         }
-        if (divides) {
+        if (divides) {      // through shared memory, so that rows leave in whole sectors: eight rows of 64 bytes a store
+          __syncwarp();
+#pragma unroll
+          for (unsigned i = 0; i < 32; i += 8) *reinterpret_cast<Bf16x8*>(staged + lane * kStagePitch + i * 2) = pack8(v + i);
+          __syncwarp();
 #pragma unroll
           for (unsigned i = 0; i < 32; i += 8) {
-            float w[8];
-#pragma unroll
-            for (unsigned k = 0; k < 8; ++k) w[k] = v[i + k] * inv;
-            const Bf16x8 packed = pack8(w);
-            // rows are staged in Q's memory, so that they leave in whole lines; where it holds the other stream's share they leave as they are
-            if (!shared_rows) *cell(r, (c0 + i) / 8) = *reinterpret_cast<const uint4*>(&packed);
-            else if (is_live && covered(token)) *reinterpret_cast<Bf16x8*>(o + row_at(r, o_stride) + c0 + i) = packed;
+            const unsigned other_row = i + lane / 4;
+            const unsigned long long at = __shfl_sync(0xffffffffu, stays ? reinterpret_cast<unsigned long long>(to_row) : 0ull, other_row);
+            if (at) *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(at) + c0 + (lane & 3) * 8) =
+                *reinterpret_cast<const uint4*>(staged + other_row * kStagePitch + (lane & 3) * 16);
           }
         } else if (is_live) {
 #pragma unroll
-          for (unsigned i = 0; i < 32; i += 4) {
-            float4* const to_row = cut ? parts.sum(blockIdx.x, slot, rows_before + r, (c0 + i) / 4) : reinterpret_cast<float4*>(own_sums + flat * kDim + c0 + i);
-            *to_row = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          }
+          for (unsigned i = 0; i < 32; i += 4)
+            *(cut ? parts.sum(blockIdx.x, slot, rows_before + r, (c0 + i) / 4) : reinterpret_cast<float4*>(own_sums + flat * kDim + c0 + i)) =
+                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
       }
+      tc::tc_fence_before();
+      tc::mbar_arrive(&o_empty[stream]);
+      if (both) tc::mbar_arrive(&o_empty[1]);
       if (!divides && is_live) *(cut ? parts.end(blockIdx.x, slot, rows_before + r) : reinterpret_cast<float2*>(own_ends + flat * 2)) = make_float2(top, sum);
-      if (shared_rows) {
-        both_sync();          // Q's memory is free
-      } else if (divides) {
-        stream_sync();
-#pragma unroll 4
-        for (unsigned i = tid & 127; i < live * (kDim / 8); i += 128) {
-          const unsigned row = i / (kDim / 8), c = i % (kDim / 8);
-          unsigned token_of, sub_of;
-          pairs.at(row, token_of, sub_of);
-          if (covered(token_of)) *reinterpret_cast<uint4*>(o + row_at(row, o_stride) + c * 8) = *cell(row, c);
-        }
-        stream_sync();
-      }
       if (cut && begin == 0 && tid == 0) {
         Note& note = parts.notes[blockIdx.x];
         note.row = it.row;
         note.row0 = it.row0;
         note.rows = it.rows;
         note.head = it.head;
-        note.pieces = (item_first + it.seen.count - 1) / per - blockIdx.x + 1;
+        note.pieces = (tiles_at + it.seen.count - 1) / per - blockIdx.x + 1;
       }
     });
   }
@@ -720,7 +700,7 @@ __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned s
 
 }  // namespace many
 
-// grid: one CTA an SM (or fewer), block = 384, dynamic shared memory = 512 * head_dim (Q) + stages * 256 * head_dim + 1024.
+// grid: one CTA an SM (or fewer), block = 384, dynamic shared memory = 512 * head_dim (Q) + stages * 256 * head_dim + 20480 (staging) + 1024.
 // own_only: the rows' own sequences' part of prefix attention, left in own_sums and own_ends instead of o.
 #define AGI_PAGED_MANY(NAME, HD16, PREFIX)                                                                                              \
   extern "C" __global__ void __launch_bounds__(many::kThreads, 1)                                                                       \

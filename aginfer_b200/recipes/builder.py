@@ -528,8 +528,9 @@ def paged_many_tiling(cache: PagedCache, blocks: int, tokens: int) -> dict[str, 
     d = cache.head_dim
     units = blocks * cache.kv_heads * ceil_div(tokens, PAGED_MANY_KEYS)
     grid = min(SM_COUNT, ceil_div(units, PAGED_MANY_LEAST))
-    stages = min(12, (MAX_DYNAMIC_SHARED - 1024 - 2048 - 512 * d) // (256 * d))
-    return {"grid": grid, "stages": stages, "least": PAGED_MANY_LEAST, "shared_bytes": 512 * d + stages * 256 * d + 1024,
+    rest = 512 * d + 20480 + 1024          # queries, staging of outputs, alignment
+    stages = min(12, (MAX_DYNAMIC_SHARED - 2048 - rest) // (256 * d))
+    return {"grid": grid, "stages": stages, "least": PAGED_MANY_LEAST, "shared_bytes": rest + stages * 256 * d,
             "scratch_bytes": grid * 2 * (PAGED_MANY_ROWS * d + 2 * PAGED_MANY_ROWS) * 4}
 
 
