@@ -31,7 +31,7 @@ constexpr unsigned kKeys = 128, kStreamRows = 128, kRows = 256, kThreads = 384;
 // bytes), the group of the loading and the issuing warp gives its own for that (2 x 208 + 88 = 3 x 168).
 constexpr unsigned kSoftmaxRegs = 208, kHelperRegs = 88;
 constexpr unsigned kStagePitch = 80;        // bytes of a row's 32 columns in a warp's staging memory, and 16 against bank conflicts
-constexpr unsigned kItemCost = 1;           // what an item costs besides its tiles (queries in, outputs out), in tiles
+constexpr unsigned kItemCost = 3;           // what an item costs besides its tiles (queries in, outputs out), in tiles
 constexpr unsigned kOutColumn = 256;
 constexpr float kSlack = 8.f;               // log2 of how far scores may exceed the maximum that weights are relative to
 
@@ -70,6 +70,13 @@ __device__ __forceinline__ void tmem_store16(unsigned addr, const unsigned* r) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ bool is_done(unsigned long long* bar, unsigned parity) {
+  unsigned done;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(done) : "r"(tc::smem_u32(bar)), "r"(parity) : "memory");
+  return done != 0;
+}
 
 // D[128 x N] (+)= A . B with A (bf16 pairs) in tensor memory.
 __device__ __forceinline__ void mma_from_tmem(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned accumulate) {
@@ -167,9 +174,9 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
                                                unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,
                                                unsigned least, unsigned own_only) {
   constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kBlockBytes = kKeys * 128, kSlotBytes = kBlocks * kBlockBytes;
-  constexpr unsigned kQBytes = kStreamRows * kDim * 2, kMaxStages = 12;
+  constexpr unsigned kQBytes = kStreamRows * kDim * 2, kMaxStages = 6;
   extern __shared__ unsigned char dynamic_smem[];
-  __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages];
+  __shared__ __align__(8) unsigned long long k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
   __shared__ __align__(8) unsigned long long q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
   __shared__ float2 shared_end[kStreamRows];
   __shared__ unsigned block_base[kThreads / 32], tile_base[kThreads / 32], run_seq, run_block, run_first, gave_up, tmem_slot;
@@ -182,8 +189,10 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 
   if (tid == 0) {
     for (unsigned s = 0; s < stages; ++s) {
-      tc::mbar_init(&full_bar[s], 1);
-      tc::mbar_init(&empty_bar[s], 1);
+      tc::mbar_init(&k_full[s], 1);
+      tc::mbar_init(&k_empty[s], 1);
+      tc::mbar_init(&v_full[s], 1);
+      tc::mbar_init(&v_empty[s], 1);
     }
     for (unsigned s = 0; s < 2; ++s) {
       tc::mbar_init(&q_full[s], 32);
@@ -279,6 +288,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 
   auto give_up = [&] { *(volatile unsigned*)&gave_up = 1; };
   auto await = [&](unsigned long long* bar, unsigned parity, unsigned code) {
+    if (is_done(bar, parity)) return;
     if (!*(volatile unsigned*)&gave_up && !tc::mbar_wait(bar, parity, batch.status, code)) give_up();
   };
   // f(item, first key tile, last key tile + 1, number of the item's first unit, sequence)
@@ -315,29 +325,39 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
-  if (warp == 9) {
-    // ---- loading warp: a lane per piece (64-column block, page or part of one) of a tile; keys run ahead of values ----
-    const unsigned run = min(batch.page, kKeys), pieces = kKeys / run;
+  if (warp == 9 || warp == 10) {
+    // ---- a warp each for keys and values: a lane per piece (64-column block, page or part of one) of a tile ----
+    const bool values = warp == 10;
+    const unsigned shift = 31 - __clz(batch.page), run = min(batch.page, kKeys), pieces = kKeys / run;
     const unsigned block = (lane / pieces) % kBlocks, piece = lane % pieces;
     const bool live = lane < kBlocks * pieces;
+    const unsigned page_bytes = kv_heads * kBlocks * batch.page * 128, slots = ring + (values ? stages * kSlotBytes : 0u);
+    unsigned long long* const full = values ? v_full : k_full;
+    unsigned long long* const empty = values ? v_empty : k_empty;
     unsigned s = 0, phase = 1;
     walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned seq) {
       const int* const pages_of = kPrefix ? prefix_table : batch.table + size_t(seq) * batch.width;
-      auto bring = [&](unsigned t, bool values) {
-        const unsigned token = it.seen.tile(t) * kKeys + piece * run;
-        unsigned count = 0;
-        const bf16* from_page = nullptr;
-        if (live && token < it.seen.end && (token < it.seen.sink_end || token + run > it.seen.start)) {
-          const unsigned page_id = unsigned(*(pages_of + token / batch.page));
-          if (page_id < batch.pages) {
-            count = min(run, it.seen.end - token);
-            from_page = (values ? v_pool : k_pool) + (block_offset(page_id, kv_heads, it.head, kBlocks, block, batch.page) + token % batch.page) * 64;
-          } else {
-            report(batch.status, kBadPage);
-          }
+      const unsigned char* const pool = reinterpret_cast<const unsigned char*>(values ? v_pool : k_pool) + size_t((it.head * kBlocks + block) * batch.page) * 128;
+      auto token_of = [&](unsigned t) { return it.seen.tile(t) * kKeys + piece * run; };
+      auto tokens_of = [&](unsigned t) {      // that this lane brings in
+        const unsigned token = token_of(t);
+        return live && token < it.seen.end && (token < it.seen.sink_end || token + run > it.seen.start) ? min(run, it.seen.end - token) : 0u;
+      };
+      unsigned count = tokens_of(begin), page_id = count ? unsigned(pages_of[token_of(begin) >> shift]) : 0u;
+#pragma unroll 1
+      for (unsigned t = begin; t < end; ++t) {
+        if (page_id >= batch.pages) {
+          report(batch.status, kBadPage);
+          count = 0;
         }
-        const unsigned slot = ring + s * kSlotBytes, all = __reduce_add_sync(0xffffffffu, count * 128);
-        if (lane == 0) await(&empty_bar[s], phase, tc::kTimeoutEmpty | s);
+        const unsigned char* const from_page = pool + size_t(page_id) * page_bytes + (token_of(t) & (batch.page - 1)) * 128;
+        const unsigned slot = slots + s * kSlotBytes, all = __reduce_add_sync(0xffffffffu, count * 128);
+        unsigned next_count = 0, next_page = 0;      // the page of the tile behind it, while this one's slot is awaited
+        if (t + 1 < end) {
+          next_count = tokens_of(t + 1);
+          if (next_count) next_page = unsigned(pages_of[token_of(t + 1) >> shift]);
+        }
+        if (lane == 0) await(&empty[s], phase, tc::kTimeoutEmpty | s);
         __syncwarp();
         if (values && all < kSlotBytes) {      // zero what is not copied
           for (unsigned p = 0; p < pieces; ++p) {
@@ -351,23 +371,19 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
           tc::fence_async_shared();
           __syncwarp();
         }
-        if (lane == 0) tc::expect_bytes(&full_bar[s], all);
+        if (lane == 0) tc::expect_bytes(&full[s], all);
         __syncwarp();
-        if (count) tc::bulk_copy(slot + block * kBlockBytes + piece * run * 128, from_page, count * 128, &full_bar[s]);
+        if (count) tc::bulk_copy(slot + block * kBlockBytes + piece * run * 128, from_page, count * 128, &full[s]);
+        count = next_count;
+        page_id = next_page;
         if (++s == stages) { s = 0; phase ^= 1; }
-      };
-      const unsigned n = end - begin, lead = min(n, it.rows <= kStreamRows ? 2u : 1u);
-      for (unsigned j = 0; j < lead; ++j) bring(begin + j, false);
-      for (unsigned j = 0; j < n; ++j) {
-        bring(begin + j, true);
-        if (j + lead < n) bring(begin + j + lead, false);
       }
     });
   } else if (warp == 8) {
     // ---- one thread issues the products ----
     if (elect_one()) {
       constexpr unsigned kScores = instruction(kKeys, false), kOutputs = instruction(kDim, true);
-      unsigned s = 0, phase = 0, q_phases = 0, p_phases = 0, o_phases = 3;       // a bit per stream
+      unsigned ks = 0, k_phase = 0, vs = 0, v_phase = 0, q_phases = 0, p_phases = 0, o_phases = 3;       // the last three: a bit per stream
       auto flips = [&](unsigned long long* bars, unsigned& phases, unsigned stream, unsigned code) {
         await(&bars[stream], (phases >> stream) & 1, tc::kTimeoutAccum | code | stream);
         phases ^= 1u << stream;
@@ -381,16 +397,15 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
                          kScores, k != 0);
         tc::tc_commit(&s_full[stream]);
       };
-      auto arrived = [&] {      // the next slot of the ring has landed: its number
-        await(&full_bar[s], phase, tc::kTimeoutFull | s);
-        tc::tc_fence_after();
+      auto arrived = [&](unsigned long long* bars, unsigned& s, unsigned& phase) {      // the next tile has landed: its slot
+        await(&bars[s], phase, tc::kTimeoutFull | s);
         const unsigned slot = s;
         if (++s == stages) { s = 0; phase ^= 1; }
         return slot;
       };
       // P V of a stream's tile: the first half of the keys while the weights of the second half are still being formed
       auto outputs = [&](unsigned stream, unsigned slot, bool first) {
-        const unsigned long long b = mn_descriptor(ring + slot * kSlotBytes, kBlockBytes);
+        const unsigned long long b = mn_descriptor(ring + (stages + slot) * kSlotBytes, kBlockBytes);
         const unsigned d = tmem + kOutColumn + stream * 128, a = tmem + stream * kKeys;
         if (first) flips(o_empty, o_phases, stream, 0x80);
         await(&p_half[stream], (p_phases >> stream) & 1, tc::kTimeoutAccum | 0x30 | stream);
@@ -413,18 +428,19 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
           for (unsigned half = 0; half < (shared_rows ? 1u : 2u); ++half) {
             const unsigned stream = shared_rows ? (i >= lead ? (i - lead) & 1 : i) : half, area = shared_rows ? 0u : stream;
             const bool last_use = shared_rows || half == 1;
+            if (i >= lead && half == 0) values = arrived(v_full, vs, v_phase);
+            if (i < n && half == 0) keys = arrived(k_full, ks, k_phase);
             if (i >= lead) {
               const unsigned j = i - lead;
-              if (half == 0) values = arrived();
               outputs(stream, values, j < lead);
-              if (last_use) tc::tc_commit(&empty_bar[values]);
+              if (last_use) tc::tc_commit(&v_empty[values]);
               if (j + lead >= n) tc::tc_commit(&o_full[stream]);
             }
             if (i < n) {
-              if (half == 0) keys = arrived();
               if (i == 0) flips(q_full, q_phases, area, 0x10);
+              tc::tc_fence_after();
               scores(stream, area, keys);
-              if (last_use) tc::tc_commit(&empty_bar[keys]);
+              if (last_use) tc::tc_commit(&k_empty[keys]);
               if (i == n - 1) tc::tc_commit(&q_empty[area]);
             }
           }
@@ -433,36 +449,41 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     }
     __syncwarp();
   } else {
-    // ---- a warp per stream brings the queries in (zero past the item's rows), as soon as the item before has formed its last scores ----
-    const unsigned stream = warp - 10;
+    // ---- a warp brings the queries in (zero past the item's rows), as soon as the item before has formed its last scores ----
     constexpr unsigned kChunks = kDim / 8, kStep = 32 / kChunks;      // 16-byte chunks of a row, rows that the warp copies at a time
-    const unsigned c = lane % kChunks, q_area = base + stream * kQBytes + (c / 8) * (kStreamRows * 128);
-    unsigned phase = 1;
+    const unsigned c = lane % kChunks, lane_row = lane / kChunks, token_step = kStep / group, sub_step = kStep % group;
+    const size_t ahead = (size_t(token_step) * q_stride + sub_step * kDim) * 2, wraps = (size_t(q_stride) - group * kDim) * 2;
+    unsigned phases = 3;
     walk([&](const Item& it, unsigned, unsigned, unsigned, unsigned) {
-      const bool shared_rows = it.rows <= kStreamRows;
-      if (shared_rows && stream == 1) return;
-      const unsigned rows_before = stream * kStreamRows, live = min(it.rows - rows_before, kStreamRows);
-      await(&q_empty[stream], phase, tc::kTimeoutAccum | 0x50 | stream);
-      phase ^= 1;
-      __syncwarp();
-      const unsigned first = it.row0 + rows_before + lane / kChunks, token_step = kStep / group, sub_step = kStep % group;
-      unsigned token = first / group, sub = first % group;
-#pragma unroll 4
-      for (unsigned row = lane / kChunks; row < kStreamRows; row += kStep) {
-        const bool held = row < live;
-        const bf16* from_row = q + (held ? size_t(it.row + token) * q_stride + (it.head * group + sub) * kDim : 0) + c * 8;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_area + row * 128 + (((c & 7) ^ (row & 7)) << 4)), "l"(from_row),
-                     "r"(held ? 16u : 0u) : "memory");
-        token += token_step;
-        sub += sub_step;
-        if (sub >= group) {
-          sub -= group;
-          ++token;
+#pragma unroll 1
+      for (unsigned stream = 0; stream < (it.rows <= kStreamRows ? 1u : 2u); ++stream) {
+        const unsigned rows_before = stream * kStreamRows, live = min(it.rows - rows_before, kStreamRows);
+        const unsigned q_area = base + stream * kQBytes + (c / 8) * (kStreamRows * 128) + lane_row * 128;
+        const unsigned first = it.row0 + rows_before + lane_row, token = first / group;
+        unsigned sub = first - token * group;
+        const unsigned char* from_row = reinterpret_cast<const unsigned char*>(q + size_t(it.row + token) * q_stride + (it.head * group + sub) * kDim + c * 8);
+        await(&q_empty[stream], (phases >> stream) & 1, tc::kTimeoutAccum | 0x50 | stream);
+        phases ^= 1u << stream;
+        __syncwarp();
+#pragma unroll 1
+        for (unsigned row = 0; row < kStreamRows; row += 8) {
+#pragma unroll
+          for (unsigned i = 0; i < 8; i += kStep) {      // a row in front of the item's end is read, one behind it is zero
+            const bool held = row + i + lane_row < live;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_area + (row + i) * 128 + (((c & 7) ^ (i + lane_row)) << 4)),
+                         "l"(held ? from_row : reinterpret_cast<const unsigned char*>(q)), "r"(held ? 16u : 0u) : "memory");
+            from_row += ahead;
+            sub += sub_step;
+            if (sub >= group) {
+              sub -= group;
+              from_row += wraps;
+            }
+          }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        tc::fence_async_shared();
+        tc::mbar_arrive(&q_full[stream]);
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      tc::fence_async_shared();
-      tc::mbar_arrive(&q_full[stream]);
     });
   }
   } else {
@@ -471,7 +492,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     const unsigned stream = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;       // row of the stream
     const unsigned lanes = (quarter * 32u) << 16;
     const unsigned score_at = tmem + stream * kKeys + lanes, out_at = tmem + kOutColumn + stream * 128 + lanes;
-    unsigned char* const staged = base_ptr + 2 * kQBytes + stages * kSlotBytes + warp * (32 * kStagePitch);
+    unsigned char* const staged = base_ptr + 2 * kQBytes + 2 * stages * kSlotBytes + warp * (32 * kStagePitch);
     unsigned s_phase = 0, o_phases = 0, shared_items = 0;
     auto outputs_done = [&](unsigned of_stream) {
       await(&o_full[of_stream], (o_phases >> of_stream) & 1, tc::kTimeoutAccum | 0x40 | of_stream);
@@ -700,7 +721,7 @@ __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned s
 
 }  // namespace many
 
-// grid: one CTA an SM (or fewer), block = 384, dynamic shared memory = 512 * head_dim (Q) + stages * 256 * head_dim + 20480 (staging) + 1024.
+// grid: one CTA an SM (or fewer), block = 384, dynamic shared memory = 512 * head_dim (Q) + stages * 512 * head_dim (keys, values) + 20480 (staging) + 1024.
 // own_only: the rows' own sequences' part of prefix attention, left in own_sums and own_ends instead of o.
 #define AGI_PAGED_MANY(NAME, HD16, PREFIX)                                                                                              \
   extern "C" __global__ void __launch_bounds__(many::kThreads, 1)                                                                       \

@@ -529,8 +529,8 @@ def paged_many_tiling(cache: PagedCache, blocks: int, tokens: int) -> dict[str, 
     units = blocks * cache.kv_heads * ceil_div(tokens, PAGED_MANY_KEYS)
     grid = min(SM_COUNT, ceil_div(units, PAGED_MANY_LEAST))
     rest = 512 * d + 20480 + 1024          # queries, staging of outputs, alignment
-    stages = min(12, (MAX_DYNAMIC_SHARED - 2048 - rest) // (256 * d))
-    return {"grid": grid, "stages": stages, "least": PAGED_MANY_LEAST, "shared_bytes": rest + stages * 256 * d,
+    stages = min(6, (MAX_DYNAMIC_SHARED - 2048 - rest) // (512 * d))
+    return {"grid": grid, "stages": stages, "least": PAGED_MANY_LEAST, "shared_bytes": rest + stages * 512 * d,
             "scratch_bytes": grid * 2 * (PAGED_MANY_ROWS * d + 2 * PAGED_MANY_ROWS) * 4}
 
 
