@@ -8,8 +8,10 @@
 //
 // A CTA: one loading warp that brings tiles in by bulk copies, a copy per page (or the part of it in the tile) and 64-column
 // block, into a ring; four warps that share a tile's keys, 16 each, with maximum, sum and outputs of their own until the item ends.
-// The rows of the query heads that share a key head are the rows of one mma.sync tile (m16n8k16; twice that with kM = 2).  Keys
-// and values lie in shared memory as they lie in the pool, swizzled, so ldmatrix reads them without bank conflicts.
+// The rows of the query heads that share a key head are columns of one, two or four mma.sync tiles (m16n8k16) with the keys as rows:
+// S^T = K Q^T, O^T += V^T P^T.  With the rows as rows, seven or eight of them would pay for sixteen, and these products (30 clocks of
+// a scheduler's tensor pipe each) took longer than the bytes.  Keys and values lie in shared memory as they lie in the pool,
+// swizzled, so ldmatrix reads them without bank conflicts.
 //
 // A value behind the sequence's end is whatever the page held before, NaN perhaps, and weight zero does not make it zero: such
 // values are masked as they are read.
@@ -24,7 +26,7 @@ namespace few {
 using namespace paged;
 
 constexpr unsigned kKeys = 64, kConsumers = 128, kThreads = 160;
-constexpr unsigned kMergeColumns = 32;      // columns of the outputs that the four warps exchange at a time
+constexpr float kSlack = 8.f;               // log2 of how far scores may exceed the maximum that weights are relative to
 
 // How many units one sequence is: its key heads x row blocks x key tiles.
 struct Items {
@@ -52,21 +54,69 @@ struct Scratch {
   __device__ __forceinline__ float* end(unsigned cta, unsigned slot, unsigned row) const { return ends + (size_t(cta * 2 + slot) * kRows + row) * 2; }
 };
 
-template <int HD16, int kM>
+// The run of a CTA in the line of units, found by every warp for itself, a lane per sequence: no barrier, one trip to memory for up to
+// 32 sequences.
+struct Run {
+  unsigned per, from, to;             // units of a run; this one's
+  unsigned seq, first;                // the sequence that holds unit `from`, and its first unit
+};
+template <unsigned kRows>
+__device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsigned kv_heads, unsigned window, unsigned sinks, unsigned least) {
+  const unsigned lane = threadIdx.x & 31;
+  auto units_of = [&](unsigned i) { return i < batch.sequences ? items_of<kRows>(batch, i, group, kv_heads, window, sinks).units : 0u; };
+  bool ordered = true;
+  unsigned units = 0, total = 0;
+#pragma unroll 2
+  for (unsigned i = lane; i < batch.sequences; i += 32) {
+    ordered = in_order(batch, i) && ordered;
+    units = units_of(i);
+    total += units;
+  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (!__all_sync(0xffffffffu, ordered)) total = 0;
+  Run run;
+  run.per = max((total + gridDim.x - 1) / gridDim.x, least);
+  run.from = min(run.per * blockIdx.x, total);
+  run.to = min(run.from + run.per, total);
+  run.seq = run.first = 0;
+  if (run.from >= run.to) return run;
+  unsigned below = 0;
+#pragma unroll 1
+  for (unsigned base = 0;; base += 32) {
+    if (batch.sequences > 32) units = units_of(base + lane);
+    unsigned up_to = units;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned other = __shfl_up_sync(0xffffffffu, up_to, d);
+      if (lane >= unsigned(d)) up_to += other;
+    }
+    const unsigned holds = __ballot_sync(0xffffffffu, run.from < below + up_to);
+    if (holds) {
+      const unsigned at = __ffs(holds) - 1;
+      run.seq = base + at;
+      run.first = below + __shfl_sync(0xffffffffu, up_to - units, at);
+      return run;
+    }
+    below += __shfl_sync(0xffffffffu, up_to, 31);
+  }
+}
+
+template <int HD16, int kN>
 __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const Batch& batch, float* own_sums,
-                                               float* own_ends, float* scratch, unsigned* counters, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride,
-                                               unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned least,
-                                               unsigned own_only) {
-  constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kRows = 16 * kM;
+                                               float* own_ends, float* scratch, unsigned* counters, unsigned q_heads, unsigned kv_heads,
+                                               unsigned q_stride, unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,
+                                               unsigned least, unsigned own_only) {
+  constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kRows = 8 * kN;
   constexpr unsigned kTileBytes = kKeys * kDim * 2, kStageBytes = 2 * kTileBytes, kBlockBytes = kKeys * 128;
-  constexpr unsigned kMaxStages = 8;
+  constexpr unsigned kMaxStages = 6;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages];
-  __shared__ unsigned run_base[kThreads / 32], run_seq, run_first, gave_up, last_flag;
+  __shared__ unsigned gave_up, last_flag;
   __shared__ float warp_max_of[4][kRows], warp_sum_of[4][kRows];
   const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const unsigned ring = (tc::smem_u32(dynamic_smem) + 1023u) & ~1023u;
-  float* const exchange = reinterpret_cast<float*>(dynamic_smem + (ring - tc::smem_u32(dynamic_smem)) + stages * kStageBytes);   // [4][16][32]
+  const unsigned ring = (tc::smem_u32(dynamic_smem) + 127u) & ~127u;
+  float* const exchange = reinterpret_cast<float*>(dynamic_smem + (ring - tc::smem_u32(dynamic_smem)) + stages * kStageBytes);   // [4][8][head_dim]
+  auto cell = [&](unsigned w, unsigned r8, unsigned d) { return exchange + (w * 8 + r8) * kDim + (d ^ ((r8 >> 1) * 8)); };      // no bank conflicts
   const unsigned group = q_heads / kv_heads;
 
   if (tid == 0) {
@@ -77,47 +127,25 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncthreads();
   grid_dependency_wait();
   if (!(aligned16(q) && aligned16(o) && aligned16(k_pool) && aligned16(v_pool))) {
     if (tid == 0) report(batch.status, kMisaligned);
     return;
   }
-
-  // ---- this CTA's run: units [from, to) of all, and the sequence that holds the first of them ----
-  unsigned mine = 0, total;
-  bool ordered = true;
-  const unsigned share = (batch.sequences + kThreads - 1) / kThreads, seq0 = min(tid * share, batch.sequences), seq1 = min(seq0 + share, batch.sequences);
-#pragma unroll 1
-  for (unsigned i = seq0; i < seq1; ++i) {
-    ordered = in_order(batch, i) && ordered;
-    mine += items_of<kRows>(batch, i, group, kv_heads, window, sinks).units;
-  }
-  unsigned below = sum_before<kThreads>(mine, run_base, &total);
-  const unsigned per = max((total + gridDim.x - 1) / gridDim.x, least), from = min(per * blockIdx.x, total), to = min(from + per, total);
-  if (from < to && from >= below && from < below + mine) {
-#pragma unroll 1
-    for (unsigned i = seq0; i < seq1; ++i) {
-      const unsigned units = items_of<kRows>(batch, i, group, kv_heads, window, sinks).units;
-      if (from < below + units) {
-        run_seq = i;
-        run_first = below;
-        break;
-      }
-      below += units;
-    }
-  }
-  if (__syncthreads_or(!ordered) || from >= to) return;
+  const Run run = run_of<kRows>(batch, group, kv_heads, window, sinks, least);
+  if (run.from >= run.to) return;
 
   // Walks the run item by item: f(sequence, key head, row block, its items, first tile, last tile + 1, first unit of the item).
   auto walk = [&](auto&& f) {
-    unsigned seq = run_seq, first = run_first, unit = from;
+    unsigned seq = run.seq, first = run.first, unit = run.from;
 #pragma unroll 1
-    while (unit < to && seq < batch.sequences) {
+    while (unit < run.to && seq < batch.sequences) {
       const Items it = items_of<kRows>(batch, seq, group, kv_heads, window, sinks);
 #pragma unroll 1
-      while (unit < to && unit < first + it.units) {
+      while (unit < run.to && unit < first + it.units) {
         const unsigned at = (unit - first) / it.seen.count;                // which item of the sequence
-        const unsigned item_first = first + at * it.seen.count, begin = unit - item_first, end = min(it.seen.count, begin + (to - unit));
+        const unsigned item_first = first + at * it.seen.count, begin = unit - item_first, end = min(it.seen.count, begin + (run.to - unit));
         const unsigned head = at / it.blocks;
         f(seq, head, at - head * it.blocks, it, begin, end, item_first);
         unit += end - begin;
@@ -126,41 +154,44 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       ++seq;
     }
   };
+  auto await = [&](unsigned long long* bar, unsigned parity, unsigned code) {
+    if (!*(volatile unsigned*)&gave_up && !tc::mbar_wait(bar, parity, batch.status, code)) *(volatile unsigned*)&gave_up = 1;
+  };
 
   if (warp == 4) {
     // ---- loading warp: a lane per piece (keys or values, 64-column block, page or part of one) of a tile ----
-    const unsigned run = min(batch.page, kKeys), pieces = kKeys / run;
+    const unsigned shift = 31 - __clz(batch.page), run_tokens = min(batch.page, kKeys), pieces = kKeys / run_tokens;
     const bool values = lane >= pieces * kBlocks;
     const unsigned block = (lane / pieces) % kBlocks, piece = lane % pieces;
     const bool live = lane < 2 * kBlocks * pieces;
-    const unsigned to_slot = (values ? kTileBytes : 0u) + block * kBlockBytes + piece * run * 128;
-    const bf16* const pool = values ? v_pool : k_pool;
+    const unsigned to_slot = (values ? kTileBytes : 0u) + block * kBlockBytes + piece * run_tokens * 128;
+    const unsigned page_bytes = kv_heads * kBlocks * batch.page * 128;
     unsigned s = 0, phase = 1;
     walk([&](unsigned seq, unsigned head, unsigned, const Items& it, unsigned begin, unsigned end, unsigned) {
       const int* const pages_of = batch.table + size_t(seq) * batch.width;
-      // tokens of a tile that this lane brings in, and the page that holds them
-      auto tokens_of = [&](unsigned t) {
-        const unsigned token = it.seen.tile(t) * kKeys + piece * run;
-        const bool wanted = live && token < it.seen.end && (token < it.seen.sink_end || token + run > it.seen.start);
-        return wanted ? min(run, it.seen.end - token) : 0u;
+      const unsigned char* const pool = reinterpret_cast<const unsigned char*>(values ? v_pool : k_pool) + size_t((head * kBlocks + block) * batch.page) * 128;
+      auto token_of = [&](unsigned t) { return it.seen.tile(t) * kKeys + piece * run_tokens; };
+      auto tokens_of = [&](unsigned t) {      // that this lane brings in
+        const unsigned token = token_of(t);
+        const bool wanted = live && token < it.seen.end && (token < it.seen.sink_end || token + run_tokens > it.seen.start);
+        return wanted ? min(run_tokens, it.seen.end - token) : 0u;
       };
-      auto page_of = [&](unsigned t) { return unsigned(pages_of[(it.seen.tile(t) * kKeys + piece * run) / batch.page]); };
-      unsigned count = tokens_of(begin), page_id = count ? page_of(begin) : 0u;
+      unsigned count = tokens_of(begin), page_id = count ? unsigned(pages_of[token_of(begin) >> shift]) : 0u;
+#pragma unroll 1
       for (unsigned t = begin; t < end; ++t) {
         if (page_id >= batch.pages) {
           report(batch.status, kBadPage);
           count = 0;
         }
-        const unsigned token = it.seen.tile(t) * kKeys + piece * run;
-        const bf16* const from_page = pool + (block_offset(page_id, kv_heads, head, kBlocks, block, batch.page) + token % batch.page) * 64;
+        const unsigned char* const from_page = pool + size_t(page_id) * page_bytes + (token_of(t) & (batch.page - 1)) * 128;
         const unsigned bytes = count * 128, all = __reduce_add_sync(0xffffffffu, bytes);
-        unsigned next_count = 0, next_page = 0;      // the page numbers of the tile behind it, while this one's slot is awaited
+        unsigned next_count = 0, next_page = 0;      // the page of the tile behind it, while this one's slot is awaited
         if (t + 1 < end) {
           next_count = tokens_of(t + 1);
-          if (next_count) next_page = page_of(t + 1);
+          if (next_count) next_page = unsigned(pages_of[token_of(t + 1) >> shift]);
         }
         if (lane == 0) {
-          if (!*(volatile unsigned*)&gave_up && !tc::mbar_wait(&empty_bar[s], phase, batch.status, tc::kTimeoutEmpty | s)) *(volatile unsigned*)&gave_up = 1;
+          await(&empty_bar[s], phase, tc::kTimeoutEmpty | s);
           tc::expect_bytes(&full_bar[s], all);
         }
         __syncwarp();
@@ -182,92 +213,107 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     const Span& span = it.span;
     const unsigned row0 = block * kRows, rows = min(kRows, span.fresh * group - row0);
     const Rows pairs(row0, group);
-    // Q fragments: row r of the item is token r / group, query head head * group + r % group
-    unsigned qa[kM][HD16][4];
-    int index[kM][2];
+    // Q as the B operand: row r of the item (token, query head) is column r
+    unsigned qb[kN][HD16][2];
+    int index[kN][2];                // of rows 2 t and 2 t + 1, whose scores this thread holds
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
+    for (int j = 0; j < kN; ++j) {
+      unsigned token, sub;
+      pairs.at(j * 8 + g, token, sub);
+      const bool live = j * 8 + g < rows;
+      const unsigned* from_row = reinterpret_cast<const unsigned*>(q + (live ? size_t(span.row + token) * q_stride + (head * group + sub) * kDim : 0)) + t4;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned r = m * 16 + g + h * 8;
-        unsigned token, sub;
-        pairs.at(r, token, sub);
-        const bool live = r < rows;
-        index[m][h] = live ? span.first + int(token) : -1;
-        const bf16* from_row = q + size_t(span.row + token) * q_stride + (head * group + sub) * kDim + 2 * t4;
-#pragma unroll
-        for (int ks = 0; ks < HD16; ++ks) {
-          qa[m][ks][h] = live ? __ldcg(reinterpret_cast<const unsigned*>(from_row + ks * 16)) : 0u;
-          qa[m][ks][h + 2] = live ? __ldcg(reinterpret_cast<const unsigned*>(from_row + ks * 16 + 8)) : 0u;
-        }
+      for (int ks = 0; ks < HD16; ++ks) {
+        qb[j][ks][0] = live ? __ldcg(from_row + ks * 8) : 0u;
+        qb[j][ks][1] = live ? __ldcg(from_row + ks * 8 + 4) : 0u;
       }
-    float top[kM][2], sum[kM][2], out[kM][2 * HD16][4];
 #pragma unroll
-    for (int m = 0; m < kM; ++m) {
-      top[m][0] = top[m][1] = -INFINITY;
-      sum[m][0] = sum[m][1] = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        pairs.at(j * 8 + 2 * t4 + e, token, sub);
+        index[j][e] = j * 8 + 2 * t4 + e < rows ? span.first + int(token) : -1;
+      }
+    }
+    float top[kN][2], sum[kN][2], out[kN][HD16][4];
 #pragma unroll
-      for (int c = 0; c < 2 * HD16; ++c) out[m][c][0] = out[m][c][1] = out[m][c][2] = out[m][c][3] = 0.f;
+    for (int j = 0; j < kN; ++j) {
+      top[j][0] = top[j][1] = -INFINITY;
+      sum[j][0] = sum[j][1] = 0.f;
+#pragma unroll
+      for (int m = 0; m < HD16; ++m) out[j][m][0] = out[j][m][1] = out[j][m][2] = out[j][m][3] = 0.f;
     }
     const int low = span.first + int(pairs.token);                 // the item's first row
+#pragma unroll 1
     for (unsigned t = begin; t < end; ++t) {
-      if (!*(volatile unsigned*)&gave_up && !tc::mbar_wait(&full_bar[s], phase, batch.status, tc::kTimeoutFull | s)) *(volatile unsigned*)&gave_up = 1;
+      await(&full_bar[s], phase, tc::kTimeoutFull | s);
       __syncwarp();
       const unsigned key0 = it.seen.tile(t) * kKeys + warp * 16, slot = ring + s * kStageBytes;
       if (key0 < it.seen.end) {
-        // scores of 16 keys: lanes 0-7 | 8-15 | 16-23 | 24-31 address the 8 x 8 blocks (keys 0-7, chunk c) | (0-7, c + 1) | (8-15, c) | (8-15, c + 1)
-        float score[kM][2][4];
+        // scores, keys as rows: S^T = K Q^T.  Lanes 0-7 | 8-15 | 16-23 | 24-31 address the 8 x 8 blocks (keys 0-7, chunk c) | (8-15, c) |
+        // (0-7, c + 1) | (8-15, c + 1).  Two accumulators a column group: half the chain of dependent products.
+        float score[kN][2][4];
 #pragma unroll
-        for (int m = 0; m < kM; ++m)
+        for (int j = 0; j < kN; ++j)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) score[m][n][0] = score[m][n][1] = score[m][n][2] = score[m][n][3] = 0.f;
-        const unsigned k_row = slot + (warp * 16 + (lane >> 4) * 8 + (lane & 7)) * 128;
+          for (int n = 0; n < 2; ++n) score[j][n][0] = score[j][n][1] = score[j][n][2] = score[j][n][3] = 0.f;
+        const unsigned k_row = slot + (warp * 16 + (lane & 15)) * 128;
 #pragma unroll
         for (int ks = 0; ks < HD16; ++ks) {
-          unsigned b0, b1, b2, b3;
+          unsigned a0, a1, a2, a3;
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(b0), "=r"(b1), "=r"(b2), "=r"(b3)
-                       : "r"(k_row + (ks / 4) * kBlockBytes + ((((ks % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4)));
+                       : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
+                       : "r"(k_row + (ks / 4) * kBlockBytes + ((((ks % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4)));
 #pragma unroll
-          for (int m = 0; m < kM; ++m) {
-            skinny_mma_bf16(score[m][0], qa[m][ks][0], qa[m][ks][1], qa[m][ks][2], qa[m][ks][3], b0, b1);
-            skinny_mma_bf16(score[m][1], qa[m][ks][0], qa[m][ks][1], qa[m][ks][2], qa[m][ks][3], b2, b3);
-          }
+          for (int j = 0; j < kN; ++j) skinny_mma_bf16(score[j][ks & 1], a0, a1, a2, a3, qb[j][ks][0], qb[j][ks][1]);
         }
         // does every row see all of these keys?
-        const bool whole = int(key0) + 15 <= low && key0 + 16 <= it.seen.end && rows == kRows &&
-                           (window == 0 || int(key0) > int(it.span.length) - 1 - int(window));
-        unsigned pa[kM][4];
+        const bool whole = int(key0) + 15 <= low && key0 + 16 <= it.seen.end && rows == kRows && (window == 0 || int(key0) > int(span.length) - 1 - int(window));
+        unsigned pb[kN][2];
+        bool grows = false;
+        float x[kN][4], now[kN][2];
 #pragma unroll
-        for (int m = 0; m < kM; ++m)
+        for (int j = 0; j < kN; ++j) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const unsigned key = key0 + (i >> 1) * 8 + 2 * t4 + (i & 1);
-              const float v = score[m][i >> 1][2 * h + (i & 1)] * scale_log2;
-              x[i] = whole || (key < it.seen.end && sees(index[m][h], key, window, sinks)) ? v : -INFINITY;
-            }
-            float peak = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-            peak = fmaxf(peak, top[m][h]);
-            const float base = peak == -INFINITY ? 0.f : peak, old = exp2_of(top[m][h] - base);
-            top[m][h] = peak;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = exp2_of(x[i] - base);
-            sum[m][h] = sum[m][h] * old + ((x[0] + x[1]) + (x[2] + x[3]));
-#pragma unroll
-            for (int c = 0; c < 2 * HD16; ++c) {
-              out[m][c][2 * h] *= old;
-              out[m][c][2 * h + 1] *= old;
-            }
-            // the scores' layout is that of P as the next product's A operand: a0 | a1 rows g | g + 8 of keys 0-7, a2 | a3 of keys 8-15
-            const bf162 first = __floats2bfloat162_rn(x[0], x[1]), second = __floats2bfloat162_rn(x[2], x[3]);
-            pa[m][h] = *reinterpret_cast<const unsigned*>(&first);
-            pa[m][h + 2] = *reinterpret_cast<const unsigned*>(&second);
+          for (int i = 0; i < 4; ++i) {       // key g (+ 8), row 2 t (+ 1)
+            x[j][i] = (score[j][0][i] + score[j][1][i]) * scale_log2;
+            const unsigned key = key0 + g + (i >> 1) * 8;
+            if (!whole && !(key < it.seen.end && sees(index[j][i & 1], key, window, sinks))) x[j][i] = -INFINITY;
           }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float peak = fmaxf(x[j][e], x[j][e + 2]);
+            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 4));
+            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 8));
+            peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 16));
+            now[j][e] = peak;
+            grows = grows || peak > top[j][e] + kSlack;
+          }
+        }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+          for (int j = 0; j < kN; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float next = fmaxf(top[j][e], now[j][e]), old = next == -INFINITY ? 1.f : exp2_of(top[j][e] - next);
+              top[j][e] = next;
+              sum[j][e] *= old;
+#pragma unroll
+              for (int m = 0; m < HD16; ++m) {
+                out[j][m][e] *= old;
+                out[j][m][e + 2] *= old;
+              }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][i] = exp2_of(x[j][i] - (top[j][i & 1] == -INFINITY ? 0.f : top[j][i & 1]));
+          sum[j][0] += x[j][0] + x[j][2];
+          sum[j][1] += x[j][1] + x[j][3];
+          const bf162 first = __floats2bfloat162_rn(x[j][0], x[j][1]), second = __floats2bfloat162_rn(x[j][2], x[j][3]);
+          // keys as rows -> keys as columns: P^T as the B operand of O^T += V^T P^T
+          asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[j][0]) : "r"(*reinterpret_cast<const unsigned*>(&first)));
+          asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[j][1]) : "r"(*reinterpret_cast<const unsigned*>(&second)));
+        }
         // values: keys 2 t, 2 t + 1 (and + 8) of a column; those that no row of the sequence sees are taken as zero
         unsigned keep[2];
 #pragma unroll
@@ -276,22 +322,19 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
           auto held = [&](unsigned j) { return j < it.seen.end && (j >= it.seen.start || j < it.seen.sink_end); };
           keep[i] = (held(key) ? 0xffffu : 0u) | (held(key + 1) ? 0xffff0000u : 0u);
         }
-        const unsigned v_row = slot + kTileBytes + (warp * 16 + (lane & 15)) * 128;
+        const unsigned v_row = slot + kTileBytes + (warp * 16 + (lane >> 4) * 8 + (lane & 7)) * 128;
 #pragma unroll
-        for (int c = 0; c < HD16; ++c) {
-          unsigned b0, b1, b2, b3;
+        for (int m = 0; m < HD16; ++m) {
+          unsigned a0, a1, a2, a3;
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(b0), "=r"(b1), "=r"(b2), "=r"(b3)
-                       : "r"(v_row + (c / 4) * kBlockBytes + ((((c % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4)));
-          b0 &= keep[0];
-          b1 &= keep[1];
-          b2 &= keep[0];
-          b3 &= keep[1];
+                       : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
+                       : "r"(v_row + (m / 4) * kBlockBytes + ((((m % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4)));
+          a0 &= keep[0];
+          a1 &= keep[0];
+          a2 &= keep[1];
+          a3 &= keep[1];
 #pragma unroll
-          for (int m = 0; m < kM; ++m) {
-            skinny_mma_bf16(out[m][2 * c], pa[m][0], pa[m][1], pa[m][2], pa[m][3], b0, b1);
-            skinny_mma_bf16(out[m][2 * c + 1], pa[m][0], pa[m][1], pa[m][2], pa[m][3], b2, b3);
-          }
+          for (int j = 0; j < kN; ++j) skinny_mma_bf16(out[j][m], a0, a1, a2, a3, pb[j][0], pb[j][1]);
         }
       }
       __syncwarp();
@@ -299,7 +342,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       if (++s == stages) { s = 0; phase ^= 1; }
     }
 
-    // ---- the four warps' shares meet: maxima and weights first, then the outputs, 32 columns at a time ----
+    // ---- the four warps' shares meet, eight rows at a time ----
     const bool whole_item = begin == 0 && end == it.seen.count;
     const unsigned slot = begin > 0 ? 0u : 1u;
     // four columns of a row, divided, or as they are with the row's maximum and weight
@@ -318,70 +361,75 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       *reinterpret_cast<uint2*>(o + size_t(row) * o_stride + q_head * kDim + c) = *reinterpret_cast<const uint2*>(pair);
     };
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
+    for (int j = 0; j < kN; ++j) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
-        sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
-        if (t4 == 0) {
-          warp_max_of[warp][m * 16 + g + h * 8] = top[m][h];
-          warp_sum_of[warp][m * 16 + g + h * 8] = sum[m][h];
+      for (int e = 0; e < 2; ++e) {
+        float all = sum[j][e];
+        all += __shfl_xor_sync(0xffffffffu, all, 4);
+        all += __shfl_xor_sync(0xffffffffu, all, 8);
+        all += __shfl_xor_sync(0xffffffffu, all, 16);
+        if (g == 0) {
+          warp_max_of[warp][j * 8 + 2 * t4 + e] = top[j][e];
+          warp_sum_of[warp][j * 8 + 2 * t4 + e] = all;
         }
       }
-    consumers_sync();
-    const unsigned r16 = tid / 8, c4 = (tid % 8) * 4;      // a thread per row and four of 32 columns
 #pragma unroll
-    for (int m = 0; m < kM; ++m) {
-      const unsigned r = m * 16 + r16;
-      const float peak = fmaxf(fmaxf(warp_max_of[0][r], warp_max_of[1][r]), fmaxf(warp_max_of[2][r], warp_max_of[3][r]));
-      float by[4], weight = 0.f;
+      for (int m = 0; m < HD16; ++m)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        by[w] = peak == -INFINITY ? 0.f : exp2_of(warp_max_of[w][r] - peak);
-        weight += warp_sum_of[w][r] * by[w];
-      }
-#pragma unroll
-      for (unsigned c0 = 0; c0 < kDim; c0 += kMergeColumns) {
-#pragma unroll
-        for (unsigned n = 0; n < kMergeColumns / 8; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<float2*>(exchange + (warp * 16 + g + h * 8) * kMergeColumns + n * 8 + 2 * t4) =
-                make_float2(out[m][c0 / 8 + n][2 * h], out[m][c0 / 8 + n][2 * h + 1]);
-        consumers_sync();
+        for (int i = 0; i < 4; ++i) *cell(warp, 2 * t4 + (i & 1), m * 16 + g + (i >> 1) * 8) = out[j][m][i];
+      consumers_sync();
+#pragma unroll 1
+      for (unsigned i = tid; i < 8 * (kDim / 4); i += kConsumers) {
+        const unsigned r8 = i / (kDim / 4), c = (i % (kDim / 4)) * 4, r = j * 8 + r8;
+        const float peak = fmaxf(fmaxf(warp_max_of[0][r], warp_max_of[1][r]), fmaxf(warp_max_of[2][r], warp_max_of[3][r]));
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float weight = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float4 part = *reinterpret_cast<const float4*>(exchange + (w * 16 + r16) * kMergeColumns + c4);
-          v.x += part.x * by[w]; v.y += part.y * by[w]; v.z += part.z * by[w]; v.w += part.w * by[w];
+          const float by = peak == -INFINITY ? 0.f : exp2_of(warp_max_of[w][r] - peak);
+          const float4 part = *reinterpret_cast<const float4*>(cell(w, r8, c));
+          v.x += part.x * by; v.y += part.y * by; v.z += part.z * by; v.w += part.w * by;
+          weight += warp_sum_of[w][r] * by;
         }
         if (r < rows) {
           if (whole_item) {
-            leave(r, c0 + c4, v, peak, weight);
+            leave(r, c, v, peak, weight);
           } else {
-            *reinterpret_cast<float4*>(parts.sum(blockIdx.x, slot, r) + c0 + c4) = v;
-            if (c0 == 0 && c4 == 0) *reinterpret_cast<float2*>(parts.end(blockIdx.x, slot, r)) = make_float2(peak, weight);
+            *reinterpret_cast<float4*>(parts.sum(blockIdx.x, slot, r) + c) = v;
+            if (c == 0) *reinterpret_cast<float2*>(parts.end(blockIdx.x, slot, r)) = make_float2(peak, weight);
           }
         }
-        consumers_sync();
       }
+      consumers_sync();
     }
     if (whole_item) return;
 
     // ---- an item of several CTAs: the last of them to arrive adds the parts, in order ----
-    const unsigned first_cta = item_first / per, last_cta = (item_first + it.seen.count - 1) / per;
-    __threadfence();
-    consumers_sync();
-    if (tid == 0) last_flag = atomicAdd(&counters[first_cta], 1u) == last_cta - first_cta;
+    const unsigned first_cta = item_first / run.per, last_cta = (item_first + it.seen.count - 1) / run.per;
+    if (tid == 0) {
+      __threadfence();
+      last_flag = atomicAdd(&counters[first_cta], 1u) == last_cta - first_cta;
+      __threadfence();
+    }
     consumers_sync();
     if (!last_flag) return;
-    __threadfence();
+    {   // every row's maximum: kConsumers / kRows threads a row look at the parts side by side
+      const unsigned r = tid % kRows;
+      float peak = -INFINITY;
+#pragma unroll 4
+      for (unsigned a = first_cta + tid / kRows; a <= last_cta; a += kConsumers / kRows)
+        if (r < rows) peak = fmaxf(peak, __ldcg(parts.end(a, a == first_cta, r)));
+      exchange[tid] = peak;
+      consumers_sync();
+    }
+#pragma unroll 1
     for (unsigned i = tid; i < rows * (kDim / 4); i += kConsumers) {
       const unsigned r = i / (kDim / 4), c = (i % (kDim / 4)) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       float peak = -INFINITY, weight = 0.f;
-      for (unsigned a = first_cta; a <= last_cta; ++a) peak = fmaxf(peak, __ldcg(parts.end(a, a == first_cta, r)));
-#pragma unroll 4
+#pragma unroll
+      for (unsigned k = 0; k < kConsumers / kRows; ++k) peak = fmaxf(peak, exchange[k * kRows + r]);
+#pragma unroll 8
       for (unsigned a = first_cta; a <= last_cta; ++a) {
         const float2 end_of = __ldcg(reinterpret_cast<const float2*>(parts.end(a, a == first_cta, r)));
         const float4 part = __ldcg(reinterpret_cast<const float4*>(parts.sum(a, a == first_cta, r) + c));
@@ -397,21 +445,23 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 
 }  // namespace few
 
-// grid: any number of CTAs that `scratch` has room for, block = 160, dynamic shared memory = stages * 256 * head_dim + 8192 + 1024.
+// grid: any number of CTAs that `scratch` has room for, block = 160, dynamic shared memory = stages * 256 * head_dim + 128 * head_dim + 128.
 // least: units that a CTA takes at the least; counters: one word per CTA, zero between launches.  own_only: sums, maxima and
 // weights to own_sums [rows][q_heads][head_dim] and own_ends [rows][q_heads][2] instead of o (prefix attention adds the prefix to them).
-#define AGI_PAGED_FEW(NAME, HD16, M, PER_SM)                                                                                          \
+#define AGI_PAGED_FEW(NAME, HD16, N, PER_SM)                                                                                          \
   extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM)                                                                 \
   NAME(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const int* starts, const int* lengths, const int* table,       \
        float* own_sums, float* own_ends, float* scratch, unsigned* counters, unsigned* status, unsigned rows, unsigned sequences,     \
        unsigned pages, unsigned page, unsigned width, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride,      \
        unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned least, unsigned own_only) {                       \
     const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                    \
-    few::attention_body<HD16, M>(q, o, k_pool, v_pool, batch, own_sums, own_ends, scratch, counters, q_heads, kv_heads, q_stride,     \
+    few::attention_body<HD16, N>(q, o, k_pool, v_pool, batch, own_sums, own_ends, scratch, counters, q_heads, kv_heads, q_stride,     \
                                  o_stride, window, sinks, scale_log2, stages, least, own_only);                                       \
   }
-AGI_PAGED_FEW(agi_paged_few_bf16_d64_m1, 4, 1, 2)
-AGI_PAGED_FEW(agi_paged_few_bf16_d64_m2, 4, 2, 1)
-AGI_PAGED_FEW(agi_paged_few_bf16_d128_m1, 8, 1, 2)
-AGI_PAGED_FEW(agi_paged_few_bf16_d128_m2, 8, 2, 1)
+AGI_PAGED_FEW(agi_paged_few_bf16_d64_r8, 4, 1, 2)
+AGI_PAGED_FEW(agi_paged_few_bf16_d64_r16, 4, 2, 2)
+AGI_PAGED_FEW(agi_paged_few_bf16_d64_r32, 4, 4, 2)
+AGI_PAGED_FEW(agi_paged_few_bf16_d128_r8, 8, 1, 2)
+AGI_PAGED_FEW(agi_paged_few_bf16_d128_r16, 8, 2, 2)
+AGI_PAGED_FEW(agi_paged_few_bf16_d128_r32, 8, 4, 1)
 #undef AGI_PAGED_FEW

@@ -505,17 +505,16 @@ PAGED_FEW_LEAST = 2
 
 
 def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> dict[str, int]:
-    """Launch geometry of ``agi_paged_few_bf16_*``: 16-row MMA tiles of an item ``m``, CTAs, ring depth.  The CTAs share out all
-    key tiles of the batch evenly, so there are as many as the SMs hold, or as the tables have room for tiles."""
-    m = 1 if longest * group <= 16 else 2
-    per_sm = 3 - m
-    stage = 4 * PAGED_FEW_KEYS * cache.head_dim
-    exchange = 4 * 16 * 32 * 4
-    stages = min(8, ((227 - per_sm) * 1024 // per_sm - 2048 - exchange) // stage)
-    blocks = min(cache.sequences, rows) * ceil_div(longest * group, 16 * m) * cache.kv_heads
+    """Launch geometry of ``agi_paged_few_bf16_*``: rows of an item, CTAs, ring depth.  The CTAs share out all key tiles of the
+    batch evenly, so there are as many as the SMs hold, or as the tables have room for tiles."""
+    item = next(r for r in (8, 16, 32) if r >= longest * group or r == 32)
+    per_sm = 1 if item == 32 and cache.head_dim == 128 else 2
+    stage, exchange = 4 * PAGED_FEW_KEYS * cache.head_dim, 128 * cache.head_dim
+    stages = min(6, ((228 - per_sm) * 1024 // per_sm - 1024 - exchange) // stage)      # 1 KB of static shared memory
+    blocks = min(cache.sequences, rows) * ceil_div(longest * group, item) * cache.kv_heads
     tiles = blocks * ceil_div(cache.pages_per_sequence * cache.page, PAGED_FEW_KEYS)
-    return {"m": m, "grid": min(SM_COUNT * per_sm, ceil_div(tiles, PAGED_FEW_LEAST)), "stages": stages, "least": PAGED_FEW_LEAST,
-            "shared_bytes": stages * stage + exchange + 1024}
+    return {"rows": item, "grid": min(SM_COUNT * per_sm, ceil_div(tiles, PAGED_FEW_LEAST)), "stages": stages, "least": PAGED_FEW_LEAST,
+            "shared_bytes": stages * stage + exchange + 128}
 
 
 PAGED_MANY_ROWS, PAGED_MANY_KEYS = 256, 128
@@ -952,10 +951,10 @@ class RecipeBuilder:
         if longest * group <= PAGED_FEW_ROWS:
             t = paged_few_tiling(cache, rows, longest, group)
             scratch, counters = self._tc_scratch
-            self.launch(f"agi_paged_few_bf16_d{d}_m{t['m']}", (t["grid"], 1, 1), (160, 1, 1),
+            self.launch(f"agi_paged_few_bf16_d{d}_r{t['rows']}", (t["grid"], 1, 1), (160, 1, 1),
                         [q, o, cache.k, cache.v, *batch, *own, scratch, counters, Arena(STATUS_WORD), *shape, *heads, U32(t["stages"]),
                          U32(t["least"]), U32(1 if prefix else 0)],
-                        shared_bytes=t["shared_bytes"], op=op, algorithm=f"mma_key_tiles_m{t['m']}")
+                        shared_bytes=t["shared_bytes"], op=op, algorithm=f"mma_key_tiles_r{t['rows']}")
         else:
             blocks = min(rows * group // PAGED_MANY_ROWS + min(cache.sequences, rows), cache.sequences * ceil_div(longest * group, PAGED_MANY_ROWS))
             many("agi_paged_many_bf16", "agi_paged_join_bf16", blocks, cache.pages_per_sequence * cache.page, (dummy, dummy, 0), 1 if prefix else 0)
