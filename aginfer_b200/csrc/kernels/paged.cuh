@@ -26,19 +26,6 @@ enum Status : unsigned {
 
 __device__ __forceinline__ void report(unsigned* status, unsigned code) { atomicCAS(status, 0u, code); }
 
-// The sequence that holds a row: the number of sequences that end at or before it (`sequences` where none holds it).
-// Called by whole warps.
-__device__ __forceinline__ unsigned sequence_of(const int* starts, unsigned sequences, unsigned row) {
-  unsigned before = 0;
-  for (unsigned i = threadIdx.x & 31; i < sequences; i += 32) before += *(starts + i + 1) <= int(row) ? 1u : 0u;
-  return __reduce_add_sync(0xffffffffu, before);
-}
-
-// The index of a row of sequence `seq` in it; whatever the tensors hold, the difference wraps and does not trap.
-__device__ __forceinline__ int index_of(const int* starts, const int* lengths, unsigned seq, unsigned row) {
-  return int(unsigned(*(lengths + seq)) - (unsigned(*(starts + seq + 1)) - row));
-}
-
 // 2^x, zero for minus infinity; relative error 2^-22.
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
@@ -68,21 +55,24 @@ struct Span {
   int first;
   unsigned length;
 };
-__device__ __forceinline__ Span span_of(const Batch& b, unsigned seq) {
-  const int from = b.starts[seq], to = b.starts[seq + 1], length = b.lengths[seq];
+// What the batch says of a sequence, as it stands in memory.
+struct Claim {
+  int from, to, length;
+};
+__device__ __forceinline__ Claim claim_of(const Batch& b, unsigned seq) { return Claim{b.starts[seq], b.starts[seq + 1], b.lengths[seq]}; }
+__device__ __forceinline__ Span span_of(const Batch& b, const Claim& c) {
   Span s;
-  s.row = unsigned(from);
-  s.fresh = unsigned(to - from);
-  s.length = min(unsigned(max(length, 0)), b.width * b.page);
+  s.row = unsigned(c.from);
+  s.fresh = unsigned(c.to - c.from);
+  s.length = min(unsigned(max(c.length, 0)), b.width * b.page);
   s.first = int(s.length) - int(s.fresh);
   return s;
 }
 // What a launch checks of every sequence before it uses any: rows in order and a length that the table has room for.  Rows out of
 // order leave the whole launch without work, so that rows add up to no more than there are.
-__device__ __forceinline__ bool in_order(const Batch& b, unsigned seq) {
-  const int from = b.starts[seq], to = b.starts[seq + 1];
-  const bool ordered = from >= 0 && to >= from && unsigned(to) <= b.rows;
-  if (!ordered || b.lengths[seq] > int(b.width * b.page)) report(b.status, kBadLength);
+__device__ __forceinline__ bool in_order(const Batch& b, const Claim& c) {
+  const bool ordered = c.from >= 0 && c.to >= c.from && unsigned(c.to) <= b.rows;
+  if (!ordered || c.length > int(b.width * b.page)) report(b.status, kBadLength);
   return ordered;
 }
 
@@ -150,13 +140,12 @@ __device__ __forceinline__ bool sees(int index, unsigned key, unsigned window, u
 }  // namespace paged
 
 // Queries and keys of a step's new tokens turned by their positions (half-split pairs, see rope.cuh), queries written to `q_out`,
-// keys and values to their pages.  Bound by memory: every row is read and written once.  Angles are formed in 64 bits: at
-// position 100000 a product in 32 bits would already be off by more than a bf16 rounding of the result; the sixty-four frequencies
-// are computed once a block and kept for its rows.
-// A block takes rows blockIdx.x, + gridDim.x, ...; a thread turns eight pairs of a head at a time (two 16-byte vectors), and
-// requests them before it computes the angles.
+// keys and values to their pages.  Bound by memory: every row is read and written once.  A block owns a row; its threads request
+// the row's first vectors, then find the row's sequence (a lane per sequence), page and angles while those are on their way, and
+// turn eight pairs of a head at a time.  Angles are formed in 64 bits: at position 100000 a product in 32 bits would already be
+// off by more than a bf16 rounding of the result.
 // s0 says where a position comes from (below).  log2_theta + log2_theta_rest: log2 of theta in two pieces.
-// block = 128.  head_dim 64 or 128, strides multiples of 8.
+// grid = rows, block = 128.  head_dim 64 or 128, strides multiples of 8.
 constexpr unsigned kPositionsFromCache = 0xffffffffu;   // s0: the index in the sequence, plus *offset where has_offset
 constexpr unsigned kPositionsOneAxis = 0xfffffffeu;     // s0: pos[row]; otherwise pos[3][rows] with sections s0, s1, rest
 extern "C" __global__ void __launch_bounds__(128)
@@ -168,8 +157,8 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
                    unsigned has_offset) {
   __shared__ __align__(16) float cosine[64], sine[64];
   grid_dependency_wait();
-  const unsigned half = head_dim / 2, vecs = half / 8, turned = (q_heads + kv_heads) * vecs;
-  const unsigned blocks = head_dim / 64, copied = kv_heads * head_dim / 8;
+  const unsigned half = head_dim / 2, vec_shift = head_dim == 128 ? 3 : 2, turned = (q_heads + kv_heads) << vec_shift;
+  const unsigned blocks = head_dim / 64, copied = kv_heads * blocks * 8, row = blockIdx.x, lane = threadIdx.x & 31;
   k += k_column;
   v += v_column;
   if (!(paged::aligned16(q) && paged::aligned16(k) && paged::aligned16(v) && paged::aligned16(q_out) && paged::aligned16(k_pool) &&
@@ -177,73 +166,114 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
     if (threadIdx.x == 0) paged::report(status, paged::kMisaligned);
     return;
   }
-  const unsigned pair = threadIdx.x;
-  // turns per position of this thread's pair
+  const bf16* const q_row = q + size_t(row) * q_stride;
+  const bf16* const k_row = k + size_t(row) * kv_stride;
+  const bf16* const v_row = v + size_t(row) * kv_stride;
+  auto from_of = [&](unsigned item) {
+    const unsigned head = item >> vec_shift, c = item & ((1u << vec_shift) - 1);
+    return (head < q_heads ? q_row + head * head_dim : k_row + (head - q_heads) * head_dim) + c * 8;
+  };
+  constexpr unsigned kAhead = 2;      // vectors of a thread that do not wait for where the row goes
+  Bf16x8 lo[kAhead], hi[kAhead];
+  uint4 value = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (unsigned u = 0; u < kAhead; ++u)
+    if (threadIdx.x + u * 128 < turned) {
+      lo[u] = *reinterpret_cast<const Bf16x8*>(from_of(threadIdx.x + u * 128));
+      hi[u] = *reinterpret_cast<const Bf16x8*>(from_of(threadIdx.x + u * 128) + half);
+    }
+  if (threadIdx.x < copied) value = *reinterpret_cast<const uint4*>(v_row + threadIdx.x * 8);
+
+  // A position that does not follow from the cache is asked for here too, and turns per position, 1 / (2 pi theta^(pair mod ladder /
+  // ladder)), are computed while all of this is on its way.
+  const unsigned pair = threadIdx.x, first = min(lane, sequences - 1);
+  int from = starts[first], to = starts[first + 1], length = lengths[first], at_position = 0;
+  if (s0 < kPositionsOneAxis && pair < half) at_position = pos[size_t(pair < s0 ? 0u : pair < s0 + s1 ? 1u : 2u) * rows + row];
+  if (s0 == kPositionsOneAxis) at_position = pos[row];
   double frequency = 0.;
   if (pair < half)
     frequency = exp2(-(double(log2_theta) + double(log2_theta_rest)) * (double(pair % ladder) / double(ladder))) * 0.15915494309189534;
-  for (unsigned row = blockIdx.x; row < rows; row += gridDim.x) {
-    const unsigned seq = paged::sequence_of(starts, sequences, row);
-    if (seq >= sequences) continue;      // the same for the whole block
-    const int index = paged::index_of(starts, lengths, seq, row);
-    unsigned page_id = 0;
-    bool stored = index >= 0;
-    if (stored) {
-      if (unsigned(index) / page >= width) {
-        stored = false;
-        if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
-      } else {
-        page_id = unsigned(*(table + size_t(seq) * width + unsigned(index) / page));
-        if (page_id >= pages) {
-          stored = false;
-          if (threadIdx.x == 0) paged::report(status, paged::kBadPage);
-        }
-      }
+
+  // the row's sequence: the first that ends behind it
+  int index = 0;
+  unsigned seq = sequences;
+  for (unsigned base = 0; base < sequences; base += 32) {
+    if (base > 0) {
+      const unsigned i = min(base + lane, sequences - 1);
+      from = starts[i];
+      to = starts[i + 1];
+      length = lengths[i];
     }
-    const unsigned token = unsigned(index) % page;
-    const bf16* const q_row = q + size_t(row) * q_stride;
-    const bf16* const k_row = k + size_t(row) * kv_stride;
-    __syncthreads();      // the angles of the row before are no longer needed
-    if (pair < half) {
-      int at;
-      if (s0 == kPositionsFromCache) at = int(unsigned(index) + (has_offset ? unsigned(*offset) : 0u));
-      else if (s0 == kPositionsOneAxis) at = *(pos + row);
-      else at = *(pos + size_t(pair < s0 ? 0u : pair < s0 + s1 ? 1u : 2u) * rows + row);
-      const double turns = double(at) * frequency;
-      sincospif(2.f * float(turns - rint(turns)), &sine[pair], &cosine[pair]);
-    }
-    __syncthreads();
-    for (unsigned item = threadIdx.x; item < turned; item += 128) {
-      const unsigned head = item / vecs, c = item - head * vecs;
-      const bf16* from = (head < q_heads ? q_row + head * head_dim : k_row + (head - q_heads) * head_dim) + c * 8;
-      float a[8], b[8], x[8], y[8];
-      unpack8(*reinterpret_cast<const Bf16x8*>(from), a);
-      unpack8(*reinterpret_cast<const Bf16x8*>(from + half), b);
+    const unsigned behind = __ballot_sync(0xffffffffu, base + lane < sequences && to > int(row));
+    if (behind == 0) continue;
+    const int at = __ffs(behind) - 1;
+    if (__shfl_sync(0xffffffffu, from, at) <= int(row)) seq = base + at;
+    index = int(unsigned(__shfl_sync(0xffffffffu, length, at)) - (unsigned(__shfl_sync(0xffffffffu, to, at)) - row));
+    break;
+  }
+  if (seq >= sequences) return;      // the same for the whole block
+  unsigned page_id = 0;
+  bool stored = index >= 0;
+  if (stored && unsigned(index) / page >= width) {
+    stored = false;
+    if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
+  }
+  if (stored) page_id = unsigned(table[size_t(seq) * width + unsigned(index) / page]);
+  if (pair < half) {
+    if (s0 == kPositionsFromCache) at_position = int(unsigned(index) + (has_offset ? unsigned(*offset) : 0u));
+    const double turns = double(at_position) * frequency;
+    sincospif(2.f * float(turns - rint(turns)), &sine[pair], &cosine[pair]);
+  }
+  if (stored && page_id >= pages) {
+    stored = false;
+    if (threadIdx.x == 0) paged::report(status, paged::kBadPage);
+  }
+  const unsigned token = unsigned(index) % page;
+  __syncthreads();
+  const unsigned c = threadIdx.x & ((1u << vec_shift) - 1);      // the same pairs in every head that this thread turns
+  float co[8], si[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float co = cosine[c * 8 + j], si = sine[c * 8 + j];
-        x[j] = a[j] * co - b[j] * si;
-        y[j] = b[j] * co + a[j] * si;
-      }
-      if (head < q_heads) {
-        bf16* to = q_out + size_t(row) * out_stride + head * head_dim + c * 8;
-        *reinterpret_cast<Bf16x8*>(to) = pack8(x);
-        *reinterpret_cast<Bf16x8*>(to + half) = pack8(y);
-      } else if (stored) {
-        // chunk c of the head's first half, chunk c + vecs of the whole row: columns of one block (64 wide) or of two
-        const unsigned lo = c, hi = c + vecs;
-        bf16* first = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, lo / 8, page) + token) * 64;
-        bf16* second = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, hi / 8, page) + token) * 64;
-        *reinterpret_cast<Bf16x8*>(first + (((lo & 7) ^ (token & 7)) * 8)) = pack8(x);
-        *reinterpret_cast<Bf16x8*>(second + (((hi & 7) ^ (token & 7)) * 8)) = pack8(y);
-      }
+  for (int j = 0; j < 8; j += 4) {
+    *reinterpret_cast<float4*>(co + j) = *reinterpret_cast<const float4*>(cosine + c * 8 + j);
+    *reinterpret_cast<float4*>(si + j) = *reinterpret_cast<const float4*>(sine + c * 8 + j);
+  }
+  auto turn = [&](unsigned item, const Bf16x8& l, const Bf16x8& h) {
+    const unsigned head = item >> vec_shift;
+    float a[8], b[8], x[8], y[8];
+    unpack8(l, a);
+    unpack8(h, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = a[j] * co[j] - b[j] * si[j];
+      y[j] = b[j] * co[j] + a[j] * si[j];
     }
-    if (stored)
-      for (unsigned item = threadIdx.x; item < copied; item += 128) {
-        const unsigned head = item / (blocks * 8), c = item % (blocks * 8);
-        bf16* to = v_pool + (paged::block_offset(page_id, kv_heads, head, blocks, c / 8, page) + token) * 64;
-        *reinterpret_cast<uint4*>(to + (((c & 7) ^ (token & 7)) * 8)) =
-            *reinterpret_cast<const uint4*>(v + size_t(row) * kv_stride + head * head_dim + c * 8);
-      }
+    if (head < q_heads) {
+      bf16* to = q_out + size_t(row) * out_stride + head * head_dim + c * 8;
+      *reinterpret_cast<Bf16x8*>(to) = pack8(x);
+      *reinterpret_cast<Bf16x8*>(to + half) = pack8(y);
+    } else if (stored) {
+      // chunk c of the head's first half and the same chunk of its second half: of one 64-column block, or of two
+      const unsigned behind = c + (1u << vec_shift);
+      bf16* first = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, c / 8, page) + token) * 64;
+      bf16* second = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, behind / 8, page) + token) * 64;
+      *reinterpret_cast<Bf16x8*>(first + (((c & 7) ^ (token & 7)) * 8)) = pack8(x);
+      *reinterpret_cast<Bf16x8*>(second + (((behind & 7) ^ (token & 7)) * 8)) = pack8(y);
+    }
+  };
+  auto keep = [&](unsigned item, const uint4& from) {
+    const unsigned head = item / (blocks * 8), c = item % (blocks * 8);
+    bf16* to = v_pool + (paged::block_offset(page_id, kv_heads, head, blocks, c / 8, page) + token) * 64;
+    *reinterpret_cast<uint4*>(to + (((c & 7) ^ (token & 7)) * 8)) = from;
+  };
+#pragma unroll
+  for (unsigned u = 0; u < kAhead; ++u)
+    if (threadIdx.x + u * 128 < turned) turn(threadIdx.x + u * 128, lo[u], hi[u]);
+  if (stored && threadIdx.x < copied) keep(threadIdx.x, value);
+#pragma unroll 1
+  for (unsigned item = threadIdx.x + kAhead * 128; item < turned; item += 128)
+    turn(item, *reinterpret_cast<const Bf16x8*>(from_of(item)), *reinterpret_cast<const Bf16x8*>(from_of(item) + half));
+  if (stored) {
+#pragma unroll 1
+    for (unsigned item = threadIdx.x + 128; item < copied; item += 128) keep(item, *reinterpret_cast<const uint4*>(v_row + item * 8));
   }
 }

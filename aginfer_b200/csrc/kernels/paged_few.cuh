@@ -35,9 +35,9 @@ struct Items {
   unsigned blocks, units;             // row blocks of a key head; units of the sequence
 };
 template <unsigned kRows>
-__device__ __forceinline__ Items items_of(const Batch& batch, unsigned seq, unsigned group, unsigned kv_heads, unsigned window, unsigned sinks) {
+__device__ __forceinline__ Items items_of(const Batch& batch, const Claim& claim, unsigned group, unsigned kv_heads, unsigned window, unsigned sinks) {
   Items it;
-  it.span = span_of(batch, seq);
+  it.span = span_of(batch, claim);
   it.seen = visible_of<kKeys>(it.span.first, int(it.span.length) - 1, it.span.length, window, sinks);
   it.blocks = (it.span.fresh * group + kRows - 1) / kRows;
   it.units = it.blocks * kv_heads * it.seen.count;
@@ -59,17 +59,19 @@ struct Scratch {
 struct Run {
   unsigned per, from, to;             // units of a run; this one's
   unsigned seq, first;                // the sequence that holds unit `from`, and its first unit
+  Claim claim;                        // what the batch says of it
 };
 template <unsigned kRows>
 __device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsigned kv_heads, unsigned window, unsigned sinks, unsigned least) {
   const unsigned lane = threadIdx.x & 31;
-  auto units_of = [&](unsigned i) { return i < batch.sequences ? items_of<kRows>(batch, i, group, kv_heads, window, sinks).units : 0u; };
   bool ordered = true;
   unsigned units = 0, total = 0;
+  Claim claim{0, 0, 0};
 #pragma unroll 2
   for (unsigned i = lane; i < batch.sequences; i += 32) {
-    ordered = in_order(batch, i) && ordered;
-    units = units_of(i);
+    claim = claim_of(batch, i);
+    ordered = in_order(batch, claim) && ordered;
+    units = items_of<kRows>(batch, claim, group, kv_heads, window, sinks).units;
     total += units;
   }
   total = __reduce_add_sync(0xffffffffu, total);
@@ -79,11 +81,18 @@ __device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsign
   run.from = min(run.per * blockIdx.x, total);
   run.to = min(run.from + run.per, total);
   run.seq = run.first = 0;
+  run.claim = claim;
   if (run.from >= run.to) return run;
   unsigned below = 0;
 #pragma unroll 1
   for (unsigned base = 0;; base += 32) {
-    if (batch.sequences > 32) units = units_of(base + lane);
+    if (batch.sequences > 32) {
+      units = 0;
+      if (base + lane < batch.sequences) {
+        claim = claim_of(batch, base + lane);
+        units = items_of<kRows>(batch, claim, group, kv_heads, window, sinks).units;
+      }
+    }
     unsigned up_to = units;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -95,6 +104,7 @@ __device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsign
       const unsigned at = __ffs(holds) - 1;
       run.seq = base + at;
       run.first = below + __shfl_sync(0xffffffffu, up_to - units, at);
+      run.claim = Claim{__shfl_sync(0xffffffffu, claim.from, at), __shfl_sync(0xffffffffu, claim.to, at), __shfl_sync(0xffffffffu, claim.length, at)};
       return run;
     }
     below += __shfl_sync(0xffffffffu, up_to, 31);
@@ -139,9 +149,10 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   // Walks the run item by item: f(sequence, key head, row block, its items, first tile, last tile + 1, first unit of the item).
   auto walk = [&](auto&& f) {
     unsigned seq = run.seq, first = run.first, unit = run.from;
+    Claim claim = run.claim;
 #pragma unroll 1
-    while (unit < run.to && seq < batch.sequences) {
-      const Items it = items_of<kRows>(batch, seq, group, kv_heads, window, sinks);
+    while (unit < run.to) {
+      const Items it = items_of<kRows>(batch, claim, group, kv_heads, window, sinks);
 #pragma unroll 1
       while (unit < run.to && unit < first + it.units) {
         const unsigned at = (unit - first) / it.seen.count;                // which item of the sequence
@@ -151,7 +162,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         unit += end - begin;
       }
       first += it.units;
-      ++seq;
+      if (unit < run.to && ++seq < batch.sequences) claim = claim_of(batch, seq);
     }
   };
   auto await = [&](unsigned long long* bar, unsigned parity, unsigned code) {
@@ -413,31 +424,47 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     }
     consumers_sync();
     if (!last_flag) return;
-    {   // every row's maximum: kConsumers / kRows threads a row look at the parts side by side
-      const unsigned r = tid % kRows;
-      float peak = -INFINITY;
-#pragma unroll 4
-      for (unsigned a = first_cta + tid / kRows; a <= last_cta; a += kConsumers / kRows)
-        if (r < rows) peak = fmaxf(peak, __ldcg(parts.end(a, a == first_cta, r)));
-      exchange[tid] = peak;
-      consumers_sync();
-    }
 #pragma unroll 1
-    for (unsigned i = tid; i < rows * (kDim / 4); i += kConsumers) {
-      const unsigned r = i / (kDim / 4), c = (i % (kDim / 4)) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float peak = -INFINITY, weight = 0.f;
+    for (unsigned i = tid; i < rows * (kDim / 4); i += 2 * kConsumers) {      // two places a thread, the loads of four parts side by side
+      constexpr unsigned kBatch = 4;
+      float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+      float peak[2] = {-INFINITY, -INFINITY}, weight[2] = {0.f, 0.f};
+      unsigned r[2], c[2];
 #pragma unroll
-      for (unsigned k = 0; k < kConsumers / kRows; ++k) peak = fmaxf(peak, exchange[k * kRows + r]);
-#pragma unroll 8
-      for (unsigned a = first_cta; a <= last_cta; ++a) {
-        const float2 end_of = __ldcg(reinterpret_cast<const float2*>(parts.end(a, a == first_cta, r)));
-        const float4 part = __ldcg(reinterpret_cast<const float4*>(parts.sum(a, a == first_cta, r) + c));
-        const float f = end_of.x == -INFINITY ? 0.f : exp2_of(end_of.x - peak);
-        v.x += part.x * f; v.y += part.y * f; v.z += part.z * f; v.w += part.w * f;
-        weight += end_of.y * f;
+      for (int e = 0; e < 2; ++e) {
+        const unsigned place = min(i + e * kConsumers, rows * (kDim / 4) - 1);
+        r[e] = place / (kDim / 4);
+        c[e] = (place % (kDim / 4)) * 4;
       }
-      leave(r, c, v, peak, weight);
+#pragma unroll 1
+      for (unsigned a0 = first_cta; a0 <= last_cta; a0 += kBatch) {
+        float2 ends[2][kBatch];
+        float4 sums[2][kBatch];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (unsigned b = 0; b < kBatch; ++b) {
+            const unsigned a = min(a0 + b, last_cta);
+            ends[e][b] = __ldcg(reinterpret_cast<const float2*>(parts.end(a, a == first_cta, r[e])));
+            sums[e][b] = __ldcg(reinterpret_cast<const float4*>(parts.sum(a, a == first_cta, r[e]) + c[e]));
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (unsigned b = 0; b < kBatch; ++b) {
+            if (a0 + b > last_cta) continue;
+            const float next = fmaxf(peak[e], ends[e][b].x);
+            const float before = next == -INFINITY ? 0.f : exp2_of(peak[e] - next), by = next == -INFINITY ? 0.f : exp2_of(ends[e][b].x - next);
+            v[e].x = v[e].x * before + sums[e][b].x * by;
+            v[e].y = v[e].y * before + sums[e][b].y * by;
+            v[e].z = v[e].z * before + sums[e][b].z * by;
+            v[e].w = v[e].w * before + sums[e][b].w * by;
+            weight[e] = weight[e] * before + ends[e][b].y * by;
+            peak[e] = next;
+          }
+      }
+      leave(r[0], c[0], v[0], peak[0], weight[0]);
+      if (i + kConsumers < rows * (kDim / 4)) leave(r[1], c[1], v[1], peak[1], weight[1]);
     }
     if (tid == 0) counters[first_cta] = 0;               // as the next launch expects it
   });

@@ -195,7 +195,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       tc::mbar_init(&v_empty[s], 1);
     }
     for (unsigned s = 0; s < 2; ++s) {
-      tc::mbar_init(&q_full[s], 32);
+      tc::mbar_init(&q_full[s], 1);
       tc::mbar_init(&q_empty[s], 1);
       tc::mbar_init(&s_full[s], 1);
       tc::mbar_init(&p_half[s], kStreamRows);
@@ -221,7 +221,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   // ---- the run of this CTA: key tiles [from, to) of all ----
   const unsigned sequences = kPrefix ? 1u : batch.sequences;
   auto span_at = [&](unsigned seq) {
-    if (!kPrefix) return span_of(batch, seq);
+    if (!kPrefix) return span_of(batch, claim_of(batch, seq));
     return Span{0u, batch.rows, 0, min(unsigned(max(*prefix_length, 0)), prefix_pages * batch.page)};
   };
   auto seen_at = [&](const Span& s, unsigned block) {
@@ -230,56 +230,71 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     return visible_of<kKeys>(s.first + int(block * kRows / group), s.first + int(last / group), s.length, window, sinks);
   };
   auto blocks_of = [&](const Span& s) { return (s.fresh * group + kRows - 1) / kRows; };
-  // blocks of rows first: where the blocks of every sequence begin (in Q's memory, before Q is there) ...
-  unsigned* const block_begin = reinterpret_cast<unsigned*>(base_ptr);
-  const unsigned seq_share = (sequences + kThreads - 1) / kThreads, seq0 = min(tid * seq_share, sequences), seq1 = min(seq0 + seq_share, sequences);
-  unsigned blocks_mine = 0, all_blocks;
-  bool usable = aligned;
-#pragma unroll 1
-  for (unsigned i = seq0; i < seq1; ++i) {
-    usable = (kPrefix || in_order(batch, i)) && usable;
-    blocks_mine += blocks_of(span_at(i));
-  }
-  if (kPrefix && tid == 0 && *prefix_length > int(prefix_pages * batch.page)) report(batch.status, kBadLength);
-  unsigned blocks_below = sum_before<kThreads>(blocks_mine, block_base, &all_blocks);
-#pragma unroll 1
-  for (unsigned i = seq0; i < seq1; ++i) {
-    block_begin[i] = blocks_below;
-    blocks_below += blocks_of(span_at(i));
-  }
-  const bool stop = __syncthreads_or(!usable);
-  if (stop) all_blocks = 0;
-  // ... then their key tiles: a run of blocks a thread
-  const unsigned share = (all_blocks + kThreads - 1) / kThreads, b0 = min(tid * share, all_blocks), b1 = min(b0 + share, all_blocks);
-  unsigned holder = 0;      // the sequence with block b0: the last one that begins at or before it
-  for (unsigned above = sequences; above - holder > 1;) {
-    const unsigned middle = (holder + above) / 2;
-    if (block_begin[middle] <= b0) holder = middle; else above = middle;
-  }
-  unsigned mine = 0, total, below = 0, from = 0, to = 0, per = 1;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {      // counts the thread's tiles; then, in the thread that has it, finds the block of tile `from`
-    if (pass == 1) {
-      below = sum_before<kThreads>(mine, tile_base, &total);
-      per = max((total + gridDim.x - 1) / gridDim.x, least);
-      from = min(per * blockIdx.x, total);
-      to = min(from + per, total);
-      if (from >= to || from < below || from >= below + mine) break;
+  unsigned from = 0, to = 0, per = 1;
+  if (kPrefix) {      // blocks are alike: every thread finds the run by itself
+    const Span span = span_at(0);
+    const unsigned tiles = (seen_at(span, 0).count + kItemCost) * kv_heads, total = aligned ? blocks_of(span) * tiles : 0u;
+    if (tid == 0 && *prefix_length > int(prefix_pages * batch.page)) report(batch.status, kBadLength);
+    per = max((total + gridDim.x - 1) / gridDim.x, least);
+    from = min(per * blockIdx.x, total);
+    to = min(from + per, total);
+    if (tid == 0) {
+      run_seq = 0;
+      run_block = from / tiles;
+      run_first = from / tiles * tiles;
     }
-    unsigned seq = holder;
+  } else {
+    // blocks of rows first: where the blocks of every sequence begin (in Q's memory, before Q is there) ...
+    unsigned* const block_begin = reinterpret_cast<unsigned*>(base_ptr);
+    const unsigned seq_share = (sequences + kThreads - 1) / kThreads, seq0 = min(tid * seq_share, sequences), seq1 = min(seq0 + seq_share, sequences);
+    unsigned blocks_mine = 0, all_blocks;
+    bool usable = aligned;
 #pragma unroll 1
-    for (unsigned b = b0; b < b1; ++b) {
-      while (seq + 1 < sequences && block_begin[seq + 1] <= b) ++seq;
-      const unsigned tiles = (seen_at(span_at(seq), b - block_begin[seq]).count + kItemCost) * kv_heads;
-      if (pass == 0) {
-        mine += tiles;
-      } else if (from < below + tiles) {
-        run_seq = seq;
-        run_block = b - block_begin[seq];
-        run_first = below;
-        break;
-      } else {
-        below += tiles;
+    for (unsigned i = seq0; i < seq1; ++i) {
+      const Claim claim = claim_of(batch, i);
+      usable = in_order(batch, claim) && usable;
+      blocks_mine += blocks_of(span_of(batch, claim));
+    }
+    unsigned blocks_below = sum_before<kThreads>(blocks_mine, block_base, &all_blocks);
+#pragma unroll 1
+    for (unsigned i = seq0; i < seq1; ++i) {
+      block_begin[i] = blocks_below;
+      blocks_below += blocks_of(span_at(i));
+    }
+    const bool stop = __syncthreads_or(!usable);
+    if (stop) all_blocks = 0;
+    // ... then their key tiles: a run of blocks a thread
+    const unsigned share = (all_blocks + kThreads - 1) / kThreads, b0 = min(tid * share, all_blocks), b1 = min(b0 + share, all_blocks);
+    unsigned holder = 0;      // the sequence with block b0: the last one that begins at or before it
+    for (unsigned above = sequences; above - holder > 1;) {
+      const unsigned middle = (holder + above) / 2;
+      if (block_begin[middle] <= b0) holder = middle; else above = middle;
+    }
+    unsigned mine = 0, total, below = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {      // counts the thread's tiles; then, in the thread that has it, finds the block of tile `from`
+      if (pass == 1) {
+        below = sum_before<kThreads>(mine, tile_base, &total);
+        per = max((total + gridDim.x - 1) / gridDim.x, least);
+        from = min(per * blockIdx.x, total);
+        to = min(from + per, total);
+        if (from >= to || from < below || from >= below + mine) break;
+      }
+      unsigned seq = holder;
+#pragma unroll 1
+      for (unsigned b = b0; b < b1; ++b) {
+        while (seq + 1 < sequences && block_begin[seq + 1] <= b) ++seq;
+        const unsigned tiles = (seen_at(span_at(seq), b - block_begin[seq]).count + kItemCost) * kv_heads;
+        if (pass == 0) {
+          mine += tiles;
+        } else if (from < below + tiles) {
+          run_seq = seq;
+          run_block = b - block_begin[seq];
+          run_first = below;
+          break;
+        } else {
+          below += tiles;
+        }
       }
     }
   }
@@ -454,7 +469,13 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     const unsigned c = lane % kChunks, lane_row = lane / kChunks, token_step = kStep / group, sub_step = kStep % group;
     const size_t ahead = (size_t(token_step) * q_stride + sub_step * kDim) * 2, wraps = (size_t(q_stride) - group * kDim) * 2;
     unsigned phases = 3;
+    bool first_item = true;            // its queries the softmax warps bring in, which have nothing else to do yet
     walk([&](const Item& it, unsigned, unsigned, unsigned, unsigned) {
+      if (first_item) {
+        first_item = false;
+        phases ^= it.rows <= kStreamRows ? 1u : 3u;
+        return;
+      }
 #pragma unroll 1
       for (unsigned stream = 0; stream < (it.rows <= kStreamRows ? 1u : 2u); ++stream) {
         const unsigned rows_before = stream * kStreamRows, live = min(it.rows - rows_before, kStreamRows);
@@ -482,7 +503,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         tc::fence_async_shared();
-        tc::mbar_arrive(&q_full[stream]);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&q_full[stream]);
       }
     });
   }
@@ -494,6 +516,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     const unsigned score_at = tmem + stream * kKeys + lanes, out_at = tmem + kOutColumn + stream * 128 + lanes;
     unsigned char* const staged = base_ptr + 2 * kQBytes + 2 * stages * kSlotBytes + warp * (32 * kStagePitch);
     unsigned s_phase = 0, o_phases = 0, shared_items = 0;
+    bool first_item = true;
     auto outputs_done = [&](unsigned of_stream) {
       await(&o_full[of_stream], (o_phases >> of_stream) & 1, tc::kTimeoutAccum | 0x40 | of_stream);
       __syncwarp();
@@ -504,8 +527,35 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       const bool shared_rows = it.rows <= kStreamRows;
       const unsigned rows_before = shared_rows ? 0u : stream * kStreamRows;                 // of the item's, in front of this stream's
       const bool is_live = rows_before + r < it.rows;
+      const Rows pairs(it.row0 + rows_before, group);
+      if (first_item && (!shared_rows || stream == 0)) {
+        constexpr unsigned kBatch = 8;
+        const unsigned live = min(it.rows - rows_before, kStreamRows);
+#pragma unroll 1
+        for (unsigned i0 = r; i0 < kStreamRows * (kDim / 8); i0 += 128 * kBatch) {
+          uint4 v[kBatch];
+#pragma unroll
+          for (unsigned b = 0; b < kBatch; ++b) {
+            const unsigned row = (i0 + b * 128) / (kDim / 8), c = (i0 + b * 128) % (kDim / 8);
+            unsigned token, sub;
+            pairs.at(row, token, sub);
+            const bf16* from_row = q + size_t(it.row + token) * q_stride + (it.head * group + sub) * kDim + c * 8;
+            v[b] = row < live ? __ldcg(reinterpret_cast<const uint4*>(from_row)) : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (unsigned b = 0; b < kBatch; ++b) {
+            const unsigned row = (i0 + b * 128) / (kDim / 8), c = (i0 + b * 128) % (kDim / 8);
+            *reinterpret_cast<uint4*>(base_ptr + stream * kQBytes + (c / 8) * (kStreamRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[b];
+          }
+        }
+        tc::fence_async_shared();
+        if (stream == 0) asm volatile("bar.sync 3, 128;" ::: "memory");
+        else asm volatile("bar.sync 4, 128;" ::: "memory");
+        if (r == 0) tc::mbar_arrive(&q_full[stream]);
+      }
+      first_item = false;
       unsigned token, sub;
-      Rows(it.row0 + rows_before, group).at(r, token, sub);
+      pairs.at(r, token, sub);
       const int index = kPrefix ? 0x3fffffff : is_live ? it.first + int(token) : -1;
       // the rows of this warp: does a tile need a mask?
       const int low = it.first + int(__shfl_sync(0xffffffffu, token, 0)), high = it.first + int(__shfl_sync(0xffffffffu, token, 31));
@@ -678,45 +728,89 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   }
 }
 
-// The parts of items that runs cut, added in order: CTA (i, cta) takes rows i * kJoinRows and on of the item that begins in slot 1 of `cta`.
-// A thread takes four columns of a row: eight rows of a column group are one line of a slot.
-constexpr unsigned kJoinRows = 8;
+// The parts of items that runs cut, added in order.  Every block reads the notes of all CTAs and counts the groups of eight rows that
+// cut items have; it takes groups blockIdx.x, + gridDim.x, ...  A thread takes four columns of a row: eight rows of a column group
+// are one line of a slot.
+constexpr unsigned kJoinRows = 8, kMaxCtas = 160;
 template <int HD16, bool kPrefix>
 __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned sequences, float* own_sums, float* own_ends, float* scratch, Note* notes,
-                                          unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {
-  constexpr unsigned kDim = HD16 * 16;
+                                          unsigned ctas, unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {
+  constexpr unsigned kDim = HD16 * 16, kJoinThreads = kJoinRows * kDim / 4, kBatch = 6;
+  __shared__ unsigned begins[kMaxCtas + 1];
+  const unsigned tid = threadIdx.x, lane = tid & 31, group = q_heads / kv_heads;
   grid_dependency_wait();
   const Parts<kDim> parts{scratch, notes};
-  const unsigned first = blockIdx.y, group = q_heads / kv_heads;
-  const uint4 a = __ldcg(reinterpret_cast<const uint4*>(notes + first));
-  const unsigned pieces = a.x, row_first = a.y, row0 = a.z, rows = a.w;
-  const unsigned r = blockIdx.x * kJoinRows + threadIdx.x % kJoinRows, c4 = threadIdx.x / kJoinRows;
-  if (pieces == 0 || r >= rows) return;
-  const unsigned head = __ldcg(&notes[first].head);
-  const unsigned row = row_first + (row0 + r) / group, q_head = head * group + (row0 + r) % group;
-  if (kPrefix && !(int(row) >= starts[0] && int(row) < starts[sequences])) return;
-  const size_t flat = size_t(row) * q_heads + q_head;
-  float top = -INFINITY, sum = 0.f;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](const float2 end, const float4 part) {
-    float mine_by, other_by;
-    join(top, sum, end, mine_by, other_by);
-    v.x = v.x * mine_by + part.x * other_by;
-    v.y = v.y * mine_by + part.y * other_by;
-    v.z = v.z * mine_by + part.z * other_by;
-    v.w = v.w * mine_by + part.w * other_by;
-  };
-#pragma unroll 2
-  for (unsigned p = 0; p < pieces; ++p) add(__ldcg(parts.end(first + p, p == 0, r)), __ldcg(parts.sum(first + p, p == 0, r, c4)));
-  if (own_only) {
-    *reinterpret_cast<float4*>(own_sums + flat * kDim + c4 * 4) = v;
-    if (c4 == 0) *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(top, sum);
-    return;
+  for (unsigned i = tid; i < kMaxCtas; i += kJoinThreads) {
+    uint4 a = make_uint4(0u, 0u, 0u, 0u);
+    if (i < ctas) a = __ldcg(reinterpret_cast<const uint4*>(notes + i));
+    begins[i + 1] = a.x ? (a.w + kJoinRows - 1) / kJoinRows : 0u;
   }
-  if (kPrefix) add(__ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c4 * 4)));
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  const bf162 pair[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv), __floats2bfloat162_rn(v.z * inv, v.w * inv)};
-  *reinterpret_cast<uint2*>(o + size_t(row) * o_stride + q_head * kDim + c4 * 4) = *reinterpret_cast<const uint2*>(pair);
+  __syncthreads();
+  if (tid < 32) {
+    constexpr unsigned kEach = kMaxCtas / 32;
+    unsigned sum = 0, of[kEach];
+#pragma unroll
+    for (unsigned i = 0; i < kEach; ++i) sum += of[i] = begins[lane * kEach + i + 1];
+    unsigned up_to = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned other = __shfl_up_sync(0xffffffffu, up_to, d);
+      if (lane >= unsigned(d)) up_to += other;
+    }
+    up_to -= sum;
+    if (lane == 0) begins[0] = 0;
+#pragma unroll
+    for (unsigned i = 0; i < kEach; ++i) begins[lane * kEach + i + 1] = up_to += of[i];
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (unsigned work = blockIdx.x; work < begins[kMaxCtas]; work += gridDim.x) {
+    unsigned first = 0;       // the CTA whose item has this group of rows: the last one that begins at or before it (none without groups)
+    for (unsigned above = kMaxCtas; above - first > 1;) {
+      const unsigned middle = (first + above) / 2;
+      if (begins[middle] <= work) first = middle; else above = middle;
+    }
+    const uint4 a = __ldcg(reinterpret_cast<const uint4*>(notes + first));
+    const unsigned pieces = a.x, rows = a.w, head = __ldcg(&notes[first].head);
+    const unsigned r = (work - begins[first]) * kJoinRows + tid % kJoinRows, c4 = tid / kJoinRows;
+    if (r >= rows) continue;
+    const unsigned row = a.y + (a.z + r) / group, q_head = head * group + (a.z + r) % group;
+    if (kPrefix && !(int(row) >= starts[0] && int(row) < starts[sequences])) continue;
+    const size_t flat = size_t(row) * q_heads + q_head;
+    float top = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float2 end, const float4 part) {
+      float mine_by, other_by;
+      join(top, sum, end, mine_by, other_by);
+      v.x = v.x * mine_by + part.x * other_by;
+      v.y = v.y * mine_by + part.y * other_by;
+      v.z = v.z * mine_by + part.z * other_by;
+      v.w = v.w * mine_by + part.w * other_by;
+    };
+#pragma unroll 1
+    for (unsigned p0 = 0; p0 < pieces; p0 += kBatch) {
+      float2 ends[kBatch];
+      float4 sums[kBatch];
+#pragma unroll
+      for (unsigned b = 0; b < kBatch; ++b) {
+        const unsigned p = min(p0 + b, pieces - 1);
+        ends[b] = __ldcg(parts.end(first + p, p == 0, r));
+        sums[b] = __ldcg(parts.sum(first + p, p == 0, r, c4));
+      }
+#pragma unroll
+      for (unsigned b = 0; b < kBatch; ++b)
+        if (p0 + b < pieces) add(ends[b], sums[b]);
+    }
+    if (own_only) {
+      *reinterpret_cast<float4*>(own_sums + flat * kDim + c4 * 4) = v;
+      if (c4 == 0) *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(top, sum);
+      continue;
+    }
+    if (kPrefix) add(__ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c4 * 4)));
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const bf162 pair[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv), __floats2bfloat162_rn(v.z * inv, v.w * inv)};
+    *reinterpret_cast<uint2*>(o + size_t(row) * o_stride + q_head * kDim + c4 * 4) = *reinterpret_cast<const uint2*>(pair);
+  }
 }
 
 }  // namespace many
@@ -741,12 +835,13 @@ AGI_PAGED_MANY(agi_paged_prefix_bf16_d64, 4, true)
 AGI_PAGED_MANY(agi_paged_prefix_bf16_d128, 8, true)
 #undef AGI_PAGED_MANY
 
-// grid = (256 / 8, CTAs of the launch before), block = 2 * head_dim.
+// grid: any number of blocks, block = 2 * head_dim; ctas: the CTAs of the launch before, 160 at most.
 #define AGI_PAGED_JOIN(NAME, HD16, PREFIX)                                                                                             \
   extern "C" __global__ void __launch_bounds__(many::kJoinRows * HD16 * 4)                                                             \
   NAME(bf16* o, const int* starts, unsigned sequences, float* own_sums, float* own_ends, float* scratch, many::Note* notes,            \
-       unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {                                                    \
-    many::join_body<HD16, PREFIX>(o, starts, sequences, own_sums, own_ends, scratch, notes, q_heads, kv_heads, o_stride, own_only);    \
+       unsigned ctas, unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {                                     \
+    many::join_body<HD16, PREFIX>(o, starts, sequences, own_sums, own_ends, scratch, notes, ctas, q_heads, kv_heads, o_stride,         \
+                                  own_only);                                                                                           \
   }
 AGI_PAGED_JOIN(agi_paged_join_bf16_d64, 4, false)
 AGI_PAGED_JOIN(agi_paged_join_bf16_d128, 8, false)

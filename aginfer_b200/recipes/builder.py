@@ -886,7 +886,7 @@ class RecipeBuilder:
         s0, s1 = (sections[0], sections[1]) if sections is not None else (POSITIONS_FROM_CACHE if positions is None else POSITIONS_ONE_AXIS, 0)
         log2_theta = struct.unpack("f", struct.pack("f", math.log2(theta)))[0]
         dummy = Arena(0)
-        self.launch("agi_kv_append_bf16", (min(rows, SM_COUNT * 8), 1, 1), (128, 1, 1),
+        self.launch("agi_kv_append_bf16", (rows, 1, 1), (128, 1, 1),
                     [q, k, v, U32(k_column), U32(v_column), q_out, cache.k, cache.v, cache.starts, cache.lengths, cache.table,
                      positions or dummy, offset or dummy, Arena(STATUS_WORD), U32(rows), U32(cache.sequences), U32(cache.pages),
                      U32(cache.page), U32(cache.pages_per_sequence), U32(q_heads), U32(cache.kv_heads), U32(d), U32(row_stride),
@@ -944,8 +944,8 @@ class RecipeBuilder:
                         [q, o, cache.k, cache.v, *batch, shared[0], shared[1], *own, scratch, notes, Arena(STATUS_WORD), *shape, U32(shared[2]),
                          *heads, U32(t["stages"]), U32(t["least"]), U32(own_only)],
                         shared_bytes=t["shared_bytes"], op=op, algorithm="tcgen05_row_blocks")
-            self.launch(f"{join}_d{d}", (ceil_div(min(PAGED_MANY_ROWS, rows * group), 8), t["grid"], 1), (2 * d, 1, 1),
-                        [o, cache.starts, U32(cache.sequences), *own, scratch, notes, U32(q_heads), U32(cache.kv_heads), U32(o_stride),
+            self.launch(f"{join}_d{d}", (min(8 * SM_COUNT, ceil_div(min(PAGED_MANY_ROWS, rows * group), 8) * t["grid"]), 1, 1), (2 * d, 1, 1),
+                        [o, cache.starts, U32(cache.sequences), *own, scratch, notes, U32(t["grid"]), U32(q_heads), U32(cache.kv_heads), U32(o_stride),
                          U32(own_only)], op=op, algorithm="join_parts")
 
         if longest * group <= PAGED_FEW_ROWS:
