@@ -76,7 +76,8 @@ __device__ __forceinline__ bool in_order(const Batch& b, const Claim& c) {
   return ordered;
 }
 
-// Sum over the threads in front of this one, and over all.  `of_warp`: a word per warp, used once a kernel.
+// Sum over the threads in front of this one, and over all.  `of_warp`: a word per warp; a barrier goes in front of its
+// next use.
 template <unsigned kThreads>
 __device__ __forceinline__ unsigned sum_before(unsigned mine, unsigned* of_warp, unsigned* all) {
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

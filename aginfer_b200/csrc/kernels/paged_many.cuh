@@ -180,6 +180,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   __shared__ __align__(8) unsigned long long q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
   __shared__ float2 shared_end[kStreamRows];
   __shared__ unsigned block_base[kThreads / 32], tile_base[kThreads / 32], run_seq, run_block, run_first, gave_up, tmem_slot;
+  __shared__ Span run_span;
   const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const unsigned base = (tc::smem_u32(dynamic_smem) + 1023u) & ~1023u;
   unsigned char* const base_ptr = dynamic_smem + (base - tc::smem_u32(dynamic_smem));
@@ -242,59 +243,62 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       run_seq = 0;
       run_block = from / tiles;
       run_first = from / tiles * tiles;
+      run_span = span;
     }
   } else {
-    // blocks of rows first: where the blocks of every sequence begin (in Q's memory, before Q is there) ...
-    unsigned* const block_begin = reinterpret_cast<unsigned*>(base_ptr);
-    const unsigned seq_share = (sequences + kThreads - 1) / kThreads, seq0 = min(tid * seq_share, sequences), seq1 = min(seq0 + seq_share, sequences);
-    unsigned blocks_mine = 0, all_blocks;
-    bool usable = aligned;
+    // what the batch says of every sequence and where its blocks of rows begin (in Q's memory, before Q is there) ...
+    int4* const places = reinterpret_cast<int4*>(base_ptr);
+    unsigned below_blocks = 0, ordered = aligned;
 #pragma unroll 1
-    for (unsigned i = seq0; i < seq1; ++i) {
-      const Claim claim = claim_of(batch, i);
-      usable = in_order(batch, claim) && usable;
-      blocks_mine += blocks_of(span_of(batch, claim));
+    for (unsigned i0 = 0; i0 < sequences; i0 += kThreads) {
+      const unsigned i = i0 + tid;
+      Claim claim{0, 0, 0};
+      if (i < sequences) {
+        claim = claim_of(batch, i);
+        if (!in_order(batch, claim)) {
+          ordered = 0;
+          claim = Claim{0, 0, 0};
+        }
+      }
+      unsigned all;
+      const unsigned begins = below_blocks + sum_before<kThreads>(blocks_of(span_of(batch, claim)), block_base, &all);
+      if (i < sequences) places[i] = make_int4(claim.from, claim.to, claim.length, int(begins));
+      below_blocks += all;
+      ordered = __syncthreads_and(ordered);
     }
-    unsigned blocks_below = sum_before<kThreads>(blocks_mine, block_base, &all_blocks);
-#pragma unroll 1
-    for (unsigned i = seq0; i < seq1; ++i) {
-      block_begin[i] = blocks_below;
-      blocks_below += blocks_of(span_at(i));
-    }
-    const bool stop = __syncthreads_or(!usable);
-    if (stop) all_blocks = 0;
+    const unsigned all_blocks = ordered ? below_blocks : 0u;
     // ... then their key tiles: a run of blocks a thread
     const unsigned share = (all_blocks + kThreads - 1) / kThreads, b0 = min(tid * share, all_blocks), b1 = min(b0 + share, all_blocks);
     unsigned holder = 0;      // the sequence with block b0: the last one that begins at or before it
     for (unsigned above = sequences; above - holder > 1;) {
       const unsigned middle = (holder + above) / 2;
-      if (block_begin[middle] <= b0) holder = middle; else above = middle;
+      if (unsigned(places[middle].w) <= b0) holder = middle; else above = middle;
     }
-    unsigned mine = 0, total, below = 0;
+    auto tiles_of = [&](unsigned& seq, unsigned b) {
+      while (seq + 1 < sequences && unsigned(places[seq + 1].w) <= b) ++seq;
+      const int4 place = places[seq];
+      return (seen_at(span_of(batch, Claim{place.x, place.y, place.z}), b - unsigned(place.w)).count + kItemCost) * kv_heads;
+    };
+    unsigned mine = 0, total, seq = holder;
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {      // counts the thread's tiles; then, in the thread that has it, finds the block of tile `from`
-      if (pass == 1) {
-        below = sum_before<kThreads>(mine, tile_base, &total);
-        per = max((total + gridDim.x - 1) / gridDim.x, least);
-        from = min(per * blockIdx.x, total);
-        to = min(from + per, total);
-        if (from >= to || from < below || from >= below + mine) break;
-      }
-      unsigned seq = holder;
-#pragma unroll 1
-      for (unsigned b = b0; b < b1; ++b) {
-        while (seq + 1 < sequences && block_begin[seq + 1] <= b) ++seq;
-        const unsigned tiles = (seen_at(span_at(seq), b - block_begin[seq]).count + kItemCost) * kv_heads;
-        if (pass == 0) {
-          mine += tiles;
-        } else if (from < below + tiles) {
+    for (unsigned b = b0; b < b1; ++b) mine += tiles_of(seq, b);
+    unsigned below = sum_before<kThreads>(mine, tile_base, &total);
+    per = max((total + gridDim.x - 1) / gridDim.x, least);
+    from = min(per * blockIdx.x, total);
+    to = min(from + per, total);
+    if (from < to && from >= below && from < below + mine) {      // this thread's blocks hold the run's first tile
+      seq = holder;
+      for (unsigned b = b0;; ++b) {
+        const unsigned tiles = tiles_of(seq, b);
+        if (from < below + tiles) {
+          const int4 place = places[seq];
           run_seq = seq;
-          run_block = b - block_begin[seq];
+          run_block = b - unsigned(place.w);
           run_first = below;
+          run_span = span_of(batch, Claim{place.x, place.y, place.z});
           break;
-        } else {
-          below += tiles;
         }
+        below += tiles;
       }
     }
   }
@@ -309,12 +313,13 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   // f(item, first key tile, last key tile + 1, number of the item's first unit, sequence)
   auto walk = [&](auto&& f) {
     unsigned seq = run_seq, block = run_block, first = run_first, unit = from;
+    Span span = run_span;
 #pragma unroll 1
-    while (unit < to && seq < sequences) {
-      const Span span = span_at(seq);
+    while (unit < to) {
       if (block >= blocks_of(span)) {
         block = 0;
-        ++seq;
+        if (++seq >= sequences) break;
+        span = span_at(seq);
         continue;
       }
       Item it;
@@ -529,7 +534,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       const bool is_live = rows_before + r < it.rows;
       const Rows pairs(it.row0 + rows_before, group);
       if (first_item && (!shared_rows || stream == 0)) {
-        constexpr unsigned kBatch = 8;
+        constexpr unsigned kBatch = kDim / 8;
         const unsigned live = min(it.rows - rows_before, kStreamRows);
 #pragma unroll 1
         for (unsigned i0 = r; i0 < kStreamRows * (kDim / 8); i0 += 128 * kBatch) {
