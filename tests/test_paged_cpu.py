@@ -101,3 +101,43 @@ def test_attention_that_is_refused(kw):
 def test_prefixes_that_are_refused(kw):
     with pytest.raises(ValueError):
         share(builder(), **kw)
+
+
+def test_every_kernel_of_the_paged_decoder_is_an_entry_point():
+    from aginfer_b200.build import build_all
+    from aginfer_b200.recipes import paged_decode
+    from aginfer_b200.recipes.decoder_layer import LayerConfig
+    from aginfer_b200.recipes.package import describe
+    from tests.test_cubin_symbols_cpu import function_symbols
+    entry_points = function_symbols(build_all()[1].read_bytes())
+    for window, heads in ((0, (4, 2, 64)), (64, (7, 1, 128)), (0, (64, 1, 64))):
+        layer = LayerConfig(hidden=256, heads=heads[0], kv_heads=heads[1], head_dim=heads[2], intermediate=704, tokens=64)
+        cfg = paged_decode.ServeConfig(layer=layer, layers=2, sequences=3, page=16, new_tokens=40, window=window)
+        plan = paged_decode.build_recipe(cfg, describe(paged_decode.synthetic_weights(cfg))).plan()
+        used = {l["kernel"] for p in plan["shape_dispatch"] for l in p["launches"]}
+        assert used <= entry_points, sorted(used - entry_points)
+        assert {p["profile"] for p in plan["shape_dispatch"]} == {"prompt", "step"}
+
+
+@pytest.mark.parametrize("kw", [dict(window=64, tokens=70), dict(fp8=True)], ids=str)
+def test_paged_decoders_that_are_refused(kw):
+    from aginfer_b200.recipes import paged_decode
+    from aginfer_b200.recipes.decoder_layer import LayerConfig
+    with pytest.raises(ValueError):
+        paged_decode.ServeConfig(layer=LayerConfig(tokens=kw.get("tokens", 64), fp8=kw.get("fp8", False)), window=kw.get("window", 0))
+
+
+def test_tilings_stay_inside_what_an_sm_and_the_scratch_hold():
+    from aginfer_b200.recipes.builder import SM_COUNT, TC_COUNTER_BYTES, TC_SCRATCH_BYTES, paged_few_tiling, paged_many_tiling
+    for d in (64, 128):
+        for page in (16, 128):
+            cache = PagedCache(**CACHE | dict(head_dim=d, page=page, sequences=4096, pages_per_sequence=1000))
+            for rows in range(1, 33):
+                t = paged_few_tiling(cache, 4096, 1, rows)
+                assert t["rows"] >= min(rows, 32) and t["stages"] >= 2 and t["grid"] * 4 <= TC_COUNTER_BYTES
+                per_sm = 1 if t["rows"] == 32 and d == 128 else 2
+                static = {8: 384, 16: 640, 32: 1152}[t["rows"]]      # barriers, maxima and weights of the warps
+                assert per_sm * (t["shared_bytes"] + static + 1024) <= 228 * 1024
+                assert t["grid"] * 2 * t["rows"] * (d + 2) * 4 <= TC_SCRATCH_BYTES
+            t = paged_many_tiling(cache, 100, 128000)
+            assert t["grid"] <= SM_COUNT and 2 <= t["stages"] <= 6 and t["shared_bytes"] + 2048 <= 227 * 1024
