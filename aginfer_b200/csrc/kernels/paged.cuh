@@ -113,6 +113,17 @@ struct Rows {
   }
 };
 
+// The part of prefix attention that a row's own sequence makes, unnormalised: [kv_heads][head_dim / 4][rows x group][4] sums and
+// [kv_heads][rows x group][2] (maximum in units of log2, weight).  Rows lie side by side, as the threads that own one read them.
+struct Own {
+  float *sums, *ends;
+  unsigned rows, dim;
+  __device__ __forceinline__ float4* sum(unsigned head, unsigned c4, unsigned row) const {
+    return reinterpret_cast<float4*>(sums) + (size_t(head) * (dim / 4) + c4) * rows + row;
+  }
+  __device__ __forceinline__ float2* end(unsigned head, unsigned row) const { return reinterpret_cast<float2*>(ends) + size_t(head) * rows + row; }
+};
+
 // The key tiles that rows at indices [low, high] see: those of the first `sinks` tokens that lie before the window of the first
 // row, then those from that window to the last row.  At least one, which may hold no visible key: it makes a row that sees
 // nothing zero.

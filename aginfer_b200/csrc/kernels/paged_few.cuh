@@ -26,6 +26,9 @@ namespace few {
 using namespace paged;
 
 constexpr unsigned kKeys = 64, kConsumers = 128, kThreads = 160;
+// CTAs that share an item: a small batch could have more, but adding their parts then takes longer than the tiles that it saves
+// (one token over 1500 keys, 24 tiles: 24 parts 14.5 us, 12 or 8 or 6 parts 12.4, 4 parts 14.6).
+constexpr unsigned kMostParts = 12;
 constexpr float kSlack = 8.f;               // log2 of how far scores may exceed the maximum that weights are relative to
 
 // How many units one sequence is: its key heads x row blocks x key tiles.
@@ -62,22 +65,25 @@ struct Run {
   Claim claim;                        // what the batch says of it
 };
 template <unsigned kRows>
-__device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsigned kv_heads, unsigned window, unsigned sinks, unsigned least) {
+__device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsigned kv_heads, unsigned window, unsigned sinks) {
   const unsigned lane = threadIdx.x & 31;
   bool ordered = true;
-  unsigned units = 0, total = 0;
+  unsigned units = 0, total = 0, longest = 0;
   Claim claim{0, 0, 0};
 #pragma unroll 2
   for (unsigned i = lane; i < batch.sequences; i += 32) {
     claim = claim_of(batch, i);
     ordered = in_order(batch, claim) && ordered;
-    units = items_of<kRows>(batch, claim, group, kv_heads, window, sinks).units;
+    const Items it = items_of<kRows>(batch, claim, group, kv_heads, window, sinks);
+    units = it.units;
     total += units;
+    if (units) longest = max(longest, it.seen.count);
   }
   total = __reduce_add_sync(0xffffffffu, total);
+  longest = __reduce_max_sync(0xffffffffu, longest);
   if (!__all_sync(0xffffffffu, ordered)) total = 0;
   Run run;
-  run.per = max((total + gridDim.x - 1) / gridDim.x, least);
+  run.per = max((total + gridDim.x - 1) / gridDim.x, (longest + kMostParts - 1) / kMostParts);
   run.from = min(run.per * blockIdx.x, total);
   run.to = min(run.from + run.per, total);
   run.seq = run.first = 0;
@@ -115,7 +121,7 @@ template <int HD16, int kN>
 __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const Batch& batch, float* own_sums,
                                                float* own_ends, float* scratch, unsigned* counters, unsigned q_heads, unsigned kv_heads,
                                                unsigned q_stride, unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,
-                                               unsigned least, unsigned own_only) {
+                                               unsigned own_only) {
   constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kRows = 8 * kN;
   constexpr unsigned kTileBytes = kKeys * kDim * 2, kStageBytes = 2 * kTileBytes, kBlockBytes = kKeys * 128;
   constexpr unsigned kMaxStages = 6;
@@ -138,12 +144,14 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  grid_dependency_wait();
+  // In front of a prefix's launch, which begins without waiting for this one, what this one waits for has to be complete.
+  if (own_only) grid_dependency_wait_then_release();
+  else grid_dependency_wait();
   if (!(aligned16(q) && aligned16(o) && aligned16(k_pool) && aligned16(v_pool))) {
     if (tid == 0) report(batch.status, kMisaligned);
     return;
   }
-  const Run run = run_of<kRows>(batch, group, kv_heads, window, sinks, least);
+  const Run run = run_of<kRows>(batch, group, kv_heads, window, sinks);
   if (run.from >= run.to) return;
 
   // Walks the run item by item: f(sequence, key head, row block, its items, first tile, last tile + 1, first unit of the item).
@@ -362,9 +370,9 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       pairs.at(r, token, sub);
       const unsigned row = span.row + token, q_head = head * group + sub;
       if (own_only) {
-        const size_t flat = size_t(row) * q_heads + q_head;
-        *reinterpret_cast<float4*>(own_sums + flat * kDim + c) = v;
-        if (c == 0) *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(peak, weight);
+        const Own own{own_sums, own_ends, batch.rows * group, kDim};
+        *own.sum(head, c / 4, row * group + sub) = v;
+        if (c == 0) *own.end(head, row * group + sub) = make_float2(peak, weight);
         return;
       }
       const float inv = weight > 0.f ? 1.f / weight : 0.f;
@@ -391,7 +399,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       consumers_sync();
 #pragma unroll 1
       for (unsigned i = tid; i < 8 * (kDim / 4); i += kConsumers) {
-        const unsigned r8 = i / (kDim / 4), c = (i % (kDim / 4)) * 4, r = j * 8 + r8;
+        // columns side by side for a row of outputs, rows side by side for sums that are kept
+        const unsigned r8 = own_only ? i % 8 : i / (kDim / 4), c = (own_only ? i / 8 : i % (kDim / 4)) * 4, r = j * 8 + r8;
         const float peak = fmaxf(fmaxf(warp_max_of[0][r], warp_max_of[1][r]), fmaxf(warp_max_of[2][r], warp_max_of[3][r]));
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float weight = 0.f;
@@ -473,17 +482,17 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 }  // namespace few
 
 // grid: any number of CTAs that `scratch` has room for, block = 160, dynamic shared memory = stages * 256 * head_dim + 128 * head_dim + 128.
-// least: units that a CTA takes at the least; counters: one word per CTA, zero between launches.  own_only: sums, maxima and
-// weights to own_sums [rows][q_heads][head_dim] and own_ends [rows][q_heads][2] instead of o (prefix attention adds the prefix to them).
+// counters: one word per CTA, zero between launches.  own_only: sums, maxima and
+// weights to own_sums and own_ends instead of o (prefix attention adds the prefix to them).
 #define AGI_PAGED_FEW(NAME, HD16, N, PER_SM)                                                                                          \
   extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM)                                                                 \
   NAME(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const int* starts, const int* lengths, const int* table,       \
        float* own_sums, float* own_ends, float* scratch, unsigned* counters, unsigned* status, unsigned rows, unsigned sequences,     \
        unsigned pages, unsigned page, unsigned width, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride,      \
-       unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned least, unsigned own_only) {                       \
+       unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned own_only) {                       \
     const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                    \
     few::attention_body<HD16, N>(q, o, k_pool, v_pool, batch, own_sums, own_ends, scratch, counters, q_heads, kv_heads, q_stride,     \
-                                 o_stride, window, sinks, scale_log2, stages, least, own_only);                                       \
+                                 o_stride, window, sinks, scale_log2, stages, own_only);                                       \
   }
 AGI_PAGED_FEW(agi_paged_few_bf16_d64_r8, 4, 1, 2)
 AGI_PAGED_FEW(agi_paged_few_bf16_d64_r16, 4, 2, 2)

@@ -122,8 +122,6 @@ struct Parts {
   }
 };
 
-// own_sums, own_ends: the rows' own sequences' part of prefix attention, [rows][q_heads][head_dim] and [rows][q_heads][2], written by the
-// launch before (own_only).
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -187,6 +185,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   const unsigned ring = base + 2 * kQBytes;
   const unsigned group = q_heads / kv_heads;
   const Parts<kDim> parts{scratch, notes};
+  const Own own{own_sums, own_ends, batch.rows * group, kDim};
 
   if (tid == 0) {
     for (unsigned s = 0; s < stages; ++s) {
@@ -214,7 +213,10 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   __syncthreads();
   tc::tc_fence_after();
   const unsigned tmem = tmem_slot;
-  grid_dependency_wait();
+  // The prefix does not wait for its rows' own sequences, which the launch before is still working on, until it adds them; that launch
+  // has let this one begin only when everything in front of it was complete.
+  if (kPrefix) grid_dependency_release();
+  else grid_dependency_wait();
 
   const bool aligned = aligned16(q) && aligned16(o) && aligned16(k_pool) && aligned16(v_pool);
   if (!aligned && tid == 0) report(batch.status, kMisaligned);
@@ -652,12 +654,13 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       // rows of no sequence are left alone
       const unsigned row = it.row + token;
       const bool stays = is_live && (!kPrefix || (int(row) >= batch.starts[0] && int(row) < batch.starts[batch.sequences]));
-      const size_t flat = size_t(row) * q_heads + it.head * group + sub;
+      const unsigned flat = row * group + sub;
       const bool merges = kPrefix && !cut && stays, divides = !cut && !own_only;
       float own_by = 0.f;
       if (merges) {
         float all_by;
-        join(top, sum, __ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), all_by, own_by);
+        grid_dependency_only_wait();
+        join(top, sum, __ldcg(own.end(it.head, flat)), all_by, own_by);
         mine_by *= all_by;
         other_by *= all_by;
       }
@@ -685,7 +688,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         if (merges) {
 #pragma unroll
           for (unsigned i = 0; i < 32; i += 4) {
-            const float4 w = __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c0 + i));
+            const float4 w = __ldcg(own.sum(it.head, (c0 + i) / 4, flat));
             v[i] = fmaf(w.x, own_by, v[i]);
             v[i + 1] = fmaf(w.y, own_by, v[i + 1]);
             v[i + 2] = fmaf(w.z, own_by, v[i + 2]);
@@ -707,14 +710,14 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         } else if (is_live) {
 #pragma unroll
           for (unsigned i = 0; i < 32; i += 4)
-            *(cut ? parts.sum(blockIdx.x, slot, rows_before + r, (c0 + i) / 4) : reinterpret_cast<float4*>(own_sums + flat * kDim + c0 + i)) =
+            *(cut ? parts.sum(blockIdx.x, slot, rows_before + r, (c0 + i) / 4) : own.sum(it.head, (c0 + i) / 4, flat)) =
                 make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
       }
       tc::tc_fence_before();
       tc::mbar_arrive(&o_empty[stream]);
       if (both) tc::mbar_arrive(&o_empty[1]);
-      if (!divides && is_live) *(cut ? parts.end(blockIdx.x, slot, rows_before + r) : reinterpret_cast<float2*>(own_ends + flat * 2)) = make_float2(top, sum);
+      if (!divides && is_live) *(cut ? parts.end(blockIdx.x, slot, rows_before + r) : own.end(it.head, flat)) = make_float2(top, sum);
       if (cut && begin == 0 && tid == 0) {
         Note& note = parts.notes[blockIdx.x];
         note.row = it.row;
@@ -725,6 +728,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
       }
     });
   }
+  if (kPrefix) grid_dependency_only_wait();       // whoever waits for this launch may rely on the one before too
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 8) {
@@ -739,12 +743,15 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 constexpr unsigned kJoinRows = 8, kMaxCtas = 160;
 template <int HD16, bool kPrefix>
 __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned sequences, float* own_sums, float* own_ends, float* scratch, Note* notes,
-                                          unsigned ctas, unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {
+                                          unsigned ctas, unsigned rows_of_launch, unsigned q_heads, unsigned kv_heads, unsigned o_stride,
+                                          unsigned own_only) {
   constexpr unsigned kDim = HD16 * 16, kJoinThreads = kJoinRows * kDim / 4, kBatch = 6;
   __shared__ unsigned begins[kMaxCtas + 1];
   const unsigned tid = threadIdx.x, lane = tid & 31, group = q_heads / kv_heads;
-  grid_dependency_wait();
+  if (own_only) grid_dependency_wait_then_release();       // a prefix's launch is next
+  else grid_dependency_wait();
   const Parts<kDim> parts{scratch, notes};
+  const Own own{own_sums, own_ends, rows_of_launch * group, kDim};
   for (unsigned i = tid; i < kMaxCtas; i += kJoinThreads) {
     uint4 a = make_uint4(0u, 0u, 0u, 0u);
     if (i < ctas) a = __ldcg(reinterpret_cast<const uint4*>(notes + i));
@@ -781,7 +788,7 @@ __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned s
     if (r >= rows) continue;
     const unsigned row = a.y + (a.z + r) / group, q_head = head * group + (a.z + r) % group;
     if (kPrefix && !(int(row) >= starts[0] && int(row) < starts[sequences])) continue;
-    const size_t flat = size_t(row) * q_heads + q_head;
+    const unsigned flat = row * group + (a.z + r) % group;
     float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](const float2 end, const float4 part) {
@@ -807,11 +814,11 @@ __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned s
         if (p0 + b < pieces) add(ends[b], sums[b]);
     }
     if (own_only) {
-      *reinterpret_cast<float4*>(own_sums + flat * kDim + c4 * 4) = v;
-      if (c4 == 0) *reinterpret_cast<float2*>(own_ends + flat * 2) = make_float2(top, sum);
+      *own.sum(head, c4, flat) = v;
+      if (c4 == 0) *own.end(head, flat) = make_float2(top, sum);
       continue;
     }
-    if (kPrefix) add(__ldcg(reinterpret_cast<const float2*>(own_ends + flat * 2)), __ldcg(reinterpret_cast<const float4*>(own_sums + flat * kDim + c4 * 4)));
+    if (kPrefix) add(__ldcg(own.end(head, flat)), __ldcg(own.sum(head, c4, flat)));
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     const bf162 pair[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv), __floats2bfloat162_rn(v.z * inv, v.w * inv)};
     *reinterpret_cast<uint2*>(o + size_t(row) * o_stride + q_head * kDim + c4 * 4) = *reinterpret_cast<const uint2*>(pair);
@@ -844,8 +851,8 @@ AGI_PAGED_MANY(agi_paged_prefix_bf16_d128, 8, true)
 #define AGI_PAGED_JOIN(NAME, HD16, PREFIX)                                                                                             \
   extern "C" __global__ void __launch_bounds__(many::kJoinRows * HD16 * 4)                                                             \
   NAME(bf16* o, const int* starts, unsigned sequences, float* own_sums, float* own_ends, float* scratch, many::Note* notes,            \
-       unsigned ctas, unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {                                     \
-    many::join_body<HD16, PREFIX>(o, starts, sequences, own_sums, own_ends, scratch, notes, ctas, q_heads, kv_heads, o_stride,         \
+       unsigned ctas, unsigned rows, unsigned q_heads, unsigned kv_heads, unsigned o_stride, unsigned own_only) {                      \
+    many::join_body<HD16, PREFIX>(o, starts, sequences, own_sums, own_ends, scratch, notes, ctas, rows, q_heads, kv_heads, o_stride,   \
                                   own_only);                                                                                           \
   }
 AGI_PAGED_JOIN(agi_paged_join_bf16_d64, 4, false)

@@ -501,7 +501,6 @@ class PagedCache:
 PAGED_MAX_SEQUENCES = 4096
 PAGED_FEW_ROWS = 32                      # rows (new tokens x query heads of a key head) of a sequence that mma.sync tiles take
 PAGED_FEW_KEYS = 64                      # keys of a tile
-PAGED_FEW_LEAST = 2
 
 
 def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> dict[str, int]:
@@ -513,12 +512,12 @@ def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> 
     stages = min(6, ((228 - per_sm) * 1024 // per_sm - 1024 - exchange) // stage)      # 1 KB of static shared memory
     blocks = min(cache.sequences, rows) * ceil_div(longest * group, item) * cache.kv_heads
     tiles = blocks * ceil_div(cache.pages_per_sequence * cache.page, PAGED_FEW_KEYS)
-    return {"rows": item, "grid": min(SM_COUNT * per_sm, ceil_div(tiles, PAGED_FEW_LEAST)), "stages": stages, "least": PAGED_FEW_LEAST,
+    return {"rows": item, "grid": min(SM_COUNT * per_sm, tiles), "stages": stages,
             "shared_bytes": stages * stage + exchange + 128}
 
 
 PAGED_MANY_ROWS, PAGED_MANY_KEYS = 256, 128
-PAGED_MANY_LEAST = 2
+PAGED_MANY_LEAST = 3         # tiles that a CTA takes at the least (288-token prompt: 2 21.9 us, 3 20.6, 4 24.4; a prefix of 288: 26.8, 24.7, 24.8)
 
 
 def paged_many_tiling(cache: PagedCache, blocks: int, tokens: int) -> dict[str, int]:
@@ -945,7 +944,8 @@ class RecipeBuilder:
                          *heads, U32(t["stages"]), U32(t["least"]), U32(own_only)],
                         shared_bytes=t["shared_bytes"], op=op, algorithm="tcgen05_row_blocks")
             self.launch(f"{join}_d{d}", (min(8 * SM_COUNT, ceil_div(min(PAGED_MANY_ROWS, rows * group), 8) * t["grid"]), 1, 1), (2 * d, 1, 1),
-                        [o, cache.starts, U32(cache.sequences), *own, scratch, notes, U32(t["grid"]), U32(q_heads), U32(cache.kv_heads), U32(o_stride),
+                        [o, cache.starts, U32(cache.sequences), *own, scratch, notes, U32(t["grid"]), U32(rows), U32(q_heads), U32(cache.kv_heads),
+                         U32(o_stride),
                          U32(own_only)], op=op, algorithm="join_parts")
 
         if longest * group <= PAGED_FEW_ROWS:
@@ -953,7 +953,7 @@ class RecipeBuilder:
             scratch, counters = self._tc_scratch
             self.launch(f"agi_paged_few_bf16_d{d}_r{t['rows']}", (t["grid"], 1, 1), (160, 1, 1),
                         [q, o, cache.k, cache.v, *batch, *own, scratch, counters, Arena(STATUS_WORD), *shape, *heads, U32(t["stages"]),
-                         U32(t["least"]), U32(1 if prefix else 0)],
+                         U32(1 if prefix else 0)],
                         shared_bytes=t["shared_bytes"], op=op, algorithm=f"mma_key_tiles_r{t['rows']}")
         else:
             blocks = min(rows * group // PAGED_MANY_ROWS + min(cache.sequences, rows), cache.sequences * ceil_div(longest * group, PAGED_MANY_ROWS))

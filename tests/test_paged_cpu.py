@@ -141,3 +141,11 @@ def test_tilings_stay_inside_what_an_sm_and_the_scratch_hold():
                 assert t["grid"] * 2 * t["rows"] * (d + 2) * 4 <= TC_SCRATCH_BYTES
             t = paged_many_tiling(cache, 100, 128000)
             assert t["grid"] <= SM_COUNT and 2 <= t["stages"] <= 6 and t["shared_bytes"] + 2048 <= 227 * 1024
+
+
+def test_no_cta_waits_for_one_that_may_lack_tensor_memory():
+    """The order that tests/test_tensor_memory_cpu.py reads off the other kernels, for the paged one."""
+    from tests.test_tensor_memory_cpu import body_events
+    events = body_events("paged_many.cuh")
+    assert events.count("tmem_alloc") == events.count("tmem_free") == 1 and "cluster_wait" not in events
+    assert all(events.index("tmem_alloc") < i for i, e in enumerate(events) if "grid_dependency" in e)
