@@ -172,6 +172,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
                                                unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,
                                                unsigned least, unsigned own_only) {
   constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kBlockBytes = kKeys * 128, kSlotBytes = kBlocks * kBlockBytes;
+  // Tiles that are not cut off an item (ragged chunks 0 57.5 us, 1 55.5, 2 56.2; a prefix's few, long items 31, 33, 35).
+  constexpr unsigned kSnap = kPrefix ? 0 : 1;
   constexpr unsigned kQBytes = kStreamRows * kDim * 2, kMaxStages = 6;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ __align__(8) unsigned long long k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
@@ -334,9 +336,14 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 #pragma unroll 1
       while (unit < to && unit < first + length * kv_heads) {
         it.head = (unit - first) / length;
-        // the item's tiles stand behind the units that it costs besides; a run that ends among those leaves the item to the next one
+        // The item's tiles stand behind the units that it costs besides.  A cut among those, or so few tiles behind the first or in front of
+        // the end that its part would cost more than it evens out, is moved there; the CTAs on both sides see it alike.
         const unsigned tiles_at = first + it.head * length + kItemCost, next = tiles_at + it.seen.count;
-        const unsigned begin = max(unit, tiles_at) - tiles_at, end = max(min(next, to), tiles_at) - tiles_at;
+        auto cut = [&](unsigned at) {
+          if (at >= next) return next;
+          return at <= tiles_at + kSnap ? tiles_at : at + kSnap >= next ? next : at;
+        };
+        const unsigned begin = cut(from) - tiles_at, end = cut(to) - tiles_at;
         if (begin < end) f(it, begin, end, tiles_at, seq);
         unit = next;
       }
@@ -724,7 +731,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         note.row0 = it.row0;
         note.rows = it.rows;
         note.head = it.head;
-        note.pieces = (tiles_at + it.seen.count - 1) / per - blockIdx.x + 1;
+        // the cuts inside the item, and one
+        note.pieces = (tiles_at + it.seen.count - kSnap - 1) / per - (tiles_at + kSnap) / per + 1;
       }
     });
   }
