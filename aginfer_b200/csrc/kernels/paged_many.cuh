@@ -8,15 +8,23 @@
 //
 // Two streams share the tensor core: while one stream's scores are exponentiated by its four warps, the other's products run.
 // An item of more than 128 rows gives each stream 128 rows and every key tile; a smaller one gives both streams the same rows
-// and every other tile, and their outputs meet in shared memory.  A warp thread owns a row: it reads the row's 128 scores from
-// tensor memory, needs no shuffles for maximum and sum, and writes P back over them as bf16.  Outputs are rescaled only when a
-// row's maximum has grown by more than 2^8 since they were last scaled (all of it cancels in the quotient).
+// and every other tile, and the first stream adds the second one's outputs where they lie in tensor memory.  A thread owns a row: it
+// reads the row's 128 scores from tensor memory, needs no shuffles for maximum and sum, and writes P back over them as bf16 (the
+// sums are of the unrounded weights, in 32 bits).  Outputs are rescaled only when a row's maximum has grown by more than 2^8 since
+// they were last scaled; all of it cancels in the quotient.
 //
 // Keys and values come in by one bulk copy per page (or its part in a tile) and 64-column block: the pool holds the image that
-// the tensor core reads, rows of keys K-major for S, the same image MN-major for P V.  Tokens behind a sequence's end are not
-// copied; their values are set to zero in shared memory, since weight zero does not make a NaN zero.
+// the tensor core reads, rows of keys K-major for S, the same image MN-major for P V.  Tokens behind a sequence's end and pages that
+// no row of the item sees are not copied; their values are set to zero in shared memory, since weight zero does not make a NaN
+// zero.  Other tokens of a tile are multiplied by weight zero where a row does not see them.
 //
+// Warps: 0-3 and 4-7 a stream each, 8 issues the products, 9 and 10 bring keys and values in, 11 the queries of the next item.
 // Tensor memory (512 columns): scores and P of the streams at 0 and 128, outputs at 256 and 384.
+//
+// What bounds it, head_dim 128: a tile of 256 rows by 128 keys takes 3200 clocks, of which the tensor core works 2100 and the
+// special-function unit 2050; the rest is the chain of a stream (scores 150 clocks to registers, maximum 450, weights 1400, products
+// 1200 until the next scores are there) that two streams do not cover.  8192 tokens, 28 query heads on 4, window 2048: 252 us =
+// 840 TFLOP/s, half the rate measured for a library product.  An item costs 8500 clocks besides, a launch 9000 before its first scores.
 #pragma once
 
 #include "gemm_tc.cuh"
@@ -353,175 +361,175 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   };
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
-  if (warp == 9 || warp == 10) {
-    // ---- a warp each for keys and values: a lane per piece (64-column block, page or part of one) of a tile ----
-    const bool values = warp == 10;
-    const unsigned shift = 31 - __clz(batch.page), run = min(batch.page, kKeys), pieces = kKeys / run;
-    const unsigned block = (lane / pieces) % kBlocks, piece = lane % pieces;
-    const bool live = lane < kBlocks * pieces;
-    const unsigned page_bytes = kv_heads * kBlocks * batch.page * 128, slots = ring + (values ? stages * kSlotBytes : 0u);
-    unsigned long long* const full = values ? v_full : k_full;
-    unsigned long long* const empty = values ? v_empty : k_empty;
-    unsigned s = 0, phase = 1;
-    walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned seq) {
-      const int* const pages_of = kPrefix ? prefix_table : batch.table + size_t(seq) * batch.width;
-      const unsigned char* const pool = reinterpret_cast<const unsigned char*>(values ? v_pool : k_pool) + size_t((it.head * kBlocks + block) * batch.page) * 128;
-      auto token_of = [&](unsigned t) { return it.seen.tile(t) * kKeys + piece * run; };
-      auto tokens_of = [&](unsigned t) {      // that this lane brings in
-        const unsigned token = token_of(t);
-        return live && token < it.seen.end && (token < it.seen.sink_end || token + run > it.seen.start) ? min(run, it.seen.end - token) : 0u;
-      };
-      unsigned count = tokens_of(begin), page_id = count ? unsigned(pages_of[token_of(begin) >> shift]) : 0u;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+    if (warp == 9 || warp == 10) {
+      // ---- a warp each for keys and values: a lane per piece (64-column block, page or part of one) of a tile ----
+      const bool values = warp == 10;
+      const unsigned shift = 31 - __clz(batch.page), run = min(batch.page, kKeys), pieces = kKeys / run;
+      const unsigned block = (lane / pieces) % kBlocks, piece = lane % pieces;
+      const bool live = lane < kBlocks * pieces;
+      const unsigned page_bytes = kv_heads * kBlocks * batch.page * 128, slots = ring + (values ? stages * kSlotBytes : 0u);
+      unsigned long long* const full = values ? v_full : k_full;
+      unsigned long long* const empty = values ? v_empty : k_empty;
+      unsigned s = 0, phase = 1;
+      walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned seq) {
+        const int* const pages_of = kPrefix ? prefix_table : batch.table + size_t(seq) * batch.width;
+        const unsigned char* const pool = reinterpret_cast<const unsigned char*>(values ? v_pool : k_pool) + size_t((it.head * kBlocks + block) * batch.page) * 128;
+        auto token_of = [&](unsigned t) { return it.seen.tile(t) * kKeys + piece * run; };
+        auto tokens_of = [&](unsigned t) {      // that this lane brings in
+          const unsigned token = token_of(t);
+          return live && token < it.seen.end && (token < it.seen.sink_end || token + run > it.seen.start) ? min(run, it.seen.end - token) : 0u;
+        };
+        unsigned count = tokens_of(begin), page_id = count ? unsigned(pages_of[token_of(begin) >> shift]) : 0u;
 #pragma unroll 1
-      for (unsigned t = begin; t < end; ++t) {
-        if (page_id >= batch.pages) {
-          report(batch.status, kBadPage);
-          count = 0;
+        for (unsigned t = begin; t < end; ++t) {
+          if (page_id >= batch.pages) {
+            report(batch.status, kBadPage);
+            count = 0;
+          }
+          const unsigned char* const from_page = pool + size_t(page_id) * page_bytes + (token_of(t) & (batch.page - 1)) * 128;
+          const unsigned slot = slots + s * kSlotBytes, all = __reduce_add_sync(0xffffffffu, count * 128);
+          unsigned next_count = 0, next_page = 0;      // the page of the tile behind it, while this one's slot is awaited
+          if (t + 1 < end) {
+            next_count = tokens_of(t + 1);
+            if (next_count) next_page = unsigned(pages_of[token_of(t + 1) >> shift]);
+          }
+          if (lane == 0) await(&empty[s], phase, tc::kTimeoutEmpty | s);
+          __syncwarp();
+          if (values && all < kSlotBytes) {      // zero what is not copied
+            for (unsigned p = 0; p < pieces; ++p) {
+              const unsigned held = __shfl_sync(0xffffffffu, count, p);       // the same for every block of the piece
+              for (unsigned i = lane; i < (run - held) * 8 * kBlocks; i += 32) {
+                const unsigned b = i / ((run - held) * 8), rest = i % ((run - held) * 8);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(slot + b * kBlockBytes + (p * run + held) * 128 + rest * 16), "r"(0u)
+                             : "memory");
+              }
+            }
+            tc::fence_async_shared();
+            __syncwarp();
+          }
+          if (lane == 0) tc::expect_bytes(&full[s], all);
+          __syncwarp();
+          if (count) tc::bulk_copy(slot + block * kBlockBytes + piece * run * 128, from_page, count * 128, &full[s]);
+          count = next_count;
+          page_id = next_page;
+          if (++s == stages) { s = 0; phase ^= 1; }
         }
-        const unsigned char* const from_page = pool + size_t(page_id) * page_bytes + (token_of(t) & (batch.page - 1)) * 128;
-        const unsigned slot = slots + s * kSlotBytes, all = __reduce_add_sync(0xffffffffu, count * 128);
-        unsigned next_count = 0, next_page = 0;      // the page of the tile behind it, while this one's slot is awaited
-        if (t + 1 < end) {
-          next_count = tokens_of(t + 1);
-          if (next_count) next_page = unsigned(pages_of[token_of(t + 1) >> shift]);
-        }
-        if (lane == 0) await(&empty[s], phase, tc::kTimeoutEmpty | s);
-        __syncwarp();
-        if (values && all < kSlotBytes) {      // zero what is not copied
-          for (unsigned p = 0; p < pieces; ++p) {
-            const unsigned held = __shfl_sync(0xffffffffu, count, p);       // the same for every block of the piece
-            for (unsigned i = lane; i < (run - held) * 8 * kBlocks; i += 32) {
-              const unsigned b = i / ((run - held) * 8), rest = i % ((run - held) * 8);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(slot + b * kBlockBytes + (p * run + held) * 128 + rest * 16), "r"(0u)
-                           : "memory");
+      });
+    } else if (warp == 8) {
+      // ---- one thread issues the products ----
+      if (elect_one()) {
+        constexpr unsigned kScores = instruction(kKeys, false), kOutputs = instruction(kDim, true);
+        unsigned ks = 0, k_phase = 0, vs = 0, v_phase = 0, q_phases = 0, p_phases = 0, o_phases = 3;       // the last three: a bit per stream
+        auto flips = [&](unsigned long long* bars, unsigned& phases, unsigned stream, unsigned code) {
+          await(&bars[stream], (phases >> stream) & 1, tc::kTimeoutAccum | code | stream);
+          phases ^= 1u << stream;
+          tc::tc_fence_after();
+        };
+        auto scores = [&](unsigned stream, unsigned q_stream, unsigned slot) {
+          const unsigned long long a = tc::smem_descriptor(base + q_stream * kQBytes), b = tc::smem_descriptor(ring + slot * kSlotBytes);
+#pragma unroll
+          for (unsigned k = 0; k < HD16; ++k)
+            tc::mma<false>(tmem + stream * kKeys, a + (k / 4) * (kStreamRows * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2,
+                           kScores, k != 0);
+          tc::tc_commit(&s_full[stream]);
+        };
+        auto arrived = [&](unsigned long long* bars, unsigned& s, unsigned& phase) {      // the next tile has landed: its slot
+          await(&bars[s], phase, tc::kTimeoutFull | s);
+          const unsigned slot = s;
+          if (++s == stages) { s = 0; phase ^= 1; }
+          return slot;
+        };
+        // P V of a stream's tile: the first half of the keys while the weights of the second half are still being formed
+        auto outputs = [&](unsigned stream, unsigned slot, bool first) {
+          const unsigned long long b = mn_descriptor(ring + (stages + slot) * kSlotBytes, kBlockBytes);
+          const unsigned d = tmem + kOutColumn + stream * 128, a = tmem + stream * kKeys;
+          if (first) flips(o_empty, o_phases, stream, 0x80);
+          await(&p_half[stream], (p_phases >> stream) & 1, tc::kTimeoutAccum | 0x30 | stream);
+          tc::tc_fence_after();
+#pragma unroll
+          for (unsigned k = 0; k < kKeys / 32; ++k) mma_from_tmem(d, a + k * 8, b + k * (16 * 128 >> 4), kOutputs, !first || k != 0);
+          flips(p_full, p_phases, stream, 0x20);
+#pragma unroll
+          for (unsigned k = kKeys / 32; k < kKeys / 16; ++k) mma_from_tmem(d, a + k * 8, b + k * (16 * 128 >> 4), kOutputs, 1);
+        };
+        walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned) {
+          const unsigned n = end - begin;
+          const bool shared_rows = it.rows <= kStreamRows;
+          // step i: scores of tile i (i < n), behind the outputs of the tile that used the same columns before
+          const unsigned lead = shared_rows ? min(n, 2u) : 1u;
+          unsigned values = 0, keys = 0;
+#pragma unroll 1
+          for (unsigned i = 0; i < n + lead; ++i) {
+#pragma unroll 1
+            for (unsigned half = 0; half < (shared_rows ? 1u : 2u); ++half) {
+              const unsigned stream = shared_rows ? (i >= lead ? (i - lead) & 1 : i) : half, area = shared_rows ? 0u : stream;
+              const bool last_use = shared_rows || half == 1;
+              if (i >= lead && half == 0) values = arrived(v_full, vs, v_phase);
+              if (i < n && half == 0) keys = arrived(k_full, ks, k_phase);
+              if (i >= lead) {
+                const unsigned j = i - lead;
+                outputs(stream, values, j < lead);
+                if (last_use) tc::tc_commit(&v_empty[values]);
+                if (j + lead >= n) tc::tc_commit(&o_full[stream]);
+              }
+              if (i < n) {
+                if (i == 0) flips(q_full, q_phases, area, 0x10);
+                tc::tc_fence_after();
+                scores(stream, area, keys);
+                if (last_use) tc::tc_commit(&k_empty[keys]);
+                if (i == n - 1) tc::tc_commit(&q_empty[area]);
+              }
             }
           }
+        });
+      }
+      __syncwarp();
+    } else {
+      // ---- a warp brings the queries in (zero past the item's rows), as soon as the item before has formed its last scores ----
+      constexpr unsigned kChunks = kDim / 8, kStep = 32 / kChunks;      // 16-byte chunks of a row, rows that the warp copies at a time
+      const unsigned c = lane % kChunks, lane_row = lane / kChunks, token_step = kStep / group, sub_step = kStep % group;
+      const size_t ahead = (size_t(token_step) * q_stride + sub_step * kDim) * 2, wraps = (size_t(q_stride) - group * kDim) * 2;
+      unsigned phases = 3;
+      bool first_item = true;            // its queries the softmax warps bring in, which have nothing else to do yet
+      walk([&](const Item& it, unsigned, unsigned, unsigned, unsigned) {
+        if (first_item) {
+          first_item = false;
+          phases ^= it.rows <= kStreamRows ? 1u : 3u;
+          return;
+        }
+#pragma unroll 1
+        for (unsigned stream = 0; stream < (it.rows <= kStreamRows ? 1u : 2u); ++stream) {
+          const unsigned rows_before = stream * kStreamRows, live = min(it.rows - rows_before, kStreamRows);
+          const unsigned q_area = base + stream * kQBytes + (c / 8) * (kStreamRows * 128) + lane_row * 128;
+          const unsigned first = it.row0 + rows_before + lane_row, token = first / group;
+          unsigned sub = first - token * group;
+          const unsigned char* from_row = reinterpret_cast<const unsigned char*>(q + size_t(it.row + token) * q_stride + (it.head * group + sub) * kDim + c * 8);
+          await(&q_empty[stream], (phases >> stream) & 1, tc::kTimeoutAccum | 0x50 | stream);
+          phases ^= 1u << stream;
+          __syncwarp();
+#pragma unroll 1
+          for (unsigned row = 0; row < kStreamRows; row += 8) {
+#pragma unroll
+            for (unsigned i = 0; i < 8; i += kStep) {      // a row in front of the item's end is read, one behind it is zero
+              const bool held = row + i + lane_row < live;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_area + (row + i) * 128 + (((c & 7) ^ (i + lane_row)) << 4)),
+                           "l"(held ? from_row : reinterpret_cast<const unsigned char*>(q)), "r"(held ? 16u : 0u) : "memory");
+              from_row += ahead;
+              sub += sub_step;
+              if (sub >= group) {
+                sub -= group;
+                from_row += wraps;
+              }
+            }
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
           tc::fence_async_shared();
           __syncwarp();
-        }
-        if (lane == 0) tc::expect_bytes(&full[s], all);
-        __syncwarp();
-        if (count) tc::bulk_copy(slot + block * kBlockBytes + piece * run * 128, from_page, count * 128, &full[s]);
-        count = next_count;
-        page_id = next_page;
-        if (++s == stages) { s = 0; phase ^= 1; }
-      }
-    });
-  } else if (warp == 8) {
-    // ---- one thread issues the products ----
-    if (elect_one()) {
-      constexpr unsigned kScores = instruction(kKeys, false), kOutputs = instruction(kDim, true);
-      unsigned ks = 0, k_phase = 0, vs = 0, v_phase = 0, q_phases = 0, p_phases = 0, o_phases = 3;       // the last three: a bit per stream
-      auto flips = [&](unsigned long long* bars, unsigned& phases, unsigned stream, unsigned code) {
-        await(&bars[stream], (phases >> stream) & 1, tc::kTimeoutAccum | code | stream);
-        phases ^= 1u << stream;
-        tc::tc_fence_after();
-      };
-      auto scores = [&](unsigned stream, unsigned q_stream, unsigned slot) {
-        const unsigned long long a = tc::smem_descriptor(base + q_stream * kQBytes), b = tc::smem_descriptor(ring + slot * kSlotBytes);
-#pragma unroll
-        for (unsigned k = 0; k < HD16; ++k)
-          tc::mma<false>(tmem + stream * kKeys, a + (k / 4) * (kStreamRows * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2,
-                         kScores, k != 0);
-        tc::tc_commit(&s_full[stream]);
-      };
-      auto arrived = [&](unsigned long long* bars, unsigned& s, unsigned& phase) {      // the next tile has landed: its slot
-        await(&bars[s], phase, tc::kTimeoutFull | s);
-        const unsigned slot = s;
-        if (++s == stages) { s = 0; phase ^= 1; }
-        return slot;
-      };
-      // P V of a stream's tile: the first half of the keys while the weights of the second half are still being formed
-      auto outputs = [&](unsigned stream, unsigned slot, bool first) {
-        const unsigned long long b = mn_descriptor(ring + (stages + slot) * kSlotBytes, kBlockBytes);
-        const unsigned d = tmem + kOutColumn + stream * 128, a = tmem + stream * kKeys;
-        if (first) flips(o_empty, o_phases, stream, 0x80);
-        await(&p_half[stream], (p_phases >> stream) & 1, tc::kTimeoutAccum | 0x30 | stream);
-        tc::tc_fence_after();
-#pragma unroll
-        for (unsigned k = 0; k < kKeys / 32; ++k) mma_from_tmem(d, a + k * 8, b + k * (16 * 128 >> 4), kOutputs, !first || k != 0);
-        flips(p_full, p_phases, stream, 0x20);
-#pragma unroll
-        for (unsigned k = kKeys / 32; k < kKeys / 16; ++k) mma_from_tmem(d, a + k * 8, b + k * (16 * 128 >> 4), kOutputs, 1);
-      };
-      walk([&](const Item& it, unsigned begin, unsigned end, unsigned, unsigned) {
-        const unsigned n = end - begin;
-        const bool shared_rows = it.rows <= kStreamRows;
-        // step i: scores of tile i (i < n), behind the outputs of the tile that used the same columns before
-        const unsigned lead = shared_rows ? min(n, 2u) : 1u;
-        unsigned values = 0, keys = 0;
-#pragma unroll 1
-        for (unsigned i = 0; i < n + lead; ++i) {
-#pragma unroll 1
-          for (unsigned half = 0; half < (shared_rows ? 1u : 2u); ++half) {
-            const unsigned stream = shared_rows ? (i >= lead ? (i - lead) & 1 : i) : half, area = shared_rows ? 0u : stream;
-            const bool last_use = shared_rows || half == 1;
-            if (i >= lead && half == 0) values = arrived(v_full, vs, v_phase);
-            if (i < n && half == 0) keys = arrived(k_full, ks, k_phase);
-            if (i >= lead) {
-              const unsigned j = i - lead;
-              outputs(stream, values, j < lead);
-              if (last_use) tc::tc_commit(&v_empty[values]);
-              if (j + lead >= n) tc::tc_commit(&o_full[stream]);
-            }
-            if (i < n) {
-              if (i == 0) flips(q_full, q_phases, area, 0x10);
-              tc::tc_fence_after();
-              scores(stream, area, keys);
-              if (last_use) tc::tc_commit(&k_empty[keys]);
-              if (i == n - 1) tc::tc_commit(&q_empty[area]);
-            }
-          }
+          if (lane == 0) tc::mbar_arrive(&q_full[stream]);
         }
       });
     }
-    __syncwarp();
-  } else {
-    // ---- a warp brings the queries in (zero past the item's rows), as soon as the item before has formed its last scores ----
-    constexpr unsigned kChunks = kDim / 8, kStep = 32 / kChunks;      // 16-byte chunks of a row, rows that the warp copies at a time
-    const unsigned c = lane % kChunks, lane_row = lane / kChunks, token_step = kStep / group, sub_step = kStep % group;
-    const size_t ahead = (size_t(token_step) * q_stride + sub_step * kDim) * 2, wraps = (size_t(q_stride) - group * kDim) * 2;
-    unsigned phases = 3;
-    bool first_item = true;            // its queries the softmax warps bring in, which have nothing else to do yet
-    walk([&](const Item& it, unsigned, unsigned, unsigned, unsigned) {
-      if (first_item) {
-        first_item = false;
-        phases ^= it.rows <= kStreamRows ? 1u : 3u;
-        return;
-      }
-#pragma unroll 1
-      for (unsigned stream = 0; stream < (it.rows <= kStreamRows ? 1u : 2u); ++stream) {
-        const unsigned rows_before = stream * kStreamRows, live = min(it.rows - rows_before, kStreamRows);
-        const unsigned q_area = base + stream * kQBytes + (c / 8) * (kStreamRows * 128) + lane_row * 128;
-        const unsigned first = it.row0 + rows_before + lane_row, token = first / group;
-        unsigned sub = first - token * group;
-        const unsigned char* from_row = reinterpret_cast<const unsigned char*>(q + size_t(it.row + token) * q_stride + (it.head * group + sub) * kDim + c * 8);
-        await(&q_empty[stream], (phases >> stream) & 1, tc::kTimeoutAccum | 0x50 | stream);
-        phases ^= 1u << stream;
-        __syncwarp();
-#pragma unroll 1
-        for (unsigned row = 0; row < kStreamRows; row += 8) {
-#pragma unroll
-          for (unsigned i = 0; i < 8; i += kStep) {      // a row in front of the item's end is read, one behind it is zero
-            const bool held = row + i + lane_row < live;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_area + (row + i) * 128 + (((c & 7) ^ (i + lane_row)) << 4)),
-                         "l"(held ? from_row : reinterpret_cast<const unsigned char*>(q)), "r"(held ? 16u : 0u) : "memory");
-            from_row += ahead;
-            sub += sub_step;
-            if (sub >= group) {
-              sub -= group;
-              from_row += wraps;
-            }
-          }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        tc::fence_async_shared();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&q_full[stream]);
-      }
-    });
-  }
   } else {
     // ---- softmax and outputs: four warps a stream, a thread a row ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -753,7 +761,7 @@ template <int HD16, bool kPrefix>
 __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned sequences, float* own_sums, float* own_ends, float* scratch, Note* notes,
                                           unsigned ctas, unsigned rows_of_launch, unsigned q_heads, unsigned kv_heads, unsigned o_stride,
                                           unsigned own_only) {
-  constexpr unsigned kDim = HD16 * 16, kJoinThreads = kJoinRows * kDim / 4, kBatch = 6;
+  constexpr unsigned kDim = HD16 * 16, kJoinThreads = kJoinRows * kDim / 4, kBatch = kPrefix ? 6 : 4;
   __shared__ unsigned begins[kMaxCtas + 1];
   const unsigned tid = threadIdx.x, lane = tid & 31, group = q_heads / kv_heads;
   if (own_only) grid_dependency_wait_then_release();       // a prefix's launch is next
@@ -813,7 +821,8 @@ __device__ __forceinline__ void join_body(bf16* o, const int* starts, unsigned s
       float4 sums[kBatch];
 #pragma unroll
       for (unsigned b = 0; b < kBatch; ++b) {
-        const unsigned p = min(p0 + b, pieces - 1);
+        const unsigned p = kPrefix ? min(p0 + b, pieces - 1) : p0 + b;
+        if (p >= pieces) continue;
         ends[b] = __ldcg(parts.end(first + p, p == 0, r));
         sums[b] = __ldcg(parts.sum(first + p, p == 0, r, c4));
       }
