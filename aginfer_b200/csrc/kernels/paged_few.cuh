@@ -284,8 +284,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 #pragma unroll
           for (int j = 0; j < kN; ++j) skinny_mma_bf16(score[j][ks & 1], a0, a1, a2, a3, qb[j][ks][0], qb[j][ks][1]);
         }
-        // does every row see all of these keys?
-        const bool whole = int(key0) + 15 <= low && key0 + 16 <= it.seen.end && rows == kRows && (window == 0 || int(key0) > int(span.length) - 1 - int(window));
+        // does every row see all of these keys?  (columns behind the item's rows may hold anything)
+        const bool whole = int(key0) + 15 <= low && key0 + 16 <= it.seen.end && (window == 0 || int(key0) > int(span.length) - 1 - int(window));
         unsigned pb[kN][2];
         bool grows = false;
         float x[kN][4], now[kN][2];

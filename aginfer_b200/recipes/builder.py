@@ -930,6 +930,10 @@ class RecipeBuilder:
         q_stride = self._paged_rows("queries", q, rows, q_heads * cache.head_dim, q_stride)
         o_stride = self._paged_rows("outputs", o, rows, q_heads * cache.head_dim, o_stride)
         dummy, group, d, mark = Arena(0), q_heads // cache.kv_heads, cache.head_dim, self.mark()
+        # what the kernels number in 32 bits: key tiles of all blocks of rows, whatever the lengths turn out to be
+        tokens = max(cache.pages_per_sequence, prefix[2] if prefix else 0) * cache.page
+        if (rows * group // 8 + min(cache.sequences, rows)) * cache.kv_heads * (ceil_div(tokens, PAGED_FEW_KEYS) + 8) >= 1 << 31:
+            raise ValueError("more key tiles than a launch numbers: fewer rows or a shorter table")
         # prefix attention: the sequences' own part, unnormalised, goes in front of the prefix's launch
         own = (self.alloc(rows * q_heads * d * 4), self.alloc(rows * q_heads * 8)) if prefix else (dummy, dummy)
         shape = [U32(rows), U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence)]

@@ -86,6 +86,36 @@ def test_a_shared_prefix(tmp_path, new, total, page, heads, prefix):
     run_and_check(tmp_path, batch, longest=max(new))
 
 
+@pytest.mark.parametrize("prefix", [0, 90], ids=str)
+@pytest.mark.parametrize("sequences,long", [(33, 1), (70, 1), (130, 3), (450, 40), (450, 1)], ids=str)
+def test_more_sequences_than_a_warp_or_a_block_looks_at(tmp_path, sequences, long, prefix):
+    lengths = torch.randint(1, 50, (sequences,), generator=torch.Generator().manual_seed(sequences)).tolist()
+    new = [0 if i % 17 == 3 else 1 for i in range(sequences)]
+    new[sequences - 2], lengths[sequences - 2] = long, 150
+    batch = Batch(new, lengths, 16, (2, 1, 64), prefix=prefix, seed=long)
+    run_and_check(tmp_path, batch, longest=long)
+
+
+@pytest.mark.parametrize("new,total", [([1, 1], [9, 80]), ([50, 1], [60, 30])], ids=["few", "chunk"])
+def test_prefixes_that_are_empty_too_long_or_not_in_the_pool(tmp_path, new, total):
+    batch = Batch(new, total, 16, (4, 2, 128), prefix=40, seed=21)
+    got, status, _ = attend(tmp_path, batch, change=lambda x: x["prefix_length"].zero_(), longest=max(new))
+    batch.prefix_kv = None
+    assert status == 0
+    check(batch, got)
+    for code, change in ((0x500, lambda x: x["prefix_length"].fill_(49)), (0x400, lambda x: x["prefix_table"].fill_(batch.pages))):
+        assert attend(tmp_path, batch, change=change, longest=max(new))[1] == code
+
+
+def test_a_prefix_without_programmatic_launch(tmp_path):
+    batch = Batch([1, 2, 1], [30, 70, 1], 32, (8, 2, 128), prefix=300, seed=22)
+    runner, x, out = packaged(tmp_path, batch.inputs(), attention_outputs(batch), lambda r: batch.attend(r, longest=2), flags=0)
+    for _ in range(2):
+        runner.run(x, out)
+    assert int(out["status"].cpu()) == 0
+    check(batch, out["o"].cpu())
+
+
 @pytest.mark.parametrize("new,total,prefix", [([1, 2], [90, 300], 0), ([70], [300], 0), ([1, 1], [9, 80], 70)], ids=str)
 def test_sharp_scores(tmp_path, new, total, prefix):
     """Scores up to a few hundred: one key takes (almost) all, the rest underflows."""

@@ -127,6 +127,17 @@ def test_paged_decoders_that_are_refused(kw):
         paged_decode.ServeConfig(layer=LayerConfig(tokens=kw.get("tokens", 64), fp8=kw.get("fp8", False)), window=kw.get("window", 0))
 
 
+def test_more_key_tiles_than_a_launch_numbers_are_refused():
+    r = RecipeBuilder({"w": ("BF16", (8,))})
+    r.begin_profile("default", [], [])
+    at = Arena(1 << 20)
+    cache = PagedCache(k=at, v=at, table=at, lengths=at, starts=at, sequences=4096, pages=1 << 20, page=128, pages_per_sequence=1 << 14, kv_heads=8,
+                       head_dim=128)
+    r.paged_attention(at, at, cache, rows=4, q_heads=8)
+    with pytest.raises(ValueError):
+        r.paged_attention(at, at, cache, rows=4096, q_heads=64)
+
+
 def test_tilings_stay_inside_what_an_sm_and_the_scratch_hold():
     from aginfer_b200.recipes.builder import SM_COUNT, TC_COUNTER_BYTES, TC_SCRATCH_BYTES, paged_few_tiling, paged_many_tiling
     for d in (64, 128):
