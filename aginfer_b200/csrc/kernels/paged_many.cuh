@@ -23,8 +23,9 @@
 //
 // What bounds it, head_dim 128: a tile of 256 rows by 128 keys takes 3200 clocks, of which the tensor core works 2100 and the
 // special-function unit 2050; the rest is the chain of a stream (scores 150 clocks to registers, maximum 450, weights 1400, products
-// 1200 until the next scores are there) that two streams do not cover.  8192 tokens, 28 query heads on 4, window 2048: 252 us =
-// 840 TFLOP/s, half the rate measured for a library product.  An item costs 8500 clocks besides, a launch 9000 before its first scores.
+// 1200 until the next scores are there) that two streams do not cover.  8192 tokens, 28 query heads on 4, window 2048: 253 us in
+// short runs, 279 in long ones: 830 and 760 TFLOP/s, about half the rate measured for a library product.  An item costs 8500 clocks
+// besides, a launch 9000 before its first scores.
 #pragma once
 
 #include "gemm_tc.cuh"
