@@ -848,12 +848,27 @@ class RecipeBuilder:
         self._declared(what, pointer, "BF16", (rows - 1) * stride + columns)
         return stride
 
+    @staticmethod
+    def _written_apart(what: str, written: tuple[Pointer, int, int], other: str, read: tuple[Pointer, int, int], rows: int) -> None:
+        """Rows that a launch writes share no memory with rows that it reads, each (pointer, pitch, columns) of BF16: every block of a
+        launch reads rows of its own, so a row written over another one's would be read before or after, as blocks happen to run."""
+        (a, a_pitch, a_columns), (b, b_pitch, b_columns) = written, read
+        if isinstance(a, Arena) and isinstance(b, Arena):
+            ahead = (b.offset - a.offset) // 2
+            apart = ahead >= (rows - 1) * a_pitch + a_columns or -ahead >= (rows - 1) * b_pitch + b_columns
+            if a_pitch == b_pitch:       # side by side in rows of one pitch
+                apart = apart or (ahead % a_pitch >= a_columns and ahead % a_pitch + b_columns <= a_pitch)
+        else:
+            apart = a != b
+        if not apart:
+            raise ValueError(f"{what}: written over the {other} that other blocks of the launch still read")
+
     def kv_append(self, q: Pointer, q_out: Pointer, cache: PagedCache, *, rows: int, q_heads: int, theta: float,
                   row_stride: int | None = None, out_stride: int | None = None, k: Pointer | None = None, v: Pointer | None = None,
                   kv_stride: int | None = None, positions: Pointer | None = None, sections: Sequence[int] | None = None,
                   ladder: int | None = None, offset: Pointer | None = None) -> None:
-        """The new tokens' queries turned by their positions into ``q_out`` (which may be ``q``), keys turned and values as they
-        are into the pages of ``cache``.  ``q``: rows of queries | keys | values side by side (pitch ``row_stride``), or the
+        """The new tokens' queries turned by their positions into ``q_out`` (which may be ``q``, at the pitch of ``q``; it shares no
+        other memory with what is read), keys turned and values as they are into the pages of ``cache``.  ``q``: rows of queries | keys | values side by side (pitch ``row_stride``), or the
         queries alone with ``k`` and ``v`` (pitch ``kv_stride``) beside them.  A position is the token's index in its sequence
         plus the I32 at ``offset`` (a shared prefix in front of the sequences), or it comes from ``positions``: I32 [rows], or with
         ``sections`` (pairs of the time, height and width axes) [3, rows].  ``ladder`` as in ``mrope``."""
@@ -868,13 +883,19 @@ class RecipeBuilder:
         if not theta > 0 or (ladder is not None and not 1 <= ladder <= d // 2):
             raise ValueError("theta is positive and a ladder has one to head_dim / 2 pairs")
         q_dim = q_heads * d
-        row_stride = self._paged_rows("queries", q, rows, q_dim + (2 * kv_dim if k is None else 0), row_stride)
-        out_stride = self._paged_rows("turned queries", q_out, rows, q_dim, out_stride)
+        columns = q_dim + (2 * kv_dim if k is None else 0)
+        row_stride = self._paged_rows("queries", q, rows, columns, row_stride)
+        out_stride = self._paged_rows("turned queries", q_out, rows, q_dim, row_stride if out_stride is None and q_out == q else out_stride)
+        written = (q_out, out_stride, q_dim)
+        if q_out != q or out_stride != row_stride:
+            self._written_apart("turned queries", written, "queries, keys or values", (q, row_stride, columns), rows)
         if k is None:
             k, v, k_column, v_column, kv_stride = q, q, q_dim, q_dim + kv_dim, row_stride
         else:
             kv_stride, k_column, v_column = self._paged_rows("keys", k, rows, kv_dim, kv_stride), 0, 0
             self._paged_rows("values", v, rows, kv_dim, kv_stride)
+            for what, p in (("keys", k), ("values", v)):
+                self._written_apart("turned queries", written, what, (p, kv_stride, kv_dim), rows)
         for name in (p.name for p in (q_out, cache.k, cache.v) if isinstance(p, Tensor)):
             if all(t["name"] != name for t in self._profile.outputs):
                 raise ValueError(f"{name!r} is written: it has to be an output of the profile")
@@ -898,7 +919,8 @@ class RecipeBuilder:
         """Causal attention of the new tokens over their sequences' pages (their own keys among them: ``kv_append`` comes first).
         ``window``: a token sees itself and the ``window`` - 1 before it (0: everything), and the first ``sinks`` tokens.
         ``longest``: the most new tokens that one sequence has (``rows`` where it is left out); it says which kernel is
-        launched, the result does not depend on it.  A row that sees nothing is zero; rows of no sequence are left alone."""
+        launched, the result does not depend on it.  A row that sees nothing is zero; rows of no sequence are left alone.
+        ``o`` may be ``q`` at the same pitch; it shares no other memory with it."""
         self._paged_attention(q, o, cache, None, rows=rows, q_heads=q_heads, longest=longest, window=window, sinks=sinks,
                               q_stride=q_stride, o_stride=o_stride, scale=scale, op="paged_attention")
 
@@ -929,6 +951,8 @@ class RecipeBuilder:
             raise ValueError("the scale of the scores is positive")
         q_stride = self._paged_rows("queries", q, rows, q_heads * cache.head_dim, q_stride)
         o_stride = self._paged_rows("outputs", o, rows, q_heads * cache.head_dim, o_stride)
+        if o != q or o_stride != q_stride:       # an item's queries are read before its outputs are written
+            self._written_apart("outputs", (o, o_stride, q_heads * cache.head_dim), "queries", (q, q_stride, q_heads * cache.head_dim), rows)
         dummy, group, d, mark = Arena(0), q_heads // cache.kv_heads, cache.head_dim, self.mark()
         # what the kernels number in 32 bits: key tiles of all blocks of rows, whatever the lengths turn out to be
         tokens = max(cache.pages_per_sequence, prefix[2] if prefix else 0) * cache.page

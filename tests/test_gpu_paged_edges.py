@@ -1,0 +1,37 @@
+"""Paged K/V cache where operands, orders and sizes meet the edges of what the entry points promise, against the definitions in 64 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from aginfer_b200.recipes import Tensor
+from oracle import paged
+from tests.paged_util import BF, Batch, packaged
+from tests.test_gpu_paged import check_append
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("new,total,heads", [([700, 1, 300], [700, 40, 333], (8, 2, 128)), ([5], [5], (4, 2, 64))], ids=str)
+def test_append_in_place_without_a_pitch(tmp_path, new, total, heads):
+    """Queries | keys | values side by side, the queries turned where they stand."""
+    batch = Batch(new, total, 16, heads, seed=31)
+    hq, hk, d = heads
+    x = torch.randn(batch.rows, (hq + 2 * hk) * d, generator=torch.Generator().manual_seed(1)).to(BF)
+    inputs = {n: t for n, t in batch.inputs().items() if n in ("table", "lengths", "starts")}
+    outputs = {"k": batch.k, "v": batch.v, "x": x, "status": torch.zeros(1, dtype=torch.int32)}
+
+    def body(r):
+        r.kv_append(Tensor("x"), Tensor("x"), batch.cache(), rows=batch.rows, q_heads=hq, theta=1e6)
+        r.export_status(Tensor("status"))
+
+    runner, dev, out = packaged(tmp_path, inputs, outputs, body)
+    runner.run(dev, out)
+    got = {n: t.cpu() for n, t in out.items()}
+    assert torch.equal(got["x"][:, hq * d:], x[:, hq * d:])
+    got["q_out"] = got["x"][:, :hq * d]
+    q, k, v = (t.reshape(batch.rows, -1, d) for t in x.split([hq * d, hk * d, hk * d], dim=1))
+    index = torch.tensor([batch.index(b, i) for b, n in enumerate(batch.new) for i in range(n)])
+    angles = paged.rotary_angles(index, 1e6, d)
+    turned = lambda t: (paged.turn(t, angles), t.double().abs())  # noqa: E731
+    check_append(batch, got, turned(q), turned(k), v)
