@@ -161,7 +161,10 @@ class Serving:
         return self.out[profile]["hidden_out"]
 
     def prompt(self, hidden):
-        """Hidden states [tokens, hidden] of the prompt -> those behind the last layer (the buffer of the next call too)."""
+        """Hidden states [tokens, hidden] of the prompt -> those behind the last layer (the buffer of the next call too).  The
+        samples begin anew behind it: what they generated from the prompt before is not looked at any more."""
+        self.steps = 0
+        self.batch["step"]["lengths"].fill_(self.cfg.layer.tokens if self.cfg.window else 0)      # in place: the graphs keep its address
         return self._run("prompt", hidden)
 
     def step(self, hidden):
