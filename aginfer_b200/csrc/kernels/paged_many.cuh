@@ -572,6 +572,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
           }
         }
         tc::fence_async_shared();
+        __syncwarp();
         if (stream == 0) asm volatile("bar.sync 3, 128;" ::: "memory");
         else asm volatile("bar.sync 4, 128;" ::: "memory");
         if (r == 0) tc::mbar_arrive(&q_full[stream]);
@@ -690,6 +691,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 #pragma unroll 1
       for (unsigned c0 = 0; c0 < kDim; c0 += 32) {
         float v[32];
+        __syncwarp();       // rows that merge, stay or are live took branches of their own; tensor memory is read by the whole warp
         tmem_load32(out_at + c0, v);
         tmem_loaded<32>(v);
 #pragma unroll

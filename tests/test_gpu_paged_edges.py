@@ -7,7 +7,7 @@ import torch
 from aginfer_b200.recipes import Tensor
 from oracle import paged
 from tests.paged_util import BF, Batch, packaged
-from tests.test_gpu_paged import check_append
+from tests.test_gpu_paged import check_append, run_and_check
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,12 @@ def test_append_in_place_without_a_pitch(tmp_path, new, total, heads):
     angles = paged.rotary_angles(index, 1e6, d)
     turned = lambda t: (paged.turn(t, angles), t.double().abs())  # noqa: E731
     check_append(batch, got, turned(q), turned(k), v)
+
+
+# rows of an item that end inside a warp, where that warp's lanes part: whole items, items that CTAs share, both streams on the same rows
+@pytest.mark.parametrize("new,total,heads,prefix,spare", [
+    ([45], [2000], (4, 2, 64), 0, 0), ([45, 300], [100, 1500], (3, 1, 128), 0, 5), ([141], [141], (1, 1, 128), 0, 0),
+    ([5, 0, 8], [60, 2, 700], (5, 1, 64), 300, 3), ([1] * 37, list(range(1, 38)), (4, 1, 128), 2500, 4), ([70, 1], [70, 90], (3, 1, 128), 40, 7)], ids=str)
+def test_rows_that_end_inside_a_warp(tmp_path, new, total, heads, prefix, spare):
+    batch = Batch(new, total, 32, heads, prefix=prefix, spare_rows=spare, seed=41)
+    run_and_check(tmp_path, batch, repeats=3, longest=max(new))
