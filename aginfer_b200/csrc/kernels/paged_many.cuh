@@ -316,6 +316,8 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     }
   }
   if (tid == 0) parts.notes[blockIdx.x].pieces = 0;
+  // `places` of a batch of many sequences reaches into the keys' ring, which bulk copies write next
+  if (!kPrefix) tc::fence_async_shared();
   __syncthreads();
 
   auto give_up = [&] { *(volatile unsigned*)&gave_up = 1; };

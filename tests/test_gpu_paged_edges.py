@@ -44,3 +44,11 @@ def test_append_in_place_without_a_pitch(tmp_path, new, total, heads):
 def test_rows_that_end_inside_a_warp(tmp_path, new, total, heads, prefix, spare):
     batch = Batch(new, total, 32, heads, prefix=prefix, spare_rows=spare, seed=41)
     run_and_check(tmp_path, batch, repeats=3, longest=max(new))
+
+
+def test_more_sequences_than_the_queries_memory_holds(tmp_path):
+    """The schedule of 2600 sequences lies in the ring of keys as well (64-wide heads)."""
+    lengths = torch.randint(1, 40, (2600,), generator=torch.Generator().manual_seed(5)).tolist()
+    new = [0 if i % 19 == 7 else 1 for i in range(2600)]
+    new[2000], lengths[2000], new[0], lengths[0] = 150, 700, 60, 60
+    run_and_check(tmp_path, Batch(new, lengths, 16, (2, 1, 64), seed=42), repeats=3, longest=150)
