@@ -68,10 +68,11 @@ __device__ __forceinline__ Span span_of(const Batch& b, const Claim& c) {
   s.first = int(s.length) - int(s.fresh);
   return s;
 }
-// What a launch checks of every sequence before it uses any: rows in order and a length that the table has room for.  Rows out of
-// order leave the whole launch without work, so that rows add up to no more than there are.
+// What a launch checks of every sequence before it uses any: rows in order and, where it reads keys, a length that the table has
+// room for.  Rows out of order leave the whole launch without work, so that rows add up to no more than there are.
+__device__ __forceinline__ bool rows_in_order(int from, int to, unsigned rows) { return from >= 0 && to >= from && unsigned(to) <= rows; }
 __device__ __forceinline__ bool in_order(const Batch& b, const Claim& c) {
-  const bool ordered = c.from >= 0 && c.to >= c.from && unsigned(c.to) <= b.rows;
+  const bool ordered = rows_in_order(c.from, c.to, b.rows);
   if (!ordered || c.length > int(b.width * b.page)) report(b.status, kBadLength);
   return ordered;
 }
@@ -206,6 +207,10 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
   if (pair < half)
     frequency = exp2(-(double(log2_theta) + double(log2_theta_rest)) * (double(pair % ladder) / double(ladder))) * 0.15915494309189534;
 
+  // Rows out of order leave the whole launch without work.  The first 32 sequences are at hand; more of them cost a trip per 128.
+  bool ordered = paged::rows_in_order(from, to, rows);
+  for (unsigned i = 32 + threadIdx.x; i < sequences; i += 128) ordered = paged::rows_in_order(starts[i], starts[i + 1], rows) && ordered;
+
   // the row's sequence: the first that ends behind it
   int index = 0;
   unsigned seq = sequences;
@@ -223,9 +228,9 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
     index = int(unsigned(__shfl_sync(0xffffffffu, length, at)) - (unsigned(__shfl_sync(0xffffffffu, to, at)) - row));
     break;
   }
-  if (seq >= sequences) return;      // the same for the whole block
+  const bool nobodys = seq >= sequences;      // as all that follows from the row alone, the same for the whole block
   unsigned page_id = 0;
-  bool stored = index >= 0;
+  bool stored = index >= 0 && !nobodys;
   if (stored && unsigned(index) / page >= width) {
     stored = false;
     if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
@@ -241,7 +246,11 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
     if (threadIdx.x == 0) paged::report(status, paged::kBadPage);
   }
   const unsigned token = unsigned(index) % page;
-  __syncthreads();
+  if (!__syncthreads_and(ordered)) {
+    if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
+    return;
+  }
+  if (nobodys) return;
   const unsigned c = threadIdx.x & ((1u << vec_shift) - 1);      // the same pairs in every head that this thread turns
   float co[8], si[8];
 #pragma unroll

@@ -467,8 +467,9 @@ class PagedCache:
     I32: rows starts[b] .. starts[b + 1) of the launch are the new tokens of sequence b, lengths[b] counts the tokens that it
     holds once they are in, table[b, i] is the page of its tokens i * page and on.  All three are read on the device when the
     launch runs, so one packaged recipe serves every step; sequences without new tokens and of length zero are fine.  A page
-    outside the pool or a sequence longer than its table leaves 0x400 or 0x500 in the status word and is not followed; a
-    tensor that does not start on a 16-byte boundary leaves 0x600."""
+    outside the pool or a sequence longer than its table leaves 0x400 or 0x500 in the status word and is not followed; rows out
+    of order (``starts`` that descend, or name rows that the launch has not) leave 0x500 and nothing is done; a tensor that does not
+    start on a 16-byte boundary leaves 0x600."""
     k: Pointer
     v: Pointer
     table: Pointer

@@ -52,3 +52,35 @@ def test_more_sequences_than_the_queries_memory_holds(tmp_path):
     new = [0 if i % 19 == 7 else 1 for i in range(2600)]
     new[2000], lengths[2000], new[0], lengths[0] = 150, 700, 60, 60
     run_and_check(tmp_path, Batch(new, lengths, 16, (2, 1, 64), seed=42), repeats=3, longest=150)
+
+
+# rows of three sequences (or, below, of many) that are not in order: they end before they begin, lie outside the launch, leave a gap to fall into
+DISORDER = ([5, 0, -3, 2], [0, 2 ** 31 - 1, -2 ** 31, 3], [-1, -1, -1, -1], [0, 2, 1, 3], [0, 1, 2, 90000], [-1, 1, 2, 3], [2, 1, 0, 0])
+
+
+@pytest.mark.parametrize("sequences,at", [(3, 0), (40, 0), (40, 36), (400, 33), (400, 396)], ids=str)
+def test_append_with_rows_out_of_order_does_nothing_and_says_so(tmp_path, sequences, at):
+    batch = Batch([1] * sequences, [20 + i % 30 for i in range(sequences)], 16, (4, 2, 64), seed=43)
+    hq, hk, d = batch.heads
+    inputs = {n: t for n, t in batch.inputs().items() if n in ("table", "lengths", "starts")}
+    inputs["x"] = torch.randn(batch.rows, (hq + 2 * hk) * d, generator=torch.Generator().manual_seed(2)).to(BF)
+    outputs = {"k": batch.k, "v": batch.v, "q_out": torch.full((batch.rows, hq * d), 77.0).to(BF), "status": torch.zeros(1, dtype=torch.int32)}
+
+    def body(r):
+        r.kv_append(Tensor("x"), Tensor("q_out"), batch.cache(), rows=batch.rows, q_heads=hq, theta=1e6)
+        r.export_status(Tensor("status"))
+
+    runner, dev, out = packaged(tmp_path, inputs, outputs, body)
+    good = dev["starts"].clone()
+    for disorder in DISORDER:
+        dev["starts"].copy_(good)
+        shifted = [min(s + (at if disorder[0] >= 0 else 0), 2 ** 31 - 1) for s in disorder]
+        dev["starts"][at:at + 4] = torch.tensor(shifted, dtype=torch.int32)
+        runner.run(dev, out)
+        assert int(out["status"].cpu()) == 0x500, disorder
+        assert bool((out["q_out"] == 77.0).all()), disorder
+        for name, before in (("k", batch.k), ("v", batch.v)):
+            assert torch.equal(out[name].cpu().view(torch.int16), before.view(torch.int16)), disorder
+    dev["starts"].copy_(good)
+    runner.run(dev, out)
+    assert int(out["status"].cpu()) == 0 and not bool((out["q_out"] == 77.0).any())
