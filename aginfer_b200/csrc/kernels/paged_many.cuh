@@ -246,8 +246,11 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   auto blocks_of = [&](const Span& s) { return (s.fresh * group + kRows - 1) / kRows; };
   unsigned from = 0, to = 0, per = 1;
   if (kPrefix) {      // blocks are alike: every thread finds the run by itself
+    // The launch before does nothing for rows out of order; no part of it would be there to be added.
+    bool ordered = true;
+    for (unsigned i = tid; i < batch.sequences; i += kThreads) ordered = rows_in_order(batch.starts[i], batch.starts[i + 1], batch.rows) && ordered;
     const Span span = span_at(0);
-    const unsigned tiles = (seen_at(span, 0).count + kItemCost) * kv_heads, total = aligned ? blocks_of(span) * tiles : 0u;
+    const unsigned tiles = (seen_at(span, 0).count + kItemCost) * kv_heads, total = __syncthreads_and(ordered && aligned) ? blocks_of(span) * tiles : 0u;
     if (tid == 0 && *prefix_length > int(prefix_pages * batch.page)) report(batch.status, kBadLength);
     per = max((total + gridDim.x - 1) / gridDim.x, least);
     from = min(per * blockIdx.x, total);

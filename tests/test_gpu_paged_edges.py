@@ -6,7 +6,7 @@ import torch
 
 from aginfer_b200.recipes import Tensor
 from oracle import paged
-from tests.paged_util import BF, Batch, packaged
+from tests.paged_util import BF, Batch, attention_outputs, check, packaged
 from tests.test_gpu_paged import check_append, run_and_check
 
 pytestmark = pytest.mark.gpu
@@ -84,3 +84,29 @@ def test_append_with_rows_out_of_order_does_nothing_and_says_so(tmp_path, sequen
     dev["starts"].copy_(good)
     runner.run(dev, out)
     assert int(out["status"].cpu()) == 0 and not bool((out["q_out"] == 77.0).any())
+
+
+@pytest.mark.parametrize("prefix", [0, 90], ids=["", "prefix"])
+@pytest.mark.parametrize("longest,sequences,at", [(1, 3, 0), (80, 3, 0), (1, 450, 440), (80, 450, 440)], ids=str)
+def test_attention_with_rows_out_of_order_does_nothing_and_says_so(tmp_path, prefix, longest, sequences, at):
+    new, total = [1] * sequences, [20 + i % 30 for i in range(sequences)]
+    new[1], total[1] = longest, 100
+    batch = Batch(new, total, 16, (4, 2, 64), prefix=prefix, seed=44)
+    runner, x, out = packaged(tmp_path, batch.inputs(), attention_outputs(batch), lambda r: batch.attend(r, longest=longest))
+    good = x["starts"].clone()
+    runner.run(x, out)            # parts of an earlier pass lie in the workspace from here on
+    assert int(out["status"].cpu()) == 0
+    for disorder in DISORDER:
+        x["starts"].copy_(good)
+        shifted = [min(s + (at if disorder[0] >= 0 else 0), 2 ** 31 - 1) for s in disorder]
+        x["starts"][at:at + 4] = torch.tensor(shifted, dtype=torch.int32)
+        if bool((x["starts"] == good).all()):
+            continue
+        out["o"].fill_(77.0)
+        runner.run(x, out)
+        assert int(out["status"].cpu()) == 0x500, disorder
+        assert bool((out["o"] == 77.0).all()), disorder
+    x["starts"].copy_(good)
+    runner.run(x, out)
+    assert int(out["status"].cpu()) == 0
+    check(batch, out["o"].cpu())
