@@ -59,13 +59,11 @@ class Runner:
                 view = rt.TensorView.from_torch("noise_override", noise_override, self._dtypes.get("noise"))
                 self._override_keep = noise_override
             options = rt.run_options(denoising_steps, view)
-        key = (*inputs, *outputs, *[t.data_ptr() for t in inputs.values()], *[t.data_ptr() for t in outputs.values()])
         tensors = (*inputs.values(), *outputs.values())
         # What the packed views say about a tensor beside its address, looked at on every call: a tensor can be given
-        # another shape or stride in place, and another one can stand at the same address.  Address, shape, strides and dtype
-        # together say which bytes are used; the storage object behind them is not asked (a call
-        # with eight tensors: 8.2 us with it, 7.3 without).
-        layout = [(t.shape, t.stride(), t.dtype) for t in tensors]
+        # another shape or stride in place, its storage can shrink, and another one can stand at the same address.
+        layout = [(t.data_ptr(), t.shape, t.stride(), t.dtype, t.storage_offset(), t.untyped_storage().nbytes()) for t in tensors]
+        key = (*inputs, *outputs, *[described[0] for described in layout])
         bound = self._bindings.get(key)
         if bound is None or bound[1] != layout:
             packed = self.session.bind(

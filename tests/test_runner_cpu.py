@@ -52,3 +52,28 @@ def test_kept_views_are_bounded(runner):
     for x in tensors + tensors[:4]:
         runner.run({"x": x}, {"y": tensors[0]})
     assert len(runner._bindings) == MAX_BINDINGS and len(runner.session.seen) == len(tensors) + 4
+
+
+def test_a_storage_that_shrank_at_its_address_is_described_anew(runner):
+    """What is behind a view is the loader's to check: it is told the bytes that are there now, not those of an earlier call."""
+    import ctypes
+    memory = (ctypes.c_float * 24)()
+    whole, cut = torch.frombuffer(memory, dtype=torch.float32, count=24), torch.frombuffer(memory, dtype=torch.float32, count=6)
+    x, y = torch.empty(0), torch.zeros(3)
+    for source, size in ((whole, 96), (cut, 24), (whole, 96)):
+        x.set_(source.untyped_storage(), 0, (3, 2), (2, 1))
+        runner.run({"x": x}, {"y": y})
+        assert runner.session.seen[-1] == [((3, 2), (2, 1), size)]
+
+
+def test_a_view_further_into_another_storage_of_the_same_size_is_described_anew(runner):
+    import ctypes
+    memory = (ctypes.c_float * 32)()
+    front = torch.frombuffer(memory, dtype=torch.float32, count=24)
+    behind = torch.frombuffer(memory, dtype=torch.float32, count=24, offset=32)
+    x, y = torch.empty(0), torch.zeros(3)
+    for source, offset in ((front, 8), (behind, 0), (front, 8)):      # one address, 64 and 96 bytes behind it
+        x.set_(source.untyped_storage(), offset, (3, 2), (2, 1))
+        assert x.data_ptr() == ctypes.addressof(memory) + 32
+        runner.run({"x": x}, {"y": y})
+        assert runner.session.seen[-1] == [((3, 2), (2, 1), 96 - 4 * offset)]
