@@ -3,8 +3,9 @@
 //
 // Bound by memory: a key and a value are 4 head_dim bytes and meet at most 32 rows.  So the unit of work is a tile of 64 keys of
 // one sequence and key head, all units of the batch in one line, and every CTA takes an equal run of it, however unequal the
-// sequences are: sequences and heads that a run cuts leave unnormalised sums, their maximum and weight in scratch, and the last
-// CTA of such an item to arrive adds them in order (nobody waits for another CTA; sums do not depend on who arrives when).
+// sequences are.  Runs are even shares in a batch that fills the card, and longer, on fewer CTAs, where parts to be added would cost
+// more (see run_length).  Sequences and heads that a run cuts leave unnormalised sums, their maximum and weight in scratch, and the
+// last CTA of such an item to arrive adds them in order (nobody waits for another CTA; sums do not depend on who arrives when).
 //
 // A CTA: one loading warp that brings tiles in by bulk copies, a copy per page (or the part of it in the tile) and 64-column
 // block, into a ring; four warps that share a tile's keys, 16 each, with maximum, sum and outputs of their own until the item ends.
@@ -26,9 +27,17 @@ namespace few {
 using namespace paged;
 
 constexpr unsigned kKeys = 64, kConsumers = 128, kThreads = 160;
-// CTAs that share an item: a small batch could have more, but adding their parts then takes longer than the tiles that it saves
-// (one token over 1500 keys, 24 tiles: 24 parts 14.5 us, 12 or 8 or 6 parts 12.4, 4 parts 14.6).
-constexpr unsigned kMostParts = 12;
+// The last CTA of an item adds its parts, four loads at a time, so a run is longer than an even share where that would make many parts:
+// one tile a part costs 0.7 us of a CTA on its own, four more parts 1.4 us of the last one, which n tiles balance at runs of sqrt(n / 2).
+// One token, 16 query heads on 2, us (these runs | even shares | at most 12 parts whatever the length):
+//   1500 keys 12.3 | 14.3 | 12.3, 8192 18.4 | 39.7 | 22.5, 32000 31 - 33 | 43.6 | 47, 131072 56 | 71 | 150.
+// Twelve parts are few enough below 72 tiles (700 keys 12.3, runs of sqrt(n / 2) 14.3).  Where the batch is large enough to keep memory
+// busy, a third more than an even share is better than more parts (four sequences of 32000 keys on 4 heads 59.6, without it 62.4).
+constexpr unsigned kFewParts = 12;
+__device__ __forceinline__ unsigned run_length(unsigned total, unsigned longest, unsigned ctas) {
+  const unsigned even = (total + ctas - 1) / ctas, balanced = unsigned(ceilf(sqrtf(float(longest) * 0.5f)));
+  return max(even, min((longest + kFewParts - 1) / kFewParts, max(balanced, even + even / 3)));
+}
 constexpr float kSlack = 8.f;               // log2 of how far scores may exceed the maximum that weights are relative to
 
 // How many units one sequence is: its key heads x row blocks x key tiles.
@@ -83,7 +92,7 @@ __device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsign
   longest = __reduce_max_sync(0xffffffffu, longest);
   if (!__all_sync(0xffffffffu, ordered)) total = 0;
   Run run;
-  run.per = max((total + gridDim.x - 1) / gridDim.x, (longest + kMostParts - 1) / kMostParts);
+  run.per = run_length(total, longest, gridDim.x);
   run.from = min(run.per * blockIdx.x, total);
   run.to = min(run.from + run.per, total);
   run.seq = run.first = 0;

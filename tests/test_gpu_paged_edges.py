@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from aginfer_b200.recipes import Tensor
+from aginfer_b200.recipes import PagedCache, Tensor
 from oracle import paged
 from tests.paged_util import BF, Batch, attention_outputs, check, packaged
 from tests.test_gpu_paged import check_append, run_and_check
@@ -110,3 +110,40 @@ def test_attention_with_rows_out_of_order_does_nothing_and_says_so(tmp_path, pre
     runner.run(x, out)
     assert int(out["status"].cpu()) == 0
     check(batch, out["o"].cpu())
+
+
+@pytest.mark.parametrize("new,total,heads,kw", [
+    ([1], [9000], (4, 1, 64), {}), ([1], [20000], (2, 2, 128), {}), ([2, 1, 0], [30, 15000, 7], (4, 1, 128), {}), ([1, 4], [12000, 50], (16, 2, 64), {}),
+    ([1], [17000], (2, 1, 64), dict(window=12000, sinks=70)), ([1, 1], [11, 40], (2, 1, 64), {})], ids=str)
+def test_one_long_sequence(tmp_path, new, total, heads, kw):
+    """An item in more parts than a short one is ever cut into."""
+    run_and_check(tmp_path, Batch(new, total, 64, heads, seed=45), repeats=3, longest=max(new), **kw)
+
+
+def test_one_long_sequence_has_the_whole_card(tmp_path):
+    """As many keys in one sequence as in twelve: about the same time, since what CTAs share out are tiles of keys (with an item cut
+    into at most twelve parts it took three times as long)."""
+    def microseconds(sequences: int, keys: int) -> float:
+        pages = sequences * keys // 64
+        specs = {"q": torch.randn(sequences, 16 * 128).to(BF), "starts": torch.arange(sequences + 1, dtype=torch.int32),
+                 "lengths": torch.full((sequences,), keys, dtype=torch.int32), "table": torch.randperm(pages).to(torch.int32).view(sequences, -1),
+                 "k": torch.zeros(pages, 2, 2, 64, 64, dtype=BF), "v": torch.zeros(pages, 2, 2, 64, 64, dtype=BF)}
+        names = {n: Tensor(n) for n in ("k", "v", "table", "lengths", "starts")}
+        cache = PagedCache(**names, sequences=sequences, pages=pages, page=64, pages_per_sequence=keys // 64, kv_heads=2, head_dim=128)
+        where = tmp_path / str(sequences)
+        where.mkdir()
+        runner, x, out = packaged(where, specs, {"o": torch.zeros(sequences, 16 * 128).to(BF)},
+                                  lambda r: r.paged_attention(Tensor("q"), Tensor("o"), cache, rows=sequences, q_heads=16, longest=1))
+        times = []
+        for _ in range(6):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(20):
+                runner.run(x, out)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end) * 50)
+        return min(times)
+
+    many, one = microseconds(12, 64 * 170), microseconds(1, 64 * 170 * 12)
+    assert one < 1.8 * many, (one, many)
