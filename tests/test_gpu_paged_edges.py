@@ -147,3 +147,14 @@ def test_one_long_sequence_has_the_whole_card(tmp_path):
 
     many, one = microseconds(12, 64 * 170), microseconds(1, 64 * 170 * 12)
     assert one < 1.8 * many, (one, many)
+
+
+# Enough key tiles a CTA that every slot of the rings is used again (five stages with 64-wide heads, two with 128), in long items and in
+# many short ones whose last tile is zeroed behind the sequence's end
+@pytest.mark.parametrize("new,total,page,heads,prefix,kw", [
+    ([2000], [2000], 64, (16, 2, 64), 0, {}), ([300], [13000], 32, (8, 2, 64), 0, {}), ([300], [13000], 128, (4, 2, 128), 0, {}),
+    ([33] * 300, [33 + 7 * i % 260 for i in range(300)], 16, (4, 2, 64), 0, {}), ([33] * 150, [33 + 7 * i % 260 for i in range(150)], 16, (4, 2, 128), 0, {}),
+    ([600], [9000], 64, (12, 2, 64), 0, dict(window=3000, sinks=130)), ([4] * 64, [4 + i for i in range(64)], 64, (32, 4, 64), 4100, {}),
+    ([2] * 64, [2 + i for i in range(64)], 32, (28, 4, 128), 3001, {})], ids=lambda v: str(v)[:24])
+def test_rings_that_go_round(tmp_path, new, total, page, heads, prefix, kw):
+    run_and_check(tmp_path, Batch(new, total, page, heads, prefix=prefix, seed=46), repeats=3, longest=max(new), **kw)

@@ -58,3 +58,39 @@ def test_a_second_prompt_is_answered_as_if_it_were_the_first(tmp_path, tokens, w
         for b in range(3):
             whole = dense(cfg, weights, torch.cat([prompt, *[s[b:b + 1] for s in steps]]))
             assert ops.max_rel_err(torch.stack([o[b] for o in got[1:]]), whole[tokens:]) < BOUND, (request, b)
+
+
+def test_a_window_that_hides_most_of_the_prompt(tmp_path, monkeypatch):
+    """Shared pages in the samples' tables, first tokens inside the prompt, a window that begins in the prompt and leaves it."""
+    window, sinks = 12, 3
+    cfg, weights, serving = served(tmp_path, tokens=48, window=window, sinks=sinks, layers=2, new_tokens=20)
+    prompt, steps = hidden(48, 1), [hidden(3, 2 + i) for i in range(20)]
+    got = [serving.prompt(prompt.cuda()).cpu(), *[serving.step(s.cuda()).cpu() for s in steps]]
+    assert serving.status() == 0
+    samples = [torch.cat([prompt, *[s[b:b + 1] for s in steps]]) for b in range(3)]
+    everything = [dense(cfg, weights, x) for x in samples]
+
+    def windowed(q, k, v, *, mask):
+        assert mask == "causal"
+        i, j = torch.arange(q.shape[0])[:, None], torch.arange(k.shape[0])[None, :]
+        seen = (j <= i) & ((i - j < window) | (j < sinks))
+        k, v = (t.float().repeat_interleave(q.shape[1] // t.shape[1], dim=1) for t in (k, v))
+        score = torch.einsum("ihd,jhd->hij", q.float() * q.shape[2] ** -0.5, k).masked_fill(~seen, float("-inf"))
+        return ops.bf16_round(torch.einsum("hij,jhd->ihd", torch.softmax(score, dim=-1), v))
+
+    monkeypatch.setattr(ops, "attention", windowed)
+    for b in range(3):
+        want, answer = dense(cfg, weights, samples[b]), torch.cat([got[0], *[o[b:b + 1] for o in got[1:]]])
+        assert ops.max_rel_err(answer, want) < BOUND, b
+        assert ops.max_rel_err(everything[b][window:], want[window:]) > 5 * BOUND        # the window does hide something
+
+
+def test_a_sample_stops_at_its_pages_and_not_before(tmp_path):
+    _, _, serving = served(tmp_path, tokens=16, layers=1, new_tokens=2)
+    x = hidden(3, 1).cuda()
+    serving.prompt(hidden(16, 0).cuda())
+    serving.step(x)
+    serving.step(x)
+    with pytest.raises(ValueError, match="a sample generates at most 2 tokens"):
+        serving.step(x)
+    assert serving.status() == 0
