@@ -518,18 +518,21 @@ def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> 
 
 
 PAGED_MANY_ROWS, PAGED_MANY_KEYS = 256, 128
-PAGED_MANY_LEAST = 3         # tiles that a CTA takes at the least (288-token prompt: 2 21.9 us, 3 20.6, 4 24.4; a prefix of 288: 26.8, 24.7, 24.8)
 
 
 def paged_many_tiling(cache: PagedCache, blocks: int, tokens: int) -> dict[str, int]:
     """Launch geometry of ``agi_paged_many_bf16_*`` and ``agi_paged_prefix_bf16_*`` for at most ``blocks`` blocks of 256 rows a key head over
     at most ``tokens`` keys: CTAs (one an SM), ring depth, room for the parts of items that the CTAs' runs cut."""
-    d = cache.head_dim
-    units = blocks * cache.kv_heads * ceil_div(tokens, PAGED_MANY_KEYS)
-    grid = min(SM_COUNT, ceil_div(units, PAGED_MANY_LEAST))
+    d, tiles = cache.head_dim, ceil_div(tokens, PAGED_MANY_KEYS)
+    # Tiles that a CTA takes at the least: one where items are short, so that a small launch has CTAs enough, two where they are long and
+    # many parts of one would have to be joined.  28 query heads on 4, us with 1 | 2 | 3: prompts of 64 tokens 15.5 | 20.5 | 26.4, 150
+    # 19.1 | 21.0 | 24.5, 288 20.5 | 20.5 | 22.5, 800 30.7 each; 8 samples behind 500 16.4 | 20.5 | 20.5, 1500 18 | 18.4 | 19.8, 3000
+    # 19.7 | 20.5 | 20.5; 64 tokens over 3000 25.0 | 22.9 | 26.2; drafts behind 4001 (16 heads on 4, 64 wide) 34.8 | 30.8 | 31.
+    least = 1 if tiles <= 16 else 2
+    grid = min(SM_COUNT, ceil_div(blocks * cache.kv_heads * tiles, least))
     rest = 512 * d + 20480 + 1024          # queries, staging of outputs, alignment
     stages = min(6, (MAX_DYNAMIC_SHARED - 2048 - rest) // (512 * d))
-    return {"grid": grid, "stages": stages, "least": PAGED_MANY_LEAST, "shared_bytes": rest + stages * 512 * d,
+    return {"grid": grid, "stages": stages, "least": least, "shared_bytes": rest + stages * 512 * d,
             "scratch_bytes": grid * 2 * (PAGED_MANY_ROWS * d + 2 * PAGED_MANY_ROWS) * 4}
 
 
