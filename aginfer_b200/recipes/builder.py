@@ -819,8 +819,10 @@ class RecipeBuilder:
                     op=f"attention_{mask}", algorithm="warp_per_row")
 
     # ---- paged K/V cache --------------------------------------------------------------------
-    def _declared(self, what: str, pointer: Pointer, dtype: str, elements: int, shape: Sequence[int] | None = None) -> None:
-        """A caller's tensor has to be declared with this dtype and at least so many elements (or exactly this shape)."""
+    def _declared(self, what: str, pointer: Pointer, dtype: str, elements: int, shape: Sequence[int] | None = None,
+                  pitch: int | None = None) -> None:
+        """A caller's tensor has to be declared with this dtype and at least so many elements (or exactly this shape).  ``pitch``: what
+        the launch takes from one row to the next, which whole rows of the tensor have to make up."""
         if not isinstance(pointer, Tensor):
             return
         assert self._profile is not None, "begin_profile first"
@@ -830,6 +832,8 @@ class RecipeBuilder:
         if found["dtype"] != dtype or math.prod(found["shape"]) < elements or (shape is not None and list(found["shape"]) != list(shape)):
             want = f"{list(shape)}" if shape is not None else f"at least {elements} elements"
             raise ValueError(f"{what}: tensor {pointer.name!r} is {found['dtype']} {list(found['shape'])}, not {dtype} with {want}")
+        if pitch is not None and len(found["shape"]) > 1 and pitch % found["shape"][-1]:
+            raise ValueError(f"{what}: rows of tensor {pointer.name!r} are {found['shape'][-1]} wide, the launch would read them {pitch} apart")
 
     def _paged_batch(self, cache: PagedCache, rows: int, q_heads: int) -> None:
         if rows < 1 or rows >= 1 << 24:
@@ -838,7 +842,8 @@ class RecipeBuilder:
             raise ValueError(f"{q_heads} query heads do not share {cache.kv_heads} key heads evenly")
         for what, p in (("keys", cache.k), ("values", cache.v)):
             self._declared(what, p, "BF16", 0, cache.pool_shape)
-        self._declared("table", cache.table, "I32", cache.sequences * cache.pages_per_sequence)
+        self._declared("table", cache.table, "I32", cache.sequences * cache.pages_per_sequence,
+                       pitch=cache.pages_per_sequence if cache.sequences > 1 else None)
         self._declared("lengths", cache.lengths, "I32", cache.sequences)
         self._declared("starts", cache.starts, "I32", cache.sequences + 1)
 
@@ -849,7 +854,7 @@ class RecipeBuilder:
             raise ValueError(f"{what}: a row pitch of {stride} elements is no multiple of 8 that holds {columns}")
         if isinstance(pointer, Arena) and pointer.offset % 16:
             raise ValueError(f"{what}: does not start on a 16-byte boundary")
-        self._declared(what, pointer, "BF16", (rows - 1) * stride + columns)
+        self._declared(what, pointer, "BF16", (rows - 1) * stride + columns, pitch=stride if rows > 1 else None)
         return stride
 
     @staticmethod
@@ -904,7 +909,7 @@ class RecipeBuilder:
             if all(t["name"] != name for t in self._profile.outputs):
                 raise ValueError(f"{name!r} is written: it has to be an output of the profile")
         if positions is not None:
-            self._declared("positions", positions, "I32", rows * (1 if sections is None else 3))
+            self._declared("positions", positions, "I32", rows * (1 if sections is None else 3), pitch=None if sections is None else rows)
         if offset is not None:
             self._declared("offset", offset, "I32", 1)
         s0, s1 = (sections[0], sections[1]) if sections is not None else (POSITIONS_FROM_CACHE if positions is None else POSITIONS_ONE_AXIS, 0)

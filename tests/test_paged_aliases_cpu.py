@@ -15,7 +15,7 @@ def builder() -> RecipeBuilder:
     r = RecipeBuilder({"w": ("BF16", (8,))})
     pool = [9, KV, DIM // 64, 16, 64]
     r.begin_profile("default", [io("q", "BF16", [ROWS, Q]), io("table", "I32", [3, 4]), io("lengths", "I32", [3]), io("starts", "I32", [4])],
-                    [io("x", "BF16", [ROWS, QKV]), io("key", "BF16", [ROWS, Q]), io("o", "BF16", [ROWS, Q]), io("k", "BF16", pool),
+                    [io("x", "BF16", [ROWS, QKV]), io("flat", "BF16", [ROWS * QKV]), io("key", "BF16", [ROWS, Q]), io("o", "BF16", [ROWS, Q]), io("k", "BF16", pool),
                      io("v", "BF16", pool)])
     return r
 
@@ -42,14 +42,14 @@ def test_queries_turned_in_place_keep_their_pitch(x):
 
 
 @pytest.mark.parametrize("q,out,kw", [
-    (Tensor("x"), Tensor("x"), dict(out_stride=Q)),
+    (Tensor("flat"), Tensor("flat"), dict(out_stride=Q)),
     (AT, AT, dict(out_stride=QKV + 8)),
     (AT, AT + 2 * Q, {}),                                     # over the keys
     (AT, AT + 2 * KEYS, dict(out_stride=QKV)),                # over queries of the same row that other threads read
     (AT + 2 * Q, AT, dict(out_stride=Q)),                     # a block of outputs that ends inside what is read
     (AT, AT + 2 * (QKV * (ROWS - 1) + QKV - 8), {}),          # the last row's last values
-    (Tensor("q"), Tensor("key"), dict(k=Tensor("key"), v=Tensor("x"))),
-    (Tensor("q"), Tensor("key"), dict(k=Tensor("x"), v=Tensor("key"))),
+    (Tensor("q"), Tensor("key"), dict(k=Tensor("key"), v=Tensor("o"), kv_stride=Q)),
+    (Tensor("q"), Tensor("key"), dict(k=Tensor("o"), v=Tensor("key"), kv_stride=Q)),
     (AT, AT, dict(row_stride=QKV, k=AT + 2 * (Q - 8), v=AT + 2 * (Q + KEYS), kv_stride=QKV)),
 ], ids=str)
 def test_outputs_over_what_is_still_read_are_refused(q, out, kw):
@@ -76,12 +76,12 @@ def test_attention_in_place_is_at_the_same_pitch(longest, prefix):
         else:
             builder().paged_attention(q, o, cache(), **common)
 
+    attend(AT, AT)
     for x in (Tensor("x"), AT):
-        attend(x, x)
         attend(x, x, q_stride=QKV, o_stride=QKV)
-        for strides in (dict(q_stride=QKV), dict(o_stride=QKV)):
-            with pytest.raises(ValueError, match="still read"):
-                attend(x, x, **strides)
+    for strides in (dict(q_stride=QKV), dict(o_stride=QKV)):
+        with pytest.raises(ValueError, match="still read"):
+            attend(AT, AT, **strides)
     with pytest.raises(ValueError, match="still read"):
         attend(AT, AT + 16)
     attend(AT, AT + 2 * Q * ROWS)
