@@ -9,9 +9,11 @@
 // Two streams share the tensor core: while one stream's scores are exponentiated by its four warps, the other's products run.
 // An item of more than 128 rows gives each stream 128 rows and every key tile; a smaller one gives both streams the same rows
 // and every other tile, and the first stream adds the second one's outputs where they lie in tensor memory.  A thread owns a row: it
-// reads the row's 128 scores from tensor memory, needs no shuffles for maximum and sum, and writes P back over them as bf16 (the
-// sums are of the unrounded weights, in 32 bits).  Outputs are rescaled only when a row's maximum has grown by more than 2^8 since
-// they were last scaled; all of it cancels in the quotient.
+// reads the row's 128 scores from tensor memory, needs no shuffles for maximum and sum, and writes P back over them as bf16.  Sums are of
+// the unrounded weights, in 32 bits; the outputs are 1.9 - 2.3e-3 (2-norm, relative) off the definition, 1.6 - 1.7e-3 of it their own
+// rounding.  Weights in two bf16 pieces would cost half as many products again, where the tensor core works two thirds of a tile's
+// time already.  Outputs are rescaled only when a row's maximum has grown by more than 2^8 since they were last scaled; all of it
+// cancels in the quotient.
 //
 // Keys and values come in by one bulk copy per page (or its part in a tile) and 64-column block: the pool holds the image that
 // the tensor core reads, rows of keys K-major for S, the same image MN-major for P V.  Tokens behind a sequence's end and pages that

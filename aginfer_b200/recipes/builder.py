@@ -928,7 +928,8 @@ class RecipeBuilder:
         """Causal attention of the new tokens over their sequences' pages (their own keys among them: ``kv_append`` comes first).
         ``window``: a token sees itself and the ``window`` - 1 before it (0: everything), and the first ``sinks`` tokens.
         ``longest``: the most new tokens that one sequence has (``rows`` where it is left out); it says which kernel is
-        launched, the result does not depend on it.  A row that sees nothing is zero; rows of no sequence are left alone.
+        launched; results differ by roundings alone.  Weights are rounded to bf16 before they meet the values, maxima and sums are in 32
+        bits.  A row that sees nothing is zero; rows of no sequence are left alone.
         ``o`` may be ``q`` at the same pitch; it shares no other memory with it."""
         self._paged_attention(q, o, cache, None, rows=rows, q_heads=q_heads, longest=longest, window=window, sinks=sinks,
                               q_stride=q_stride, o_stride=o_stride, scale=scale, op="paged_attention")
