@@ -9,6 +9,12 @@
 // holds once they are in, table[b * width + i] the page of its tokens [i * page, (i + 1) * page).  Row r of sequence b stands at
 // index lengths[b] - (starts[b + 1] - r) of its sequence; a row at a negative index is not appended and sees no key.
 //
+// A cache in 8 bits is two pools [pages][kv_heads][page][head_dim] of E4M3 codes and two of scales, [pages][kv_heads][page] of bf16: a token's
+// values of a head are its codes times its scale, the least power of two that brings the largest of them to 448 or less.  With powers of
+// two every code times its scale is a bf16 (as long as that is a normal number), so bringing tokens back rounds nothing, and scales move
+// between operands without rounding either.  The 16-byte chunk c of token t lies at position c ^ (t & 7) of its 128-byte row, or at
+// c ^ ((t >> 1) & 3) of its 64-byte one: ldmatrix reads eight rows without bank conflicts.  A token that is not finite has the scale NaN.
+//
 // starts, lengths and table are read on the device, so that one launch serves every step of a replayed graph.  What they must not
 // say is checked here: a page outside the pool or an index outside the table leaves a code in the status word and nothing is
 // read or written there.
@@ -150,6 +156,43 @@ __device__ __forceinline__ bool sees(int index, unsigned key, unsigned window, u
   return back >= 0 && (window == 0 || unsigned(back) < window || key < sinks);
 }
 
+// ---- a cache in 8 bits ----
+// Position of 16-byte chunk c in token t's row.
+__device__ __forceinline__ unsigned code_chunk(unsigned c, unsigned t, unsigned head_dim) { return c ^ (head_dim == 128 ? t & 7u : (t >> 1) & 3u); }
+
+// The largest |x| of 16 values, as bits: these order like the numbers, infinities and NaN above all of them.
+__device__ __forceinline__ unsigned peak_bits(const float* x, unsigned count, unsigned peak = 0u) {
+#pragma unroll
+  for (unsigned i = 0; i < count; ++i) peak = max(peak, __float_as_uint(x[i]) & 0x7fffffffu);
+  return peak;
+}
+// The scale of a row with that peak, as the bits of a power of two (a bf16 too): 448 = 1.75 * 2^8, so 2^(exponent - 8), or twice that where the
+// peak's fraction is above 1.75.  One for a row of zeros, 2^-126 at the least, NaN for a row that is not finite.
+__device__ __forceinline__ unsigned scale_bits(unsigned peak) {
+  if (peak >= 0x7f800000u) return 0x7fc00000u;
+  if (peak == 0u) return 0x3f800000u;
+  const int exponent = int(peak >> 23) - 8 + ((peak & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return unsigned(max(exponent, 1)) << 23;
+}
+// What values are multiplied by to become codes: one over the scale, or zero where that is NaN.
+__device__ __forceinline__ float inverse_scale(unsigned scale) { return scale > 0x7f000000u ? 0.f : __uint_as_float((254u << 23) - scale); }
+__device__ __forceinline__ uint2 codes8(const float* x, float by) {
+  return make_uint2(float4_to_e4m3x4(x[0] * by, x[1] * by, x[2] * by, x[3] * by), float4_to_e4m3x4(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
+}
+// The largest of the peaks of `lanes` (4 or 8) lanes side by side, all of them here.
+__device__ __forceinline__ unsigned peak_of_lanes(unsigned peak, unsigned lanes) {
+  const unsigned lane = threadIdx.x & 31, mask = ((1u << lanes) - 1) << (lane & ~(lanes - 1));
+  for (unsigned o = 1; o < lanes; o <<= 1) peak = max(peak, __shfl_xor_sync(mask, peak, o));
+  return peak;
+}
+
+// Where an append leaves keys and values: pools of bf16, or codes and scales.
+template <bool kE4m3>
+struct Pools {
+  unsigned char *k, *v;
+  bf16 *k_scale, *v_scale;
+};
+
 }  // namespace paged
 
 // Queries and keys of a step's new tokens turned by their positions (half-split pairs, see rope.cuh), queries written to `q_out`,
@@ -161,22 +204,26 @@ __device__ __forceinline__ bool sees(int index, unsigned key, unsigned window, u
 // grid = rows, block = 128.  head_dim 64 or 128, strides multiples of 8.
 constexpr unsigned kPositionsFromCache = 0xffffffffu;   // s0: the index in the sequence, plus *offset where has_offset
 constexpr unsigned kPositionsOneAxis = 0xfffffffeu;     // s0: pos[row]; otherwise pos[3][rows] with sections s0, s1, rest
-extern "C" __global__ void __launch_bounds__(128)
-agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_column, unsigned v_column, bf16* q_out, bf16* k_pool,
-                   bf16* v_pool, const int* starts, const int* lengths, const int* table, const int* pos, const int* offset,
-                   unsigned* status, unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width,
-                   unsigned q_heads, unsigned kv_heads, unsigned head_dim, unsigned q_stride, unsigned kv_stride,
-                   unsigned out_stride, float log2_theta, float log2_theta_rest, unsigned s0, unsigned s1, unsigned ladder,
-                   unsigned has_offset) {
+namespace paged {
+template <bool kE4m3>
+__device__ __forceinline__ void append_body(const bf16* q, const bf16* k, const bf16* v, unsigned k_column, unsigned v_column, bf16* q_out,
+                                            const Pools<kE4m3>& into, const int* starts, const int* lengths, const int* table, const int* pos,
+                                            const int* offset, unsigned* status, unsigned rows, unsigned sequences, unsigned pages, unsigned page,
+                                            unsigned width, unsigned q_heads, unsigned kv_heads, unsigned head_dim, unsigned q_stride,
+                                            unsigned kv_stride, unsigned out_stride, float log2_theta, float log2_theta_rest, unsigned s0,
+                                            unsigned s1, unsigned ladder, unsigned has_offset) {
   __shared__ __align__(16) float cosine[64], sine[64];
   grid_dependency_wait();
   const unsigned half = head_dim / 2, vec_shift = head_dim == 128 ? 3 : 2, turned = (q_heads + kv_heads) << vec_shift;
-  const unsigned blocks = head_dim / 64, copied = kv_heads * blocks * 8, row = blockIdx.x, lane = threadIdx.x & 31;
+  // values go in pieces of eight, in 8 bits of sixteen
+  const unsigned blocks = head_dim / 64, copied = kE4m3 ? kv_heads * (head_dim / 16) : kv_heads * blocks * 8, row = blockIdx.x, lane = threadIdx.x & 31;
+  bf16* const k_pool = reinterpret_cast<bf16*>(into.k);
+  bf16* const v_pool = reinterpret_cast<bf16*>(into.v);
   k += k_column;
   v += v_column;
-  if (!(paged::aligned16(q) && paged::aligned16(k) && paged::aligned16(v) && paged::aligned16(q_out) && paged::aligned16(k_pool) &&
-        paged::aligned16(v_pool))) {
-    if (threadIdx.x == 0) paged::report(status, paged::kMisaligned);
+  if (!(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) && aligned16(into.k) && aligned16(into.v) &&
+        (!kE4m3 || (aligned16(into.k_scale) && aligned16(into.v_scale))))) {
+    if (threadIdx.x == 0) report(status, kMisaligned);
     return;
   }
   const bf16* const q_row = q + size_t(row) * q_stride;
@@ -188,14 +235,19 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
   };
   constexpr unsigned kAhead = 2;      // vectors of a thread that do not wait for where the row goes
   Bf16x8 lo[kAhead], hi[kAhead];
-  uint4 value = make_uint4(0u, 0u, 0u, 0u);
+  constexpr unsigned kVectors = kE4m3 ? 2 : 1;      // of a piece of values
+  uint4 value[kVectors] = {};
 #pragma unroll
   for (unsigned u = 0; u < kAhead; ++u)
     if (threadIdx.x + u * 128 < turned) {
       lo[u] = *reinterpret_cast<const Bf16x8*>(from_of(threadIdx.x + u * 128));
       hi[u] = *reinterpret_cast<const Bf16x8*>(from_of(threadIdx.x + u * 128) + half);
     }
-  if (threadIdx.x < copied) value = *reinterpret_cast<const uint4*>(v_row + threadIdx.x * 8);
+  auto values_of = [&](unsigned item, uint4* to_item) {
+#pragma unroll
+    for (unsigned i = 0; i < kVectors; ++i) to_item[i] = reinterpret_cast<const uint4*>(v_row)[item * kVectors + i];
+  };
+  if (threadIdx.x < copied) values_of(threadIdx.x, value);
 
   // A position that does not follow from the cache is asked for here too, and turns per position, 1 / (2 pi theta^(pair mod ladder /
   // ladder)), are computed while all of this is on its way.
@@ -208,8 +260,8 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
     frequency = exp2(-(double(log2_theta) + double(log2_theta_rest)) * (double(pair % ladder) / double(ladder))) * 0.15915494309189534;
 
   // Rows out of order leave the whole launch without work.  The first 32 sequences are at hand; more of them cost a trip per 128.
-  bool ordered = paged::rows_in_order(from, to, rows);
-  for (unsigned i = 32 + threadIdx.x; i < sequences; i += 128) ordered = paged::rows_in_order(starts[i], starts[i + 1], rows) && ordered;
+  bool ordered = rows_in_order(from, to, rows);
+  for (unsigned i = 32 + threadIdx.x; i < sequences; i += 128) ordered = rows_in_order(starts[i], starts[i + 1], rows) && ordered;
 
   // the row's sequence: the first that ends behind it
   int index = 0;
@@ -233,7 +285,7 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
   bool stored = index >= 0 && !nobodys;
   if (stored && unsigned(index) / page >= width) {
     stored = false;
-    if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
+    if (threadIdx.x == 0) report(status, kBadLength);
   }
   if (stored) page_id = unsigned(table[size_t(seq) * width + unsigned(index) / page]);
   if (pair < half) {
@@ -243,11 +295,11 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
   }
   if (stored && page_id >= pages) {
     stored = false;
-    if (threadIdx.x == 0) paged::report(status, paged::kBadPage);
+    if (threadIdx.x == 0) report(status, kBadPage);
   }
   const unsigned token = unsigned(index) % page;
   if (!__syncthreads_and(ordered)) {
-    if (threadIdx.x == 0) paged::report(status, paged::kBadLength);
+    if (threadIdx.x == 0) report(status, kBadLength);
     return;
   }
   if (nobodys) return;
@@ -274,17 +326,40 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
       *reinterpret_cast<Bf16x8*>(to + half) = pack8(y);
     } else if (stored) {
       // chunk c of the head's first half and the same chunk of its second half: of one 64-column block, or of two
-      const unsigned behind = c + (1u << vec_shift);
-      bf16* first = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, c / 8, page) + token) * 64;
-      bf16* second = k_pool + (paged::block_offset(page_id, kv_heads, head - q_heads, blocks, behind / 8, page) + token) * 64;
-      *reinterpret_cast<Bf16x8*>(first + (((c & 7) ^ (token & 7)) * 8)) = pack8(x);
-      *reinterpret_cast<Bf16x8*>(second + (((behind & 7) ^ (token & 7)) * 8)) = pack8(y);
+      const unsigned kv_head = head - q_heads, behind = c + (1u << vec_shift);
+      if constexpr (kE4m3) {
+        const unsigned scale = scale_bits(peak_of_lanes(peak_bits(y, 8, peak_bits(x, 8)), 1u << vec_shift));
+        const float by = inverse_scale(scale);
+        const size_t at = block_offset(page_id, kv_heads, kv_head, 1, 0, page) + token;
+        unsigned char* const to_row = into.k + at * head_dim;
+        *reinterpret_cast<uint2*>(to_row + code_chunk(c / 2, token, head_dim) * 16 + (c & 1) * 8) = codes8(x, by);
+        *reinterpret_cast<uint2*>(to_row + code_chunk(behind / 2, token, head_dim) * 16 + (c & 1) * 8) = codes8(y, by);
+        if (c == 0) into.k_scale[at] = __ushort_as_bfloat16((unsigned short)(scale >> 16));
+      } else {
+        bf16* first = k_pool + (block_offset(page_id, kv_heads, kv_head, blocks, c / 8, page) + token) * 64;
+        bf16* second = k_pool + (block_offset(page_id, kv_heads, kv_head, blocks, behind / 8, page) + token) * 64;
+        *reinterpret_cast<Bf16x8*>(first + (((c & 7) ^ (token & 7)) * 8)) = pack8(x);
+        *reinterpret_cast<Bf16x8*>(second + (((behind & 7) ^ (token & 7)) * 8)) = pack8(y);
+      }
     }
   };
-  auto keep = [&](unsigned item, const uint4& from) {
-    const unsigned head = item / (blocks * 8), c = item % (blocks * 8);
-    bf16* to = v_pool + (paged::block_offset(page_id, kv_heads, head, blocks, c / 8, page) + token) * 64;
-    *reinterpret_cast<uint4*>(to + (((c & 7) ^ (token & 7)) * 8)) = from;
+  auto keep = [&](unsigned item, const uint4* from) {
+    if constexpr (kE4m3) {
+      const unsigned chunks = head_dim / 16, head = item / chunks, c = item % chunks;
+      float x[16];
+      unpack8(*reinterpret_cast<const Bf16x8*>(from), x);
+      unpack8(*reinterpret_cast<const Bf16x8*>(from + 1), x + 8);
+      const unsigned scale = scale_bits(peak_of_lanes(peak_bits(x, 16), chunks));
+      const float by = inverse_scale(scale);
+      const size_t at = block_offset(page_id, kv_heads, head, 1, 0, page) + token;
+      const uint2 first = codes8(x, by), second = codes8(x + 8, by);
+      *reinterpret_cast<uint4*>(into.v + at * head_dim + code_chunk(c, token, head_dim) * 16) = make_uint4(first.x, first.y, second.x, second.y);
+      if (c == 0) into.v_scale[at] = __ushort_as_bfloat16((unsigned short)(scale >> 16));
+    } else {
+      const unsigned head = item / (blocks * 8), c = item % (blocks * 8);
+      bf16* to_row = v_pool + (block_offset(page_id, kv_heads, head, blocks, c / 8, page) + token) * 64;
+      *reinterpret_cast<uint4*>(to_row + (((c & 7) ^ (token & 7)) * 8)) = *from;
+    }
   };
 #pragma unroll
   for (unsigned u = 0; u < kAhead; ++u)
@@ -295,6 +370,34 @@ agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_colum
     turn(item, *reinterpret_cast<const Bf16x8*>(from_of(item)), *reinterpret_cast<const Bf16x8*>(from_of(item) + half));
   if (stored) {
 #pragma unroll 1
-    for (unsigned item = threadIdx.x + 128; item < copied; item += 128) keep(item, *reinterpret_cast<const uint4*>(v_row + item * 8));
+    for (unsigned item = threadIdx.x + 128; item < copied; item += 128) {
+      values_of(item, value);
+      keep(item, value);
+    }
   }
+}
+}  // namespace paged
+
+extern "C" __global__ void __launch_bounds__(128)
+agi_kv_append_bf16(const bf16* q, const bf16* k, const bf16* v, unsigned k_column, unsigned v_column, bf16* q_out, unsigned char* k_pool,
+                   unsigned char* v_pool, const int* starts, const int* lengths, const int* table, const int* pos, const int* offset,
+                   unsigned* status, unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width,
+                   unsigned q_heads, unsigned kv_heads, unsigned head_dim, unsigned q_stride, unsigned kv_stride,
+                   unsigned out_stride, float log2_theta, float log2_theta_rest, unsigned s0, unsigned s1, unsigned ladder,
+                   unsigned has_offset) {
+  paged::append_body<false>(q, k, v, k_column, v_column, q_out, paged::Pools<false>{k_pool, v_pool, nullptr, nullptr}, starts, lengths, table, pos,
+                            offset, status, rows, sequences, pages, page, width, q_heads, kv_heads, head_dim, q_stride, kv_stride, out_stride,
+                            log2_theta, log2_theta_rest, s0, s1, ladder, has_offset);
+}
+// The same into a cache in 8 bits: keys are rounded once, from the turned values in 32 bits.
+extern "C" __global__ void __launch_bounds__(128)
+agi_kv_append_e4m3(const bf16* q, const bf16* k, const bf16* v, unsigned k_column, unsigned v_column, bf16* q_out, unsigned char* k_pool,
+                   unsigned char* v_pool, bf16* k_scale, bf16* v_scale, const int* starts, const int* lengths, const int* table, const int* pos,
+                   const int* offset, unsigned* status, unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width,
+                   unsigned q_heads, unsigned kv_heads, unsigned head_dim, unsigned q_stride, unsigned kv_stride,
+                   unsigned out_stride, float log2_theta, float log2_theta_rest, unsigned s0, unsigned s1, unsigned ladder,
+                   unsigned has_offset) {
+  paged::append_body<true>(q, k, v, k_column, v_column, q_out, paged::Pools<true>{k_pool, v_pool, k_scale, v_scale}, starts, lengths, table, pos,
+                           offset, status, rows, sequences, pages, page, width, q_heads, kv_heads, head_dim, q_stride, kv_stride, out_stride,
+                           log2_theta, log2_theta_rest, s0, s1, ladder, has_offset);
 }

@@ -18,8 +18,16 @@
 // 2.0 - 2.3e-3 (2-norm, relative) off the definition where weights in 32 bits and the outputs' own rounding leave 1.6 - 1.7e-3.  Weights
 // in two bf16 pieces would take that back for twice the products of P V.
 //
+// A cache in 8 bits (kE4m3) brings half the bytes and goes through the same products after a conversion in registers.  Keys become f16,
+// which every code is (one instruction a pair), queries f16 too, times the power of two that brings a row's largest one to 2^14 .. 2^15:
+// bf16 has fewer digits, so that loses nothing but what lies 2^-39 below the row's largest.  Products are then of codes, and a score is
+// multiplied by the row's and the key's power of two.  Values become bf16 by moving bits, which makes a code 2^-120 of itself; the weight
+// that meets it carries the value's scale and 2^64, in bf16, whose range takes scales of any size side by side, and the outputs are
+// multiplied by 2^56.  Pairs of one token's columns are what ldmatrix exchanges, so rows g and g + 8 of a product of values are columns
+// 2 g and 2 g + 1 of its 16.
+//
 // A value behind the sequence's end is whatever the page held before, NaN perhaps, and weight zero does not make it zero: such
-// values are masked as they are read.
+// values are masked as they are read.  In 8 bits it is the scale that is masked: codes as bf16 are finite whatever they are.
 #pragma once
 
 #include "attention.cuh"
@@ -130,13 +138,36 @@ __device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsign
   }
 }
 
-template <int HD16, int kN>
-__device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const Batch& batch, float* own_sums,
+// Two E4M3 codes as f16, and the bytes 0 and 2 or 1 and 3 of four of them as bf16 times 2^-120: the sign stays in front, exponent and
+// fraction move to where bf16 has the low end of its exponent.
+__device__ __forceinline__ unsigned half_pair(unsigned codes) {
+  unsigned h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)codes));
+  return h;
+}
+__device__ __forceinline__ unsigned even_codes(unsigned w) { return ((w << 8) & 0x80008000u) | ((w << 4) & 0x07f007f0u); }
+__device__ __forceinline__ unsigned odd_codes(unsigned w) { return (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u); }
+constexpr float kWeightUnit = 0x1p64f, kOutUnit = 0x1p56f;      // 2^64 * 2^56 * 2^-120 = 1
+__device__ __forceinline__ void skinny_mma_f16(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float scale_at(unsigned addr) {      // a bf16 in shared memory
+  unsigned short bits;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(addr));
+  return __uint_as_float(unsigned(bits) << 16);
+}
+
+template <int HD16, int kN, bool kE4m3>
+__device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const void* k_pool, const void* v_pool, const bf16* k_scale,
+                                               const bf16* v_scale, const Batch& batch, float* own_sums,
                                                float* own_ends, float* scratch, unsigned* counters, unsigned q_heads, unsigned kv_heads,
                                                unsigned q_stride, unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,
                                                unsigned own_only) {
   constexpr unsigned kDim = HD16 * 16, kBlocks = kDim / 64, kRows = 8 * kN;
-  constexpr unsigned kTileBytes = kKeys * kDim * 2, kStageBytes = 2 * kTileBytes, kBlockBytes = kKeys * 128;
+  constexpr unsigned kTileBytes = kKeys * kDim * (kE4m3 ? 1 : 2), kBlockBytes = kKeys * 128, kScaleBytes = kE4m3 ? kKeys * 2 : 0;
+  constexpr unsigned kStageBytes = 2 * kTileBytes + 2 * kScaleBytes;
   constexpr unsigned kMaxStages = 6;
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ __align__(8) unsigned long long full_bar[kMaxStages], empty_bar[kMaxStages];
@@ -160,7 +191,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   // In front of a prefix's launch, which begins without waiting for this one, what this one waits for has to be complete.
   if (own_only) grid_dependency_wait_then_release();
   else grid_dependency_wait();
-  if (!(aligned16(q) && aligned16(o) && aligned16(k_pool) && aligned16(v_pool))) {
+  if (!(aligned16(q) && aligned16(o) && aligned16(k_pool) && aligned16(v_pool) && (!kE4m3 || (aligned16(k_scale) && aligned16(v_scale))))) {
     if (tid == 0) report(batch.status, kMisaligned);
     return;
   }
@@ -193,15 +224,17 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
   if (warp == 4) {
     // ---- loading warp: a lane per piece (keys or values, 64-column block, page or part of one) of a tile ----
     const unsigned shift = 31 - __clz(batch.page), run_tokens = min(batch.page, kKeys), pieces = kKeys / run_tokens;
-    const bool values = lane >= pieces * kBlocks;
-    const unsigned block = (lane / pieces) % kBlocks, piece = lane % pieces;
-    const bool live = lane < 2 * kBlocks * pieces;
-    const unsigned to_slot = (values ? kTileBytes : 0u) + block * kBlockBytes + piece * run_tokens * 128;
-    const unsigned page_bytes = kv_heads * kBlocks * batch.page * 128;
+    // In 8 bits a token of a head is one row, and its scales are a word of two more lines: lanes for keys, values and the scales of both.
+    const unsigned kind = lane / (kE4m3 ? pieces : pieces * kBlocks), block = kE4m3 ? 0u : (lane / pieces) % kBlocks, piece = lane % pieces;
+    const bool values = kE4m3 ? kind & 1 : kind >= 1, scales = kE4m3 && kind >= 2, live = kind < (kE4m3 ? 4u : 2u);
+    const unsigned token_bytes = !kE4m3 ? 128u : scales ? 2u : kDim;
+    const unsigned to_slot = (scales ? 2 * kTileBytes + (values ? kScaleBytes : 0u) : values ? kTileBytes : 0u) + block * kBlockBytes + piece * run_tokens * token_bytes;
+    const unsigned page_bytes = kv_heads * (kE4m3 ? 1u : kBlocks) * batch.page * token_bytes;
+    const unsigned char* const source = reinterpret_cast<const unsigned char*>(scales ? (values ? v_scale : k_scale) : values ? v_pool : k_pool);
     unsigned s = 0, phase = 1;
     walk([&](unsigned seq, unsigned head, unsigned, const Items& it, unsigned begin, unsigned end, unsigned) {
       const int* const pages_of = batch.table + size_t(seq) * batch.width;
-      const unsigned char* const pool = reinterpret_cast<const unsigned char*>(values ? v_pool : k_pool) + size_t((head * kBlocks + block) * batch.page) * 128;
+      const unsigned char* const pool = source + size_t((head * (kE4m3 ? 1u : kBlocks) + block) * batch.page) * token_bytes;
       auto token_of = [&](unsigned t) { return it.seen.tile(t) * kKeys + piece * run_tokens; };
       auto tokens_of = [&](unsigned t) {      // that this lane brings in
         const unsigned token = token_of(t);
@@ -215,8 +248,9 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
           report(batch.status, kBadPage);
           count = 0;
         }
-        const unsigned char* const from_page = pool + size_t(page_id) * page_bytes + (token_of(t) & (batch.page - 1)) * 128;
-        const unsigned bytes = count * 128, all = __reduce_add_sync(0xffffffffu, bytes);
+        const unsigned char* const from_page = pool + size_t(page_id) * page_bytes + (token_of(t) & (batch.page - 1)) * token_bytes;
+        // scales of whole eights of tokens: a copy is of 16 bytes, and a page holds at least 16
+        const unsigned bytes = (scales ? (count + 7) & ~7u : count) * token_bytes, all = __reduce_add_sync(0xffffffffu, bytes);
         unsigned next_count = 0, next_page = 0;      // the page of the tile behind it, while this one's slot is awaited
         if (t + 1 < end) {
           next_count = tokens_of(t + 1);
@@ -248,16 +282,47 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
     // Q as the B operand: row r of the item (token, query head) is column r
     unsigned qb[kN][HD16][2];
     int index[kN][2];                // of rows 2 t and 2 t + 1, whose scores this thread holds
+    float q_unit[kN][2];             // in 8 bits: what these rows' products are multiplied by
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
       unsigned token, sub;
       pairs.at(j * 8 + g, token, sub);
       const bool live = j * 8 + g < rows;
-      const unsigned* from_row = reinterpret_cast<const unsigned*>(q + (live ? size_t(span.row + token) * q_stride + (head * group + sub) * kDim : 0)) + t4;
+      const bf16* const q_row = q + (live ? size_t(span.row + token) * q_stride + (head * group + sub) * kDim : 0);
+      if constexpr (kE4m3) {
+        // columns 4 t .. 4 t + 3 of a chunk of 16 are columns 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of its product, as they are of the keys
+        uint2 pair[HD16];
+        unsigned peak = 0;
 #pragma unroll
-      for (int ks = 0; ks < HD16; ++ks) {
-        qb[j][ks][0] = live ? __ldcg(from_row + ks * 8) : 0u;
-        qb[j][ks][1] = live ? __ldcg(from_row + ks * 8 + 4) : 0u;
+        for (int ks = 0; ks < HD16; ++ks) {
+          pair[ks] = live ? __ldcg(reinterpret_cast<const uint2*>(q_row) + ks * 4 + t4) : make_uint2(0u, 0u);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const unsigned w = e ? pair[ks].y : pair[ks].x;
+            peak = max(peak, max((w << 16) & 0x7fff0000u, w & 0x7fff0000u));
+          }
+        }
+        peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+        peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+        const unsigned unit = min(268u - (peak >> 23), 253u) << 23;       // the power of two that brings the largest to 2^14 .. 2^15
+        const float by = __uint_as_float(unit), back = __uint_as_float((254u << 23) - unit);
+#pragma unroll
+        for (int ks = 0; ks < HD16; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const unsigned w = e ? pair[ks].y : pair[ks].x;
+            const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * by, __uint_as_float(w & 0xffff0000u) * by);
+            qb[j][ks][e] = *reinterpret_cast<const unsigned*>(&h);
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q_unit[j][e] = __shfl_sync(0xffffffffu, back, (2 * t4 + e) * 4) * scale_log2;
+      } else {
+        const unsigned* from_row = reinterpret_cast<const unsigned*>(q_row) + t4;
+#pragma unroll
+        for (int ks = 0; ks < HD16; ++ks) {
+          qb[j][ks][0] = live ? __ldcg(from_row + ks * 8) : 0u;
+          qb[j][ks][1] = live ? __ldcg(from_row + ks * 8 + 4) : 0u;
+        }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -287,18 +352,45 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         for (int j = 0; j < kN; ++j)
 #pragma unroll
           for (int n = 0; n < 2; ++n) score[j][n][0] = score[j][n][1] = score[j][n][2] = score[j][n][3] = 0.f;
-        const unsigned k_row = slot + (warp * 16 + (lane & 15)) * 128;
+        if constexpr (kE4m3) {
+          const unsigned k_row = slot + (warp * 16 + (lane & 15)) * kDim, turn = kDim == 128 ? lane & 7 : (lane >> 1) & 3;
 #pragma unroll
-        for (int ks = 0; ks < HD16; ++ks) {
-          unsigned a0, a1, a2, a3;
-          asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
-                       : "r"(k_row + (ks / 4) * kBlockBytes + ((((ks % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4)));
+          for (int kp = 0; kp < HD16 / 2; ++kp) {
+            unsigned w[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(k_row + (((kp * 2 + (lane >> 4)) ^ turn) << 4)));
 #pragma unroll
-          for (int j = 0; j < kN; ++j) skinny_mma_bf16(score[j][ks & 1], a0, a1, a2, a3, qb[j][ks][0], qb[j][ks][1]);
+            for (int e = 0; e < 2; ++e) {
+              const unsigned a0 = half_pair(w[2 * e]), a1 = half_pair(w[2 * e + 1]), a2 = half_pair(w[2 * e] >> 16), a3 = half_pair(w[2 * e + 1] >> 16);
+#pragma unroll
+              for (int j = 0; j < kN; ++j) skinny_mma_f16(score[j][e], a0, a1, a2, a3, qb[j][2 * kp + e][0], qb[j][2 * kp + e][1]);
+            }
+          }
+        } else {
+          const unsigned k_row = slot + (warp * 16 + (lane & 15)) * 128;
+#pragma unroll
+          for (int ks = 0; ks < HD16; ++ks) {
+            unsigned a0, a1, a2, a3;
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
+                         : "r"(k_row + (ks / 4) * kBlockBytes + ((((ks % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4)));
+#pragma unroll
+            for (int j = 0; j < kN; ++j) skinny_mma_bf16(score[j][ks & 1], a0, a1, a2, a3, qb[j][ks][0], qb[j][ks][1]);
+          }
         }
         // does every row see all of these keys?  (columns behind the item's rows may hold anything)
         const bool whole = int(key0) + 15 <= low && key0 + 16 <= it.seen.end && (window == 0 || int(key0) > int(span.length) - 1 - int(window));
+        auto held = [&](unsigned j) { return j < it.seen.end && (j >= it.seen.start || j < it.seen.sink_end); };
+        float k_unit[2] = {1.f, 1.f}, v_unit[2] = {1.f, 1.f};       // in 8 bits: of keys g and g + 8
+        if constexpr (kE4m3) {
+          const unsigned scales = slot + 2 * kTileBytes + (warp * 16 + g) * 2;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            k_unit[i] = scale_at(scales + i * 16);
+            v_unit[i] = whole || held(key0 + g + i * 8) ? scale_at(scales + kScaleBytes + i * 16) * kWeightUnit : 0.f;
+          }
+        }
         unsigned pb[kN][2];
         bool grows = false;
         float x[kN][4], now[kN][2];
@@ -306,7 +398,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         for (int j = 0; j < kN; ++j) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {       // key g (+ 8), row 2 t (+ 1)
-            x[j][i] = (score[j][0][i] + score[j][1][i]) * scale_log2;
+            x[j][i] = (score[j][0][i] + score[j][1][i]) * (kE4m3 ? q_unit[j][i & 1] * k_unit[i >> 1] : scale_log2);
             const unsigned key = key0 + g + (i >> 1) * 8;
             if (!whole && !(key < it.seen.end && sees(index[j][i & 1], key, window, sinks))) x[j][i] = -INFINITY;
           }
@@ -341,32 +433,52 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
           for (int i = 0; i < 4; ++i) x[j][i] = exp2_of(x[j][i] - (top[j][i & 1] == -INFINITY ? 0.f : top[j][i & 1]));
           sum[j][0] += x[j][0] + x[j][2];
           sum[j][1] += x[j][1] + x[j][3];
+          if constexpr (kE4m3) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] *= v_unit[i >> 1];
+          }
           const bf162 first = __floats2bfloat162_rn(x[j][0], x[j][1]), second = __floats2bfloat162_rn(x[j][2], x[j][3]);
           // keys as rows -> keys as columns: P^T as the B operand of O^T += V^T P^T
           asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[j][0]) : "r"(*reinterpret_cast<const unsigned*>(&first)));
           asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[j][1]) : "r"(*reinterpret_cast<const unsigned*>(&second)));
         }
-        // values: keys 2 t, 2 t + 1 (and + 8) of a column; those that no row of the sequence sees are taken as zero
-        unsigned keep[2];
+        if constexpr (kE4m3) {
+          const unsigned v_row = slot + kTileBytes + (warp * 16 + (lane & 15)) * kDim, turn = kDim == 128 ? lane & 7 : (lane >> 1) & 3;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const unsigned key = key0 + i * 8 + 2 * t4;
-          auto held = [&](unsigned j) { return j < it.seen.end && (j >= it.seen.start || j < it.seen.sink_end); };
-          keep[i] = (held(key) ? 0xffffu : 0u) | (held(key + 1) ? 0xffff0000u : 0u);
-        }
-        const unsigned v_row = slot + kTileBytes + (warp * 16 + (lane >> 4) * 8 + (lane & 7)) * 128;
+          for (int mp = 0; mp < HD16 / 2; ++mp) {
+            unsigned w[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(v_row + (((mp * 2 + (lane >> 4)) ^ turn) << 4)));
 #pragma unroll
-        for (int m = 0; m < HD16; ++m) {
-          unsigned a0, a1, a2, a3;
-          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
-                       : "r"(v_row + (m / 4) * kBlockBytes + ((((m % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4)));
-          a0 &= keep[0];
-          a1 &= keep[0];
-          a2 &= keep[1];
-          a3 &= keep[1];
+            for (int e = 0; e < 2; ++e) {
+              const unsigned a0 = even_codes(w[2 * e]), a1 = odd_codes(w[2 * e]), a2 = even_codes(w[2 * e + 1]), a3 = odd_codes(w[2 * e + 1]);
 #pragma unroll
-          for (int j = 0; j < kN; ++j) skinny_mma_bf16(out[j][m], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+              for (int j = 0; j < kN; ++j) skinny_mma_bf16(out[j][2 * mp + e], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+            }
+          }
+        } else {
+          // values: keys 2 t, 2 t + 1 (and + 8) of a column; those that no row of the sequence sees are taken as zero
+          unsigned keep[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const unsigned key = key0 + i * 8 + 2 * t4;
+            keep[i] = (held(key) ? 0xffffu : 0u) | (held(key + 1) ? 0xffff0000u : 0u);
+          }
+          const unsigned v_row = slot + kTileBytes + (warp * 16 + (lane >> 4) * 8 + (lane & 7)) * 128;
+#pragma unroll
+          for (int m = 0; m < HD16; ++m) {
+            unsigned a0, a1, a2, a3;
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
+                         : "r"(v_row + (m / 4) * kBlockBytes + ((((m % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4)));
+            a0 &= keep[0];
+            a1 &= keep[0];
+            a2 &= keep[1];
+            a3 &= keep[1];
+#pragma unroll
+            for (int j = 0; j < kN; ++j) skinny_mma_bf16(out[j][m], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+          }
         }
       }
       __syncwarp();
@@ -406,9 +518,16 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
         }
       }
 #pragma unroll
-      for (int m = 0; m < HD16; ++m)
+      for (int m = 0; m < HD16; ++m) {
+        if constexpr (kE4m3) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *cell(warp, 2 * t4 + (i & 1), m * 16 + g + (i >> 1) * 8) = out[j][m][i];
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float2*>(cell(warp, 2 * t4 + e, m * 16 + 2 * g)) = make_float2(out[j][m][e] * kOutUnit, out[j][m][e + 2] * kOutUnit);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *cell(warp, 2 * t4 + (i & 1), m * 16 + g + (i >> 1) * 8) = out[j][m][i];
+        }
+      }
       consumers_sync();
 #pragma unroll 1
       for (unsigned i = tid; i < 8 * (kDim / 4); i += kConsumers) {
@@ -494,23 +613,33 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const bf1
 
 }  // namespace few
 
-// grid: any number of CTAs that `scratch` has room for, block = 160, dynamic shared memory = stages * 256 * head_dim + 128 * head_dim + 128.
-// counters: one word per CTA, zero between launches.  own_only: sums, maxima and
+// grid: any number of CTAs that `scratch` has room for, block = 160, dynamic shared memory = stages * 256 * head_dim + 128 * head_dim + 128
+// (in 8 bits stages * (128 * head_dim + 256) + ...).  counters: one word per CTA, zero between launches.  own_only: sums, maxima and
 // weights to own_sums and own_ends instead of o (prefix attention adds the prefix to them).
-#define AGI_PAGED_FEW(NAME, HD16, N, PER_SM)                                                                                          \
+#define AGI_PAGED_FEW_REST                                                                                                            \
+  const int *starts, const int *lengths, const int *table, float *own_sums, float *own_ends, float *scratch, unsigned *counters,      \
+      unsigned *status, unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width, unsigned q_heads,           \
+      unsigned kv_heads, unsigned q_stride, unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,    \
+      unsigned own_only
+#define AGI_PAGED_FEW(SHAPE, HD16, N, PER_SM)                                                                                         \
   extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM)                                                                 \
-  NAME(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, const int* starts, const int* lengths, const int* table,       \
-       float* own_sums, float* own_ends, float* scratch, unsigned* counters, unsigned* status, unsigned rows, unsigned sequences,     \
-       unsigned pages, unsigned page, unsigned width, unsigned q_heads, unsigned kv_heads, unsigned q_stride, unsigned o_stride,      \
-       unsigned window, unsigned sinks, float scale_log2, unsigned stages, unsigned own_only) {                       \
+  agi_paged_few_bf16_##SHAPE(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, AGI_PAGED_FEW_REST) {                    \
     const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                    \
-    few::attention_body<HD16, N>(q, o, k_pool, v_pool, batch, own_sums, own_ends, scratch, counters, q_heads, kv_heads, q_stride,     \
-                                 o_stride, window, sinks, scale_log2, stages, own_only);                                       \
+    few::attention_body<HD16, N, false>(q, o, k_pool, v_pool, nullptr, nullptr, batch, own_sums, own_ends, scratch, counters,         \
+                                        q_heads, kv_heads, q_stride, o_stride, window, sinks, scale_log2, stages, own_only);          \
+  }                                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM)                                                                 \
+  agi_paged_few_e4m3_##SHAPE(const bf16* q, bf16* o, const unsigned char* k_pool, const unsigned char* v_pool, const bf16* k_scale,   \
+                             const bf16* v_scale, AGI_PAGED_FEW_REST) {                                                               \
+    const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                    \
+    few::attention_body<HD16, N, true>(q, o, k_pool, v_pool, k_scale, v_scale, batch, own_sums, own_ends, scratch, counters,          \
+                                       q_heads, kv_heads, q_stride, o_stride, window, sinks, scale_log2, stages, own_only);           \
   }
-AGI_PAGED_FEW(agi_paged_few_bf16_d64_r8, 4, 1, 2)
-AGI_PAGED_FEW(agi_paged_few_bf16_d64_r16, 4, 2, 2)
-AGI_PAGED_FEW(agi_paged_few_bf16_d64_r32, 4, 4, 2)
-AGI_PAGED_FEW(agi_paged_few_bf16_d128_r8, 8, 1, 2)
-AGI_PAGED_FEW(agi_paged_few_bf16_d128_r16, 8, 2, 2)
-AGI_PAGED_FEW(agi_paged_few_bf16_d128_r32, 8, 4, 1)
+AGI_PAGED_FEW(d64_r8, 4, 1, 2)
+AGI_PAGED_FEW(d64_r16, 4, 2, 2)
+AGI_PAGED_FEW(d64_r32, 4, 4, 2)
+AGI_PAGED_FEW(d128_r8, 8, 1, 2)
+AGI_PAGED_FEW(d128_r16, 8, 2, 2)
+AGI_PAGED_FEW(d128_r32, 8, 4, 1)
 #undef AGI_PAGED_FEW
+#undef AGI_PAGED_FEW_REST

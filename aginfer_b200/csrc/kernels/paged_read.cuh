@@ -1,0 +1,138 @@
+// Pages of a cache in 8 bits brought back as pages of bf16: x = code * scale, exact (see paged.cuh).
+//
+// Bound by memory: head_dim + 2 bytes are read and 2 head_dim written for a token, key head and pool.  Only pages are read that hold a
+// token which some row of the batch sees; page i of sequence b goes to page b * width + i of the pools behind, and `table_out` says so to
+// the launches that read them (a page outside the pool is left out and named so that they leave it out too).  Pages of the batch
+// form one line, found by every block as in the attention kernels, of which a warp takes 16 tokens of a page and head at a time: its
+// keys and values are up to eight 16-byte loads a lane, asked for before the first of them is used.
+//
+// Measured: see `read_long` and `read_window` of perf/more_operators.py.
+#pragma once
+
+#include "paged.cuh"
+
+namespace reading {
+
+using namespace paged;
+
+constexpr unsigned kThreads = 256, kTokens = 16, kMaxSequences = 4096;
+enum Flag : unsigned {
+  kFreshOnly = 1,      // sequences without new tokens are left out
+  kNoStarts = 2,       // `starts` is not there: no sequence has new tokens
+};
+
+// The pages of a sequence that hold a visible token: [0, sink) and [window, end).
+struct Seen {
+  unsigned sink, window, count, length;
+};
+
+// 16 codes times a scale, as two 16-byte pieces of bf16.
+__device__ __forceinline__ void widen(const uint4& codes, float scale, Bf16x8 (&to)[2]) {
+  const unsigned word[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __half2 pair(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word[i / 2] >> (16 * (i & 1))), __NV_E4M3));
+    const float2 f = __half22float2(pair);
+    to[i / 4].v[i % 4] = __floats2bfloat162_rn(f.x * scale, f.y * scale);
+  }
+}
+
+}  // namespace reading
+
+// grid: any number of blocks, block = 256.  At most 4096 sequences; head_dim 64 or 128; page a power of two from 16 to 128.
+extern "C" __global__ void __launch_bounds__(reading::kThreads)
+agi_kv_read_e4m3(const unsigned char* k_pool, const unsigned char* v_pool, const bf16* k_scale, const bf16* v_scale, const int* starts,
+                 const int* lengths, const int* table, bf16* k_out, bf16* v_out, int* table_out, unsigned* status, unsigned rows,
+                 unsigned sequences, unsigned pages, unsigned page, unsigned width, unsigned kv_heads, unsigned head_dim, unsigned window,
+                 unsigned sinks, unsigned flags) {
+  using namespace reading;
+  __shared__ unsigned begins[kMaxSequences + 1], of_warp[kThreads / 32];
+  const unsigned tid = threadIdx.x, lane = tid & 31, page_shift = 31 - __clz(page);
+  const Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};
+  grid_dependency_wait();
+  if (!(aligned16(k_pool) && aligned16(v_pool) && aligned16(k_scale) && aligned16(v_scale) && aligned16(k_out) && aligned16(v_out))) {
+    if (tid == 0) report(status, kMisaligned);
+    return;
+  }
+  auto claimed = [&](unsigned seq) { return flags & kNoStarts ? Claim{0, 0, lengths[seq]} : claim_of(batch, seq); };
+  auto seen_of = [&](const Claim& claim) {
+    const Span span = span_of(batch, claim);
+    Seen s{0, 0, 0, span.length};
+    if (span.length == 0 || ((flags & kFreshOnly) && span.fresh == 0)) return s;
+    const unsigned start = window == 0 ? 0u : unsigned(max(span.first - int(window) + 1, 0)), end = (span.length + page - 1) >> page_shift;
+    s.sink = (min(sinks, start) + page - 1) >> page_shift;
+    s.sink = min(s.sink, end);
+    s.window = start < span.length ? max(start >> page_shift, s.sink) : end;      // the next row may see no token that is there
+    s.count = s.sink + (end > s.window ? end - s.window : 0u);
+    return s;
+  };
+  unsigned below = 0;
+  int ordered = 1;
+#pragma unroll 1
+  for (unsigned i0 = 0; i0 < sequences; i0 += kThreads) {
+    const unsigned i = i0 + tid;
+    unsigned mine = 0, all;
+    if (i < sequences) {
+      const Claim claim = claimed(i);
+      if (in_order(batch, claim)) mine = seen_of(claim).count;
+      else ordered = 0;
+    }
+    const unsigned first = below + sum_before<kThreads>(mine, of_warp, &all);
+    if (i < sequences) begins[i] = first;
+    below += all;
+    ordered = __syncthreads_and(ordered);
+  }
+  if (!ordered) return;
+
+  const unsigned pieces = page / kTokens, chunk_shift = head_dim == 128 ? 3 : 2, chunks = 1u << chunk_shift, blocks = head_dim / 64;
+  const unsigned step = 32 >> chunk_shift, loads = kTokens / step;        // tokens that the lanes cover at a time
+  const unsigned items = below * kv_heads * pieces, stride = gridDim.x * (kThreads / 32);
+  const unsigned position = lane & (chunks - 1), lane_token = lane >> chunk_shift;
+#pragma unroll 1
+  for (unsigned item = blockIdx.x * (kThreads / 32) + (tid >> 5); item < items; item += stride) {
+    const unsigned piece = item & (pieces - 1), rest = item / pieces, line = rest / kv_heads, head = rest - line * kv_heads;
+    unsigned seq = 0;      // the last sequence that begins at or before the page
+    for (unsigned above = sequences; above - seq > 1;) {
+      const unsigned middle = (seq + above) / 2;
+      if (begins[middle] <= line) seq = middle; else above = middle;
+    }
+    const Seen seen = seen_of(claimed(seq));
+    const unsigned at = line - begins[seq], slot = at < seen.sink ? at : seen.window + (at - seen.sink), to = seq * width + slot;
+    const unsigned page_id = unsigned(table[to]);
+    if (piece == 0 && head == 0 && lane == 0) {
+      table_out[to] = page_id < pages ? int(to) : -1;
+      if (page_id >= pages) report(status, kBadPage);
+    }
+    if (page_id >= pages) continue;
+    const unsigned held = min(seen.length - slot * page, page);       // tokens of the page
+    const size_t from = block_offset(page_id, kv_heads, head, 1, 0, page), to_row = block_offset(to, kv_heads, head, blocks, 0, page);
+    uint4 codes[2][4];
+    float scale[2][4];
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+      const unsigned token = piece * kTokens + lane_token + i * step;
+      if (i < loads && token < held) {
+        codes[0][i] = reinterpret_cast<const uint4*>(k_pool + (from + token) * head_dim)[position];
+        codes[1][i] = reinterpret_cast<const uint4*>(v_pool + (from + token) * head_dim)[position];
+        scale[0][i] = __bfloat162float(k_scale[from + token]);
+        scale[1][i] = __bfloat162float(v_scale[from + token]);
+      }
+    }
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+      const unsigned token = piece * kTokens + lane_token + i * step;
+      if (i >= loads || token >= held) continue;
+      const unsigned chunk = code_chunk(position, token, head_dim);       // exchanging chunks is its own inverse
+      const size_t row = (to_row + size_t(chunk / 4) * page + token) * 64;
+      const unsigned c = (chunk & 3) * 2;
+#pragma unroll
+      for (unsigned which = 0; which < 2; ++which) {
+        Bf16x8 out[2];
+        widen(codes[which][i], scale[which][i], out);
+        bf16* const to_block = (which ? v_out : k_out) + row;
+        *reinterpret_cast<Bf16x8*>(to_block + ((c ^ (token & 7)) * 8)) = out[0];
+        *reinterpret_cast<Bf16x8*>(to_block + (((c + 1) ^ (token & 7)) * 8)) = out[1];
+      }
+    }
+  }
+}

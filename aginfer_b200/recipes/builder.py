@@ -18,7 +18,7 @@ from __future__ import annotations
 import functools
 import math
 import struct
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Any, Mapping, Sequence
 
 from ..target import CHECKPOINT_DTYPE_BYTES
@@ -469,7 +469,11 @@ class PagedCache:
     launch runs, so one packaged recipe serves every step; sequences without new tokens and of length zero are fine.  A page
     outside the pool or a sequence longer than its table leaves 0x400 or 0x500 in the status word and is not followed; rows out
     of order (``starts`` that descend, or name rows that the launch has not) leave 0x500 and nothing is done; a tensor that does not
-    start on a 16-byte boundary leaves 0x600."""
+    start on a 16-byte boundary leaves 0x600.
+
+    With ``k_scale`` and ``v_scale`` the cache is held in 8 bits: ``k`` and ``v`` are pools [pages, kv_heads, page, head_dim] of E4M3 codes and
+    the scales [pages, kv_heads, page] of bf16, in the layout of ``layout.quantize_kv_pages``.  A token's values of a head are its codes
+    times its scale, the least power of two that brings the largest of them to 448 or less; a token that is not finite has the scale NaN."""
     k: Pointer
     v: Pointer
     table: Pointer
@@ -481,8 +485,12 @@ class PagedCache:
     pages_per_sequence: int
     kv_heads: int
     head_dim: int
+    k_scale: Pointer | None = None
+    v_scale: Pointer | None = None
 
     def __post_init__(self) -> None:
+        if (self.k_scale is None) != (self.v_scale is None):
+            raise ValueError("keys and values are both held in 8 bits, with scales, or neither is")
         if self.page not in PAGE_TOKENS:
             raise ValueError(f"a page holds {PAGE_TOKENS} tokens, not {self.page}")
         if self.head_dim not in PAGED_HEAD_DIMS:
@@ -495,11 +503,27 @@ class PagedCache:
             raise ValueError("a sequence holds fewer than 2^30 tokens and a pool fewer than 2^31 pages")
 
     @property
+    def quantized(self) -> bool:
+        return self.k_scale is not None
+
+    @property
     def pool_shape(self) -> list[int]:
+        if self.quantized:
+            return [self.pages, self.kv_heads, self.page, self.head_dim]
         return [self.pages, self.kv_heads, self.head_dim // 64, self.page, 64]
+
+    @property
+    def scale_shape(self) -> list[int]:
+        return [self.pages, self.kv_heads, self.page]
+
+    @property
+    def pools(self) -> list[Pointer]:
+        """What an append writes: keys, values and, in 8 bits, their scales."""
+        return [self.k, self.v, *([self.k_scale, self.v_scale] if self.quantized else [])]
 
 
 PAGED_MAX_SEQUENCES = 4096
+KV_READ_FRESH_ONLY, KV_READ_NO_STARTS = 1, 2
 PAGED_FEW_ROWS = 32                      # rows (new tokens x query heads of a key head) of a sequence that mma.sync tiles take
 PAGED_FEW_KEYS = 64                      # keys of a tile
 
@@ -509,7 +533,7 @@ def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> 
     batch evenly, so there are as many as the SMs hold, or as the tables have room for tiles."""
     item = next(r for r in (8, 16, 32) if r >= longest * group or r == 32)
     per_sm = 1 if item == 32 and cache.head_dim == 128 else 2
-    stage, exchange = 4 * PAGED_FEW_KEYS * cache.head_dim, 128 * cache.head_dim
+    stage, exchange = PAGED_FEW_KEYS * (2 * cache.head_dim + 4 if cache.quantized else 4 * cache.head_dim), 128 * cache.head_dim
     stages = min(6, ((228 - per_sm) * 1024 // per_sm - 1024 - exchange) // stage)      # 1 KB of static shared memory
     blocks = min(cache.sequences, rows) * ceil_div(longest * group, item) * cache.kv_heads
     tiles = blocks * ceil_div(cache.pages_per_sequence * cache.page, PAGED_FEW_KEYS)
@@ -840,12 +864,27 @@ class RecipeBuilder:
             raise ValueError(f"a launch works on 1 to 2^24 - 1 rows, not {rows}")
         if q_heads < 1 or q_heads % cache.kv_heads:
             raise ValueError(f"{q_heads} query heads do not share {cache.kv_heads} key heads evenly")
-        for what, p in (("keys", cache.k), ("values", cache.v)):
-            self._declared(what, p, "BF16", 0, cache.pool_shape)
+        self._paged_pools(cache)
         self._declared("table", cache.table, "I32", cache.sequences * cache.pages_per_sequence,
                        pitch=cache.pages_per_sequence if cache.sequences > 1 else None)
         self._declared("lengths", cache.lengths, "I32", cache.sequences)
         self._declared("starts", cache.starts, "I32", cache.sequences + 1)
+
+    def _paged_pools(self, cache: PagedCache) -> None:
+        for what, p, dtype, shape in (("keys", cache.k, "F8_E4M3" if cache.quantized else "BF16", cache.pool_shape),
+                                      ("values", cache.v, "F8_E4M3" if cache.quantized else "BF16", cache.pool_shape),
+                                      ("scales of keys", cache.k_scale, "BF16", cache.scale_shape),
+                                      ("scales of values", cache.v_scale, "BF16", cache.scale_shape)):
+            if p is None:
+                continue
+            if isinstance(p, Arena) and p.offset % 16:
+                raise ValueError(f"{what}: do not start on a 16-byte boundary")
+            self._declared(what, p, dtype, 0, shape)
+
+    def _written(self, *pointers: Pointer) -> None:
+        for name in (p.name for p in pointers if isinstance(p, Tensor)):
+            if all(t["name"] != name for t in self._profile.outputs):
+                raise ValueError(f"{name!r} is written: it has to be an output of the profile")
 
     def _paged_rows(self, what: str, pointer: Pointer, rows: int, columns: int, stride: int | None) -> int:
         """The row pitch of a [rows, columns] operand; 16-byte vectors need rows that start on one."""
@@ -880,7 +919,8 @@ class RecipeBuilder:
         other memory with what is read), keys turned and values as they are into the pages of ``cache``.  ``q``: rows of queries | keys | values side by side (pitch ``row_stride``), or the
         queries alone with ``k`` and ``v`` (pitch ``kv_stride``) beside them.  A position is the token's index in its sequence
         plus the I32 at ``offset`` (a shared prefix in front of the sequences), or it comes from ``positions``: I32 [rows], or with
-        ``sections`` (pairs of the time, height and width axes) [3, rows].  ``ladder`` as in ``mrope``."""
+        ``sections`` (pairs of the time, height and width axes) [3, rows].  ``ladder`` as in ``mrope``.  Into a cache in 8 bits turned keys
+        are rounded once, to their codes, and so are values; rotation and scales are as in 32 bits."""
         self._paged_batch(cache, rows, q_heads)
         d, kv_dim = cache.head_dim, cache.kv_heads * cache.head_dim
         if (k is None) != (v is None) or (k is None and kv_stride is not None):
@@ -905,9 +945,7 @@ class RecipeBuilder:
             self._paged_rows("values", v, rows, kv_dim, kv_stride)
             for what, p in (("keys", k), ("values", v)):
                 self._written_apart("turned queries", written, what, (p, kv_stride, kv_dim), rows)
-        for name in (p.name for p in (q_out, cache.k, cache.v) if isinstance(p, Tensor)):
-            if all(t["name"] != name for t in self._profile.outputs):
-                raise ValueError(f"{name!r} is written: it has to be an output of the profile")
+        self._written(q_out, *cache.pools)
         if positions is not None:
             self._declared("positions", positions, "I32", rows * (1 if sections is None else 3), pitch=None if sections is None else rows)
         if offset is not None:
@@ -915,12 +953,51 @@ class RecipeBuilder:
         s0, s1 = (sections[0], sections[1]) if sections is not None else (POSITIONS_FROM_CACHE if positions is None else POSITIONS_ONE_AXIS, 0)
         log2_theta = struct.unpack("f", struct.pack("f", math.log2(theta)))[0]
         dummy = Arena(0)
-        self.launch("agi_kv_append_bf16", (rows, 1, 1), (128, 1, 1),
-                    [q, k, v, U32(k_column), U32(v_column), q_out, cache.k, cache.v, cache.starts, cache.lengths, cache.table,
+        self.launch("agi_kv_append_e4m3" if cache.quantized else "agi_kv_append_bf16", (rows, 1, 1), (128, 1, 1),
+                    [q, k, v, U32(k_column), U32(v_column), q_out, *cache.pools, cache.starts, cache.lengths, cache.table,
                      positions or dummy, offset or dummy, Arena(STATUS_WORD), U32(rows), U32(cache.sequences), U32(cache.pages),
                      U32(cache.page), U32(cache.pages_per_sequence), U32(q_heads), U32(cache.kv_heads), U32(d), U32(row_stride),
                      U32(kv_stride), U32(out_stride), F32(log2_theta), F32(math.log2(theta) - log2_theta), U32(s0), U32(s1),
                      U32(ladder or d // 2), U32(0 if offset is None else 1)], op="kv_append", algorithm="row_per_block")
+
+    def kv_read(self, cache: PagedCache, to: PagedCache, *, rows: int, window: int = 0, sinks: int = 0) -> None:
+        """The batch's pages of a cache in 8 bits as bf16 pages, exactly: page i of sequence b goes to page b * pages_per_sequence + i of the
+        pools of ``to``, which has as many pages at least, and ``to.table`` says so, so that ``to`` is a cache of the same batch.  With
+        ``window`` only pages are brought back that hold a token which the next rows of their sequence see (as in ``paged_attention``; rows
+        that are not there yet where a sequence has no new ones); other pages, tokens behind a sequence's end and their places in the
+        table are left as they are.  ``rows``: those that ``cache.starts`` shares out.  A page outside the pool is -1 in ``to.table``."""
+        if not cache.quantized or to.quantized:
+            raise ValueError("kv_read goes from a cache in 8 bits to one of bf16")
+        same = ("sequences", "page", "pages_per_sequence", "kv_heads", "head_dim", "starts", "lengths")
+        if any(getattr(cache, n) != getattr(to, n) for n in same):
+            raise ValueError("both caches of kv_read hold the same batch: " + ", ".join(same))
+        if to.pages < to.sequences * to.pages_per_sequence:
+            raise ValueError(f"{to.sequences} sequences of {to.pages_per_sequence} pages do not fit {to.pages} pages")
+        if not (0 <= window < 1 << 30 and 0 <= sinks < 1 << 30) or (sinks and not window):
+            raise ValueError("window and sinks are counts of tokens, and sinks go with a window")
+        self._paged_batch(cache, rows, cache.kv_heads)
+        self._paged_batch(to, rows, to.kv_heads)
+        self._written(to.k, to.v, to.table)
+        if len({to.k, to.v, to.table, *cache.pools, cache.table, cache.starts, cache.lengths}) < 10:
+            raise ValueError("kv_read writes into tensors of their own")
+        self._kv_read(cache, to, rows, window, sinks, 0)
+
+    def _kv_read(self, cache: PagedCache, to: PagedCache, rows: int, window: int, sinks: int, flags: int) -> None:
+        pieces = cache.sequences * cache.pages_per_sequence * cache.kv_heads * (cache.page // 16)
+        if pieces >= 1 << 31:
+            raise ValueError("more pages than a launch numbers: fewer sequences or a shorter table")
+        self.launch("agi_kv_read_e4m3", (min(8 * SM_COUNT, ceil_div(pieces, 8)), 1, 1), (256, 1, 1),
+                    [*cache.pools, cache.starts, cache.lengths, cache.table, to.k, to.v, to.table, Arena(STATUS_WORD), U32(rows),
+                     U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence), U32(cache.kv_heads),
+                     U32(cache.head_dim), U32(window), U32(sinks), U32(flags)], op="kv_read", algorithm="warp_per_16_tokens")
+
+    def _read_into_scratch(self, cache: PagedCache, rows: int, window: int, sinks: int, flags: int) -> PagedCache:
+        """The batch's visible pages as bf16 pages in the arena, for the kernels that read these (given back with the caller's mark)."""
+        pages = cache.sequences * cache.pages_per_sequence
+        pool = pages * cache.kv_heads * cache.page * cache.head_dim * 2
+        to = replace(cache, k=self.alloc(pool), v=self.alloc(pool), table=self.alloc(pages * 4), pages=pages, k_scale=None, v_scale=None)
+        self._kv_read(cache, to, rows, window, sinks, flags)
+        return to
 
     def paged_attention(self, q: Pointer, o: Pointer, cache: PagedCache, *, rows: int, q_heads: int, longest: int | None = None,
                         window: int = 0, sinks: int = 0, q_stride: int | None = None, o_stride: int | None = None,
@@ -970,34 +1047,44 @@ class RecipeBuilder:
             raise ValueError("more key tiles than a launch numbers: fewer rows or a shorter table")
         # prefix attention: the sequences' own part, unnormalised, goes in front of the prefix's launch
         own = (self.alloc(rows * q_heads * d * 4), self.alloc(rows * q_heads * 8)) if prefix else (dummy, dummy)
-        shape = [U32(rows), U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence)]
         heads = [U32(q_heads), U32(cache.kv_heads), U32(q_stride), U32(o_stride), U32(window), U32(sinks), F32(scale * math.log2(math.e))]
-        batch = [cache.starts, cache.lengths, cache.table]
+        shape = lambda held: [U32(rows), U32(held.sequences), U32(held.pages), U32(held.page), U32(held.pages_per_sequence)]  # noqa: E731
 
-        def many(kernel: str, join: str, blocks: int, tokens: int, shared: tuple[Pointer, Pointer, int], own_only: int) -> None:
-            t = paged_many_tiling(cache, blocks, tokens)
+        def many(kernel: str, join: str, blocks: int, tokens: int, held: PagedCache, shared: tuple[Pointer, Pointer, int], own_only: int) -> None:
+            t = paged_many_tiling(held, blocks, tokens)
             scratch, notes = self.alloc(t["scratch_bytes"]), self.alloc(t["grid"] * 32)
             self.launch(f"{kernel}_d{d}", (t["grid"], 1, 1), (384, 1, 1),
-                        [q, o, cache.k, cache.v, *batch, shared[0], shared[1], *own, scratch, notes, Arena(STATUS_WORD), *shape, U32(shared[2]),
-                         *heads, U32(t["stages"]), U32(t["least"]), U32(own_only)],
+                        [q, o, held.k, held.v, held.starts, held.lengths, held.table, shared[0], shared[1], *own, scratch, notes, Arena(STATUS_WORD),
+                         *shape(held), U32(shared[2]), *heads, U32(t["stages"]), U32(t["least"]), U32(own_only)],
                         shared_bytes=t["shared_bytes"], op=op, algorithm="tcgen05_row_blocks")
             self.launch(f"{join}_d{d}", (min(8 * SM_COUNT, ceil_div(min(PAGED_MANY_ROWS, rows * group), 8) * t["grid"]), 1, 1), (2 * d, 1, 1),
-                        [o, cache.starts, U32(cache.sequences), *own, scratch, notes, U32(t["grid"]), U32(rows), U32(q_heads), U32(cache.kv_heads),
+                        [o, held.starts, U32(held.sequences), *own, scratch, notes, U32(t["grid"]), U32(rows), U32(q_heads), U32(held.kv_heads),
                          U32(o_stride),
                          U32(own_only)], op=op, algorithm="join_parts")
 
-        if longest * group <= PAGED_FEW_ROWS:
+        # The tensor-core kernel takes bf16 pages: a cache in 8 bits is read back for it, once, whatever the number of row blocks that see a
+        # page.  The prefix's pages come first: its attention begins before the launch in front of it has ended, but not before this one has.
+        few = longest * group <= PAGED_FEW_ROWS
+        held, behind = cache, cache
+        if prefix and cache.quantized:
+            behind = self._read_into_scratch(replace(cache, table=prefix[0], lengths=prefix[1], sequences=1, pages_per_sequence=prefix[2]), rows, 0, 0,
+                                             KV_READ_NO_STARTS)
+            prefix = (behind.table, prefix[1], prefix[2])
+            behind = replace(cache, k=behind.k, v=behind.v, k_scale=None, v_scale=None, pages=behind.pages)
+        if not few and cache.quantized:
+            held = self._read_into_scratch(cache, rows, window, sinks, KV_READ_FRESH_ONLY)
+        if few:
             t = paged_few_tiling(cache, rows, longest, group)
             scratch, counters = self._tc_scratch
-            self.launch(f"agi_paged_few_bf16_d{d}_r{t['rows']}", (t["grid"], 1, 1), (160, 1, 1),
-                        [q, o, cache.k, cache.v, *batch, *own, scratch, counters, Arena(STATUS_WORD), *shape, *heads, U32(t["stages"]),
-                         U32(1 if prefix else 0)],
+            self.launch(f"agi_paged_few_{'e4m3' if cache.quantized else 'bf16'}_d{d}_r{t['rows']}", (t["grid"], 1, 1), (160, 1, 1),
+                        [q, o, *cache.pools, cache.starts, cache.lengths, cache.table, *own, scratch, counters, Arena(STATUS_WORD), *shape(cache),
+                         *heads, U32(t["stages"]), U32(1 if prefix else 0)],
                         shared_bytes=t["shared_bytes"], op=op, algorithm=f"mma_key_tiles_r{t['rows']}")
         else:
             blocks = min(rows * group // PAGED_MANY_ROWS + min(cache.sequences, rows), cache.sequences * ceil_div(longest * group, PAGED_MANY_ROWS))
-            many("agi_paged_many_bf16", "agi_paged_join_bf16", blocks, cache.pages_per_sequence * cache.page, (dummy, dummy, 0), 1 if prefix else 0)
+            many("agi_paged_many_bf16", "agi_paged_join_bf16", blocks, cache.pages_per_sequence * cache.page, held, (dummy, dummy, 0), 1 if prefix else 0)
         if prefix:
-            many("agi_paged_prefix_bf16", "agi_paged_join_prefix_bf16", ceil_div(rows * group, PAGED_MANY_ROWS), prefix[2] * cache.page, prefix, 0)
+            many("agi_paged_prefix_bf16", "agi_paged_join_prefix_bf16", ceil_div(rows * group, PAGED_MANY_ROWS), prefix[2] * cache.page, behind, prefix, 0)
         self.release(mark)
 
     def swiglu(self, gate: Pointer, up: Pointer, out: Pointer, rows: int, cols: int, in_stride: int,

@@ -69,6 +69,41 @@ def unpack_kv_pages(p):
     return t.permute(0, 3, 1, 2, 4, 5).reshape(pages, page, heads, blocks * 64)
 
 
+def quantize_kv_pages(t):
+    """Keys or values [pages, page, kv_heads, head_dim] (head_dim 64 or 128) -> (codes, scales) of a paged cache in 8 bits: E4M3 codes
+    [pages, kv_heads, page, head_dim] as uint8, in which 16-byte chunk c of token t sits at position ``c ^ (t & 7)``, or at
+    ``c ^ ((t >> 1) & 3)`` of a row of 64; scales [pages, kv_heads, page] in bf16, the least power of two that brings the largest |value|
+    of a token and head to 448 or less (one for zeros, 2^-126 at the least, NaN, with codes of zero, where a value is not finite)."""
+    import torch
+    x = t.permute(0, 2, 1, 3).float()
+    peak = x.abs().amax(dim=-1)
+    finite = x.isfinite().all(dim=-1)
+    fraction, exponent = torch.frexp(torch.where(finite, peak, 1.0))        # fraction in [0.5, 1); 448 = 0.875 * 2^9
+    exponent = torch.where(peak > 0, (exponent - 9 + (fraction > 0.875).int()).clamp_min(-126), 0)
+    scale = torch.where(finite, torch.ldexp(torch.ones_like(peak), exponent), float("nan"))
+    codes = torch.where(finite[..., None], x / scale[..., None], 0.0).clamp(-448, 448).to(torch.float8_e4m3fn)
+    return _swap_code_chunks(codes.view(torch.uint8)), scale.to(torch.bfloat16)
+
+
+def read_kv_pages(codes, scales):
+    """Inverse of ``quantize_kv_pages`` but for the rounding: [pages, page, kv_heads, head_dim] in fp32."""
+    import torch
+    t = _swap_code_chunks(codes.view(torch.uint8)).view(torch.float8_e4m3fn).float() * scales.float()[..., None]
+    return t.permute(0, 2, 1, 3).contiguous()
+
+
+def _swap_code_chunks(t):
+    """[..., page, head_dim] bytes with the 16-byte chunks of every token exchanged (its own inverse)."""
+    import torch
+    page, d = t.shape[-2:]
+    if d not in (64, 128):
+        raise ValueError(f"a cache in 8 bits holds heads 64 or 128 wide, not {d}")
+    token = torch.arange(page, device=t.device)[:, None]
+    source = torch.arange(d // 16, device=t.device)[None, :] ^ (token % 8 if d == 128 else token // 2 % 4)
+    chunks = t.reshape(*t.shape[:-1], d // 16, 16)
+    return torch.gather(chunks, -2, source[:, :, None].expand(chunks.shape)).reshape(t.shape).contiguous()
+
+
 def _swap_chunks(t):
     """[..., token, chunk, 8] with chunk c of token r exchanged with chunk c ^ (r & 7) (its own inverse)."""
     import torch
