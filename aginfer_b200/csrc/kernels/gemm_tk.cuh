@@ -314,6 +314,7 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
     }
     __syncwarp();
   }
+  if (!kPacked && (flags & kFlagLateWeights)) grid_dependency_only_wait();      // the launch before writes them
   if (!kPacked && warp < kW && nkb > 0) copy_weights(0);
   if (warp == kMmaWarp) tmem_alloc(&tmem_slot, columns);
   tc_fence_before();

@@ -4,7 +4,8 @@
 // token which some row of the batch sees; page i of sequence b goes to page b * width + i of the pools behind, and `table_out` says so to
 // the launches that read them (a page outside the pool is left out and named so that they leave it out too).  Pages of the batch
 // form one line, found by every block as in the attention kernels, of which a warp takes 16 tokens of a page and head at a time: its
-// keys and values are up to eight 16-byte loads a lane, asked for before the first of them is used.
+// keys and values are up to sixteen 8-byte loads a lane, asked for before the first of them is used.  Eight codes are one 16-byte store,
+// so that a warp's store fills whole lines (with 16 codes and two stores of every other 16 bytes 527 MB took 290 us).
 //
 // Measured: see `read_long` and `read_window` of perf/more_operators.py.
 #pragma once
@@ -26,15 +27,16 @@ struct Seen {
   unsigned sink, window, count, length;
 };
 
-// 16 codes times a scale, as two 16-byte pieces of bf16.
-__device__ __forceinline__ void widen(const uint4& codes, float scale, Bf16x8 (&to)[2]) {
-  const unsigned word[4] = {codes.x, codes.y, codes.z, codes.w};
+// Eight codes times a scale.
+__device__ __forceinline__ Bf16x8 widen(const uint2& codes, float scale) {
+  Bf16x8 to;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __half2 pair(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(word[i / 2] >> (16 * (i & 1))), __NV_E4M3));
+  for (int i = 0; i < 4; ++i) {
+    const __half2 pair(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? codes.x : codes.y) >> (16 * (i & 1))), __NV_E4M3));
     const float2 f = __half22float2(pair);
-    to[i / 4].v[i % 4] = __floats2bfloat162_rn(f.x * scale, f.y * scale);
+    to.v[i] = __floats2bfloat162_rn(f.x * scale, f.y * scale);
   }
+  return to;
 }
 
 }  // namespace reading
@@ -84,10 +86,10 @@ agi_kv_read_e4m3(const unsigned char* k_pool, const unsigned char* v_pool, const
   }
   if (!ordered) return;
 
-  const unsigned pieces = page / kTokens, chunk_shift = head_dim == 128 ? 3 : 2, chunks = 1u << chunk_shift, blocks = head_dim / 64;
-  const unsigned step = 32 >> chunk_shift, loads = kTokens / step;        // tokens that the lanes cover at a time
+  const unsigned pieces = page / kTokens, lane_shift = head_dim == 128 ? 4 : 3, blocks = head_dim / 64;       // lanes of a token: eight codes each
+  const unsigned step = 32 >> lane_shift, loads = kTokens / step;        // tokens that the lanes cover at a time
   const unsigned items = below * kv_heads * pieces, stride = gridDim.x * (kThreads / 32);
-  const unsigned position = lane & (chunks - 1), lane_token = lane >> chunk_shift;
+  const unsigned eight = lane & ((1u << lane_shift) - 1), lane_token = lane >> lane_shift;
 #pragma unroll 1
   for (unsigned item = blockIdx.x * (kThreads / 32) + (tid >> 5); item < items; item += stride) {
     const unsigned piece = item & (pieces - 1), rest = item / pieces, line = rest / kv_heads, head = rest - line * kv_heads;
@@ -106,33 +108,26 @@ agi_kv_read_e4m3(const unsigned char* k_pool, const unsigned char* v_pool, const
     if (page_id >= pages) continue;
     const unsigned held = min(seen.length - slot * page, page);       // tokens of the page
     const size_t from = block_offset(page_id, kv_heads, head, 1, 0, page), to_row = block_offset(to, kv_heads, head, blocks, 0, page);
-    uint4 codes[2][4];
-    float scale[2][4];
+    uint2 codes[2][8];
+    float scale[2][8];
 #pragma unroll
-    for (unsigned i = 0; i < 4; ++i) {
+    for (unsigned i = 0; i < 8; ++i) {
       const unsigned token = piece * kTokens + lane_token + i * step;
       if (i < loads && token < held) {
-        codes[0][i] = reinterpret_cast<const uint4*>(k_pool + (from + token) * head_dim)[position];
-        codes[1][i] = reinterpret_cast<const uint4*>(v_pool + (from + token) * head_dim)[position];
+        codes[0][i] = reinterpret_cast<const uint2*>(k_pool + (from + token) * head_dim)[eight];
+        codes[1][i] = reinterpret_cast<const uint2*>(v_pool + (from + token) * head_dim)[eight];
         scale[0][i] = __bfloat162float(k_scale[from + token]);
         scale[1][i] = __bfloat162float(v_scale[from + token]);
       }
     }
 #pragma unroll
-    for (unsigned i = 0; i < 4; ++i) {
+    for (unsigned i = 0; i < 8; ++i) {
       const unsigned token = piece * kTokens + lane_token + i * step;
       if (i >= loads || token >= held) continue;
-      const unsigned chunk = code_chunk(position, token, head_dim);       // exchanging chunks is its own inverse
-      const size_t row = (to_row + size_t(chunk / 4) * page + token) * 64;
-      const unsigned c = (chunk & 3) * 2;
-#pragma unroll
-      for (unsigned which = 0; which < 2; ++which) {
-        Bf16x8 out[2];
-        widen(codes[which][i], scale[which][i], out);
-        bf16* const to_block = (which ? v_out : k_out) + row;
-        *reinterpret_cast<Bf16x8*>(to_block + ((c ^ (token & 7)) * 8)) = out[0];
-        *reinterpret_cast<Bf16x8*>(to_block + (((c + 1) ^ (token & 7)) * 8)) = out[1];
-      }
+      const unsigned chunk = code_chunk(eight >> 1, token, head_dim);       // exchanging chunks is its own inverse
+      const size_t to_eight = (to_row + size_t(chunk / 4) * page + token) * 64 + (((chunk & 3) * 2 + (eight & 1)) ^ (token & 7)) * 8;
+      *reinterpret_cast<Bf16x8*>(k_out + to_eight) = widen(codes[0][i], scale[0][i]);
+      *reinterpret_cast<Bf16x8*>(v_out + to_eight) = widen(codes[1][i], scale[1][i]);
     }
   }
 }

@@ -31,7 +31,7 @@ SM_COUNT = 148
 
 FLAG_BIAS, FLAG_RESIDUAL, FLAG_OUT_F32, FLAG_SCALED = 1, 2, 1 << 8, 1 << 9
 FLAG_LAYERNORM, FLAG_LN_MODULATE, FLAG_SLAB = 1 << 10, 1 << 11, 1 << 12
-FLAG_SWIGLU, FLAG_MUL_SILU, FLAG_AMAX, FLAG_GROUPS_FIRST = 1 << 13, 1 << 14, 1 << 15, 1 << 16
+FLAG_SWIGLU, FLAG_MUL_SILU, FLAG_AMAX, FLAG_GROUPS_FIRST, FLAG_LATE_WEIGHTS = 1 << 13, 1 << 14, 1 << 15, 1 << 16, 1 << 17
 ACT = {None: 0, "gelu_tanh": 1 << 4, "silu": 2 << 4, "relu": 3 << 4}
 PLAN_DTYPE_BYTES = {"F32": 4, "F16": 2, "BF16": 2, "F8_E4M3": 1, "I32": 4}
 
@@ -329,6 +329,50 @@ def tcs_tiling(M: int, tiles: int, K: int, cluster: int | None = None, groups: i
     gather = cluster * ceil_div(32, cluster) * 512 if cluster > 1 else 0
     return {"cluster": cluster, "groups": groups, "kb": kb, "slices": slices, "ctas": tiles * slices,
             "shared_bytes": kb * 20480 + 1024 + gather}
+
+
+W4_GROUPS = (32, 64, 128)                 # columns that share a scale
+# Tokens up to which codes go straight into products; beyond, they are brought into scratch as bf16 for `gemm`, whose tensor-core kernel begins
+# there.  us, codes | bf16 and gemm: 32 tokens 2560 x 2048 8.5 | 11.7, 22016 x 2048 34 | 138 (the streaming gemm), 48 tokens 10.5 | 11, 45 | 36,
+# 64 tokens 12.5 | 10.9, 62 | 36.
+W4_MAX_ROWS = 32
+
+
+@functools.lru_cache(maxsize=4096)
+def w4_tiling(M: int, N: int, K: int, group: int = 64) -> Mapping[str, Any] | None:
+    """Launch geometry of ``agi_gemm_w4_*``: eights of columns (two a token), parts of K, warps that share a tile's columns, blocks of a copy,
+    ring depth; None where scratch or shared memory do not suffice.
+
+    The least estimate in clocks over parts and ways: rounds of the row tiles over the warps, each 480 clocks a block (what sixteen warps of an SM
+    together take from memory) and 900 besides, 14 a block of tokens laid out; where parts of K meet 1500, 2500 a round, 100 a part and tile.
+    Sixteen tokens of a CTA share a pass over the codes
+    where these are many (16 x 22016 x 2048: 20.4 us, in fours 21.8; 4608 x 3584 11.7 and 10.5)."""
+    eights = 2 if M > 8 and N * K >= 1 << 25 else 1
+    groups, tiles, blocks = ceil_div(M, 4 * eights), ceil_div(N, 16), K // 64
+    best: dict[str, Any] | None = None
+    for splits in range(1, 33):
+        per = ceil_div(blocks, splits)
+        held, ctas = per * eights * (672 if group == 32 else 608), SM_COUNT // (splits * groups)
+        if ctas < 1 or ceil_div(blocks, per) != splits:
+            continue
+        if splits > 1 and (tiles * groups * splits * 256 * eights > TC_SCRATCH_BYTES or tiles * groups * 4 > TC_COUNTER_BYTES):
+            break
+        room = MAX_DYNAMIC_SHARED - W4_STATIC_BYTES - held
+        chunk = next((c for c in (8, 4) if room >= 2 * 16 * c * 576), None)
+        if chunk is None:
+            continue
+        for ways in (8, 4, 2, 1):
+            rounds, mine = ceil_div(tiles, ctas * 2 * 8 // ways), ceil_div(per, ways)
+            cost = rounds * (mine * (480 if eights == 1 else 770) + 900) + per * eights * 14
+            cost += 1500 + 2500 * rounds + 100 * splits * 8 // ways if splits > 1 else 0
+            if best is None or cost < best["cost"]:
+                stages = min(8, room // (16 * chunk * 576))
+                best = {"eights": eights, "splits": splits, "ways": ways, "chunk": chunk, "stages": stages, "cost": cost,
+                        "grid": (min(ceil_div(tiles, 8 // ways), ctas), groups, splits), "shared_bytes": 16 * stages * chunk * 576 + held}
+    return best
+
+
+W4_STATIC_BYTES = 2 * 2 * 8 * 8 * 80 + 2048      # sums of the warps, barriers
 
 
 GRID_SECOND = 65535          # the most a grid's second and third dimensions take
@@ -1099,8 +1143,10 @@ class RecipeBuilder:
              bias: Pointer | None = None, residual: Pointer | None = None, act: str | None = None,
              scale_a: Pointer | None = None, scale_w: Pointer | None = None, ldx: int | None = None,
              ldy: int | None = None, out_f32: bool = False, tactic: str = "auto",
-             splits: int | None = None, packed: bool = False, fixed_order: bool = False) -> None:
+             splits: int | None = None, packed: bool = False, fixed_order: bool = False, late_weights: bool = False) -> None:
         """Y[M, N] = epilogue(X[M, K] . W[N, K]^T); ``dtype`` names the operand type (bf16 or e4m3).
+        ``late_weights``: ``w`` is written by an earlier launch of the profile (the kernels otherwise ask for it before that has ended); with
+        the row-major tcgen05 tactics of the planner.
         ``fixed_order``: K is summed as ``k_runs`` says whatever the tile, for products inside a stack of FP8 blocks.
         ``packed`` (E4M3 only): both operands are in the packed layout of ``recipes/layout.py`` (weights packed
         at packaging time, activations by ``quantize_e4m3(..., packed=)``) and ring slots are filled by bulk copies."""
@@ -1167,6 +1213,8 @@ class RecipeBuilder:
                 tactic = "stream"
             else:
                 tactic = "simt"
+        if late_weights and tactic != "tcgen05_plan":
+            raise ValueError("weights that an earlier launch writes go with the planner's tcgen05 tactic")
         if tactic == "stream":
             # both operands reach shared memory by bulk copies; K is cut into chunks of <= ~100 KB per slot
             if M > 64 or (K * elem) % 64 or not aligned:
@@ -1222,7 +1270,7 @@ class RecipeBuilder:
                 clusters = TK_CLUSTERS[f"agi_gemm_tk_{dtype}"] if runs else (1, 2, 4, 8)
                 t = tk_tiling(M, (N,), K, elem, runs=runs, clusters=clusters)
             self._gemm_tk(f"agi_gemm_tk_{dtype}", f"gemm_{dtype}", t, x, [(w, bias, scale_w, y, N, ldy or N)], M, K, ldx or K,
-                          flags, scale_a=scale_a, other=residual)
+                          flags | (FLAG_LATE_WEIGHTS if late_weights else 0), scale_a=scale_a, other=residual)
             return
         partial, counters = self._tc_scratch
         t = tc_tiling(M, N, K, elem, splits)
@@ -1233,6 +1281,55 @@ class RecipeBuilder:
                     args[:7] + [partial, counters, Arena(STATUS_WORD)] + args[7:] + [U32(t["TN"]), U32(t["stages"])],
                     shared_bytes=t["shared_bytes"], op=f"gemm_{dtype}",
                     algorithm=f"tcgen05_128x{t['TN']}_s{t['stages']}_k{t['splits']}")
+
+    def gemm_w4(self, x: Pointer, w: Pointer, scales: Pointer, y: Pointer, M: int, N: int, K: int, *, group: int = 64, bias: Pointer | None = None,
+                residual: Pointer | None = None, act: str | None = None, ldx: int | None = None, ldy: int | None = None) -> None:
+        """Y[M, N] = epilogue(X[M, K] . W[N, K]^T) with 4-bit weights: W[n, k] = (code - 8) * scale of n's group of ``group`` columns.  ``w`` and
+        ``scales``: the two tensors of ``layout.pack_w4``, from the checkpoint or the caller (codes then I32).  The epilogue is that of ``gemm``.
+        Up to W4_MAX_ROWS tokens codes are multiplied as they are, exactly, with tokens that are off by at most 2^-14 of the largest value of
+        their 64 columns (or 2^-127, if that is more), and sums in 32 bits; beyond, the weights are brought into scratch as bf16, rounded, and ``gemm`` takes them.
+        A token that is not finite makes its outputs NaN."""
+        if group not in W4_GROUPS or K < 64 or K % 64 or K % group:
+            raise ValueError(f"columns come in groups of {W4_GROUPS}, and K is a multiple of the group and of 64, not {K} in groups of {group}")
+        if not (1 <= M < 1 << 24 and 1 <= N < 1 << 24 and K < 1 << 24):
+            raise ValueError(f"a product of {M} x {N} x {K} has a size below 1 or beyond 2^24")
+        tiles = ceil_div(N, 16)
+        ldx, ldy = ldx or K, ldy or N
+        if ldx < K or ldx % 8 or ldy < N:
+            raise ValueError(f"rows of {ldx} and {ldy} elements: those of x hold K and are a multiple of 8, those of y hold N")
+        self._declared("x", x, "BF16", (M - 1) * ldx + K, pitch=ldx if M > 1 else None)
+        self._declared("y", y, "BF16", (M - 1) * ldy + N, pitch=ldy if M > 1 else None)
+        self._declared("codes", w, "I32", 0, [tiles, K // 64, 32, 4])
+        self._declared("scales", scales, "BF16", 0, [tiles, K // group, 8, 2])
+        for what, p, size in (("codes", w, tiles * K * 8), ("scales", scales, tiles * (K // group) * 32)):
+            if isinstance(p, Weight) and self.weight_sizes.get(p.name) != size:
+                raise ValueError(f"{what}: weight {p.name!r} is not the {size} bytes of {N} x {K} in groups of {group}")
+        for what, p, extra in (("bias", bias, N), ("residual", residual, (M - 1) * ldy + N)):
+            if p is not None:
+                self._declared(what, p, "BF16", extra, pitch=ldy if what == "residual" and M > 1 else None)
+        for what, p in (("x", x), ("codes", w), ("scales", scales)):
+            if isinstance(p, Arena) and p.offset % 16:
+                raise ValueError(f"{what}: does not start on a 16-byte boundary")
+        self._written(y)
+        self._written_apart("outputs", (y, ldy, N), "activations", (x, ldx, K), M)
+        dummy = Arena(0)
+        # The codes may be asked for while the launch before is still at work, unless a launch can have written them.
+        early = int(isinstance(w, Weight) or (isinstance(w, Tensor) and all(t["name"] != w.name for t in self._profile.outputs)))
+        t = w4_tiling(M, N, K, group) if M <= W4_MAX_ROWS else None
+        if t is None:
+            mark = self.mark()
+            wide = self.alloc(N * K * 2)
+            self.launch("agi_dequantize_w4_bf16", (min(8 * SM_COUNT, ceil_div(tiles * (K // 64), 8)), 1, 1), (256, 1, 1),
+                        [w, scales, wide, Arena(STATUS_WORD), U32(N), U32(K), U32(group), U32(early)], op="dequantize_w4", algorithm="warp_per_tile")
+            self.gemm(x, wide, y, M, N, K, bias=bias, residual=residual, act=act, ldx=ldx, ldy=ldy, tactic="tcgen05_plan", late_weights=True)
+            self.release(mark)
+            return
+        partial, counters = self._tc_scratch
+        flags = ACT[act] | (FLAG_BIAS if bias else 0) | (FLAG_RESIDUAL if residual else 0)
+        self.launch(f"agi_gemm_w4_g{group}_t{t['eights']}", t["grid"], (576, 1, 1),
+                    [x, w, scales, y, bias or dummy, residual or dummy, partial, counters, Arena(STATUS_WORD), U32(M), U32(N), U32(K),
+                     U32(ldx), U32(ldy), U32(flags), U32(t["ways"]), U32(t["chunk"]), U32(t["stages"]), U32(early)], shared_bytes=t["shared_bytes"], op="gemm_w4",
+                    algorithm=f"mma_t{t['eights']}_w{t['ways']}_k{t['splits']}")
 
     def _gemm_tk(self, family: str, op: str, t: Mapping[str, int], x: Pointer,
                  parts: Sequence[tuple[Pointer, Pointer | None, Pointer | None, Pointer, int, int]], M: int, K: int, ldx: int,

@@ -53,6 +53,56 @@ def unpack_kblock_swizzled(p, rows: int):
     return flat.view(p.dtype)
 
 
+def quantize_w4(t, group: int = 64):
+    """A weight matrix [N, K] -> (codes [N, K] from 0 to 15 as uint8, scales [N, K / group] in bf16): the weight is (code - 8) * scale.  The
+    scale is the largest |weight| of the group over 7, rounded up to a bf16 where rounding down would take it below (none is
+    clipped then); a group of zeros has the scale zero."""
+    import torch
+    n, k = t.shape
+    if k % group:
+        raise ValueError(f"{k} columns do not fall into groups of {group}")
+    x = t.float().reshape(n, k // group, group)
+    least = x.abs().amax(dim=-1) / 7
+    scale = least.to(torch.bfloat16)
+    scale = torch.where(scale.float() < least, torch.nextafter(scale, torch.full_like(scale, float("inf"))), scale)
+    codes = torch.where(scale[..., None] > 0, (x / scale.float()[..., None]).round().clamp(-8, 7) + 8, 8.0)
+    return codes.to(torch.uint8).reshape(n, k), scale
+
+
+def pack_w4(codes, scales):
+    """Codes [N, K] and scales [N, K / group] (``quantize_w4``, or a checkpoint's own) as ``gemm_w4`` takes them: int32
+    [N / 16, K / 64, 32, 4] and bf16 [N / 16, K / group, 8, 2], N rounded up to 16 rows (a checkpoint stores the codes' bits as F32).
+    The four bits from 4 p of word j of lane 4 g + t are the code of row g + 8 (p & 1), column 32 (j >> 1) + 8 t + 4 (j & 1) + (p & 2) + (p >> 2)
+    of a tile of 16 rows and 64 columns: a lane's words are its operands of four matrix products, and its columns are eight in a row."""
+    import torch
+    n, k = codes.shape
+    if k % 64 or k % scales.shape[1] or scales.shape[0] != n:
+        raise ValueError(f"codes {list(codes.shape)} and scales {list(scales.shape)}: K is a multiple of 64 and of the group")
+    tiles, groups = (n + 15) // 16, scales.shape[1]
+    padded = torch.full((tiles * 16, k), 8, dtype=torch.int64, device=codes.device)
+    padded[:n] = codes
+    units = torch.zeros(tiles * 16, groups, dtype=torch.bfloat16, device=codes.device)
+    units[:n] = scales
+    # row: half h, g; column: j >> 1, t, j & 1, p & 2, p >> 2
+    c = padded.reshape(tiles, 2, 8, k // 64, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)      # [tile, block, g, t, j, j, p >> 2, p & 2, p & 1]
+    shift = 4 * torch.arange(8, device=codes.device)
+    words = (c.reshape(tiles, k // 64, 32, 4, 8) << shift).sum(dim=-1)
+    words = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    return words, units.reshape(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+
+
+def unpack_w4(words, scales, rows: int):
+    """Inverse of ``pack_w4``, with the scales applied: the weights [rows, K] in fp32, exact."""
+    import torch
+    tiles, blocks = words.shape[:2]
+    groups = scales.shape[1]
+    shift = 4 * torch.arange(8, device=words.device, dtype=torch.int32)
+    c = (words.view(torch.int32)[..., None] >> shift & 15).reshape(tiles, blocks, 8, 4, 2, 2, 2, 2, 2)
+    c = c.permute(0, 8, 2, 1, 4, 3, 5, 7, 6).reshape(tiles * 16, groups, blocks * 64 // groups)
+    units = scales.permute(0, 3, 2, 1).reshape(tiles * 16, groups, 1)
+    return ((c - 8).float() * units.float()).reshape(tiles * 16, blocks * 64)[:rows]
+
+
 def pack_kv_pages(t):
     """Keys or values [pages, page, kv_heads, head_dim] (2-byte dtype, head_dim a multiple of 64) -> the pool of a paged cache,
     [pages, kv_heads, head_dim / 64, page, 64]: 16-byte chunk c of a token's 64 columns sits at position ``c ^ (token & 7)``, so
