@@ -118,3 +118,26 @@ def test_many_tokens_go_through_bf16_weights_in_scratch():
 def test_what_does_not_fit_is_refused(kw, match):
     with pytest.raises(ValueError, match=match):
         product(builder(), **kw)
+
+
+def test_a_served_decoder_of_fewer_bits_packages():
+    from aginfer_b200.recipes import paged_decode
+    from aginfer_b200.recipes.decoder_layer import LayerConfig
+    from aginfer_b200.recipes.package import describe
+    layer = LayerConfig(hidden=256, heads=4, kv_heads=2, head_dim=64, intermediate=704, tokens=48)
+    for window in (0, 128):
+        cfg = paged_decode.ServeConfig(layer=layer, layers=2, sequences=3, page=16, new_tokens=6, window=window, weight_bits=4, cache_bits=8)
+        weights = paged_decode.quantize_weights(cfg, paged_decode.synthetic_weights(cfg))
+        assert not any(".q_proj" in n or ".gate_proj" in n for n in weights) and weights["model.layers.1.self_attn.qkv_proj.bias"].shape == (512,)
+        plan = paged_decode.build_recipe(cfg, describe(weights)).plan()
+        prompt, step = ([l["kernel"] for l in p["launches"]] for p in plan["shape_dispatch"])
+        assert prompt.count("agi_dequantize_w4_bf16") == 8 and step.count("agi_gemm_w4_g64_t1") == 8      # 48 tokens, three
+        assert prompt.count("agi_kv_append_e4m3") == step.count("agi_kv_append_e4m3") == 2
+        assert step.count("agi_paged_few_e4m3_d64_r8") == 2 and step.count("agi_kv_read_e4m3") == (0 if window else 2)
+
+
+@pytest.mark.parametrize("kw", [dict(weight_bits=8), dict(cache_bits=4), dict(weight_bits=0)], ids=str)
+def test_served_decoders_that_are_refused(kw):
+    from aginfer_b200.recipes import paged_decode
+    with pytest.raises(ValueError, match="bits"):
+        paged_decode.ServeConfig(**kw)
