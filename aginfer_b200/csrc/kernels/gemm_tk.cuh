@@ -30,11 +30,18 @@
 // ~99 cycles and a bulk copy ~54 in operand moves; elected, 39 and 17.  Row-major operands complete on the ring's
 // mbarriers (cp.async.mbarrier.arrive), so the whole ring is in flight.
 //
+// 4-bit weights (kW4, bf16 tokens; the codes and scales of gemm_w4.cuh): the weight warps bring a block's codes into registers, three
+// blocks ahead, and write the slot's B operand themselves: code - 8 times the group's scale, rounded to bf16, four 16-byte pieces of a row a
+// lane and tile.  A tile's codes of all of K are asked into L2 when the CTA begins, a quarter of the bytes that bf16 weights take from memory.
+// What bounds it is a block's turn through the ring, some 500 clocks whatever the tile (with copies, conversion, stores and products taken out
+// 22016 x 2048 still takes 12.5 of 24 us); eight converting warps, or one arrival a warp instead of one a thread, change nothing.
+//
 // Every mbarrier wait is bounded and reports through the status word; nobody waits for another CTA except at the
 // cluster barrier.
 #pragma once
 
 #include "gemm_tc.cuh"
+#include "gemm_w4.cuh"
 
 namespace tk {
 
@@ -235,12 +242,13 @@ __device__ __forceinline__ void add_runs(const float4* filed, float* tile, unsig
 // slot's A tiles overhang (rows past the tokens are read by the MMA, never stored), and the epilogue's tile,
 // min(tg, 128) (in a cluster: ceil(tg / (8 ranks)) * 8) * (NB + 4) * 4.  `partial` holds
 // gridDim.x * gridDim.y * runs * NB * (tg rounded up to 32) floats for a cluster.
-template <bool kFp8, bool kPacked, bool kCluster>
+// With kW4 NB is at most 128, `group` the columns that share a scale, part.w the codes and part.scale the scales (bf16).
+template <bool kFp8, bool kPacked, bool kCluster, bool kW4 = false>
 __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, const bf16* other, float* partial,
                                      unsigned* amax_bits, unsigned* status, unsigned M, unsigned K, unsigned ldx,
                                      unsigned flags, unsigned NB, unsigned stages, unsigned tg, unsigned runs,
                                      unsigned per_run, const Part& p0,
-                                     const Part& p1, const Part& p2, unsigned tile) {
+                                     const Part& p1, const Part& p2, unsigned tile, unsigned group = 64) {
   constexpr unsigned kRowStep = 4 * kW;   // rows a copy pass covers
   extern __shared__ unsigned char dynamic_smem[];
   __shared__ __align__(8) unsigned long long full_bar[kMaxRing], empty_bar[kMaxRing], accum_bar;
@@ -302,6 +310,38 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
     }
   };
   const size_t w_block = kPacked ? size_t(((part.N + 255u) / 256u) * 256u) * kRowBytes : kRowBytes;   // to the next K block
+  // 4-bit weights: warp w takes row tiles w, w + kW of the CTA's, kAhead blocks in flight
+  constexpr unsigned kAhead = 3, kTiles = 2;
+  const unsigned first16 = n0 / w4::kTileRows, tiles16 = kW4 ? min(NB / w4::kTileRows, (part.N + w4::kTileRows - 1) / w4::kTileRows - first16) : 0u;
+  const unsigned group_shift = 31 - __clz(group), groups = K >> group_shift;
+  uint4 codes[kAhead][kTiles];
+  unsigned units[kAhead][kTiles][2];
+  auto tile_of = [&](unsigned j) { return first16 + min(warp + j * kW, tiles16 - 1); };      // past the last tile it is that again, and is not stored
+  auto load_codes = [&](unsigned i, unsigned a) {
+    if (i >= nkb) return;
+#pragma unroll
+    for (unsigned j = 0; j < kTiles; ++j) {
+      const unsigned block = kb0 + i;
+      const unsigned* const unit = reinterpret_cast<const unsigned*>(part.scale) + size_t(tile_of(j)) * groups * 8 + (lane >> 2);
+      codes[a][j] = w4::stream_load(reinterpret_cast<const uint4*>(part.w) + (size_t(tile_of(j)) * k_blocks + block) * 32 + lane);
+      units[a][j][0] = __ldg(unit + ((block * w4::kBlock) >> group_shift) * 8);
+      units[a][j][1] = __ldg(unit + ((block * w4::kBlock + 32) >> group_shift) * 8);
+    }
+  };
+  if (kW4) {
+    if (flags & kFlagLateWeights) grid_dependency_only_wait();
+    if (warp < kW && nkb > 0) {
+      if (lane < kTiles && warp + lane * kW < tiles16) {
+        const unsigned group0 = (kb0 * w4::kBlock) >> group_shift, group1 = ((kb0 + nkb) * w4::kBlock + group - 1) >> group_shift;
+        const uint8_t* const from = part.w + (size_t(tile_of(lane)) * k_blocks + kb0) * w4::kBlockBytes;
+        const uint8_t* const scales = reinterpret_cast<const uint8_t*>(part.scale) + (size_t(tile_of(lane)) * groups + group0) * 32;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(nkb * w4::kBlockBytes) : "memory");
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(scales), "r"((group1 - group0) * 32) : "memory");
+      }
+#pragma unroll
+      for (unsigned a = 0; a < kAhead; ++a) load_codes(a, a);
+    }
+  }
   if (warp == 0) {
     if (elect_one()) {
       for (unsigned s = 0; s < stages; ++s) {
@@ -314,8 +354,8 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
     }
     __syncwarp();
   }
-  if (!kPacked && (flags & kFlagLateWeights)) grid_dependency_only_wait();      // the launch before writes them
-  if (!kPacked && warp < kW && nkb > 0) copy_weights(0);
+  if (!kPacked && !kW4 && (flags & kFlagLateWeights)) grid_dependency_only_wait();      // the launch before writes them
+  if (!kPacked && !kW4 && warp < kW && nkb > 0) copy_weights(0);
   if (warp == kMmaWarp) tmem_alloc(&tmem_slot, columns);
   tc_fence_before();
   __syncthreads();
@@ -335,7 +375,44 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
   };
   if (warp < kW) {
     // ---------------- weights ----------------
-    if (kPacked) {
+    if (kW4) {
+      unsigned s = 0, phase = 1;
+      const unsigned g = lane >> 2, t4 = lane & 3;
+#pragma unroll 1
+      for (unsigned i0 = 0; i0 < nkb; i0 += kAhead) {
+#pragma unroll
+        for (unsigned a = 0; a < kAhead; ++a) {
+          const unsigned i = i0 + a;
+          if (i >= nkb) break;
+          if (i >= stages) mbar_wait(&empty_bar[s], phase, status, kTimeoutEmpty | s);
+#pragma unroll
+          for (unsigned j = 0; j < kTiles; ++j) {
+            if (warp + j * kW >= tiles16) break;
+            const unsigned word[4] = {codes[a][j].x, codes[a][j].y, codes[a][j].z, codes[a][j].w};
+#pragma unroll
+            for (unsigned half = 0; half < 2; ++half) {      // rows g and g + 8: 16-byte pieces t4 and 4 + t4 of 128 bytes
+              const unsigned row = (warp + j * kW) * w4::kTileRows + half * 8 + g, at = ring + s * stage_bytes + a_bytes + row * kRowBytes;
+#pragma unroll
+              for (unsigned h = 0; h < 2; ++h) {
+                const unsigned unit = units[a][j][h], both = __byte_perm(unit, unit, half ? 0x3232 : 0x1010);
+                unsigned v[4];
+#pragma unroll
+                for (unsigned e = 0; e < 4; ++e) {
+                  const unsigned weight = w4::weights_of(word[2 * h + (e >> 1)], 2 * (e & 1) + half);
+                  const bf162 scaled = __hmul2(*reinterpret_cast<const bf162*>(&weight), *reinterpret_cast<const bf162*>(&both));
+                  v[e] = *reinterpret_cast<const unsigned*>(&scaled);
+                }
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((h * 4 + t4) ^ g) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+              }
+            }
+          }
+          load_codes(i + kAhead, a);
+          fence_async_shared();       // the tensor core reads what this thread wrote
+          mbar_arrive(&full_bar[s]);
+          if (++s == stages) { s = 0; phase ^= 1; }
+        }
+      }
+    } else if (kPacked) {
       if (warp == 0) {
         if (elect_one()) {
           unsigned s = 0, phase = 1;
@@ -589,6 +666,29 @@ AGI_TK_CLUSTER(agi_gemm_tc_e4m3_x3, uint8_t, true, false, 4)
 AGI_TK_CLUSTER(agi_gemm_tc_e4m3_x3, uint8_t, true, false, 8)
 #undef AGI_TK_CLUSTER
 #undef AGI_TK_KERNEL
+
+// 4-bit weights, bf16 tokens.
+#define AGI_TK_W4(NAME, CLUSTER, IN_CLUSTER)                                                                                             \
+  extern "C" __global__ void CLUSTER __launch_bounds__(tk::kThreads, 2)                                                                 \
+  NAME(const bf16* x, const bf16* other, float* partial, unsigned* status, unsigned M, unsigned K, unsigned ldx, unsigned flags,        \
+       unsigned NB, unsigned stages, unsigned tg, unsigned runs, unsigned per_run, const uint4* codes, const bf16* scales,              \
+       const bf16* bias, bf16* y, unsigned N, unsigned ldy, unsigned group) {                                                           \
+    if (!(paged::aligned16(codes) && paged::aligned16(scales) && paged::aligned16(x))) {                                                \
+      grid_dependency_wait();                                                                                                           \
+      if (threadIdx.x == 0) paged::report(status, paged::kMisaligned);                                                                  \
+      return;                                                                                                                           \
+    }                                                                                                                                   \
+    const tk::Part part = {reinterpret_cast<const uint8_t*>(codes), bias, reinterpret_cast<const float*>(scales), y, N, ldy};           \
+    const tk::Part none = {nullptr, nullptr, nullptr, nullptr, 0, 0};                                                                   \
+    tk::body<false, false, IN_CLUSTER, true>(reinterpret_cast<const uint8_t*>(x), nullptr, other, partial, nullptr, status, M, K, ldx,   \
+                                             flags, NB, stages, tg, runs, per_run, part, none, none,                                     \
+                                             (flags & kFlagGroupsFirst) ? blockIdx.y : blockIdx.x, group);                              \
+  }
+AGI_TK_W4(agi_gemm_tk_w4, , false)
+AGI_TK_W4(agi_gemm_tk_w4_c2, __cluster_dims__(1, 1, 2), true)
+AGI_TK_W4(agi_gemm_tk_w4_c4, __cluster_dims__(1, 1, 4), true)
+AGI_TK_W4(agi_gemm_tk_w4_c8, __cluster_dims__(1, 1, 8), true)
+#undef AGI_TK_W4
 
 // Up to 16 independent bf16 GEMMs that share the activation matrix (the K and V projections of every cross-attention
 // block over the context tokens, every block's AdaLN projection) as ONE launch: grid = (segments * ceil(N / NB), token groups), or the other way round;

@@ -621,25 +621,25 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const voi
       unsigned *status, unsigned rows, unsigned sequences, unsigned pages, unsigned page, unsigned width, unsigned q_heads,           \
       unsigned kv_heads, unsigned q_stride, unsigned o_stride, unsigned window, unsigned sinks, float scale_log2, unsigned stages,    \
       unsigned own_only
-#define AGI_PAGED_FEW(SHAPE, HD16, N, PER_SM)                                                                                         \
+#define AGI_PAGED_FEW(SHAPE, HD16, N, PER_SM, PER_SM_E4M3)                                                                            \
   extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM)                                                                 \
   agi_paged_few_bf16_##SHAPE(const bf16* q, bf16* o, const bf16* k_pool, const bf16* v_pool, AGI_PAGED_FEW_REST) {                    \
     const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                    \
     few::attention_body<HD16, N, false>(q, o, k_pool, v_pool, nullptr, nullptr, batch, own_sums, own_ends, scratch, counters,         \
                                         q_heads, kv_heads, q_stride, o_stride, window, sinks, scale_log2, stages, own_only);          \
   }                                                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM)                                                                 \
+  extern "C" __global__ void __launch_bounds__(few::kThreads, PER_SM_E4M3)                                                            \
   agi_paged_few_e4m3_##SHAPE(const bf16* q, bf16* o, const unsigned char* k_pool, const unsigned char* v_pool, const bf16* k_scale,   \
                              const bf16* v_scale, AGI_PAGED_FEW_REST) {                                                               \
     const paged::Batch batch{starts, lengths, table, status, rows, sequences, pages, page, width};                                    \
     few::attention_body<HD16, N, true>(q, o, k_pool, v_pool, k_scale, v_scale, batch, own_sums, own_ends, scratch, counters,          \
                                        q_heads, kv_heads, q_stride, o_stride, window, sinks, scale_log2, stages, own_only);           \
   }
-AGI_PAGED_FEW(d64_r8, 4, 1, 2)
-AGI_PAGED_FEW(d64_r16, 4, 2, 2)
-AGI_PAGED_FEW(d64_r32, 4, 4, 2)
-AGI_PAGED_FEW(d128_r8, 8, 1, 2)
-AGI_PAGED_FEW(d128_r16, 8, 2, 2)
-AGI_PAGED_FEW(d128_r32, 8, 4, 1)
+AGI_PAGED_FEW(d64_r8, 4, 1, 2, 3)
+AGI_PAGED_FEW(d64_r16, 4, 2, 2, 3)
+AGI_PAGED_FEW(d64_r32, 4, 4, 2, 2)
+AGI_PAGED_FEW(d128_r8, 8, 1, 2, 3)
+AGI_PAGED_FEW(d128_r16, 8, 2, 2, 2)
+AGI_PAGED_FEW(d128_r32, 8, 4, 1, 1)
 #undef AGI_PAGED_FEW
 #undef AGI_PAGED_FEW_REST

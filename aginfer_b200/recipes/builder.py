@@ -332,10 +332,34 @@ def tcs_tiling(M: int, tiles: int, K: int, cluster: int | None = None, groups: i
 
 
 W4_GROUPS = (32, 64, 128)                 # columns that share a scale
-# Tokens up to which codes go straight into products; beyond, they are brought into scratch as bf16 for `gemm`, whose tensor-core kernel begins
-# there.  us, codes | bf16 and gemm: 32 tokens 2560 x 2048 8.5 | 11.7, 22016 x 2048 34 | 138 (the streaming gemm), 48 tokens 10.5 | 11, 45 | 36,
-# 64 tokens 12.5 | 10.9, 62 | 36.
-W4_MAX_ROWS = 32
+# Tokens up to which the products are integer ones, a pass over the codes for every few tokens; beyond, the codes become bf16 operands of
+# tcgen05 tiles, and beyond W4_FUSED_ROWS, where every group of tokens would convert them again, bf16 weights in scratch for `gemm`.
+# us, integer | tcgen05 | scratch and gemm:  16 tokens 22016 x 2048 20.4 | 23.1, 2048 x 11008 17.6 | 16.6, 37888 x 3584 48 | 51;  32 tokens 35 | 24,
+# 27 | 17, 82 | 52;  64 tokens 62 | 25 | 36, 45 | 18 | 24, 162 | 54 | 118;  288 tokens - | 56 | 64, - | 35 | 36, - | 123 | 174;  600 tokens - | 88 | 87,
+# - | 46 | 56, - | 248 | 220.
+W4_MAX_ROWS, W4_FUSED_ROWS = 16, 400
+
+
+@functools.lru_cache(maxsize=4096)
+def w4_tk_tiling(M: int, N: int, K: int) -> Mapping[str, int]:
+    """Tile of ``agi_gemm_tk_w4*``: of the tiles of 16 to 128 weight rows and clusters of 1 to 8 with the token group that ``tk_tiling`` gives each, the
+    one with the least estimate.  A CTA takes 500 clocks a block of 64 columns whatever it holds, 30 for each 16 rows and its tokens' bytes;
+    two that share an SM take turns at the conversion (28 clocks) and the intake."""
+    best: tuple[float, int, Mapping[str, int]] | None = None
+    for C in (1, 2, 4, 8):
+        for NB in range(16, 129, 16):
+            t = tk_tiling(M, (N,), K, 2, clusters=(C,), rows_per_tile=NB, must_fit=False)
+            if t is None:
+                continue
+            per_sm = 2 if t["shared_bytes"] <= TK_PAIR_BUDGET else 1
+            ctas, intake = t["tiles"] * t["groups"] * C, t["tg"] * 128 / 57
+            busy = NB // 16 * 28 + intake
+            block = max(500 + NB // 16 * 30 + intake, min(per_sm, ceil_div(ctas, SM_COUNT)) * busy)
+            cost = ceil_div(ctas, SM_COUNT * per_sm) * (min(K // 64, t["per_run"] * ceil_div(t["runs"], C)) * block + 4000 + (3000 + 0.083 * min(t["tg"], M) * NB if C > 1 else 0))
+            if best is None or cost < best[0]:
+                best = (cost, NB, t)
+    assert best is not None, "no tile of the tensor-core GEMM fits"
+    return best[2]
 
 
 @functools.lru_cache(maxsize=4096)
@@ -577,6 +601,10 @@ def paged_few_tiling(cache: PagedCache, rows: int, longest: int, group: int) -> 
     batch evenly, so there are as many as the SMs hold, or as the tables have room for tiles."""
     item = next(r for r in (8, 16, 32) if r >= longest * group or r == 32)
     per_sm = 1 if item == 32 and cache.head_dim == 128 else 2
+    # In 8 bits a tile has half the bytes and its latency shows: three CTAs where 128 registers a thread suffice.  64 sequences of 10000 keys, us
+    # with two | three: 28 heads on 4 129 | 119, 16 on 4 of 64 columns 101 | 84, four drafts a sequence of these 138 | 117.
+    if cache.quantized and item * cache.head_dim <= 1024:
+        per_sm = 3
     stage, exchange = PAGED_FEW_KEYS * (2 * cache.head_dim + 4 if cache.quantized else 4 * cache.head_dim), 128 * cache.head_dim
     stages = min(6, ((228 - per_sm) * 1024 // per_sm - 1024 - exchange) // stage)      # 1 KB of static shared memory
     blocks = min(cache.sequences, rows) * ceil_div(longest * group, item) * cache.kv_heads
@@ -1287,8 +1315,8 @@ class RecipeBuilder:
         """Y[M, N] = epilogue(X[M, K] . W[N, K]^T) with 4-bit weights: W[n, k] = (code - 8) * scale of n's group of ``group`` columns.  ``w`` and
         ``scales``: the two tensors of ``layout.pack_w4``, from the checkpoint or the caller (codes then I32).  The epilogue is that of ``gemm``.
         Up to W4_MAX_ROWS tokens codes are multiplied as they are, exactly, with tokens that are off by at most 2^-14 of the largest value of
-        their 64 columns (or 2^-127, if that is more), and sums in 32 bits; beyond, the weights are brought into scratch as bf16, rounded, and ``gemm`` takes them.
-        A token that is not finite makes its outputs NaN."""
+        their 64 columns (or 2^-127, if that is more), and a token that is not finite makes its outputs NaN; beyond, a weight is rounded to
+        bf16 on its way into the tensor core, or, for more than W4_FUSED_ROWS tokens, into scratch that ``gemm`` reads.  Sums are in 32 bits."""
         if group not in W4_GROUPS or K < 64 or K % 64 or K % group:
             raise ValueError(f"columns come in groups of {W4_GROUPS}, and K is a multiple of the group and of 64, not {K} in groups of {group}")
         if not (1 <= M < 1 << 24 and 1 <= N < 1 << 24 and K < 1 << 24):
@@ -1314,21 +1342,30 @@ class RecipeBuilder:
         self._written_apart("outputs", (y, ldy, N), "activations", (x, ldx, K), M)
         dummy = Arena(0)
         # The codes may be asked for while the launch before is still at work, unless a launch can have written them.
-        early = int(isinstance(w, Weight) or (isinstance(w, Tensor) and all(t["name"] != w.name for t in self._profile.outputs)))
-        t = w4_tiling(M, N, K, group) if M <= W4_MAX_ROWS else None
-        if t is None:
-            mark = self.mark()
-            wide = self.alloc(N * K * 2)
-            self.launch("agi_dequantize_w4_bf16", (min(8 * SM_COUNT, ceil_div(tiles * (K // 64), 8)), 1, 1), (256, 1, 1),
-                        [w, scales, wide, Arena(STATUS_WORD), U32(N), U32(K), U32(group), U32(early)], op="dequantize_w4", algorithm="warp_per_tile")
-            self.gemm(x, wide, y, M, N, K, bias=bias, residual=residual, act=act, ldx=ldx, ldy=ldy, tactic="tcgen05_plan", late_weights=True)
-            self.release(mark)
-            return
+        early = all(isinstance(p, Weight) or (isinstance(p, Tensor) and all(t["name"] != p.name for t in self._profile.outputs)) for p in (w, scales))
         partial, counters = self._tc_scratch
         flags = ACT[act] | (FLAG_BIAS if bias else 0) | (FLAG_RESIDUAL if residual else 0)
+        t = w4_tiling(M, N, K, group) if M <= W4_MAX_ROWS else None
+        if t is None:
+            if M > W4_FUSED_ROWS:
+                mark = self.mark()
+                wide = self.alloc(N * K * 2)
+                self.launch("agi_dequantize_w4_bf16", (min(8 * SM_COUNT, ceil_div(tiles * (K // 64), 8)), 1, 1), (256, 1, 1),
+                            [w, scales, wide, Arena(STATUS_WORD), U32(N), U32(K), U32(group), U32(int(early))], op="dequantize_w4", algorithm="warp_per_tile")
+                self.gemm(x, wide, y, M, N, K, bias=bias, residual=residual, act=act, ldx=ldx, ldy=ldy, tactic="tcgen05_plan", late_weights=True)
+                self.release(mark)
+                return
+            t = w4_tk_tiling(M, N, K)
+            grid, order = tk_order(t, M, N, K, 2)
+            self.launch("agi_gemm_tk_w4" if t["C"] == 1 else f"agi_gemm_tk_w4_c{t['C']}", (*grid, t["C"]), (288, 1, 1),
+                        [x, residual or dummy, partial, Arena(STATUS_WORD), U32(M), U32(K), U32(ldx),
+                         U32(flags | order | (0 if early else FLAG_LATE_WEIGHTS)), U32(t["NB"]), U32(t["stages"]), U32(t["tg"]), U32(t["runs"]),
+                         U32(t["per_run"]), w, scales, bias or dummy, y, U32(N), U32(ldy), U32(group)], shared_bytes=t["shared_bytes"], op="gemm_w4",
+                        algorithm=f"tcgen05_{t['tg']}x{t['NB']}_s{t['stages']}_r{t['runs']}_c{t['C']}")
+            return
         self.launch(f"agi_gemm_w4_g{group}_t{t['eights']}", t["grid"], (576, 1, 1),
                     [x, w, scales, y, bias or dummy, residual or dummy, partial, counters, Arena(STATUS_WORD), U32(M), U32(N), U32(K),
-                     U32(ldx), U32(ldy), U32(flags), U32(t["ways"]), U32(t["chunk"]), U32(t["stages"]), U32(early)], shared_bytes=t["shared_bytes"], op="gemm_w4",
+                     U32(ldx), U32(ldy), U32(flags), U32(t["ways"]), U32(t["chunk"]), U32(t["stages"]), U32(int(early))], shared_bytes=t["shared_bytes"], op="gemm_w4",
                     algorithm=f"mma_t{t['eights']}_w{t['ways']}_k{t['splits']}")
 
     def _gemm_tk(self, family: str, op: str, t: Mapping[str, int], x: Pointer,

@@ -95,14 +95,42 @@ def test_forms():
     r.plan()
 
 
-def test_many_tokens_go_through_bf16_weights_in_scratch():
+def recipe(m: int) -> RecipeBuilder:
     r = RecipeBuilder({"w": ("BF16", (8,))})
-    r.begin_profile("default", [io("x", "BF16", [33, K]), io("c", *SHAPES["codes"]), io("s", *SHAPES["scales"])], [io("y", "BF16", [33, N])])
+    r.begin_profile("default", [io("x", "BF16", [m, K]), io("c", *SHAPES["codes"]), io("s", *SHAPES["scales"])], [io("y", "BF16", [m, N]), io("s_out", *SHAPES["scales"])])
+    return r
+
+
+@pytest.mark.parametrize("m", [17, 400])
+def test_more_tokens_are_tiles_of_converted_weights(m):
+    r = recipe(m)
+    launch = product(r, m=m)
+    assert launch["kernel"].startswith("agi_gemm_tk_w4") and len(r._profile.launches) == 2
+    late = lambda: r._profile.launches[-1]["arguments"][7]["scalar_u32"] & B.FLAG_LATE_WEIGHTS  # noqa: E731
+    assert not late()
+    product(r, m=m, w=Arena(1 << 20))
+    assert late()
+    product(r, m=m, s=Tensor("s_out"))
+    assert late()
+
+
+def test_many_tokens_go_through_bf16_weights_in_scratch():
+    r = recipe(401)
     before = r.mark()
-    r.gemm_w4(Tensor("x"), Tensor("c"), Tensor("s"), Tensor("y"), 33, N, K, group=G)
+    product(r, m=401)
     first, second = r._profile.launches[-2:]
-    assert first["kernel"] == "agi_dequantize_w4_bf16" and second["kernel"].startswith("agi_gemm_t") and r.mark() == before
+    assert first["kernel"] == "agi_dequantize_w4_bf16" and second["kernel"].startswith("agi_gemm_tk_bf16") and r.mark() == before
     assert second["arguments"][15] == first["arguments"][2], "the product's weights are those that were brought out"
+    assert second["arguments"][9]["scalar_u32"] & B.FLAG_LATE_WEIGHTS, "and not asked for before that"
+
+
+def test_tiles_of_converted_weights_fit():
+    rng = random.Random(8)
+    for _ in range(300):
+        m, n, k = rng.choice((rng.randint(17, 400), rng.randint(1, 400))), int(10 ** rng.uniform(0, 4.8)), 64 * int(10 ** rng.uniform(0, 2.6))
+        t = B.w4_tk_tiling(m, max(n, 1), max(k, 64))
+        assert t["NB"] % 16 == 0 and 16 <= t["NB"] <= 128 and t["C"] in (1, 2, 4, 8) and t["stages"] >= 2 and t["shared_bytes"] <= B.TK_SMEM_BUDGET
+        assert t["tiles"] * t["NB"] >= n and t["groups"] * t["tg"] >= m
 
 
 @pytest.mark.parametrize("kw,match", [
@@ -131,7 +159,7 @@ def test_a_served_decoder_of_fewer_bits_packages():
         assert not any(".q_proj" in n or ".gate_proj" in n for n in weights) and weights["model.layers.1.self_attn.qkv_proj.bias"].shape == (512,)
         plan = paged_decode.build_recipe(cfg, describe(weights)).plan()
         prompt, step = ([l["kernel"] for l in p["launches"]] for p in plan["shape_dispatch"])
-        assert prompt.count("agi_dequantize_w4_bf16") == 8 and step.count("agi_gemm_w4_g64_t1") == 8      # 48 tokens, three
+        assert sum("gemm_tk_w4" in k for k in prompt) == 8 and step.count("agi_gemm_w4_g64_t1") == 8      # 48 tokens, three
         assert prompt.count("agi_kv_append_e4m3") == step.count("agi_kv_append_e4m3") == 2
         assert step.count("agi_paged_few_e4m3_d64_r8") == 2 and step.count("agi_kv_read_e4m3") == (0 if window else 2)
 
