@@ -370,8 +370,8 @@ def w4_tiling(M: int, N: int, K: int, group: int = 64) -> Mapping[str, Any] | No
     The least estimate in clocks over parts and ways: rounds of the row tiles over the warps, each 350 clocks a block (770 with two eights) and 1730
     besides, 300 a block of one round for the warps that end last, 14 a block of tokens laid out; where parts of K meet 1500, 3880 a round, 90 a
     part and tile.  Fitted to seven shapes with 1, 4, 8 and 16 tokens in groups of 64;
-    of parts 1 to 10 and 12 and all ways it takes one within 3 % of the fastest there, but for 3584 x 18944, where it takes five parts: 4 tokens
-    19.8 to 20.5 us (four parts 18.0), 8 tokens 30.9 (two 26.9), 16 tokens 53 (four 45).  1 token, us with 8 | 4 | 2 | 1 ways: 37888 x 3584 17.7 |
+    of parts 1 to 10 and 12 and all ways it takes one within 3 % of the fastest there, but for 3584 x 18944, where it takes five parts: 1 token
+    16.3 us (fastest 15.1), 4 tokens 20.5 (four parts 18.0), 8 tokens 30.9 (two 26.9), 16 tokens 53 (four 45).  1 token, us with 8 | 4 | 2 | 1 ways: 37888 x 3584 17.7 |
     17.0 | 17.4 | 17.8, 22016 x 2048 8.8 | 8.5 | 8.9 | 10.3; four ways in 1 | 2 | 4 parts: 2048 x 11008 13.8 | 10.0 | 8.4.
     Sixteen tokens of a CTA share a pass over the codes
     where these are many (16 x 22016 x 2048: 20.4 us, in fours 21.8; 4608 x 3584 11.7 and 10.5)."""
