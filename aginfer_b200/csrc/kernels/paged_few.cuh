@@ -21,10 +21,11 @@
 // A cache in 8 bits (kE4m3) brings half the bytes and goes through the same products after a conversion in registers.  Keys become f16,
 // which every code is (one instruction a pair), queries f16 too, times the power of two that brings a row's largest one to 2^14 .. 2^15:
 // bf16 has fewer digits, so that loses nothing but what lies 2^-39 below the row's largest.  Products are then of codes, and a score is
-// multiplied by the row's and the key's power of two.  Values become bf16 by moving bits, which makes a code 2^-120 of itself; the weight
-// that meets it carries the value's scale and 2^64, in bf16, whose range takes scales of any size side by side, and the outputs are
-// multiplied by 2^56.  Pairs of one token's columns are what ldmatrix exchanges, so rows g and g + 8 of a product of values are columns
-// 2 g and 2 g + 1 of its 16.
+// multiplied by the row's and the key's power of two.  Values become bf16 by moving bits, which makes a code 2^-120 of itself, and one
+// exact multiplication a pair; the weight that meets them carries the value's scale, in bf16, whose range is the scales' own.  So sums
+// are what they are of bf16 values, of any size side by side (a weight that carried part of the 2^120 instead would be infinite for
+// values of 2^72 and more, or sums of values below 2^-70 would lose digits).  Pairs of one token's columns are what ldmatrix exchanges, so
+// rows g and g + 8 of a product of values are columns 2 g and 2 g + 1 of its 16.
 //
 // A value behind the sequence's end is whatever the page held before, NaN perhaps, and weight zero does not make it zero: such
 // values are masked as they are read.  In 8 bits it is the scale that is masked: codes as bf16 are finite whatever they are.
@@ -138,16 +139,20 @@ __device__ __forceinline__ Run run_of(const Batch& batch, unsigned group, unsign
   }
 }
 
-// Two E4M3 codes as f16, and the bytes 0 and 2 or 1 and 3 of four of them as bf16 times 2^-120: the sign stays in front, exponent and
-// fraction move to where bf16 has the low end of its exponent.
+// Two E4M3 codes as f16, and the bytes 0 and 2 or 1 and 3 of four of them as bf16: the sign stays in front, exponent and fraction move to
+// where bf16 has the low end of its exponent, which is 2^-120 of the code (subnormal ones too), and are multiplied by 2^120.
 __device__ __forceinline__ unsigned half_pair(unsigned codes) {
   unsigned h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)codes));
   return h;
 }
-__device__ __forceinline__ unsigned even_codes(unsigned w) { return ((w << 8) & 0x80008000u) | ((w << 4) & 0x07f007f0u); }
-__device__ __forceinline__ unsigned odd_codes(unsigned w) { return (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u); }
-constexpr float kWeightUnit = 0x1p64f, kOutUnit = 0x1p56f;      // 2^64 * 2^56 * 2^-120 = 1
+__device__ __forceinline__ unsigned raised(unsigned pair) {
+  constexpr unsigned k2p120 = 0x7b807b80u;
+  const bf162 v = __hmul2(*reinterpret_cast<const bf162*>(&pair), *reinterpret_cast<const bf162*>(&k2p120));
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ unsigned even_codes(unsigned w) { return raised(((w << 8) & 0x80008000u) | ((w << 4) & 0x07f007f0u)); }
+__device__ __forceinline__ unsigned odd_codes(unsigned w) { return raised((w & 0x80008000u) | ((w >> 4) & 0x07f007f0u)); }
 __device__ __forceinline__ void skinny_mma_f16(float* c, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -388,7 +393,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const voi
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             k_unit[i] = scale_at(scales + i * 16);
-            v_unit[i] = whole || held(key0 + g + i * 8) ? scale_at(scales + kScaleBytes + i * 16) * kWeightUnit : 0.f;
+            v_unit[i] = whole || held(key0 + g + i * 8) ? scale_at(scales + kScaleBytes + i * 16) : 0.f;
           }
         }
         unsigned pb[kN][2];
@@ -522,7 +527,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const voi
         if constexpr (kE4m3) {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float2*>(cell(warp, 2 * t4 + e, m * 16 + 2 * g)) = make_float2(out[j][m][e] * kOutUnit, out[j][m][e + 2] * kOutUnit);
+            *reinterpret_cast<float2*>(cell(warp, 2 * t4 + e, m * 16 + 2 * g)) = make_float2(out[j][m][e], out[j][m][e + 2]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) *cell(warp, 2 * t4 + (i & 1), m * 16 + g + (i >> 1) * 8) = out[j][m][i];
