@@ -28,7 +28,8 @@
 // rows g and g + 8 of a product of values are columns 2 g and 2 g + 1 of its 16.
 //
 // A value behind the sequence's end is whatever the page held before, NaN perhaps, and weight zero does not make it zero: such
-// values are masked as they are read.  In 8 bits it is the scale that is masked: codes as bf16 are finite whatever they are.
+// values are masked as they are read.  In 8 bits codes as bf16 are finite whatever they are, and a scale meets only the weights of rows that
+// see its token, so that a token that is not finite leaves the drafts before it alone, too.
 #pragma once
 
 #include "attention.cuh"
@@ -393,7 +394,7 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const voi
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             k_unit[i] = scale_at(scales + i * 16);
-            v_unit[i] = whole || held(key0 + g + i * 8) ? scale_at(scales + kScaleBytes + i * 16) : 0.f;
+            v_unit[i] = scale_at(scales + kScaleBytes + i * 16);
           }
         }
         unsigned pb[kN][2];
@@ -434,15 +435,18 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const voi
         }
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
+          float weight[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[j][i] = exp2_of(x[j][i] - (top[j][i & 1] == -INFINITY ? 0.f : top[j][i & 1]));
+          for (int i = 0; i < 4; ++i) {
+            const float at = x[j][i];
+            x[j][i] = exp2_of(at - (top[j][i & 1] == -INFINITY ? 0.f : top[j][i & 1]));
+            // not the weight: one that is zero in 32 bits alone takes a value that is not finite as it is
+            if constexpr (kE4m3) weight[i] = at == -INFINITY ? 0.f : x[j][i] * v_unit[i >> 1];
+            else weight[i] = x[j][i];
+          }
           sum[j][0] += x[j][0] + x[j][2];
           sum[j][1] += x[j][1] + x[j][3];
-          if constexpr (kE4m3) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[j][i] *= v_unit[i >> 1];
-          }
-          const bf162 first = __floats2bfloat162_rn(x[j][0], x[j][1]), second = __floats2bfloat162_rn(x[j][2], x[j][3]);
+          const bf162 first = __floats2bfloat162_rn(weight[0], weight[1]), second = __floats2bfloat162_rn(weight[2], weight[3]);
           // keys as rows -> keys as columns: P^T as the B operand of O^T += V^T P^T
           asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[j][0]) : "r"(*reinterpret_cast<const unsigned*>(&first)));
           asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[j][1]) : "r"(*reinterpret_cast<const unsigned*>(&second)));

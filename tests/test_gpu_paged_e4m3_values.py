@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests.paged_e4m3_util import Batch8
-from tests.paged_util import check
+from tests.paged_util import BOUND, check
 from tests.test_gpu_paged_e4m3 import attend
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +77,25 @@ def test_a_huge_value_whose_weight_vanishes(tmp_path, longest):
     q = batch.q.view(batch.rows, 4, 64)
     q[..., 0] = q[..., 0].abs() + 1.0
     attend_and_check(tmp_path, batch, longest)
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (8, 1, 128)], ids=str)
+@pytest.mark.parametrize("new,total,unseen", [([4, 1], [100, 90], [(0, 99)]), ([3, 2], [66, 18], [(0, 65), (0, 64), (1, 17)])], ids=str)
+def test_rows_that_do_not_see_a_draft_are_not_touched_by_it(tmp_path, new, total, unseen, heads):
+    """Later drafts whose keys and values are not finite: earlier rows are what they are without them, the others NaN."""
+    batch = Batch8(new, total, 16, heads, seed=5)
+    for b, j in unseen:
+        for name in ("k_scale", "v_scale"):
+            batch.pools[name][batch.table[b, j // 16], :, j % 16] = float("nan")
+    got, status, _ = attend(tmp_path, batch, longest=max(new))
+    assert status == 0
+    want, mass = batch.expected()
+    row = 0
+    for b, n in enumerate(new):
+        first = min((j for c, j in unseen if c == b), default=total[b])
+        for i in range(n):
+            if batch.index(b, i) < first:
+                assert bool(((got[row].double() - want[row]).abs() <= BOUND * mass[row]).all()), (b, i)
+            else:
+                assert bool(got[row].isnan().all()), (b, i)
+            row += 1
