@@ -618,6 +618,14 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
   }
 }
 
+// Operands come in by copies of 16 bytes and more: one off its boundary is reported, in every CTA, and nothing is read.
+__device__ __forceinline__ bool operands_aligned(unsigned* status, const void* x, const void* w0, const void* w1, const void* w2) {
+  if (paged::aligned16(x) && paged::aligned16(w0) && paged::aligned16(w1) && paged::aligned16(w2)) return true;
+  grid_dependency_wait();
+  if (threadIdx.x == 0) paged::report(status, paged::kMisaligned);
+  return false;
+}
+
 }  // namespace tk
 
 #define AGI_TK_KERNEL(NAME, CLUSTER, TYPE, FP8, PACKED, IN_CLUSTER)                                                   \
@@ -627,6 +635,7 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
        unsigned tg, unsigned runs, unsigned per_run, const TYPE* w0, const bf16* bias0, const float* sw0, void* y0,   \
        unsigned N0, unsigned ldy0, const TYPE* w1, const bf16* bias1, const float* sw1, void* y1, unsigned N1,       \
        unsigned ldy1, const TYPE* w2, const bf16* bias2, const float* sw2, void* y2, unsigned N2, unsigned ldy2) {   \
+    if (!tk::operands_aligned(status, x, w0, w1, w2)) return;                                                        \
     const tk::Part p0 = {reinterpret_cast<const uint8_t*>(w0), bias0, sw0, y0, N0, ldy0};                            \
     const tk::Part p1 = {reinterpret_cast<const uint8_t*>(w1), bias1, sw1, y1, N1, ldy1};                            \
     const tk::Part p2 = {reinterpret_cast<const uint8_t*>(w2), bias2, sw2, y2, N2, ldy2};                            \
@@ -673,11 +682,7 @@ AGI_TK_CLUSTER(agi_gemm_tc_e4m3_x3, uint8_t, true, false, 8)
   NAME(const bf16* x, const bf16* other, float* partial, unsigned* status, unsigned M, unsigned K, unsigned ldx, unsigned flags,        \
        unsigned NB, unsigned stages, unsigned tg, unsigned runs, unsigned per_run, const uint4* codes, const bf16* scales,              \
        const bf16* bias, bf16* y, unsigned N, unsigned ldy, unsigned group) {                                                           \
-    if (!(paged::aligned16(codes) && paged::aligned16(scales) && paged::aligned16(x))) {                                                \
-      grid_dependency_wait();                                                                                                           \
-      if (threadIdx.x == 0) paged::report(status, paged::kMisaligned);                                                                  \
-      return;                                                                                                                           \
-    }                                                                                                                                   \
+    if (!tk::operands_aligned(status, x, codes, scales, nullptr)) return;                                                               \
     const tk::Part part = {reinterpret_cast<const uint8_t*>(codes), bias, reinterpret_cast<const float*>(scales), y, N, ldy};           \
     const tk::Part none = {nullptr, nullptr, nullptr, nullptr, 0, 0};                                                                   \
     tk::body<false, false, IN_CLUSTER, true>(reinterpret_cast<const uint8_t*>(x), nullptr, other, partial, nullptr, status, M, K, ldx,   \
