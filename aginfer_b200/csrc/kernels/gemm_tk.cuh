@@ -324,8 +324,8 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
       const unsigned block = kb0 + i;
       const unsigned* const unit = reinterpret_cast<const unsigned*>(part.scale) + size_t(tile_of(j)) * groups * 8 + (lane >> 2);
       codes[a][j] = w4::stream_load(reinterpret_cast<const uint4*>(part.w) + (size_t(tile_of(j)) * k_blocks + block) * 32 + lane);
-      units[a][j][0] = __ldg(unit + ((block * w4::kBlock) >> group_shift) * 8);
-      units[a][j][1] = __ldg(unit + ((block * w4::kBlock + 32) >> group_shift) * 8);
+      units[a][j][0] = unit[((block * w4::kBlock) >> group_shift) * 8];
+      units[a][j][1] = unit[((block * w4::kBlock + 32) >> group_shift) * 8];
     }
   };
   if (kW4) {

@@ -62,9 +62,11 @@ __device__ __forceinline__ unsigned piece_of(unsigned low, unsigned high, float 
   const unsigned v2 = __float_as_uint(fmaf(__uint_as_float(high << 16), by, kRound)), v3 = __float_as_uint(fmaf(__uint_as_float(high & 0xffff0000u), by, kRound));
   return __byte_perm(__byte_perm(v0, v2, 0x5410) >> shift, __byte_perm(v1, v3, 0x5410) >> shift, 0x6420) & mask;
 }
-__device__ __forceinline__ uint4 stream_load(const uint4* p) {      // read once: not kept in L1
+// Codes, read once: not kept in L1.  A launch before may write codes and scales while this one already lives, so they are no constants of it: with
+// ld.global.nc a product took what an earlier run had left of them in the SM's L1.
+__device__ __forceinline__ uint4 stream_load(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 
@@ -350,7 +352,7 @@ agi_dequantize_w4_bf16(const uint4* codes, const bf16* scales, bf16* out, unsign
     const uint4 c = next;
     if (item + stride < items) next = w4::stream_load(codes + size_t(item + stride) * 32 + lane);
     const unsigned* const unit = reinterpret_cast<const unsigned*>(scales) + size_t(tile) * groups * 8 + g;
-    const unsigned first = __ldg(unit + block * w4::kBlock / group * 8), second = __ldg(unit + (block * w4::kBlock + 32) / group * 8);
+    const unsigned first = unit[block * w4::kBlock / group * 8], second = unit[(block * w4::kBlock + 32) / group * 8];
     __syncwarp();       // the tile before has left
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
