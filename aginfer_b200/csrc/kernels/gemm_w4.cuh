@@ -10,10 +10,16 @@
 // instruction at all, are that of row g + 8, whose sum is then 16 times its own and once row g's, which is taken off again, exactly.
 //
 // Tokens are 15-bit integers relative to the power of two next to the largest value of their block of 64 columns, which becomes 2^13 .. 2^14: they
-// are off by half a unit, 2^-14 of that value (or 2^-127) at most, and exact where they are 2^-6 of it or more, so that one large value
-// costs its neighbours no more than its own last digits, and other blocks nothing; outputs in bf16 are off by up to 2^-8 of theirs.  They go in as two columns, the upper eight bits and the lower seven.  The 8
-// that is too much of every code is taken off the sums: they begin at -8 (or -136) times the sum of the columns.  A block's sums are exact;
-// they are multiplied by the scales and added up in fp32.
+// are off by half a unit, 2^-14 of that value at most, and exact where they are 2^-6 of it or more; outputs in bf16 are off by up to 2^-8 of
+// theirs.  They go in as two columns, the upper eight bits and the lower seven.  The 8 that is too much of every code is taken off the sums:
+// they begin at -8 (or -136) times the sum of the columns.  A block's sums are exact; they are multiplied by the scales and added up in fp32.
+//
+// That is too little for neighbours of a value thousands of times theirs, whose own weight may be zero.  So a block is one of integers only if each
+// eight of its values (what a lane holds of even or of odd columns) has one of 2^-4 of the power of two or more, 2^9 units, in all of the CTA's
+// tokens: normal values have, and so have products of two of them but for one block in ten.  Other blocks, and those below 2^-113, where
+// the unit would leave fp32, are zero as integers and go through bf16 products besides, exact but for sums in 32 bits: rows of x from L2,
+// codes - 8 as bf16 from the ring.  us with such a value in no | one | every block: 37888 x 3584, 1 token 17.9 | 18.6 | 37.9, 8 tokens 30.0 | 30.5 |
+// 73.6; 2048 x 11008, 1 token 8.8 | 8.9 | 12.9.
 //
 // A CTA is one an SM: it lays its part of the tokens (of gridDim.z parts of K) into shared memory once, as the products take them, then two
 // teams of eight warps stream row tiles past them.  `ways` warps share the columns of a tile, so that there are tiles for all warps
@@ -23,9 +29,9 @@
 // order, so sums do not depend on who that is.  Weights are no earlier launch's work (`early`): the rings fill before the launch before
 // has ended.
 //
-// Measured in a chain of launches (codes from memory, groups of 64): 37888 x 3584 with 1 token 17.0 us (4.2 TB/s), where the same copies without
-// the products took 12.9 to 13.6; with 4 tokens 17.7, 8 tokens (two groups) 28.4, 16 tokens 47 to 49.  Three teams a CTA were slower (1 token
-// 18.7 to 20.3).  Two blocks unrolled, not four: 18.1 to 17.4 at four ways, and no spills.
+// Measured in a chain of launches (codes from memory, groups of 64): 37888 x 3584 with 1 token 17.9 us (4.0 TB/s; 17.2 before blocks were looked at
+// for uneven values), where the same copies without the products took 12.9 to 13.6; with 4 tokens 18.7, 8 tokens (two groups) 30.0, 16 tokens
+// 48.2.  Three teams a CTA were slower (1 token 18.7 to 20.3 where two took 17.4).  Two blocks unrolled, not four: 18.1 to 17.4 at four ways.
 #pragma once
 
 #include "attention.cuh"
@@ -36,6 +42,7 @@
 namespace w4 {
 
 constexpr unsigned kWarps = 8, kTeams = 2, kTeamThreads = 288, kThreads = kTeams * kTeamThreads, kTileRows = 16, kBlock = 64, kBlockBytes = 512;
+constexpr unsigned kMaxBlocks = 512;       // of a part of K: shared memory holds fewer
 constexpr unsigned kMaxStages = 8, kBlockTokens = 512, kBlockOffs = 64;      // bytes of eight columns of tokens, of what their sums begin at
 constexpr unsigned kPitch = 20;            // floats from one column of a warp's sums to the next: 16 rows, no bank conflicts
 constexpr unsigned kTimeout = 0x700;       // a copy that does not arrive
@@ -80,6 +87,7 @@ __device__ __forceinline__ void body(const bf16* x, const uint4* codes, const bf
   extern __shared__ __align__(128) unsigned char w4_smem[];       // rings [warp][stage] | tokens [block][eight][lane][16] | offs [block][half][eight][t][4] | units [block][eight][8]
   __shared__ __align__(16) float sums[kTeams][2][kWarps][kColumns * kPitch];
   __shared__ __align__(8) unsigned long long full[kTeams * kWarps][kMaxStages];
+  __shared__ unsigned char apart[kMaxBlocks];       // 1: this block of the part is no block of integers; 2: its values are near the largest there are, too
   const unsigned tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t4 = lane & 3, warp = tid >> 5, team = warp / (kWarps + 1), mate = warp % (kWarps + 1);
   const unsigned tiles = (N + kTileRows - 1) / kTileRows, blocks = K / kBlock, groups = K / kGroup;
   const unsigned per = (blocks + gridDim.z - 1) / gridDim.z, part0 = min(blockIdx.z * per, blocks), part = min(per, blocks - part0);
@@ -139,12 +147,16 @@ __device__ __forceinline__ void body(const bf16* x, const uint4* codes, const bf
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       pair = larger_pair(larger_pair(larger_pair(v[h].x & 0x7fff7fffu, v[h].y & 0x7fff7fffu), larger_pair(v[h].z & 0x7fff7fffu, v[h].w & 0x7fff7fffu)), pair);
+    const unsigned least = min(pair & 0xffffu, pair >> 16);      // of the lane's eights the one with the least largest value
     pair = larger_pair(pair, __shfl_xor_sync(0xffffffffu, pair, 1));
     pair = larger_pair(pair, __shfl_xor_sync(0xffffffffu, pair, 2));
     const unsigned peak = max(pair & 0xffffu, pair >> 16), exponent = peak >> 7;
     // 2^13 / 2^exponent: values below 2^14.  A block that is not finite is zero, times NaN
     const unsigned unit = exponent == 255 ? 0u : min(267u - exponent, 253u) << 23;
-    const float by = __uint_as_float(unit);
+    const bool uneven = unit && peak && (exponent < 14 || least < (exponent - 4) << 7), any_uneven = __any_sync(0xffffffffu, uneven);
+    const bool any_huge = __any_sync(0xffffffffu, unit && exponent >= 240);
+    if (lane == 0) apart[block] = any_uneven ? 1 + any_huge : 0;       // the same for both eights, which hold the same tokens
+    const float by = __uint_as_float(any_uneven ? 0u : unit);
     const unsigned shift = lower ? 0 : 7, mask = lower ? 0x7f7f7f7fu : 0xffffffffu;
     uint4 piece = make_uint4(0u, 0u, 0u, 0u);
     if (unit) piece = make_uint4(piece_of(v[0].x, v[0].y, by, shift, mask), piece_of(v[0].z, v[0].w, by, shift, mask), piece_of(v[1].x, v[1].y, by, shift, mask),
@@ -235,6 +247,41 @@ __device__ __forceinline__ void body(const bf16* x, const uint4* codes, const bf
           units_at += 2 * kEights * 4;
         }
         if (todo) multiply(0);
+        for (unsigned left_apart = __ballot_sync(0xffffffffu, lane < held && apart[at - part0 + lane]); left_apart; left_apart &= left_apart - 1) {
+          const unsigned b = __ffs(left_apart) - 1, group0 = at * kBlock / kGroup;
+          const uint4 c = reinterpret_cast<const uint4*>(ring + s * slot_bytes)[b * 32 + lane];
+          // column g of the products is token g: columns 2 t .. and 2 t + 8 .. of two products are the lane's eight in a row of codes and tokens
+          uint4 v[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+          if (g < live_tokens) {
+            const uint4* const from = reinterpret_cast<const uint4*>(x + size_t(token0 + g) * ldx + (at + b) * kBlock + t4 * 8);
+            v[0] = from[0];
+            v[1] = from[4];
+          }
+          // 64 products of up to 8 times a value of 2^113 or more stay finite times 2^-10
+          const bool huge = apart[at - part0 + b] == 2;
+          const float back = huge ? 0x1p10f : 1.f;
+          const bf162 small = __floats2bfloat162_rn(huge ? 0x1p-10f : 1.f, huge ? 0x1p-10f : 1.f);
+          auto weights = [&](unsigned word, int i) {
+            const unsigned pair = weights_of(word, i);
+            const bf162 less = __hmul2(*reinterpret_cast<const bf162*>(&pair), small);
+            return *reinterpret_cast<const unsigned*>(&less);
+          };
+          float all[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned w0 = h ? c.z : c.x, w1 = h ? c.w : c.y;
+            skinny_mma_bf16(all, weights(w0, 0), weights(w0, 1), weights(w0, 2), weights(w0, 3), v[h].x, v[h].y);
+            skinny_mma_bf16(all, weights(w1, 0), weights(w1, 1), weights(w1, 2), weights(w1, 3), v[h].z, v[h].w);
+            if (h == 0 && kGroup != 32) continue;
+            const unsigned group = ((at + b) * kBlock + h * 32) / kGroup - group0;
+            const unsigned scale = *reinterpret_cast<const unsigned*>(ring + s * slot_bytes + chunk * kBlockBytes + group * 32 + g * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              sum[0][i] = fmaf(all[i] * __uint_as_float(i < 2 ? scale << 16 : scale & 0xffff0000u), back, sum[0][i]);
+              all[i] = 0.f;
+            }
+          }
+        }
         __syncwarp();       // the slot has been read
         if (lane == 0) ask(s);
         if (++s == stages) { s = 0; phase ^= 1; }

@@ -1319,8 +1319,9 @@ class RecipeBuilder:
         """Y[M, N] = epilogue(X[M, K] . W[N, K]^T) with 4-bit weights: W[n, k] = (code - 8) * scale of n's group of ``group`` columns.  ``w`` and
         ``scales``: the two tensors of ``layout.pack_w4``, from the checkpoint or the caller (codes then I32).  The epilogue is that of ``gemm``.
         Up to W4_MAX_ROWS tokens codes are multiplied as they are, exactly, with tokens that are off by at most 2^-14 of the largest value of
-        their 64 columns (or 2^-127, if that is more), and a token that is not finite makes its outputs NaN; beyond, a weight is rounded to
-        bf16 on its way into the tensor core, or, for more than W4_FUSED_ROWS tokens, into scratch that ``gemm`` reads.  Sums are in 32 bits."""
+        their 64 columns, or exact where some columns are far larger than the rest, and a token that is not finite makes its outputs NaN; beyond, a
+        weight is rounded to bf16 on its way into the tensor core, or, for more than W4_FUSED_ROWS tokens, into scratch that ``gemm`` reads, so
+        the same token has other digits with 17 tokens than with 16.  Sums are in 32 bits."""
         if group not in W4_GROUPS or K < 64 or K % 64 or K % group:
             raise ValueError(f"columns come in groups of {W4_GROUPS}, and K is a multiple of the group and of 64, not {K} in groups of {group}")
         if not (1 <= M < 1 << 24 and 1 <= N < 1 << 24 and K < 1 << 24):
