@@ -533,6 +533,10 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
   const unsigned R = (tg + 31u) & ~31u;      // rows of a filed partial tile: [run][column / 4][row] float4
   float4* const filed = reinterpret_cast<float4*>(partial) +
                         size_t(blockIdx.y * gridDim.x + blockIdx.x) * runs * (NB / 4) * R;
+  auto epilogue_sync = [] {
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
+  };
   if (warp < kMmaWarp) {
     // warp w reads TMEM lanes 32 * (w % 4) ..., 16-column units w / 4, w / 4 + kW / 2, ...
     const unsigned quarter = warp & 3, half = warp >> 2, units = NB / 16;
@@ -551,6 +555,7 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
           for (unsigned q = 0; q < max(my_runs, 1u); ++q) {
             unsigned r[16];
             if (q * per_run < nkb) {
+              __syncwarp();       // an instruction of the whole warp, behind stores of single lanes
               tmem_load16_nowait(addr + q * run_cols + c * 16, r);
               tmem_wait_loads();
             } else {
@@ -579,9 +584,9 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
         }
       }
       if (!kCluster) {
-        asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
+        epilogue_sync();
         finish(min(128u, rows - mt * 128), m0 + mt * 128);
-        if (mt + 1 < m_tiles) asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
+        if (mt + 1 < m_tiles) epilogue_sync();
       }
     }
     tc_fence_before();
@@ -590,6 +595,7 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
   // CTA kept its columns across the cluster barrier, two clusters that share two SMs in opposite order would each hold
   // what the other's missing rank waits for.  The epilogue warps only arrive (their partial tiles are in L2, every
   // tcgen05.ld is complete) and do not wait for the release.
+  __syncwarp();
   if (warp == kMmaWarp) {
     asm volatile("bar.sync 2, %0;" ::"n"(kEpilogue + 32) : "memory");
     tc_fence_after();
@@ -609,7 +615,7 @@ __device__ __forceinline__ void body(const uint8_t* x, const float* scale_a, con
     if (runs <= 2) add_runs<4, 2>(from, tile_rows, P, count, NB / 4, R, runs);
     else if (runs <= 4) add_runs<2, 4>(from, tile_rows, P, count, NB / 4, R, runs);
     else add_runs<1, 8>(from, tile_rows, P, count, NB / 4, R, runs);
-    asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
+    epilogue_sync();
     finish(count, m0 + first);
   }
   if ((flags & kFlagAmax) && warp < kMmaWarp) {

@@ -176,8 +176,15 @@ __device__ __forceinline__ void body(const bf16* x, const uint4* codes, const bf
     if (t4 == 0) units[i * 8 + g] = unit ? __uint_as_float((254u << 23) - unit) * (lower ? 1.f : 128.f) : __uint_as_float(0x7fc00000u);
   }
   __syncthreads();
-  auto meet = [&](unsigned bar) { asm volatile("bar.sync %0, 288;" ::"r"(1 + team * 4 + bar) : "memory"); };
-  auto pass = [&](unsigned bar) { asm volatile("bar.arrive %0, 288;" ::"r"(1 + team * 4 + bar) : "memory"); };
+  // instructions of a whole warp, behind branches of single lanes
+  auto meet = [&](unsigned bar) {
+    __syncwarp();
+    asm volatile("bar.sync %0, 288;" ::"r"(1 + team * 4 + bar) : "memory");
+  };
+  auto pass = [&](unsigned bar) {
+    __syncwarp();
+    asm volatile("bar.arrive %0, 288;" ::"r"(1 + team * 4 + bar) : "memory");
+  };
   unsigned which = 0;
 
   if (mate < kWarps) {

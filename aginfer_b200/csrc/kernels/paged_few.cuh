@@ -279,7 +279,10 @@ __device__ __forceinline__ void attention_body(const bf16* q, bf16* o, const voi
   // ---- four warps: 16 keys each of every tile ----
   const Scratch<kRows, kDim> parts{scratch, scratch + size_t(gridDim.x) * 2 * kRows * kDim};
   const unsigned g = lane >> 2, t4 = lane & 3;
-  auto consumers_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+  auto consumers_sync = [] {
+    __syncwarp();       // a barrier of whole warps, behind branches of single lanes
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  };
   unsigned s = 0, phase = 0;
   walk([&](unsigned seq, unsigned head, unsigned block, const Items& it, unsigned begin, unsigned end, unsigned item_first) {
     const Span& span = it.span;
