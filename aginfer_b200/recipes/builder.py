@@ -987,6 +987,13 @@ class RecipeBuilder:
         if not apart:
             raise ValueError(f"{what}: written over the {other} that other blocks of the launch still read")
 
+    @staticmethod
+    def _spans_apart(what: str, written: tuple[Pointer, int], other: str, read: tuple[Pointer, int]) -> None:
+        """Bytes that a launch writes, (pointer, count), are none of those that other blocks of it read."""
+        (a, a_bytes), (b, b_bytes) = written, read
+        if a == b or (isinstance(a, Arena) and isinstance(b, Arena) and a.offset < b.offset + b_bytes and b.offset < a.offset + a_bytes):
+            raise ValueError(f"{what}: written over the {other} that other blocks of the launch still read")
+
     def kv_append(self, q: Pointer, q_out: Pointer, cache: PagedCache, *, rows: int, q_heads: int, theta: float,
                   row_stride: int | None = None, out_stride: int | None = None, k: Pointer | None = None, v: Pointer | None = None,
                   kv_stride: int | None = None, positions: Pointer | None = None, sections: Sequence[int] | None = None,
@@ -1345,6 +1352,12 @@ class RecipeBuilder:
                 raise ValueError(f"{what}: does not start on a 16-byte boundary")
         self._written(y)
         self._written_apart("outputs", (y, ldy, N), "activations", (x, ldx, K), M)
+        span = ((M - 1) * ldy + N) * 2
+        for what, p, size in (("codes", w, tiles * K * 8), ("scales", scales, tiles * (K // group) * 32), ("bias", bias, N * 2)):
+            if p is not None:
+                self._spans_apart("outputs", (y, span), what, (p, size))
+        if residual is not None and residual != y:       # in place a value is read by the thread that then writes it
+            self._written_apart("outputs", (y, ldy, N), "residual", (residual, ldy, N), M)
         dummy = Arena(0)
         # The codes may be asked for while the launch before is still at work, unless a launch can have written them.
         early = all(isinstance(p, Weight) or (isinstance(p, Tensor) and all(t["name"] != p.name for t in self._profile.outputs)) for p in (w, scales))
