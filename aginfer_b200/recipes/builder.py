@@ -1061,14 +1061,27 @@ class RecipeBuilder:
         self._paged_batch(cache, rows, cache.kv_heads)
         self._paged_batch(to, rows, to.kv_heads)
         self._written(to.k, to.v, to.table)
-        if len({to.k, to.v, to.table, *cache.pools, cache.table, cache.starts, cache.lengths}) < 10:
-            raise ValueError("kv_read writes into tensors of their own")
+        self._kv_read_fits(cache)
+        slots, token = cache.sequences * cache.pages_per_sequence, cache.kv_heads * cache.page
+        spans = [(to.k, to.pages * token * cache.head_dim * 2), (to.v, to.pages * token * cache.head_dim * 2), (to.table, slots * 4),      # written
+                 (cache.k, cache.pages * token * cache.head_dim), (cache.v, cache.pages * token * cache.head_dim),
+                 (cache.k_scale, cache.pages * token * 2), (cache.v_scale, cache.pages * token * 2), (cache.table, slots * 4),
+                 (cache.starts, (cache.sequences + 1) * 4), (cache.lengths, cache.sequences * 4)]
+        for i in range(3):
+            for other in spans[i + 1:]:
+                self._spans_apart("kv_read writes into tensors of their own", spans[i], "memory", other)
         self._kv_read(cache, to, rows, window, sinks, 0)
 
-    def _kv_read(self, cache: PagedCache, to: PagedCache, rows: int, window: int, sinks: int, flags: int) -> None:
+    @staticmethod
+    def _kv_read_fits(cache: PagedCache) -> int:
+        """Pieces of 16 tokens of a head that a launch may have to bring back."""
         pieces = cache.sequences * cache.pages_per_sequence * cache.kv_heads * (cache.page // 16)
         if pieces >= 1 << 31:
             raise ValueError("more pages than a launch numbers: fewer sequences or a shorter table")
+        return pieces
+
+    def _kv_read(self, cache: PagedCache, to: PagedCache, rows: int, window: int, sinks: int, flags: int) -> None:
+        pieces = self._kv_read_fits(cache)
         self.launch("agi_kv_read_e4m3", (min(8 * SM_COUNT, ceil_div(pieces, 8)), 1, 1), (256, 1, 1),
                     [*cache.pools, cache.starts, cache.lengths, cache.table, to.k, to.v, to.table, Arena(STATUS_WORD), U32(rows),
                      U32(cache.sequences), U32(cache.pages), U32(cache.page), U32(cache.pages_per_sequence), U32(cache.kv_heads),
