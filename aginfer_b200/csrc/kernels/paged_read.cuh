@@ -2,7 +2,9 @@
 //
 // Bound by memory: head_dim + 2 bytes are read and 2 head_dim written for a token, key head and pool.  Only pages are read that hold a
 // token which some row of the batch sees; page i of sequence b goes to page b * width + i of the pools behind, and `table_out` says so to
-// the launches that read them (a page outside the pool is left out and named so that they leave it out too).  Pages of the batch
+// the launches that read them (a page outside the pool is left out and named so that they leave it out too).  With kByPage a page keeps its
+// number in the pools behind, and the batch's own table says where it is: for tables with far more places than the pool has pages (sequences
+// that share the page then write the same bytes to the same place).  Pages of the batch
 // form one line, found by every block as in the attention kernels, of which a warp takes 16 tokens of a page and head at a time: its
 // keys and values are up to sixteen 8-byte loads a lane, asked for before the first of them is used.  Eight codes are one 16-byte store,
 // so that a warp's store fills whole lines (with 16 codes and two stores of every other 16 bytes 527 MB took 290 us).
@@ -20,6 +22,7 @@ constexpr unsigned kThreads = 256, kTokens = 16, kMaxSequences = 4096;
 enum Flag : unsigned {
   kFreshOnly = 1,      // sequences without new tokens are left out
   kNoStarts = 2,       // `starts` is not there: no sequence has new tokens
+  kByPage = 4,         // pages keep their numbers, `table_out` is not written
 };
 
 // The pages of a sequence that hold a visible token: [0, sink) and [window, end).
@@ -102,12 +105,12 @@ agi_kv_read_e4m3(const unsigned char* k_pool, const unsigned char* v_pool, const
     const unsigned at = line - begins[seq], slot = at < seen.sink ? at : seen.window + (at - seen.sink), to = seq * width + slot;
     const unsigned page_id = unsigned(table[to]);
     if (piece == 0 && head == 0 && lane == 0) {
-      table_out[to] = page_id < pages ? int(to) : -1;
+      if (!(flags & kByPage)) table_out[to] = page_id < pages ? int(to) : -1;
       if (page_id >= pages) report(status, kBadPage);
     }
     if (page_id >= pages) continue;
     const unsigned held = min(seen.length - slot * page, page);       // tokens of the page
-    const size_t from = block_offset(page_id, kv_heads, head, 1, 0, page), to_row = block_offset(to, kv_heads, head, blocks, 0, page);
+    const size_t from = block_offset(page_id, kv_heads, head, 1, 0, page), to_row = block_offset(flags & kByPage ? page_id : to, kv_heads, head, blocks, 0, page);
     uint2 codes[2][8];
     float scale[2][8];
 #pragma unroll

@@ -595,7 +595,7 @@ class PagedCache:
 
 
 PAGED_MAX_SEQUENCES = 4096
-KV_READ_FRESH_ONLY, KV_READ_NO_STARTS = 1, 2
+KV_READ_FRESH_ONLY, KV_READ_NO_STARTS, KV_READ_BY_PAGE = 1, 2, 4
 PAGED_FEW_ROWS = 32                      # rows (new tokens x query heads of a key head) of a sequence that mma.sync tiles take
 PAGED_FEW_KEYS = 64                      # keys of a tile
 
@@ -1088,11 +1088,15 @@ class RecipeBuilder:
                      U32(cache.head_dim), U32(window), U32(sinks), U32(flags)], op="kv_read", algorithm="warp_per_16_tokens")
 
     def _read_into_scratch(self, cache: PagedCache, rows: int, window: int, sinks: int, flags: int) -> PagedCache:
-        """The batch's visible pages as bf16 pages in the arena, for the kernels that read these (given back with the caller's mark)."""
-        pages = cache.sequences * cache.pages_per_sequence
+        """The batch's visible pages as bf16 pages in the arena, for the kernels that read these (given back with the caller's mark): as many as
+        the table has places, in their order, or, where these are twice the pool's pages or more, as many as the pool has, under its numbers."""
+        slots = cache.sequences * cache.pages_per_sequence
+        by_page = slots >= 2 * cache.pages
+        pages = cache.pages if by_page else slots
         pool = pages * cache.kv_heads * cache.page * cache.head_dim * 2
-        to = replace(cache, k=self.alloc(pool), v=self.alloc(pool), table=self.alloc(pages * 4), pages=pages, k_scale=None, v_scale=None)
-        self._kv_read(cache, to, rows, window, sinks, flags)
+        to = replace(cache, k=self.alloc(pool), v=self.alloc(pool), table=cache.table if by_page else self.alloc(slots * 4), pages=pages, k_scale=None,
+                     v_scale=None)
+        self._kv_read(cache, to, rows, window, sinks, flags | (KV_READ_BY_PAGE if by_page else 0))
         return to
 
     def paged_attention(self, q: Pointer, o: Pointer, cache: PagedCache, *, rows: int, q_heads: int, longest: int | None = None,
