@@ -56,7 +56,7 @@ def unpack_kblock_swizzled(p, rows: int):
 def quantize_w4(t, group: int = 64):
     """A weight matrix [N, K] -> (codes [N, K] from 0 to 15 as uint8, scales [N, K / group] in bf16): the weight is (code - 8) * scale.  The
     scale is the largest |weight| of the group over 7, rounded up to a bf16 where rounding down would take it below (none is
-    clipped then); a group of zeros has the scale zero."""
+    clipped then); a group of zeros has the scale zero, one that is not finite the scale NaN."""
     import torch
     n, k = t.shape
     if k % group:
@@ -65,12 +65,13 @@ def quantize_w4(t, group: int = 64):
     least = x.abs().amax(dim=-1) / 7
     scale = least.to(torch.bfloat16)
     scale = torch.where(scale.float() < least, torch.nextafter(scale, torch.full_like(scale, float("inf"))), scale)
+    scale = torch.where(least.isfinite(), scale, torch.full_like(scale, float("nan")))
     codes = torch.where(scale[..., None] > 0, (x / scale.float()[..., None]).round().clamp(-8, 7) + 8, 8.0)
     return codes.to(torch.uint8).reshape(n, k), scale
 
 
 def pack_w4(codes, scales):
-    """Codes [N, K] and scales [N, K / group] (``quantize_w4``, or a checkpoint's own) as ``gemm_w4`` takes them: int32
+    """Codes [N, K] from 0 to 15 and scales [N, K / group] that are bf16 numbers (``quantize_w4``, or a checkpoint's own) as ``gemm_w4`` takes them: int32
     [N / 16, K / 64, 32, 4] and bf16 [N / 16, K / group, 8, 2], N rounded up to 16 rows (a checkpoint stores the codes' bits as F32).
     The four bits from 4 p of word j of lane 4 g + t are the code of row g + 8 (p & 1), column 32 (j >> 1) + 8 t + 4 (j & 1) + (p & 2) + (p >> 2)
     of a tile of 16 rows and 64 columns: a lane's words are its operands of four matrix products, and its columns are eight in a row."""
@@ -78,6 +79,10 @@ def pack_w4(codes, scales):
     n, k = codes.shape
     if k % 64 or k % scales.shape[1] or scales.shape[0] != n:
         raise ValueError(f"codes {list(codes.shape)} and scales {list(scales.shape)}: K is a multiple of 64 and of the group")
+    if codes.numel() and not (0 <= int(codes.min()) and int(codes.max()) <= 15):
+        raise ValueError(f"codes from {int(codes.min())} to {int(codes.max())}: they have four bits")
+    if not torch.equal(scales.to(torch.bfloat16).double().nan_to_num(), scales.double().nan_to_num()):
+        raise ValueError(f"scales ({scales.dtype}) that bf16 does not hold: round them, and make the codes for the rounded ones")
     tiles, groups = (n + 15) // 16, scales.shape[1]
     padded = torch.full((tiles * 16, k), 8, dtype=torch.int64, device=codes.device)
     padded[:n] = codes
