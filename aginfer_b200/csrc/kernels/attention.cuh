@@ -156,8 +156,8 @@ agi_attention_smem_bf16(const bf16* q, const bf16* k, const bf16* v, bf16* o, un
       if (i < vectors) {
         const unsigned j = i / vec_per_row, d = (i % vec_per_row) * 8;
         const size_t key = key_begin + j;
-        kk[b] = __ldg(reinterpret_cast<const uint4*>(k + key * k_stride + kv_head * head_dim + d));
-        vv[b] = __ldg(reinterpret_cast<const uint4*>(v + key * v_stride + kv_head * head_dim + d));
+        kk[b] = *reinterpret_cast<const uint4*>(k + key * k_stride + kv_head * head_dim + d);
+        vv[b] = *reinterpret_cast<const uint4*>(v + key * v_stride + kv_head * head_dim + d);
       }
     }
 #pragma unroll
@@ -284,8 +284,8 @@ agi_attention_rows_bf16(const bf16* q, const bf16* k, const bf16* v, bf16* o, un
       if (i < vectors) {
         const size_t key = i / vec_per_row;
         const unsigned d = (i % vec_per_row) * 8;
-        kk[b] = __ldg(reinterpret_cast<const uint4*>(k + key * k_stride + kv_head * head_dim + d));
-        vv[b] = __ldg(reinterpret_cast<const uint4*>(v + key * v_stride + kv_head * head_dim + d));
+        kk[b] = *reinterpret_cast<const uint4*>(k + key * k_stride + kv_head * head_dim + d);
+        vv[b] = *reinterpret_cast<const uint4*>(v + key * v_stride + kv_head * head_dim + d);
       }
     }
 #pragma unroll

@@ -31,7 +31,7 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {  // weights: read 
   return v;
 }
 __device__ __forceinline__ uint4 load_cached(const void* p) {  // activations: reused by every warp
-  return __ldg(reinterpret_cast<const uint4*>(p));
+  return *reinterpret_cast<const uint4*>(p);      // no constants of the launch: the one before may still write them when it begins
 }
 
 template <bool kFp8>
