@@ -33,8 +33,11 @@
 // 4-bit weights (kW4, bf16 tokens; the codes and scales of gemm_w4.cuh): the weight warps bring a block's codes into registers, three
 // blocks ahead, and write the slot's B operand themselves: code - 8 times the group's scale, rounded to bf16, four 16-byte pieces of a row a
 // lane and tile.  A tile's codes of all of K are asked into L2 when the CTA begins, a quarter of the bytes that bf16 weights take from memory.
+// The tensor core takes bf16, so the product of a code and a scale, up to twelve bits, loses its last ones: outputs are 1.9 - 2.2e-3 off (2-norm,
+// relative) where exact weights leave 1.7e-3; scales kept out of the operands would be a product and an addition of their own a group.
 // What bounds it is a block's turn through the ring, some 500 clocks whatever the tile (with copies, conversion, stores and products taken out
-// 22016 x 2048 still takes 12.5 of 24 us); eight converting warps, or one arrival a warp instead of one a thread, change nothing.
+// 22016 x 2048 still takes 12.5 of 24 us); eight converting warps, or one arrival a warp instead of one a thread, change nothing.  Counters of
+// 288 x 22016 x 2048: tensor pipe 28 % of active cycles, issue slots 49 %, load and store 61 %, DRAM 5 %, stalls mostly on loads.
 //
 // Every mbarrier wait is bounded and reports through the status word; nobody waits for another CTA except at the
 // cluster barrier.

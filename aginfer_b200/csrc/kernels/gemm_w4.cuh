@@ -69,8 +69,8 @@ __device__ __forceinline__ unsigned piece_of(unsigned low, unsigned high, float 
   const unsigned v2 = __float_as_uint(fmaf(__uint_as_float(high << 16), by, kRound)), v3 = __float_as_uint(fmaf(__uint_as_float(high & 0xffff0000u), by, kRound));
   return __byte_perm(__byte_perm(v0, v2, 0x5410) >> shift, __byte_perm(v1, v3, 0x5410) >> shift, 0x6420) & mask;
 }
-// Codes, read once: not kept in L1.  A launch before may write codes and scales while this one already lives, so they are no constants of it: with
-// ld.global.nc a product took what an earlier run had left of them in the SM's L1.
+// Codes, read once: not kept in L1.  A launch before may write codes and scales while this one already lives, so they are no constants of it: read
+// with ld.global.nc, behind the wait for that launch, products of 410 tokens were of an earlier run's codes.
 __device__ __forceinline__ uint4 stream_load(const uint4* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");

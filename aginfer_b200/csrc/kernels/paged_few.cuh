@@ -18,6 +18,9 @@
 // 2.0 - 2.3e-3 (2-norm, relative) off the definition where weights in 32 bits and the outputs' own rounding leave 1.6 - 1.7e-3.  Weights
 // in two bf16 pieces would take that back for twice the products of P V.
 //
+// Four mma.sync tiles of 128-wide heads (17 to 32 rows) are one CTA an SM and its latency: 64 sequences of 10000 keys, 28 heads on 4, us with 1 | 2 | 3
+// | 4 new tokens: bf16 207 | 211 | 579 | 583, 8 bits 118 | 189 | 550 | 552 (counters of the last: DRAM 1.2 TB/s, issue slots 22 %).
+//
 // A cache in 8 bits (kE4m3) brings half the bytes and goes through the same products after a conversion in registers.  Keys become f16,
 // which every code is (one instruction a pair), queries f16 too, times the power of two that brings a row's largest one to 2^14 .. 2^15:
 // bf16 has fewer digits, so that loses nothing but what lies 2^-39 below the row's largest.  Products are then of codes, and a score is
@@ -47,6 +50,7 @@ constexpr unsigned kKeys = 64, kConsumers = 128, kThreads = 160;
 //   1500 keys 12.3 | 14.3 | 12.3, 8192 18.4 | 39.7 | 22.5, 32000 31 - 33 | 43.6 | 47, 131072 56 | 71 | 150.
 // Twelve parts are few enough below 72 tiles (700 keys 12.3, runs of sqrt(n / 2) 14.3).  Where the batch is large enough to keep memory
 // busy, a third more than an even share is better than more parts (four sequences of 32000 keys on 4 heads 59.6, without it 62.4).
+// All of these with bf16 tiles; those of a cache in 8 bits go by the same rule (16 heads on 2: 1000 keys 10.5, 32000 27.3) and were not fitted.
 constexpr unsigned kFewParts = 12;
 __device__ __forceinline__ unsigned run_length(unsigned total, unsigned longest, unsigned ctas) {
   const unsigned even = (total + ctas - 1) / ctas, balanced = unsigned(ceilf(sqrtf(float(longest) * 0.5f)));

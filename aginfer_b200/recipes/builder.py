@@ -334,9 +334,11 @@ def tcs_tiling(M: int, tiles: int, K: int, cluster: int | None = None, groups: i
 W4_GROUPS = (32, 64, 128)                 # columns that share a scale
 # Tokens up to which the products are integer ones, a pass over the codes for every few tokens; beyond, the codes become bf16 operands of
 # tcgen05 tiles, and beyond W4_FUSED_ROWS, where every group of tokens would convert them again, bf16 weights in scratch for `gemm`.
-# us, integer | tcgen05 | scratch and gemm:  16 tokens 22016 x 2048 20.4 | 23.1, 2048 x 11008 17.6 | 16.6, 37888 x 3584 48 | 51;  32 tokens 35 | 24,
-# 27 | 17, 82 | 52;  64 tokens 62 | 25 | 36, 45 | 18 | 24, 162 | 54 | 118;  288 tokens - | 56 | 64, - | 35 | 36, - | 123 | 174;  600 tokens - | 88 | 87,
-# - | 46 | 56, - | 248 | 220.
+# us, integer | tcgen05, 22016 x 2048, 2048 x 11008, 37888 x 3584:  16 tokens 21.0 | 23.1, 18.8 | 16.7, 48.2 | 50.5;  32 tokens 35 | 24, 27 | 17, 82 | 52.
+# tcgen05 | scratch and gemm, these and 3584 x 18944:  48 tokens 24 | 37, 17 | 25, 53 | 120, 35 | 57;  288 58 | 62, 38 | 37, 146 | 173, 78 | 106;  400 66 | 80,
+# 40 | 41, 130 | 176, 76 | 92;  512 73 | 82, 42 | 41, 160 | 192, 82 | 97;  600 88 | 87, 45 | 57, 289 | 225, 131 | 120;  800 140 | 105, 49 | 52, 383 | 274, 149 | 173.
+# So the two meet somewhere between 512 and 600 tokens, and from 401 on to there the scratch is up to a fifth slower.  ``gemm`` on bf16 weights, for
+# comparison:  17 tokens 45, 14, 185, 38;  48 20, 15, 52, 31;  288 45, 27, 112, 80;  600 69, 46, 164, 92.
 W4_MAX_ROWS, W4_FUSED_ROWS = 16, 400
 
 
@@ -370,7 +372,8 @@ def w4_tiling(M: int, N: int, K: int, group: int = 64) -> Mapping[str, Any] | No
     The least estimate in clocks over parts and ways: rounds of the row tiles over the warps, each 350 clocks a block (770 with two eights) and 1730
     besides, 300 a block of one round for the warps that end last, 14 a block of tokens laid out; where parts of K meet 1500, 3880 a round, 90 a
     part and tile.  Fitted to seven shapes with 1, 4, 8 and 16 tokens in groups of 64;
-    of parts 1 to 10 and 12 and all ways it takes one within 3 % of the fastest there, but for 3584 x 18944, where it takes five parts: 1 token
+    of parts 1 to 10 and 12 and all ways it takes one within 3 % of the fastest there (before blocks were looked at for uneven values, which adds 0.2 to
+    1 us to each), but for 3584 x 18944, where it takes five parts: 1 token
     16.3 us (fastest 15.1), 4 tokens 20.5 (four parts 18.0), 8 tokens 30.9 (two 26.9), 16 tokens 53 (four 45).  1 token, us with 8 | 4 | 2 | 1 ways: 37888 x 3584 17.7 |
     17.0 | 17.4 | 17.8, 22016 x 2048 8.8 | 8.5 | 8.9 | 10.3; four ways in 1 | 2 | 4 parts: 2048 x 11008 13.8 | 10.0 | 8.4.
     Sixteen tokens of a CTA share a pass over the codes
@@ -1106,7 +1109,8 @@ class RecipeBuilder:
         ``window``: a token sees itself and the ``window`` - 1 before it (0: everything), and the first ``sinks`` tokens.
         ``longest``: the most new tokens that one sequence has (``rows`` where it is left out); it says which kernel is
         launched; results differ by roundings alone.  Weights are rounded to bf16 before they meet the values, maxima and sums are in 32
-        bits.  A row that sees nothing is zero; rows of no sequence are left alone.
+        bits.  A row that sees nothing is zero; rows of no sequence are left alone.  With a cache in 8 bits and at most PAGED_FEW_ROWS rows a sequence
+        and key head the codes are read as they are; beyond, the pages in view come into the arena as bf16 first.
         ``o`` may be ``q`` at the same pitch; it shares no other memory with it."""
         self._paged_attention(q, o, cache, None, rows=rows, q_heads=q_heads, longest=longest, window=window, sinks=sinks,
                               q_stride=q_stride, o_stride=o_stride, scale=scale, op="paged_attention")
