@@ -68,3 +68,35 @@ def test_of_unequal_size(tmp_path, m):
     sparse[:, [5, 40, 700]] = torch.randn(m, 3, generator=g)
     (tmp_path / "sparse").mkdir()
     run_and_check(tmp_path / "sparse", *with_outliers(m, 90, 1024, 64, 1000.0, [6, 701], rest=sparse.to(BF)))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_every_geometry(tmp_path, monkeypatch, group):
+    """Ways, parts, copies and depths of the ring over a product some of whose blocks are of integers and some are not."""
+    from aginfer_b200.recipes import builder as B
+    k, blocks = 2816, 44
+    places = [block * 64 + (block * 37) % 64 for block in range(blocks) if block % 5 in (0, 1, 3)]
+    full, clean = with_outliers(6, 1003, k, group, 2000.0, places, seed=group)
+    for i, (eights, splits, ways, chunk, stages, ctas) in enumerate(((1, 1, 1, 4, 2, 3), (1, 1, 8, 8, 2, 1), (2, 1, 2, 4, 3, 5), (1, 5, 4, 4, 2, 7), (2, 3, 1, 8, 2, 2), (1, 44, 8, 4, 5, 3))):
+        groups, per = -(-full.m // (4 * eights)), -(-blocks // splits)
+        tiling = {"eights": eights, "splits": splits, "ways": ways, "chunk": chunk, "stages": stages, "grid": (ctas, groups, splits),
+                  "shared_bytes": 16 * stages * chunk * 576 + per * eights * (672 if group == 32 else 608)}
+        assert tiling["shared_bytes"] + B.W4_STATIC_BYTES <= B.MAX_DYNAMIC_SHARED
+        monkeypatch.setattr(B, "w4_tiling", lambda *a, tiling=tiling: tiling)
+        where = tmp_path / str(i)
+        where.mkdir()
+        run_and_check(where, full, clean)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_beside_a_token_that_is_not_finite(tmp_path, value):
+    full, clean = with_outliers(7, 90, 512, 64, 5000.0, [3, 77, 300])
+    runner, x, out = packaged(tmp_path, full)
+    x["x"][2, 70] = value
+    x["x"][5, 400] = value
+    runner.run(x, out)
+    got = out["y"].cpu()
+    assert int(out["status"].cpu()) == 0 and bool(got[[2, 5]].isnan().all())
+    want, bound = clean.expected()
+    kept = [0, 1, 3, 4, 6]
+    assert bool(((got[kept].double() - want[kept]).abs()[:, ::2] <= bound[kept][:, ::2]).all())
